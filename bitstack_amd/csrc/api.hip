@@ -435,3 +435,100 @@ extern "C" int bs_argmax_advance_f16(const void *x, int64_t *out, int64_t *pos, 
     if (!bs_aligned(x, 16) || !bs_aligned(out, 8) || !bs_aligned(pos, 8) || (B > 1 && V % 8 != 0)) return BS_ERR_ALIGN;
     return bs_launch_argmax((const half_t *)x, out, pos, B, V, (hipStream_t)stream);
 }
+
+// ---- requests of unequal lengths -----------------------------------------------------------------
+// log2 of a page's positions, or -1
+static int page_shift(int page_size) {
+    if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)) != 0) return -1;
+    return __builtin_ctz((unsigned)page_size);
+}
+static bool pool_fits(int pool_pages, int page_size) { return pool_pages >= 1 && (int64_t)pool_pages * page_size <= INT32_MAX; }
+
+static int plan_shape(int B, int T, int page_size, int max_pages, int pool_pages) {
+    return B < 0 || B > 65536 || T < 0 || T > 1 << 30 || page_shift(page_size) < 0 || max_pages < 1 || max_pages > 1 << 24 || !pool_fits(pool_pages, page_size)
+               ? BS_ERR_SHAPE
+               : BS_OK;
+}
+
+extern "C" int64_t bs_page_plan_workspace_bytes(int B, int T) {
+    return B < 0 || B > 65536 || T < 0 || T > 1 << 30 ? BS_ERR_SHAPE : bs_page_plan_scratch(B, T);
+}
+
+extern "C" int bs_page_plan(const int32_t *lengths, const int32_t *new_tokens, const uint8_t *released, int32_t *block_table, int32_t *free_pages,
+                            const int32_t *free_state, int32_t *lengths_out, int32_t *free_state_out, int32_t *granted, int32_t *starts,
+                            int32_t *positions, int64_t *slots, int B, int T, int page_size, int max_pages, int pool_pages, void *workspace,
+                            int64_t workspace_bytes, void *stream) {
+    const int st = plan_shape(B, T, page_size, max_pages, pool_pages);
+    if (st != BS_OK) return st;
+    if (!free_pages || !free_state || !free_state_out || !starts || (T > 0 && (!positions || !slots)) ||
+        (B > 0 && (!lengths || !new_tokens || !block_table || !lengths_out || !granted)))
+        return BS_ERR_NULL;
+    for (const void *p : {(const void *)lengths, (const void *)new_tokens, (const void *)block_table, (const void *)free_pages, (const void *)free_state,
+                          (const void *)lengths_out, (const void *)free_state_out, (const void *)granted, (const void *)starts, (const void *)positions})
+        if (!bs_aligned(p, 4)) return BS_ERR_ALIGN;
+    if (!bs_aligned(slots, 8)) return BS_ERR_ALIGN;
+    const int64_t need = bs_page_plan_scratch(B, T);
+    if (need > 0 && (!workspace || workspace_bytes < need || !bs_aligned(workspace, 16))) return BS_ERR_WORKSPACE;
+    return bs_launch_page_plan(lengths, new_tokens, released, block_table, free_pages, free_state, lengths_out, free_state_out, granted, starts, positions, slots,
+                               B, T, page_shift(page_size), max_pages, pool_pages, workspace, (hipStream_t)stream);
+}
+
+extern "C" int bs_rope_store_paged_f16(void *q, int ldq, void *q_out, int ldq_out, const void *k, const void *v, int ldkv, const void *cos, const void *sin,
+                                       const int32_t *positions, const int64_t *slots, void *kpages, void *vpages, int T, int heads, int kv_heads,
+                                       int head_dim, int max_pos, int page_size, int pool_pages, void *stream) {
+    if (T < 0 || (head_dim != 64 && head_dim != 128) || kv_heads < 1 || max_pos < 1 || page_shift(page_size) < 0 || !pool_fits(pool_pages, page_size) ||
+        (q && heads < 1) || ((q ? heads : 0) + 3 * (int64_t)kv_heads) * head_dim > INT32_MAX || ldkv < (int64_t)kv_heads * head_dim ||
+        (q && ldq < (int64_t)heads * head_dim) || (q_out && ldq_out < (int64_t)heads * head_dim) || (q_out && !q) || (q && q_out == q && ldq_out != ldq))
+        return BS_ERR_SHAPE;
+    if (T == 0) return BS_OK;
+    if (!k || !v || !cos || !sin || !positions || !slots || !kpages || !vpages) return BS_ERR_NULL;
+    for (const void *p : {(const void *)q, (const void *)q_out, (const void *)k, (const void *)v, (const void *)cos, (const void *)sin, (const void *)kpages, (const void *)vpages})
+        if (!bs_aligned(p, 2)) return BS_ERR_ALIGN;
+    if (!bs_aligned(positions, 4) || !bs_aligned(slots, 8)) return BS_ERR_ALIGN;
+    half_t *from = q ? (half_t *)q : (half_t *)k;          // (no heads: neither read nor written)
+    return bs_launch_rope_store_paged(from, q_out ? (half_t *)q_out : from, (const half_t *)k, (const half_t *)v, (const half_t *)cos, (const half_t *)sin, positions,
+                                      slots, (half_t *)kpages, (half_t *)vpages, q ? ldq : ldkv, q ? (q_out ? ldq_out : ldq) : ldkv, ldkv, T, q ? heads : 0,
+                                      kv_heads, head_dim, max_pos, page_shift(page_size), pool_pages, (hipStream_t)stream);
+}
+
+static int attention_paged_shape(int B, int heads, int kv_heads, int head_dim, int page_size, int max_pages) {
+    return B < 0 || B > 65536 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || (head_dim != 64 && head_dim != 128) || page_shift(page_size) < 0 ||
+                   max_pages < 1 || (int64_t)max_pages * page_size > INT32_MAX || (int64_t)B * ((int64_t)max_pages * page_size / 16) > INT32_MAX ||
+                   ((int64_t)heads + 2 * (int64_t)kv_heads) * head_dim > INT32_MAX || (int64_t)B * heads > INT32_MAX
+               ? BS_ERR_SHAPE
+               : BS_OK;
+}
+
+extern "C" int64_t bs_attention_paged_workspace_bytes(int B, int heads, int kv_heads, int head_dim, int page_size, int max_pages) {
+    const int st = attention_paged_shape(B, heads, kv_heads, head_dim, page_size, max_pages);
+    return st != BS_OK ? st : B == 0 ? 0 : bs_attention_paged_scratch(B, heads, kv_heads, head_dim, max_pages, page_size);
+}
+
+extern "C" int bs_attention_paged_f16(const void *qkv, int ldqkv, void *kpages, void *vpages, const void *cos, const void *sin, const int32_t *block_table,
+                                      const int32_t *lengths, const int64_t *slots, void *out, int B, int heads, int kv_heads, int head_dim, int max_pos,
+                                      int page_size, int max_pages, int pool_pages, void *workspace, int64_t workspace_bytes, void *stream) {
+    const int st = attention_paged_shape(B, heads, kv_heads, head_dim, page_size, max_pages);
+    if (st != BS_OK) return st;
+    if (max_pos < 1 || !pool_fits(pool_pages, page_size) || ldqkv < ((int64_t)heads + 2 * (int64_t)kv_heads) * head_dim) return BS_ERR_SHAPE;
+    if (B == 0) return BS_OK;
+    if (!qkv || !kpages || !vpages || !cos || !sin || !block_table || !lengths || !slots || !out) return BS_ERR_NULL;
+    if (!bs_aligned(qkv, 2) || !bs_aligned(kpages, 16) || !bs_aligned(vpages, 16) || !bs_aligned(cos, 2) || !bs_aligned(sin, 2) || !bs_aligned(block_table, 4) ||
+        !bs_aligned(lengths, 4) || !bs_aligned(slots, 8) || !bs_aligned(out, 2))
+        return BS_ERR_ALIGN;
+    const int64_t need = bs_attention_paged_scratch(B, heads, kv_heads, head_dim, max_pages, page_size);
+    if (need > 0 && (!workspace || workspace_bytes < need || !bs_aligned(workspace, 16))) return BS_ERR_WORKSPACE;
+    return bs_launch_attention_paged((const half_t *)qkv, ldqkv, (half_t *)kpages, (half_t *)vpages, (const half_t *)cos, (const half_t *)sin, block_table, lengths,
+                                     slots, (half_t *)out, B, heads, kv_heads, head_dim, max_pos, page_shift(page_size), max_pages, pool_pages, workspace,
+                                     (hipStream_t)stream);
+}
+
+extern "C" int bs_sample_f16(const void *logits, int64_t ld, const float *uniform, const float *temperature, const int32_t *top_k, const float *top_p,
+                             const float *min_p, int64_t *out, int B, int V, void *stream) {
+    if (B < 0 || V < 1 || V > 1 << 18 || (B > 1 && ld < V)) return BS_ERR_SHAPE;
+    if (B == 0) return BS_OK;
+    if (!logits || !uniform || !out) return BS_ERR_NULL;
+    if (!bs_aligned(logits, 2) || !bs_aligned(uniform, 4) || !bs_aligned(temperature, 4) || !bs_aligned(top_k, 4) || !bs_aligned(top_p, 4) || !bs_aligned(min_p, 4) ||
+        !bs_aligned(out, 8))
+        return BS_ERR_ALIGN;
+    return bs_launch_sample((const half_t *)logits, ld, uniform, temperature, top_k, top_p, min_p, out, B, V, (hipStream_t)stream);
+}

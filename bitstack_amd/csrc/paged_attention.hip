@@ -1,0 +1,437 @@
+// One new token per request over the paged cache: out = softmax(q k^T / sqrt(D)) v over the request's positions, the last of them this
+// step's own, which is rotated and appended here.
+//
+// A unit is the up to 16 query heads of one KV head that share its rows: they are the columns of both products, so K and V are read once.
+//   scores  S[position, head] = K q     16x16x32, K rows as loaded (a lane: position l % 16, dimensions 32 c + 8 (l / 16) ..); the rotated query
+//                                       in two fp16 terms too.  Up to eight heads leave columns free: those are the second terms', and a
+//                                       score is the sum of two lanes; with more heads it is a product of its own.  (Rounded to fp16 the query alone put the
+//                                       result's error against 64 bits from 2.0e-4, the rounding of the result, to 3.4e-4.)
+//   output  O[dim, head] += V^T P       16x16x32, four positions twice: P is split into two fp16 terms, p = hi + lo to 2^-22, and the eight
+//                                       k slots of a lane hold {hi, lo} against {v, v}: the weights keep the precision of fp32 numbers
+// A lane of the scores holds positions 4 (l / 16) + i of head l % 16, which is what the second product wants of P; V needs no transposition
+// either: a lane loads dimensions W r .. W r + W - 1 (r = l % 16, W = D / 16) of its four positions, and product j takes element j of each, so that its
+// row r is dimension W r + j.  Maximum, sum and output are fp32, in base 2; K of the next tile of 16 positions is requested behind the scores, V behind the
+// output product, the tile's page one tile further ahead.
+//
+// The split: the lengths are known on the device alone, so every workgroup works out from them what it is to do.  The first B workgroups of a unit take
+// one request each, or the first part of it; if requests are longer than C = (all tiles) / (parts that fill the chip), the next ones take
+// the further parts, in order.  Parts leave (max, sum, weighted v) in the workspace, and a second launch puts them together, in order: the
+// result does not depend on which came first.
+#include "common.h"
+
+namespace {
+
+constexpr int PA_TILE = 16, PA_HEADS = 16;       // positions of a tile; query heads of a unit
+constexpr int PA_PARTS = 768;                    // workgroups (over all units) that further parts may add
+constexpr int PA_LEAST = 32;                     // tiles of a part, at least
+
+struct pa_args {
+    const half_t *qkv, *cosv, *sinv;
+    half_t *kpages, *vpages;
+    const int32_t *lengths;
+    const int64_t *slots;
+    half_t *out;
+    int32_t *heads_of;                           // workspace: {first further part, further parts} of every request
+    float *part;                                 // ... and what the parts leave
+    int ldqkv, B, heads, kv_heads, groups, per_unit, max_pos, shift, max_pages, pool, parts;
+};
+
+// positions of request b that the cache holds (without its own): 0 for a length that is none
+__device__ __forceinline__ int pa_cached(const pa_args &a, int b) {
+    const int len = a.lengths[b];
+    return len > 0 && len <= a.max_pos && (int64_t)len <= (int64_t)a.max_pages << a.shift ? len - 1 : 0;
+}
+__device__ __forceinline__ int pa_tiles(int cached) { return (cached + PA_TILE - 1) / PA_TILE; }
+__device__ __forceinline__ int pa_further(int tiles, int most) { return tiles > most ? (tiles + most - 1) / most - 1 : 0; }
+
+template <int WAVES>
+__device__ __forceinline__ int pa_sum(int v, int *to) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+    if ((threadIdx.x & 63) == 0) to[threadIdx.x >> 6] = v;
+    __syncthreads();
+    int s = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) s += to[w];
+    return s;
+}
+
+// the value of the lane eight on (or back) in the row of 16
+__device__ __forceinline__ float eight_on(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x128, 0xf, 0xf, true));    // row_ror:8
+}
+
+template <int D, int HP, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void attention_paged_kernel(const pa_args a, const int32_t *__restrict__ table) {
+    constexpr int THREADS = WAVES * 64, W = D / 16, NC = D / 32, D2 = D / 2;
+    typedef half_t vec_t __attribute__((ext_vector_type(W)));
+    __shared__ __attribute__((aligned(16))) half_t qrot[2][HP][D];             // rotated queries, first and second terms
+    __shared__ __attribute__((aligned(16))) half_t knew[D], vnew[D];           // this position's rotated k and v
+    __shared__ float wm[HP][WAVES], wl[HP][WAVES];                             // per wave: running max, sum of exp
+    __shared__ __attribute__((aligned(16))) float wacc[HP][WAVES][D];
+    __shared__ int sums[WAVES], found[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
+    const int units = a.kv_heads * a.groups, unit = blockIdx.x % units, work = blockIdx.x / units;
+    const int hk = unit % a.kv_heads, hg = unit / a.kv_heads, rep = a.heads / a.kv_heads;
+    const int head0 = hk * rep + hg * a.per_unit, nh = min(a.per_unit, rep - hg * a.per_unit);
+
+    // ---- which request, which part of it
+    int all = 0;
+    for (int i = tid; i < a.B; i += THREADS) all += pa_tiles(pa_cached(a, i));
+    int b = work, part = 0;
+    const int64_t slot0 = work < a.B ? a.slots[work] : 0;
+    all = pa_sum<WAVES>(all, sums);
+    const int most = max(PA_LEAST, (all + a.parts - 1) / max(a.parts, 1));
+    int further = 0, place = 0;                  // further parts of this request, and the first one's number
+    if (work < a.B) further = a.parts > 0 ? pa_further(pa_tiles(pa_cached(a, work)), most) : 0;
+    if (work >= a.B || further > 0) {            // numbers of the further parts: a running sum over the requests
+        if (tid == 0) found[0] = -1;
+        int before = 0;
+        const int wanted = work - a.B;
+        for (int i0 = 0; i0 < a.B; i0 += THREADS) {
+            const int i = i0 + tid, mine = i < a.B ? pa_further(pa_tiles(pa_cached(a, i)), most) : 0;
+            int s = mine;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int below = __shfl_up(s, o, 64);
+                if (lane >= o) s += below;
+            }
+            __syncthreads();
+            if (lane == 63) sums[wave] = s;
+            __syncthreads();
+            int ahead = before;
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) {
+                if (w < wave) ahead += sums[w];
+                before += sums[w];
+            }
+            const int first = ahead + s - mine;
+            if (work < a.B ? i == work : wanted >= first && wanted < first + mine) {
+                found[0] = i;
+                found[1] = first;
+                found[2] = mine;
+            }
+        }
+        __syncthreads();
+        if (found[0] < 0) return;                // no such part
+        b = __builtin_amdgcn_readfirstlane(found[0]);
+        place = __builtin_amdgcn_readfirstlane(found[1]);
+        further = __builtin_amdgcn_readfirstlane(found[2]);
+        if (work >= a.B) part = wanted - place + 1;
+    }
+    const int len = a.lengths[b];
+    const int64_t slot = work < a.B ? slot0 : a.slots[b];
+    const bool live = slot >= 0 && slot < (int64_t)a.pool << a.shift && len > 0 && len <= a.max_pos && (int64_t)len <= (int64_t)a.max_pages << a.shift;
+    half_t *orow = a.out + ((int64_t)b * a.heads + head0) * D;
+    if (part == 0 && unit == 0 && a.parts > 0 && tid == 0) {
+        a.heads_of[2 * b] = place;
+        a.heads_of[2 * b + 1] = live ? further : 0;
+    }
+    if (!live) {                                 // an idle row: zeros, and nothing is stored
+        if (part == 0)
+            for (int it = tid; it < nh * D; it += THREADS) orow[it] = (half_t)0;
+        return;
+    }
+    const int pos = len - 1, tiles = pa_tiles(pos), parts = further + 1;
+    const int t_first = (int)((int64_t)tiles * part / parts), t_end = (int)((int64_t)tiles * (part + 1) / parts);
+
+    // ---- the rows of the cache
+    const half_t *qh = a.qkv + (int64_t)b * a.ldqkv;
+    const int32_t *row = table + (int64_t)b * a.max_pages;
+    const int64_t page_step = (int64_t)a.kv_heads * D << a.shift, head_at = (int64_t)hk * D << a.shift;
+    half8_t k8[NC];
+    vec_t v8[4];
+    auto page_of = [&](int t) { return row[__builtin_amdgcn_readfirstlane((t * PA_TILE) >> a.shift)]; };
+    auto good = [&](int id) { return id >= 0 && id < a.pool; };       // (positions of a page that does not exist are left out)
+    auto at_row = [&](int id, int t, int r) {    // rows past the last are the last again; their scores are masked
+        return (int64_t)(good(id) ? id : 0) * page_step + head_at + (int64_t)(min(t * PA_TILE + r, pos - 1) & ((1 << a.shift) - 1)) * D;
+    };
+    auto fetch_k = [&](int id, int t) {
+        const half_t *p = a.kpages + at_row(id, t, r16) + 8 * g;
+#pragma unroll
+        for (int c = 0; c < NC; c++) k8[c] = *reinterpret_cast<const half8_t *>(p + 32 * c);
+    };
+    auto fetch_v = [&](int id, int t) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v8[i] = *reinterpret_cast<const vec_t *>(a.vpages + at_row(id, t, 4 * g + i) + W * r16);
+    };
+    int t = t_first + wave, id = 0, next_id = 0;
+    if (t < t_end) id = page_of(t);
+    if (t + WAVES < t_end) next_id = page_of(t + WAVES);
+
+    // ---- this position's own: pairs (i, i + D / 2) of the unit's queries, of k and of v
+    constexpr int PAIRS = (HP + 2) * D2, EACH = (PAIRS + THREADS - 1) / THREADS;
+    half_t pa[EACH], pb[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        const int it = tid + e * THREADS, h = it / D2, i = it % D2;
+        pa[e] = pb[e] = (half_t)0;
+        const int at = h < HP ? (head0 + h) * D : (a.heads + (h - HP) * a.kv_heads + hk) * D;
+        if (h < HP + 2 && (h >= HP || h < nh)) {
+            pa[e] = qh[at + i];
+            pb[e] = qh[at + i + D2];
+        }
+    }
+    if (t < t_end) {
+        fetch_k(id, t);
+        fetch_v(id, t);
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        const int it = tid + e * THREADS, h = it / D2, i = it % D2;
+        if (h < HP + 1) {
+            const float c = (float)a.cosv[(int64_t)pos * D2 + i], sn = (float)a.sinv[(int64_t)pos * D2 + i];
+            const float x = (float)pa[e] * c - (float)pb[e] * sn, y = (float)pb[e] * c + (float)pa[e] * sn;
+            half_t *to = h < HP ? qrot[0][h] : knew;
+            to[i] = (half_t)x;
+            to[i + D2] = (half_t)y;
+            if (h < HP) {
+                qrot[1][h][i] = (half_t)(x - (float)(half_t)x);
+                qrot[1][h][i + D2] = (half_t)(y - (float)(half_t)y);
+            }
+        } else if (h < HP + 2) {
+            vnew[i] = pa[e];
+            vnew[i + D2] = pb[e];
+        }
+    }
+    __syncthreads();
+    if (part == 0 && hg == 0 && tid < D) {       // one workgroup of the KV head appends this position to the cache
+        const int64_t at = (slot >> a.shift) * page_step + head_at + (slot & ((1 << a.shift) - 1)) * D + tid;
+        a.kpages[at] = knew[tid];
+        a.vpages[at] = vnew[tid];
+    }
+
+    // column r: first terms of head r; up to eight heads: column 8 + r the second terms
+    constexpr int TERMS = HP > 8 ? 2 : 1;
+    half8_t q8[TERMS][NC];
+    const int column = HP > 8 ? r16 : r16 & 7;
+#pragma unroll
+    for (int e = 0; e < TERMS; e++)
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+            q8[e][c] = column < HP ? *reinterpret_cast<const half8_t *>(&qrot[HP > 8 ? e : r16 >> 3][column < HP ? column : 0][32 * c + 8 * g]) : (half8_t)(half_t)0;
+    const float scale2 = (D == 128 ? 0.08838834764831845f : 0.125f) * 1.4426950408889634f;    // log2(e) / sqrt(D)
+    float m = -INFINITY, l = 0.f;                // of head l % 16; the sum over this lane's positions only
+    float4_t acc[W];
+#pragma unroll
+    for (int j = 0; j < W; j++) acc[j] = (float4_t)0.f;
+    auto scores = [&]() {
+        float4_t s = (float4_t)0.f;
+#pragma unroll
+        for (int e = 0; e < TERMS; e++)
+#pragma unroll
+            for (int c = 0; c < NC; c++) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8[c], q8[e][c], s, 0, 0, 0);
+        if (TERMS == 1) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[i] += eight_on(s[i]);
+        }
+        return s;
+    };
+    auto fold = [&](const float4_t s, int valid) {                      // the tile's first `valid` positions (at least one)
+        float p[4], mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            p[i] = 4 * g + i < valid ? s[i] * scale2 : -INFINITY;
+            mx = fmaxf(mx, p[i]);
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float mn = fmaxf(m, mx), r = __builtin_amdgcn_exp2f(m - mn);      // exp2(-inf) = 0 on the first tile
+        m = mn;
+        half8_t p8;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            p[i] = __builtin_amdgcn_exp2f(p[i] - mn);
+            sum += p[i];
+            p8[i] = (half_t)p[i];
+            p8[i + 4] = (half_t)(p[i] - (float)p8[i]);
+        }
+        l = l * r + sum;
+        if (__any(r != 1.f)) {
+#pragma unroll
+            for (int j = 0; j < W; j++) acc[j] *= r;
+        }
+#pragma unroll
+        for (int j = 0; j < W; j++) {
+            const half8_t v = {v8[0][j], v8[1][j], v8[2][j], v8[3][j], v8[0][j], v8[1][j], v8[2][j], v8[3][j]};
+            acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p8, acc[j], 0, 0, 0);
+        }
+    };
+    while (t < t_end) {
+        const int next = t + WAVES, now = id;
+        const float4_t s = scores();
+        id = next_id;
+        if (next < t_end) fetch_k(id, next);
+        if (next + WAVES < t_end) next_id = page_of(next + WAVES);
+        if (good(now)) fold(s, pos - t * PA_TILE);
+        if (next < t_end) fetch_v(id, next);
+        t = next;
+    }
+    // its own k and v, from LDS, by the wave whose turn is next: a tile with one position
+    const bool own = part == 0 && wave == (t_end - t_first) % WAVES;
+    auto take_own = [&]() {
+#pragma unroll
+        for (int c = 0; c < NC; c++) k8[c] = *reinterpret_cast<const half8_t *>(&knew[32 * c + 8 * g]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v8[i] = *reinterpret_cast<const vec_t *>(&vnew[W * r16]);
+    };
+    if (own) {
+        take_own();
+        fold(scores(), 1);
+    }
+
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (r16 < HP && g == 0) { wm[r16][wave] = m; wl[r16][wave] = l; }
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < W; j++) sum += (acc[j][0] + acc[j][1]) + (acc[j][2] + acc[j][3]);
+    if (__builtin_expect(__any(sum != sum), 0)) {
+        // An infinite v: times a second term of zero or below it, or a masked weight, it is NaN in the output product.  The wave's
+        // positions once more, head by head, each weight as one fp32 number: a lane owns dimensions W r16 .. W r16 + W - 1.
+#pragma unroll 1
+        for (int h = 0; h < HP; h++) {
+            float o[W];
+#pragma unroll
+            for (int e = 0; e < W; e++) o[e] = 0.f;
+            auto add = [&](const float4_t s, int valid) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float w = __shfl(__builtin_amdgcn_exp2f(s[i] * scale2 - m), (lane & 48) | h, 64);
+#pragma unroll
+                    for (int e = 0; e < W; e++)
+                        if (4 * g + i < valid) o[e] += w * (float)v8[i][e];
+                }
+            };
+            for (t = t_first + wave; t < t_end; t += WAVES) {
+                id = page_of(t);
+                if (!good(id)) continue;
+                fetch_k(id, t);
+                fetch_v(id, t);
+                add(scores(), pos - t * PA_TILE);
+            }
+            if (own) {
+                take_own();
+                add(scores(), 1);
+            }
+#pragma unroll
+            for (int e = 0; e < W; e++) {
+                o[e] += __shfl_xor(o[e], 16, 64);
+                o[e] += __shfl_xor(o[e], 32, 64);
+                if (g == 0) wacc[h][wave][W * r16 + e] = o[e];
+            }
+        }
+    } else if (r16 < HP) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)              // row 4 g + i of product j is dimension W (4 g + i) + j
+#pragma unroll
+            for (int j = 0; j < W; j += 4)
+                *reinterpret_cast<float4_t *>(&wacc[r16][wave][W * (4 * g + i) + j]) = (float4_t){acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]};
+    }
+    __syncthreads();
+    const int64_t mine = ((int64_t)(part == 0 ? b : a.B + place + part - 1) * a.kv_heads + hk) * rep + hg * a.per_unit;
+    for (int it = tid; it < nh * D; it += THREADS) {
+        const int h = it / D, dim = it % D;
+        float mx = wm[h][0];
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) mx = fmaxf(mx, wm[h][w]);
+        float o = 0.f, den = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            const float r = wl[h][w] != 0.f ? __builtin_amdgcn_exp2f(wm[h][w] - mx) : 0.f;    // 0: a wave that saw no position
+            o += wl[h][w] != 0.f ? r * wacc[h][w][dim] : 0.f;
+            den += r * wl[h][w];
+        }
+        if (further > 0) {                       // part[request or further part][head][max, sum, pad, pad, weighted v]
+            float *to = a.part + (mine + h) * (D + 4);
+            to[4 + dim] = o;
+            if (dim == 0) { to[0] = mx; to[1] = den; }
+        } else {
+            orow[it] = (half_t)(o / den);
+        }
+    }
+}
+
+// The parts of one head put together, in order, eight of them requested at once.
+template <int D>
+__global__ __launch_bounds__(D) void attention_paged_merge_kernel(const float *__restrict__ part, const int32_t *__restrict__ heads_of, half_t *__restrict__ out,
+                                                                  int B, int heads) {
+    const int dim = threadIdx.x, b = blockIdx.x / heads, head = blockIdx.x % heads;
+    const int place = heads_of[2 * b], further = heads_of[2 * b + 1];
+    if (further == 0) return;                    // written by the first launch
+    auto from = [&](int i) { return part + ((int64_t)(i == 0 ? b : B + place + i - 1) * heads + head) * (D + 4); };
+    float mx = -INFINITY, o = 0.f, den = 0.f;
+    for (int i0 = 0; i0 <= further; i0 += 8) {
+        float m[8], l[8], v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float *p = from(min(i0 + j, further));
+            m[j] = p[0];
+            l[j] = i0 + j <= further ? p[1] : 0.f;
+            v[j] = p[4 + dim];
+        }
+        float top = mx;
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = fmaxf(top, l[j] != 0.f ? m[j] : -INFINITY);
+        const float r0 = den != 0.f ? __builtin_amdgcn_exp2f(mx - top) : 0.f;
+        o = den != 0.f ? o * r0 : 0.f;
+        den *= r0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float r = l[j] != 0.f ? __builtin_amdgcn_exp2f(m[j] - top) : 0.f;
+            o += l[j] != 0.f ? r * v[j] : 0.f;
+            den += r * l[j];
+        }
+        mx = top;
+    }
+    out[(int64_t)blockIdx.x * D + dim] = (half_t)(o / den);
+}
+
+struct pa_shape {
+    int rep, groups, per_unit, units, parts;
+};
+pa_shape shape_of(int heads, int kv_heads, int64_t positions) {
+    pa_shape p;
+    p.rep = heads / kv_heads;
+    p.groups = (int)bs_cdiv(p.rep, PA_HEADS);
+    p.per_unit = (int)bs_cdiv(p.rep, p.groups);
+    p.units = kv_heads * p.groups;
+    p.parts = positions <= PA_LEAST * PA_TILE ? 0 : (int)(PA_PARTS / p.units > 1 ? PA_PARTS / p.units : 1);
+    return p;
+}
+
+template <int D, int HP>
+int launch(const pa_args &a, const int32_t *table, int64_t workgroups, hipStream_t s) {
+    attention_paged_kernel<D, HP, HP == 16 ? 4 : 8><<<(unsigned)workgroups, (HP == 16 ? 4 : 8) * 64, 0, s>>>(a, table);
+    BS_LAUNCH_CHECK();
+    return BS_OK;
+}
+
+}  // namespace
+
+int64_t bs_attention_paged_scratch(int B, int heads, int kv_heads, int head_dim, int max_pages, int page) {
+    const pa_shape p = shape_of(heads, kv_heads, (int64_t)max_pages * page);
+    return p.parts ? bs_cdiv(8ll * B, 16) * 16 + (int64_t)(B + p.parts) * heads * (head_dim + 4) * 4 : 0;
+}
+
+int bs_launch_attention_paged(const half_t *qkv, int ldqkv, half_t *kpages, half_t *vpages, const half_t *cos, const half_t *sin, const int32_t *table,
+                              const int32_t *lengths, const int64_t *slots, half_t *out, int B, int heads, int kv_heads, int head_dim, int max_pos,
+                              int shift, int max_pages, int pool, void *workspace, hipStream_t s) {
+    const pa_shape p = shape_of(heads, kv_heads, (int64_t)max_pages << shift);
+    const int64_t workgroups = (int64_t)(B + p.parts) * p.units;
+    if (workgroups > INT32_MAX) return BS_ERR_SHAPE;
+    pa_args a = {qkv, cos, sin, kpages, vpages, lengths, slots, out, (int32_t *)workspace, (float *)((char *)workspace + bs_cdiv(8ll * B, 16) * 16),
+                 ldqkv, B, heads, kv_heads, p.groups, p.per_unit, max_pos, shift, max_pages, pool, p.parts};
+    int st;
+    if (head_dim == 128)
+        st = p.per_unit > 8 ? launch<128, 16>(a, table, workgroups, s) : p.per_unit > 4 ? launch<128, 8>(a, table, workgroups, s) : p.per_unit > 2 ? launch<128, 4>(a, table, workgroups, s)
+           : p.per_unit > 1 ? launch<128, 2>(a, table, workgroups, s) : launch<128, 1>(a, table, workgroups, s);
+    else
+        st = p.per_unit > 8 ? launch<64, 16>(a, table, workgroups, s) : p.per_unit > 4 ? launch<64, 8>(a, table, workgroups, s) : p.per_unit > 2 ? launch<64, 4>(a, table, workgroups, s)
+           : p.per_unit > 1 ? launch<64, 2>(a, table, workgroups, s) : launch<64, 1>(a, table, workgroups, s);
+    if (st != BS_OK || p.parts == 0) return st;
+    (head_dim == 128 ? attention_paged_merge_kernel<128> : attention_paged_merge_kernel<64>)<<<(unsigned)((int64_t)B * heads), head_dim, 0, s>>>(a.part, a.heads_of, out, B, heads);
+    BS_LAUNCH_CHECK();
+    return BS_OK;
+}

@@ -3,6 +3,8 @@
 """
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
 from bitstack_amd import _lib
@@ -330,6 +332,138 @@ def argmax_hip(x, out=None):
     with torch.cuda.device(dev):
         _lib.check(_lib.lib().bs_argmax_f16(_lib.ptr(x), _lib.ptr(y), x.shape[0], x.shape[1], _lib.stream_ptr(dev)),
                    "bs_argmax_f16")
+    return y
+
+
+# ---- requests of unequal lengths: a cache in pages -----------------------------------------------------------------------
+def _vector(t, n, dtype, name):
+    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor [{n}], got {t.dtype} {tuple(t.shape)}")
+
+
+class PagePlan(NamedTuple):
+    """What page_plan_hip gives: positions per request and the ring's {first, count} afterwards, tokens that got slots [B], first
+    token row of every request [B + 1], position (int32) and slot (int64) of every token row, -1 without one."""
+    lengths: torch.Tensor
+    state: torch.Tensor
+    granted: torch.Tensor
+    starts: torch.Tensor
+    positions: torch.Tensor
+    slots: torch.Tensor
+
+
+def page_plan_hip(lengths, new_tokens, block_table, free_pages, free_state, page_size, tokens, released=None, inplace=False):
+    """The pages of a step's tokens, once for all layers.  Request b holds lengths[b] positions and gets new_tokens[b] more (int32 [B]); where
+    `released` [B] (bool) is set its pages go back first.  Pages come from the ring free_pages [pool] with free_state = {first, count} (int32 [2]);
+    a new pool is free_pages = arange(pool), free_state = [0, pool].  block_table [B, max_pages] and the ring are written in place, lengths and
+    free_state too with `inplace` (else new tensors are given back).  `tokens` is the number of token rows, at least sum(new_tokens)."""
+    dev = _lib.require_gpu(lengths, new_tokens, block_table, free_pages, free_state, released)
+    B, tokens = lengths.shape[0] if lengths.dim() == 1 else -1, int(tokens)
+    _vector(lengths, B, torch.int32, "lengths")
+    _vector(new_tokens, B, torch.int32, "new_tokens")
+    _vector(free_pages, free_pages.numel(), torch.int32, "free_pages")
+    _vector(free_state, 2, torch.int32, "free_state")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or not block_table.is_contiguous():
+        raise ValueError(f"block_table must be a contiguous int32 tensor [{B}, max_pages], got {block_table.dtype} {tuple(block_table.shape)}")
+    if released is not None:
+        if released.dtype not in (torch.bool, torch.uint8):
+            raise ValueError(f"released must be bool or uint8, got {released.dtype}")
+        _vector(released, B, released.dtype, "released")
+    need = int(_lib.lib().bs_page_plan_workspace_bytes(B, tokens))
+    if need < 0:
+        _lib.check(need, "bs_page_plan_workspace_bytes")
+    i32 = dict(dtype=torch.int32, device=dev)
+    plan = PagePlan(lengths if inplace else torch.empty(B, **i32), free_state if inplace else torch.empty(2, **i32), torch.empty(B, **i32),
+                    torch.empty(B + 1, **i32), torch.empty(tokens, **i32), torch.empty(tokens, dtype=torch.int64, device=dev))
+    with torch.cuda.device(dev), _lib.scratch(dev, need) as ws:
+        _lib.check(_lib.lib().bs_page_plan(_lib.ptr(lengths), _lib.ptr(new_tokens), _lib.ptr(released), _lib.ptr(block_table), _lib.ptr(free_pages),
+                                           _lib.ptr(free_state), *(_lib.ptr(t) for t in plan), B, tokens, int(page_size), block_table.shape[1],
+                                           free_pages.shape[0], _lib.ptr(ws), ws.numel(), _lib.stream_ptr(dev)), "bs_page_plan")
+    return plan
+
+
+def _pages(kpages, vpages, cos, sin):
+    """(pool, kv_heads, page_size, head_dim) of a cache in pages, and the positions of the RoPE tables."""
+    for t in (kpages, vpages):
+        if t.dtype != torch.float16 or t.dim() != 4 or t.shape != kpages.shape or not t.is_contiguous():
+            raise ValueError("kpages and vpages must be contiguous fp16 tensors [pool, kv_heads, page_size, head_dim] of one shape")
+    for t in (cos, sin):
+        if t.dtype != torch.float16 or t.dim() != 2 or t.shape != cos.shape or 2 * t.shape[1] != kpages.shape[3] or not t.is_contiguous():
+            raise ValueError("cos and sin must be contiguous fp16 tensors [positions, head_dim / 2] of one shape")
+    return (*kpages.shape, cos.shape[0])
+
+
+def rope_store_paged_hip(q, k, v, cos, sin, kpages, vpages, positions, slots, out=None):
+    """RoPE on the token rows of q [T, heads * d] (in place, or into `out`; None: keys and values alone), rotated k and v [T, kv * d] to their
+    slots in the pages [pool, kv, page_size, d].  positions (int32) and slots (int64) as page_plan_hip gives them; rows without a
+    slot are left as they are.  q, k and v may be column slices of one wider matrix.  Returns the rotated q."""
+    dev = _lib.require_gpu(q, k, v, cos, sin, kpages, vpages, positions, slots, out)
+    pool, kv, page, d, max_pos = _pages(kpages, vpages, cos, sin)
+    T = k.shape[0]
+    _vector(positions, T, torch.int32, "positions")
+    _vector(slots, T, torch.int64, "slots")
+    if q is not None and (q.dim() != 2 or q.shape[1] % d or q.shape[1] == 0):
+        raise ValueError("q must hold whole heads")
+    if out is not None and (q is None or out.shape != q.shape):
+        raise ValueError("out must be a tensor of q's shape")
+    ldk, ldv = _rows(k, (T, kv * d)), _rows(v, (T, kv * d))
+    if ldk != ldv:
+        raise ValueError("k and v must have the same row stride")
+    ldq = 0 if q is None else _rows(q, (T, q.shape[1]))
+    ldo = 0 if out is None else _rows(out, q.shape)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().bs_rope_store_paged_f16(_lib.ptr(q), ldq, _lib.ptr(out), ldo, _lib.ptr(k), _lib.ptr(v), ldk, _lib.ptr(cos), _lib.ptr(sin),
+                                                      _lib.ptr(positions), _lib.ptr(slots), _lib.ptr(kpages), _lib.ptr(vpages), T,
+                                                      0 if q is None else q.shape[1] // d, kv, d, max_pos, page, pool, _lib.stream_ptr(dev)),
+                   "bs_rope_store_paged_f16")
+    return q if out is None else out
+
+
+def attention_paged_hip(qkv, kpages, vpages, cos, sin, block_table, lengths, slots, heads, kv_heads, out=None):
+    """One new token per request: RoPE on q and k of qkv [B, (heads + 2 kv) * d] at position lengths[b] - 1, k and v to slots[b] of the pages
+    [pool, kv, page_size, d], attention over positions 0 .. lengths[b] - 1 by block_table [B, max_pages]; returns [B, heads * d].
+    lengths (int32) and slots (int64) as page_plan_hip leaves them; a request without a slot is idle and its row zeros."""
+    dev = _lib.require_gpu(qkv, kpages, vpages, cos, sin, block_table, lengths, slots, out)
+    pool, kv, page, d, max_pos = _pages(kpages, vpages, cos, sin)
+    B = qkv.shape[0]
+    if kv != kv_heads:
+        raise ValueError(f"the pages hold {kv} heads, not {kv_heads}")
+    ldqkv = _rows(qkv, (B, (heads + 2 * kv_heads) * d))
+    _vector(lengths, B, torch.int32, "lengths")
+    _vector(slots, B, torch.int64, "slots")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or not block_table.is_contiguous():
+        raise ValueError(f"block_table must be a contiguous int32 tensor [{B}, max_pages], got {block_table.dtype} {tuple(block_table.shape)}")
+    y = out if out is not None else torch.empty((B, heads * d), dtype=torch.float16, device=dev)
+    if y.dtype != torch.float16 or not y.is_contiguous() or y.numel() != B * heads * d:
+        raise ValueError("out must be a contiguous fp16 [B, heads * head_dim] tensor")
+    need = int(_lib.lib().bs_attention_paged_workspace_bytes(B, heads, kv_heads, d, page, block_table.shape[1]))
+    if need < 0:
+        _lib.check(need, "bs_attention_paged_workspace_bytes")
+    with torch.cuda.device(dev), _lib.scratch(dev, need) as ws:
+        _lib.check(_lib.lib().bs_attention_paged_f16(_lib.ptr(qkv), ldqkv, _lib.ptr(kpages), _lib.ptr(vpages), _lib.ptr(cos), _lib.ptr(sin), _lib.ptr(block_table),
+                                                     _lib.ptr(lengths), _lib.ptr(slots), _lib.ptr(y), B, heads, kv_heads, d, max_pos, page,
+                                                     block_table.shape[1], pool, _lib.ptr(ws), ws.numel(), _lib.stream_ptr(dev)), "bs_attention_paged_f16")
+    return y
+
+
+def sample_hip(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, out=None):
+    """The next token of every row of logits [B, V] (fp16, rows may be strided), int64 [B], drawn with the given random numbers uniform [B] of [0, 1).
+    temperature, top_p, min_p (fp32 [B]) and top_k (int32 [B]) may be None: temperature 1, all tokens.  A temperature of 0 is argmax_hip.
+    What stays and how it is drawn: bs_sample_f16 in include/bitstack_hip.h."""
+    dev = _lib.require_gpu(logits, uniform, temperature, top_k, top_p, min_p, out)
+    if logits.dim() != 2:
+        raise ValueError("logits must be a fp16 [B, V] tensor")
+    B, V = logits.shape
+    ld = _rows(logits, (B, V))
+    for name, t, dtype in (("uniform", uniform, torch.float32), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if t is not None:
+            _vector(t, B, dtype, name)
+    y = out if out is not None else torch.empty(B, dtype=torch.int64, device=dev)
+    _vector(y, B, torch.int64, "out")
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().bs_sample_f16(_lib.ptr(logits), ld, _lib.ptr(uniform), _lib.ptr(temperature), _lib.ptr(top_k), _lib.ptr(top_p), _lib.ptr(min_p),
+                                            _lib.ptr(y), B, V, _lib.stream_ptr(dev)), "bs_sample_f16")
     return y
 
 

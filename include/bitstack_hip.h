@@ -428,6 +428,97 @@ int bs_argmax_f16(const void *x, int64_t *out, int B, int V, void *stream);
 /* ... and *pos += 1, the position of the next token, in the same launch (pos null: bs_argmax_f16; B == 0: nothing happens). */
 int bs_argmax_advance_f16(const void *x, int64_t *out, int64_t *pos, int B, int V, void *stream);
 
+/*
+ * ---- requests of unequal lengths: a cache in pages ------------------------
+ * The cache is pool_pages pages of page_size positions (a power of two, 16 to
+ * 1024; pool_pages * page_size < 2^31), kpages and vpages [pool_pages, kv_heads,
+ * page_size, head_dim].  Row b of block_table [B, max_pages] names the pages of
+ * request b in order; a slot is page * page_size + offset.  No counterpart in the
+ * reference (generation is left to Hugging Face code).
+ *
+ * bs_page_plan, once per step (of decoding, of prompts, of both together):
+ * request b holds lengths[b] positions and gets new_tokens[b] more (0: none); with
+ * released[b] != 0 (released may be NULL) its pages go back first, and it holds 0.
+ * Pages are taken from the front of a ring, free_pages [pool_pages] with
+ * free_state = {first, count}, and go back behind its end.  Requests are granted
+ * in order: the first whose pages are not there and all later ones that need
+ * pages get nothing in this call, and neither does one whose row is too short, or
+ * whose tokens lie behind row T.
+ *   block_table     the new pages' entries are written, the others left alone
+ *   lengths_out [B], free_state_out [2]   afterwards; may be lengths, free_state
+ *   granted [B]     tokens that got slots: new_tokens[b] or 0
+ *   starts [B + 1]  first token row of every request (the exclusive sum of
+ *                   new_tokens, refused ones counted; at most T + 1)
+ *   positions [T], slots [T]   of every token row; -1 where a request was
+ *                   refused, and behind the last token
+ * Pages that go back in a call are not taken in the same one.  Negative lengths
+ * and counts are taken as 0, lengths beyond the row as a full one, a free_state
+ * that no ring has as an empty ring.  Deterministic.  Many tokens need scratch
+ * (bs_page_plan_workspace_bytes, 16-byte aligned; 0: none).  At most 65536
+ * requests and 2^30 token rows.
+ */
+int64_t bs_page_plan_workspace_bytes(int B, int T);
+int bs_page_plan(const int32_t *lengths, const int32_t *new_tokens, const uint8_t *released, int32_t *block_table, int32_t *free_pages,
+                 const int32_t *free_state, int32_t *lengths_out, int32_t *free_state_out, int32_t *granted, int32_t *starts,
+                 int32_t *positions, int64_t *slots, int B, int T, int page_size, int max_pages, int pool_pages, void *workspace,
+                 int64_t workspace_bytes, void *stream);
+
+/*
+ * The prompts' keys and values to their pages: for every token row t with a slot,
+ * q and k are rotated by positions[t] (rotate-half RoPE, cos/sin [max_pos,
+ * head_dim / 2]), q [T, heads * head_dim] in place or, if q_out is given, there; k
+ * and v [T, kv_heads * head_dim] go to slots[t].  Rows of q, q_out and of k and v
+ * are ldq, ldq_out and ldkv halves apart; q may be NULL (keys and values alone);
+ * q_out must not overlap q unless it is q.  Rows whose slot or position does not
+ * exist (negative, or too large) are stored nowhere, and their q is left as it is
+ * (copied to q_out).  Slots must differ.  head_dim 64 or 128; fp32, rounded
+ * once, as bs_rope_store_f16.  (16-byte aligned rows are read 16 bytes at a time,
+ * others one value at a time.)
+ */
+int bs_rope_store_paged_f16(void *q, int ldq, void *q_out, int ldq_out, const void *k, const void *v, int ldkv, const void *cos, const void *sin,
+                            const int32_t *positions, const int64_t *slots, void *kpages, void *vpages, int T, int heads, int kv_heads,
+                            int head_dim, int max_pos, int page_size, int pool_pages, void *stream);
+
+/*
+ * One new token for each of B requests of their own lengths: as
+ * bs_attention_decode_f16, but over the pages.  lengths[b] counts the new position
+ * (what bs_page_plan has left there): q and k of qkv [B, (heads + 2 kv_heads) *
+ * head_dim] (rows ldqkv halves apart) are rotated by lengths[b] - 1, k and v stored at
+ * slots[b], and out[B, heads * head_dim] = softmax(q k^T / sqrt(head_dim)) v over
+ * positions 0 .. lengths[b] - 1.  A row without a slot (negative, or one that
+ * does not exist), or with a length below 1, beyond its table's row or beyond
+ * max_pos, is idle: zeros, nothing stored.  Positions whose table entry is no page
+ * are left out.  Requests may share pages that none of them writes.  Any heads per
+ * KV head, head_dim 64 or 128; B <= 65536 and B * max_pages * page_size < 2^35.
+ * Long requests are cut into parts by what the lengths are at the call, and summed
+ * in order: deterministic.  Scratch: bs_attention_paged_workspace_bytes, 16-byte
+ * aligned (0: none; negative: an error status).
+ */
+int64_t bs_attention_paged_workspace_bytes(int B, int heads, int kv_heads, int head_dim, int page_size, int max_pages);
+int bs_attention_paged_f16(const void *qkv, int ldqkv, void *kpages, void *vpages, const void *cos, const void *sin, const int32_t *block_table,
+                           const int32_t *lengths, const int64_t *slots, void *out, int B, int heads, int kv_heads, int head_dim, int max_pos,
+                           int page_size, int max_pages, int pool_pages, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * The next token of each of B rows of logits (fp16, rows ld values apart, V <=
+ * 2^18), drawn with the random number uniform[b] of [0, 1) that the caller gives.
+ * With w_i = exp((x_i - max) / temperature[b]):
+ *   top_k[b]   the k largest stay (among equals the lowest indexes); <= 0: all
+ *   top_p[b]   of those, from the largest down (among equals the lowest index
+ *              first), the ones before which the sum is less than top_p times the
+ *              sum of all of those; >= 1 (or NaN): all; the largest always stays
+ *   min_p[b]   of those, the ones with w_i >= min_p, the largest weight being 1;
+ *              <= 0: all; the largest always stays
+ *   out[b]     the lowest index whose sum of kept weights up to it is more than
+ *              uniform[b] times the sum of all kept
+ * Weights and sums are those of 64 bits.  A temperature that is not above 0:
+ * bs_argmax_f16.  The four may be NULL: temperature 1, no top_k, top_p, min_p.  NaN
+ * and -inf have no weight; a row without any: 0.  A random number outside [0, 1)
+ * is taken as the nearest inside, NaN as 0.  Deterministic.  No counterpart in the reference.
+ */
+int bs_sample_f16(const void *logits, int64_t ld, const float *uniform, const float *temperature, const int32_t *top_k, const float *top_p,
+                  const float *min_p, int64_t *out, int B, int V, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
