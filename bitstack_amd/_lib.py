@@ -79,7 +79,8 @@ SIGNATURES.update({
     "bs_rope_store_paged_f16": (_I, [_P, _I, _P, _I, _P, _P, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P]),
     "bs_attention_paged_workspace_bytes": (_L, [_I, _I, _I, _I, _I, _I]),
     "bs_attention_paged_f16": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _L, _P]),
-    "bs_sample_f16": (_I, [_P, _L, _P, _P, _P, _P, _P, _P, _I, _I, _P]),
+    "bs_sample_workspace_bytes": (_L, [_I, _I]),
+    "bs_sample_f16": (_I, [_P, _L, _P, _P, _P, _P, _P, _P, _I, _I, _P, _L, _P]),
 })
 EPI_NONE, EPI_RESIDUAL, EPI_SWIGLU = 0, 1, 2
 

@@ -522,13 +522,21 @@ extern "C" int bs_attention_paged_f16(const void *qkv, int ldqkv, void *kpages, 
                                      (hipStream_t)stream);
 }
 
+static int sample_shape(int B, int V) { return B < 0 || B > 1 << 20 || V < 1 || V > 1 << 18 ? BS_ERR_SHAPE : BS_OK; }
+
+extern "C" int64_t bs_sample_workspace_bytes(int B, int V) {
+    const int st = sample_shape(B, V);
+    return st != BS_OK ? st : B == 0 ? 0 : bs_sample_scratch(B, V);
+}
+
 extern "C" int bs_sample_f16(const void *logits, int64_t ld, const float *uniform, const float *temperature, const int32_t *top_k, const float *top_p,
-                             const float *min_p, int64_t *out, int B, int V, void *stream) {
-    if (B < 0 || V < 1 || V > 1 << 18 || (B > 1 && ld < V)) return BS_ERR_SHAPE;
+                             const float *min_p, int64_t *out, int B, int V, void *workspace, int64_t workspace_bytes, void *stream) {
+    if (sample_shape(B, V) != BS_OK || (B > 1 && ld < V)) return BS_ERR_SHAPE;
     if (B == 0) return BS_OK;
     if (!logits || !uniform || !out) return BS_ERR_NULL;
     if (!bs_aligned(logits, 2) || !bs_aligned(uniform, 4) || !bs_aligned(temperature, 4) || !bs_aligned(top_k, 4) || !bs_aligned(top_p, 4) || !bs_aligned(min_p, 4) ||
         !bs_aligned(out, 8))
         return BS_ERR_ALIGN;
-    return bs_launch_sample((const half_t *)logits, ld, uniform, temperature, top_k, top_p, min_p, out, B, V, (hipStream_t)stream);
+    if (!workspace || workspace_bytes < bs_sample_scratch(B, V) || !bs_aligned(workspace, 16)) return BS_ERR_WORKSPACE;
+    return bs_launch_sample((const half_t *)logits, ld, uniform, temperature, top_k, top_p, min_p, out, B, V, workspace, (hipStream_t)stream);
 }

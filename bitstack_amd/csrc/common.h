@@ -146,5 +146,6 @@ int bs_launch_attention_paged(const half_t *qkv, int ldqkv, half_t *kpages, half
                               const int32_t *lengths, const int64_t *slots, half_t *out, int B, int heads, int kv_heads, int head_dim, int max_pos,
                               int shift, int max_pages, int pool, void *workspace, hipStream_t s);
 // the next tokens from logits (sample.hip), rows ld apart
+int64_t bs_sample_scratch(int B, int V);
 int bs_launch_sample(const half_t *logits, int64_t ld, const float *uniform, const float *temperature, const int32_t *top_k, const float *top_p,
-                     const float *min_p, int64_t *out, int B, int V, hipStream_t s);
+                     const float *min_p, int64_t *out, int B, int V, void *workspace, hipStream_t s);

@@ -461,9 +461,12 @@ def sample_hip(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=
             _vector(t, B, dtype, name)
     y = out if out is not None else torch.empty(B, dtype=torch.int64, device=dev)
     _vector(y, B, torch.int64, "out")
-    with torch.cuda.device(dev):
+    need = int(_lib.lib().bs_sample_workspace_bytes(B, V))
+    if need < 0:
+        _lib.check(need, "bs_sample_workspace_bytes")
+    with torch.cuda.device(dev), _lib.scratch(dev, need) as ws:
         _lib.check(_lib.lib().bs_sample_f16(_lib.ptr(logits), ld, _lib.ptr(uniform), _lib.ptr(temperature), _lib.ptr(top_k), _lib.ptr(top_p), _lib.ptr(min_p),
-                                            _lib.ptr(y), B, V, _lib.stream_ptr(dev)), "bs_sample_f16")
+                                            _lib.ptr(y), B, V, _lib.ptr(ws), ws.numel(), _lib.stream_ptr(dev)), "bs_sample_f16")
     return y
 
 

@@ -501,7 +501,7 @@ int bs_attention_paged_f16(const void *qkv, int ldqkv, void *kpages, void *vpage
 
 /*
  * The next token of each of B rows of logits (fp16, rows ld values apart, V <=
- * 2^18), drawn with the random number uniform[b] of [0, 1) that the caller gives.
+ * 2^18, B <= 2^20), drawn with the random number uniform[b] of [0, 1) that the caller gives.
  * With w_i = exp((x_i - max) / temperature[b]):
  *   top_k[b]   the k largest stay (among equals the lowest indexes); <= 0: all
  *   top_p[b]   of those, from the largest down (among equals the lowest index
@@ -514,10 +514,13 @@ int bs_attention_paged_f16(const void *qkv, int ldqkv, void *kpages, void *vpage
  * Weights and sums are those of 64 bits.  A temperature that is not above 0:
  * bs_argmax_f16.  The four may be NULL: temperature 1, no top_k, top_p, min_p.  NaN
  * and -inf have no weight; a row without any: 0.  A random number outside [0, 1)
- * is taken as the nearest inside, NaN as 0.  Deterministic.  No counterpart in the reference.
+ * is taken as the nearest inside, NaN as 0.  Deterministic.  Scratch:
+ * bs_sample_workspace_bytes (negative: an error status), 16-byte aligned; the first call per device must be
+ * made outside stream capture (it raises an LDS limit).  No counterpart in the reference.
  */
+int64_t bs_sample_workspace_bytes(int B, int V);
 int bs_sample_f16(const void *logits, int64_t ld, const float *uniform, const float *temperature, const int32_t *top_k, const float *top_p,
-                  const float *min_p, int64_t *out, int B, int V, void *stream);
+                  const float *min_p, int64_t *out, int B, int V, void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

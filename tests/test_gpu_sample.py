@@ -129,3 +129,19 @@ def test_frequencies():
     p = torch.softmax(row[0].double(), 0)
     count = torch.bincount(got, minlength=16)
     assert bool(((count - n * p).abs() <= 6 * (n * p * (1 - p)).sqrt()).all())
+
+
+@pytest.mark.parametrize("V", [3000, 33000])
+def test_settings_together(V):
+    """min-p drops tokens that top-p's sum still counts: every pair of settings, and all of them, with k below and above what a list holds."""
+    x = rows(6, V, V, 2.0)
+    u = numbers(6, V)
+    for k in (3, 40, 260, 900, 1024, 1025, 2000):
+        for t in (0.4, 1.0, 3.0):
+            for p in (0.2, 0.9, 0.999):
+                for m in (0.0, 0.01, 0.2):
+                    check(x, u, temperature=[t] * 6, top_k=[k] * 6, top_p=[p] * 6, min_p=[m] * 6)
+        check(x, u, top_k=[k] * 6, min_p=[0.02] * 6)
+    for p in (0.2, 0.9, 0.999):
+        check(x, u, top_p=[p] * 6, min_p=[0.02] * 6)
+        check(x, u, top_p=[p] * 6, min_p=[0.0001] * 6, temperature=[2.0] * 6)

@@ -31,7 +31,7 @@ STORE = dict(q=ONE, ldq=512, q_out=NUL, ldq_out=0, k=ONE, v=ONE, ldkv=256, cos=O
              d=128, max_pos=100, page=16, pool=100, stream=NUL)
 ATTEND = dict(qkv=ONE, ld=1024, kpages=ONE, vpages=ONE, cos=ONE, sin=ONE, table=ONE, lengths=ONE, slots=ONE, out=ONE, B=4, heads=4, kv_heads=2, d=128, max_pos=5000, page=16,
               max_pages=300, pool=100, ws=ONE, ws_bytes=1 << 30, stream=NUL)
-SAMPLE = dict(logits=ONE, ld=1000, uniform=ONE, temperature=NUL, top_k=NUL, top_p=NUL, min_p=NUL, out=ONE, B=4, V=1000, stream=NUL)
+SAMPLE = dict(logits=ONE, ld=1000, uniform=ONE, temperature=NUL, top_k=NUL, top_p=NUL, min_p=NUL, out=ONE, B=4, V=1000, ws=ONE, ws_bytes=1 << 20, stream=NUL)
 ODD = ctypes.c_void_p(4097)
 EIGHT = ctypes.c_void_p(4104)
 
@@ -85,8 +85,10 @@ def test_sample(L):
     for name in ("logits", "uniform", "temperature", "top_k", "top_p", "min_p", "out"):
         assert refused(**{name: ODD}) == ALIGN, name
     assert refused(out=ctypes.c_void_p(4100)) == refused(top_k=ctypes.c_void_p(4098)) == ALIGN
-    for change in ({"B": -1}, {"V": 0}, {"V": (1 << 18) + 1}, {"ld": 999}, {"ld": -1000}):
+    for change in ({"B": -1}, {"B": (1 << 20) + 1}, {"V": 0}, {"V": (1 << 18) + 1}, {"ld": 999}, {"ld": -1000}):
         assert refused(**change) == SHAPE, change
+    assert refused(ws=NUL) == refused(ws_bytes=10) == refused(ws=EIGHT) == WORKSPACE
+    assert L.bs_sample_workspace_bytes(4, 0) == L.bs_sample_workspace_bytes(-1, 10) == SHAPE and L.bs_sample_workspace_bytes(0, 10) == 0
     assert refused(B=0) == 0
 
 
