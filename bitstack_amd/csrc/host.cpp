@@ -532,9 +532,206 @@ PyObject *host_argmax(PyObject *, PyObject *const *a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- requests of unequal lengths -------------------------------------------------------------------
+at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType type, c10::Device dev) { return at::Tensor(at::detail::empty_cuda(sizes, type, dev, std::nullopt)); }
+
+// None, or a tensor (false: neither)
+bool optional_arg(PyObject *o, const at::Tensor *&t) {
+    t = o == Py_None ? nullptr : tensor_arg(o);
+    return t || o == Py_None;
+}
+bool vector(const at::Tensor &t, int64_t n, at::ScalarType type, c10::Device dev) { return t.dim() == 1 && t.size(0) == n && plain(t, type, dev); }
+// a fp16 matrix with contiguous rows, ld halves apart
+bool matrix_rows(const at::Tensor &t, int64_t rows, int64_t columns, c10::Device dev, int64_t &ld) {
+    if (t.scalar_type() != at::kHalf || t.device() != dev || t.dim() != 2 || t.size(0) != rows || t.size(1) != columns || t.stride(1) != 1) return false;
+    ld = t.stride(0);
+    return ld >= columns && ld < INT32_MAX;
+}
+// a cache in pages and its RoPE tables
+struct Pages {
+    int pool, kv, page, d, positions;
+    void *k, *v;
+    const void *cos, *sin;
+};
+bool pages_args(PyObject *kp, PyObject *vp, PyObject *cosp, PyObject *sinp, c10::Device dev, Pages &p) {
+    const at::Tensor *k = tensor_arg(kp), *v = tensor_arg(vp), *cos = tensor_arg(cosp), *sin = tensor_arg(sinp);
+    if (!k || !v || !cos || !sin || !plain(*k, at::kHalf, dev) || !plain(*v, at::kHalf, dev) || !plain(*cos, at::kHalf, dev) || !plain(*sin, at::kHalf, dev)) return false;
+    if (k->dim() != 4 || k->sizes() != v->sizes() || cos->dim() != 2 || cos->sizes() != sin->sizes() || 2 * cos->size(1) != k->size(3)) return false;
+    for (int64_t n : {k->size(0), k->size(1), k->size(2), k->size(3), cos->size(0)})
+        if (n < 1 || n >= INT32_MAX) return false;
+    p = {(int)k->size(0), (int)k->size(1), (int)k->size(2), (int)k->size(3), (int)cos->size(0), k->mutable_data_ptr(), v->mutable_data_ptr(), cos->const_data_ptr(), sin->const_data_ptr()};
+    return true;
+}
+
+// page_plan(lengths, new_tokens, block_table, free_pages, free_state, page_size, tokens, released or None, inplace)
+// -> (lengths, state, granted, starts, positions, slots), or None
+PyObject *host_page_plan(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 9) return PyErr_Format(PyExc_TypeError, "page_plan takes 9 arguments");
+    HANDLE_TH_ERRORS
+        const at::Tensor *lengths = tensor_arg(a[0]), *fresh = tensor_arg(a[1]), *table = tensor_arg(a[2]), *ring = tensor_arg(a[3]), *state = tensor_arg(a[4]), *released;
+        int64_t page, T;
+        if (!int_arg(a[5], page) || !int_arg(a[6], T)) return nullptr;
+        if (!lengths || !fresh || !table || !ring || !state || !optional_arg(a[7], released) || !lengths->is_cuda() || lengths->dim() != 1) Py_RETURN_NONE;
+        const c10::Device dev = lengths->device();
+        const int64_t B = lengths->size(0);
+        if (T < 0 || T >= INT32_MAX || B >= INT32_MAX || page < 1 || page >= INT32_MAX || !vector(*lengths, B, at::kInt, dev) || !vector(*fresh, B, at::kInt, dev) || !plain(*table, at::kInt, dev) ||
+            table->dim() != 2 || table->size(0) != B || table->size(1) >= INT32_MAX || ring->dim() != 1 || ring->size(0) >= INT32_MAX || !plain(*ring, at::kInt, dev) ||
+            !vector(*state, 2, at::kInt, dev))
+            Py_RETURN_NONE;
+        if (released && ((released->scalar_type() != at::kBool && released->scalar_type() != at::kByte) || !vector(*released, B, released->scalar_type(), dev))) Py_RETURN_NONE;
+        const int64_t need = bs_page_plan_workspace_bytes((int)B, (int)T);
+        if (need < 0) Py_RETURN_NONE;
+        const bool inplace = a[8] == Py_True;
+        const int32_t *lp = (const int32_t *)lengths->const_data_ptr(), *fp = (const int32_t *)fresh->const_data_ptr(), *sp = (const int32_t *)state->const_data_ptr();
+        const uint8_t *gone = released ? (const uint8_t *)released->const_data_ptr() : nullptr;
+        int32_t *tp = (int32_t *)table->mutable_data_ptr(), *rp = (int32_t *)ring->mutable_data_ptr();
+        const int max_pages = (int)table->size(1), pool = (int)ring->size(0);
+        at::Tensor out[6];
+        if (inplace) {
+            out[0] = *lengths;
+            out[1] = *state;
+        }
+        const int st = while_others_run([&] {
+            DeviceScope scope(dev);
+            const hipStream_t stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+            if (!inplace) {
+                out[0] = new_tensor({B}, at::kInt, dev);
+                out[1] = new_tensor({2}, at::kInt, dev);
+            }
+            out[2] = new_tensor({B}, at::kInt, dev);
+            out[3] = new_tensor({B + 1}, at::kInt, dev);
+            out[4] = new_tensor({T}, at::kInt, dev);
+            out[5] = new_tensor({T}, at::kLong, dev);
+            const Workspace ws = workspace_for(dev.index(), stream, need);
+            std::lock_guard<std::mutex> launching(*ws.launching);
+            return bs_page_plan(lp, fp, gone, tp, rp, sp, (int32_t *)out[0].mutable_data_ptr(), (int32_t *)out[1].mutable_data_ptr(), (int32_t *)out[2].mutable_data_ptr(),
+                                (int32_t *)out[3].mutable_data_ptr(), (int32_t *)out[4].mutable_data_ptr(), (int64_t *)out[5].mutable_data_ptr(), (int)B, (int)T, (int)page,
+                                max_pages, pool, ws.data(), ws.buffer.numel(), stream);
+        });
+        if (st != BS_OK) return raise_status(st, "bs_page_plan");
+        PyObject *all = PyTuple_New(6);
+        for (int i = 0; all && i < 6; i++) {
+            PyObject *t = THPVariable_Wrap(out[i]);
+            if (!t) {
+                Py_DECREF(all);
+                return nullptr;
+            }
+            PyTuple_SET_ITEM(all, i, t);
+        }
+        return all;
+    END_HANDLE_TH_ERRORS
+}
+
+// rope_store_paged(q or None, k, v, cos, sin, kpages, vpages, positions, slots, out or None) -> True, or None
+PyObject *host_rope_store_paged(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 10) return PyErr_Format(PyExc_TypeError, "rope_store_paged takes 10 arguments");
+    HANDLE_TH_ERRORS
+        const at::Tensor *q, *out, *k = tensor_arg(a[1]), *v = tensor_arg(a[2]), *positions = tensor_arg(a[7]), *slots = tensor_arg(a[8]);
+        if (!k || !v || !positions || !slots || !optional_arg(a[0], q) || !optional_arg(a[9], out) || !k->is_cuda() || k->dim() != 2 || (out && !q)) Py_RETURN_NONE;
+        const c10::Device dev = k->device();
+        Pages p;
+        if (!pages_args(a[5], a[6], a[3], a[4], dev, p)) Py_RETURN_NONE;
+        const int64_t T = k->size(0);
+        int64_t ldk, ldv, ldq = 0, ldo = 0, width = 0;
+        if (T >= INT32_MAX || !vector(*positions, T, at::kInt, dev) || !vector(*slots, T, at::kLong, dev) || !matrix_rows(*k, T, (int64_t)p.kv * p.d, dev, ldk) ||
+            !matrix_rows(*v, T, (int64_t)p.kv * p.d, dev, ldv) || ldk != ldv)
+            Py_RETURN_NONE;
+        if (q) {
+            if (q->dim() != 2) Py_RETURN_NONE;
+            width = q->size(1);
+            if (width == 0 || width % p.d != 0 || width >= INT32_MAX || !matrix_rows(*q, T, width, dev, ldq) || (out && !matrix_rows(*out, T, width, dev, ldo))) Py_RETURN_NONE;
+        }
+        void *qp = q ? q->mutable_data_ptr() : nullptr, *op = out ? out->mutable_data_ptr() : nullptr;
+        const void *kp = k->const_data_ptr(), *vp = v->const_data_ptr();
+        const int32_t *pp = (const int32_t *)positions->const_data_ptr();
+        const int64_t *sp = (const int64_t *)slots->const_data_ptr();
+        const int st = while_others_run([&] {
+            DeviceScope scope(dev);
+            return bs_rope_store_paged_f16(qp, (int)ldq, op, (int)ldo, kp, vp, (int)ldk, p.cos, p.sin, pp, sp, p.k, p.v, (int)T, (int)(width / p.d), p.kv, p.d, p.positions,
+                                           p.page, p.pool, c10::hip::getCurrentHIPStream(dev.index()).stream());
+        });
+        if (st != BS_OK) return raise_status(st, "bs_rope_store_paged_f16");
+        Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// attention_paged(qkv, kpages, vpages, cos, sin, block_table, lengths, slots, heads, kv_heads, out or None) -> out, or None
+PyObject *host_attention_paged(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 11) return PyErr_Format(PyExc_TypeError, "attention_paged takes 11 arguments");
+    HANDLE_TH_ERRORS
+        const at::Tensor *qkv = tensor_arg(a[0]), *table = tensor_arg(a[5]), *lengths = tensor_arg(a[6]), *slots = tensor_arg(a[7]), *out;
+        int64_t heads, kv, ld;
+        if (!int_arg(a[8], heads) || !int_arg(a[9], kv)) return nullptr;
+        if (!qkv || !table || !lengths || !slots || !optional_arg(a[10], out) || !qkv->is_cuda() || qkv->dim() != 2) Py_RETURN_NONE;
+        const c10::Device dev = qkv->device();
+        Pages p;
+        if (!pages_args(a[1], a[2], a[3], a[4], dev, p) || p.kv != kv || heads < 1 || heads > (1 << 24) || kv > (1 << 24)) Py_RETURN_NONE;
+        const int64_t B = qkv->size(0);
+        if (B >= INT32_MAX || !matrix_rows(*qkv, B, (heads + 2 * kv) * p.d, dev, ld) || !plain(*table, at::kInt, dev) || table->dim() != 2 || table->size(0) != B ||
+            table->size(1) >= INT32_MAX || !vector(*lengths, B, at::kInt, dev) || !vector(*slots, B, at::kLong, dev) ||
+            (out && (!plain(*out, at::kHalf, dev) || out->numel() != B * heads * p.d)))
+            Py_RETURN_NONE;
+        const int64_t need = bs_attention_paged_workspace_bytes((int)B, (int)heads, (int)kv, p.d, p.page, (int)table->size(1));
+        if (need < 0) Py_RETURN_NONE;
+        const void *xp = qkv->const_data_ptr();
+        const int32_t *tp = (const int32_t *)table->const_data_ptr(), *lp = (const int32_t *)lengths->const_data_ptr();
+        const int64_t *sp = (const int64_t *)slots->const_data_ptr();
+        const int max_pages = (int)table->size(1);
+        at::Tensor y;
+        if (out) y = *out;
+        const int st = while_others_run([&] {
+            DeviceScope scope(dev);
+            const hipStream_t stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+            if (!y.defined()) y = new_half({B, heads * p.d}, dev);
+            const Workspace ws = workspace_for(dev.index(), stream, need);
+            std::lock_guard<std::mutex> launching(*ws.launching);
+            return bs_attention_paged_f16(xp, (int)ld, p.k, p.v, p.cos, p.sin, tp, lp, sp, y.mutable_data_ptr(), (int)B, (int)heads, (int)kv, p.d, p.positions, p.page, max_pages,
+                                          p.pool, ws.data(), ws.buffer.numel(), stream);
+        });
+        if (st != BS_OK) return raise_status(st, "bs_attention_paged_f16");
+        return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
+// sample(logits, uniform, temperature, top_k, top_p, min_p, out; the last five or None) -> out, or None
+PyObject *host_sample(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 7) return PyErr_Format(PyExc_TypeError, "sample takes 7 arguments");
+    HANDLE_TH_ERRORS
+        const at::Tensor *x = tensor_arg(a[0]), *uniform = tensor_arg(a[1]), *temperature, *top_k, *top_p, *min_p, *out;
+        if (!x || !uniform || !optional_arg(a[2], temperature) || !optional_arg(a[3], top_k) || !optional_arg(a[4], top_p) || !optional_arg(a[5], min_p) ||
+            !optional_arg(a[6], out) || !x->is_cuda() || x->dim() != 2)
+            Py_RETURN_NONE;
+        const c10::Device dev = x->device();
+        const int64_t B = x->size(0), V = x->size(1);
+        int64_t ld;
+        if (B >= INT32_MAX || V >= INT32_MAX || !matrix_rows(*x, B, V, dev, ld) || !vector(*uniform, B, at::kFloat, dev) || (temperature && !vector(*temperature, B, at::kFloat, dev)) ||
+            (top_k && !vector(*top_k, B, at::kInt, dev)) || (top_p && !vector(*top_p, B, at::kFloat, dev)) || (min_p && !vector(*min_p, B, at::kFloat, dev)) ||
+            (out && !vector(*out, B, at::kLong, dev)))
+            Py_RETURN_NONE;
+        const int64_t need = bs_sample_workspace_bytes((int)B, (int)V);
+        if (need < 0) Py_RETURN_NONE;
+        auto data = [](const at::Tensor *t) { return t ? t->const_data_ptr() : nullptr; };
+        const void *xp = x->const_data_ptr(), *up = uniform->const_data_ptr(), *tp = data(temperature), *kp = data(top_k), *pp = data(top_p), *mp = data(min_p);
+        at::Tensor y;
+        if (out) y = *out;
+        const int st = while_others_run([&] {
+            DeviceScope scope(dev);
+            const hipStream_t stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+            if (!y.defined()) y = new_tensor({B}, at::kLong, dev);
+            const Workspace ws = workspace_for(dev.index(), stream, need);
+            std::lock_guard<std::mutex> launching(*ws.launching);
+            return bs_sample_f16(xp, ld, (const float *)up, (const float *)tp, (const int32_t *)kp, (const float *)pp, (const float *)mp, (int64_t *)y.mutable_data_ptr(), (int)B,
+                                 (int)V, ws.data(), ws.buffer.numel(), stream);
+        });
+        if (st != BS_OK) return raise_status(st, "bs_sample_f16");
+        return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
 #define HOST_METHOD(name) {#name, (PyCFunction)(void (*)(void))host_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {HOST_METHOD(forward), HOST_METHOD(rebuild), HOST_METHOD(unpack), HOST_METHOD(rebuild_from_sign), HOST_METHOD(linear), HOST_METHOD(forward_cat), HOST_METHOD(workspace),
-                         HOST_METHOD(hold), HOST_METHOD(let_go), HOST_METHOD(argmax), HOST_METHOD(make_steps), HOST_METHOD(run_steps), {nullptr, nullptr, 0, nullptr}};
+                         HOST_METHOD(hold), HOST_METHOD(let_go), HOST_METHOD(argmax), HOST_METHOD(make_steps), HOST_METHOD(run_steps),
+                         HOST_METHOD(page_plan), HOST_METHOD(rope_store_paged), HOST_METHOD(attention_paged), HOST_METHOD(sample), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Native host path over libbitstack_hip.so.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -1,6 +1,6 @@
 // A key-value cache in pages, for requests of unequal lengths: which pages a step's tokens take (page_plan_kernel), and the prompts'
 // keys and values on their way into them (rope_store_paged_kernel).
-#include "common.h"
+#include "lanes.h"
 
 namespace {
 
@@ -35,27 +35,23 @@ struct plan_row {
 
 __device__ __forceinline__ uint32_t capped(uint32_t a, uint32_t b, uint32_t cap) { return min(a + b, cap); }    // (a, b <= cap < 2^31)
 
-// exclusive capped sum over the workgroup, and the whole one; `to` is free again behind the next barrier
-__device__ __forceinline__ uint32_t sum_before(uint32_t v, uint32_t cap, uint32_t *to, uint32_t &total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint32_t s = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t below = __shfl_up(s, o, 64);
-        if (lane >= o) s = capped(s, below, cap);
+// the capped sums of the waves before this one, of all, and of what is in front of this thread
+struct plan_sum {
+    uint32_t before, total;
+    __device__ __forceinline__ plan_sum(uint32_t scanned, uint32_t cap, const uint32_t *waves) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        auto f = [cap](uint32_t a, uint32_t b) { return capped(a, b, cap); };
+        const uint32_t upto = bs_row_scan(waves[lane & 15], f);
+        total = bs_read(upto, 15);
+        before = bs_lane_before(scanned);
+        if (wave > 0) before = capped(bs_read(upto, wave - 1), before, cap);
     }
-    uint32_t mine = __shfl_up(s, 1, 64);
-    if (lane == 0) mine = 0;
-    if (lane == 63) to[wave] = s;
-    __syncthreads();
-    total = 0;
-    uint32_t before = 0;
-#pragma unroll
-    for (int w = 0; w < PLAN_THREADS / 64; w++) {
-        if (w == wave) before = total;
-        total = capped(total, to[w], cap);
-    }
-    return capped(before, mine, cap);
+};
+// a wave's capped sums up to each lane; the whole one goes to waves[wave]
+__device__ __forceinline__ uint32_t plan_scan(uint32_t v, uint32_t cap, uint32_t *waves) {
+    const uint32_t s = bs_scan(v, [cap](uint32_t a, uint32_t b) { return capped(a, b, cap); });
+    if ((threadIdx.x & 63) == 63) waves[threadIdx.x >> 6] = s;
+    return s;
 }
 
 __device__ __forceinline__ int plan_pages(int n, int shift) { return n > 0 ? ((n - 1) >> shift) + 1 : 0; }
@@ -71,32 +67,54 @@ struct plan_state {
     }
 };
 
-// entries [j0, j1) of a row by steps: pages that go back are read before the new ones take their place, by the same thread
-__device__ __forceinline__ int plan_entries(const plan_row &r, int shift) {
-    return max(r.back, plan_pages(r.held, shift) + r.need);
-}
+// The entries of a row that change, first <= j < end: pages that go back are read before new ones take their place, by the same thread.  Several at a time: a
+// load that stands behind another entry's store waits for nothing but it.
+__device__ __forceinline__ int plan_entries(const plan_row &r, int shift) { return max(r.back, plan_pages(r.held, shift) + r.need); }
 __device__ __forceinline__ int plan_first_entry(const plan_row &r, int shift) { return r.back ? 0 : plan_pages(r.held, shift); }
-__device__ __forceinline__ void plan_entry(const plan_args &a, const plan_state &st, const plan_row &r, int b, int j) {
-    int32_t *at = a.table + (int64_t)b * a.max_pages + j;
-    const int own = j - plan_pages(r.held, a.shift);
-    const bool taken = own >= 0 && own < r.need;
-    const int32_t fresh = taken ? a.ring[plan_wrap((uint32_t)st.head + r.first + own, a.pool)] : 0;
-    // (a ring that is full already takes no more: the pages of a table that does not belong to it)
-    if (j < r.back && r.back_first + j < a.pool - st.count) a.ring[plan_wrap((uint32_t)st.tail + r.back_first + j, a.pool)] = *at;
-    if (taken) *at = fresh;
-}
-__device__ __forceinline__ void plan_token(const plan_args &a, const plan_state &st, const plan_row &r, int b, int i) {
-    if (r.start + i >= a.T) return;
-    int64_t slot = -1;
-    int pos = -1;
-    if (i < r.granted) {
-        pos = r.held + i;
-        const int p = pos >> a.shift, own = p - plan_pages(r.held, a.shift);
-        const int32_t id = own >= 0 ? a.ring[plan_wrap((uint32_t)st.head + r.first + own, a.pool)] : a.table[(int64_t)b * a.max_pages + p];
-        slot = id < 0 ? -1 : ((int64_t)id << a.shift) + (pos & ((1 << a.shift) - 1));
+template <int N>
+__device__ __forceinline__ void plan_write_entries(const plan_args &a, const plan_state &st, const plan_row &r, int b, int from, int step, int end) {
+    int32_t *row = a.table + (int64_t)b * a.max_pages;
+    const int have = plan_pages(r.held, a.shift);
+    for (int j0 = from; j0 < end; j0 += N * step) {
+        int32_t fresh[N], old[N];
+        bool taken[N], back[N];
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const int j = j0 + n * step, own = j - have;
+            taken[n] = j < end && own >= 0 && own < r.need;
+            back[n] = j < end && j < r.back && r.back_first + j < a.pool - st.count;       // (a full ring takes no more: pages of a table that is not its own)
+            fresh[n] = taken[n] ? a.ring[plan_wrap((uint32_t)st.head + r.first + own, a.pool)] : 0;
+            old[n] = back[n] ? row[j] : 0;
+        }
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const int j = j0 + n * step;
+            if (back[n]) a.ring[plan_wrap((uint32_t)st.tail + r.back_first + j, a.pool)] = old[n];
+            if (taken[n]) row[j] = fresh[n];
+        }
     }
-    a.slots[r.start + i] = slot;
-    a.positions[r.start + i] = pos;
+}
+template <int N>
+__device__ __forceinline__ void plan_write_tokens(const plan_args &a, const plan_state &st, const plan_row &r, int b, int from, int step, int end) {
+    const int32_t *row = a.table + (int64_t)b * a.max_pages;
+    const int have = plan_pages(r.held, a.shift);
+    for (int i0 = from; i0 < end; i0 += N * step) {
+        int32_t id[N];
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const int i = i0 + n * step, p = (r.held + i) >> a.shift, own = p - have;
+            id[n] = -1;
+            if (i < end && i < r.granted) id[n] = own >= 0 ? a.ring[plan_wrap((uint32_t)st.head + r.first + own, a.pool)] : row[p];
+        }
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const int i = i0 + n * step, pos = r.held + i;
+            if (i < end) {
+                a.slots[r.start + i] = id[n] < 0 ? -1 : ((int64_t)id[n] << a.shift) + (pos & ((1 << a.shift) - 1));
+                a.positions[r.start + i] = i < r.granted ? pos : -1;
+            }
+        }
+    }
 }
 __device__ __forceinline__ void plan_behind(const plan_args &a, int from, int step, int total) {
     for (int t = min(total, a.T) + from; t < a.T; t += step) {
@@ -106,13 +124,16 @@ __device__ __forceinline__ void plan_behind(const plan_args &a, int from, int st
 }
 
 // The sums, by one workgroup.  ALL: it writes everything; otherwise it leaves what rows have to write in `rows` for plan_write_kernel.
-// A thread writes the first two entries and tokens of its row itself, and a wave the rest of its rows one by one: with one token per row nobody waits
-// for anybody, and a long row is written by 64 lanes.
+// A thread writes the first entry and token of its row itself, as nearly all rows of a decode step want no more; longer rows are dealt to the waves.
 // What bounds it: the chain launch -> lengths -> sums -> ring -> slots.
 template <bool ALL>
 __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(const plan_args a, plan_row *__restrict__ rows) {
     __shared__ uint32_t sums[3][PLAN_THREADS / 64];
-    const int tid = threadIdx.x, lane = tid & 63;
+    __shared__ plan_row longer[ALL ? PLAN_THREADS : 1];
+    __shared__ int longer_row[ALL ? PLAN_THREADS : 1], n_longer;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    static_assert(PLAN_THREADS == 1024, "16 waves");
+    if (tid == 0) n_longer = 0;
     const plan_state st(a.state, a.pool);
     const uint32_t token_cap = (uint32_t)a.T + 1, back_cap = (uint32_t)a.pool + 1, need_cap = (uint32_t)st.count + 1;
     uint32_t tokens = 0, back = 0, need = 0, taken = 0;
@@ -128,14 +149,17 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(const plan_args
             r.held = gone ? 0 : len;
             r.back = gone ? plan_pages(len, a.shift) : 0;
         }
-        uint32_t all_tokens, all_back, all_need;
         const uint32_t fresh = min((uint32_t)r.fresh, token_cap);
-        const uint32_t start = capped(tokens, sum_before(fresh, token_cap, sums[0], all_tokens), token_cap);
-        const uint32_t back_first = capped(back, sum_before(min((uint32_t)r.back, back_cap), back_cap, sums[1], all_back), back_cap);
+        const uint32_t fresh_upto = plan_scan(fresh, token_cap, sums[0]), back_upto = plan_scan(min((uint32_t)r.back, back_cap), back_cap, sums[1]);
+        __syncthreads();
+        const plan_sum all_fresh(fresh_upto, token_cap, sums[0]), all_back(back_upto, back_cap, sums[1]);
+        const uint32_t start = capped(tokens, all_fresh.before, token_cap), back_first = capped(back, all_back.before, back_cap);
         const bool possible = in && capped(start, fresh, token_cap) <= (uint32_t)a.T && r.fresh <= most - r.held;
         r.need = possible ? plan_pages(r.held + r.fresh, a.shift) - plan_pages(r.held, a.shift) : 0;
-        const uint32_t want = min((uint32_t)r.need, need_cap);
-        const uint32_t first = capped(need, sum_before(want, need_cap, sums[2], all_need), need_cap);
+        const uint32_t want = min((uint32_t)r.need, need_cap), need_upto = plan_scan(want, need_cap, sums[2]);
+        __syncthreads();
+        const plan_sum all_need(need_upto, need_cap, sums[2]);
+        const uint32_t first = capped(need, all_need.before, need_cap);
         const bool ok = possible && (r.need == 0 || capped(first, want, need_cap) <= (uint32_t)st.count);
         if (!ok) r.need = 0;
         r.granted = ok ? r.fresh : 0;
@@ -148,42 +172,39 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(const plan_args
             a.starts[b] = r.start;
             if (!ALL) rows[b] = r;
         }
-        tokens = capped(tokens, all_tokens, token_cap);
-        back = capped(back, all_back, back_cap);
-        need = capped(need, all_need, need_cap);
+        tokens = capped(tokens, all_fresh.total, token_cap);
+        back = capped(back, all_back.total, back_cap);
+        need = capped(need, all_need.total, need_cap);
         // the pages of the rows that were granted: the largest sum that ends with one of them (rows behind a refused one need none)
         const uint32_t end = ok && r.need ? first + (uint32_t)r.need : 0;
         taken = max(taken, end);
         if (ALL) {
             const int e0 = plan_first_entry(r, a.shift), e1 = plan_entries(r, a.shift);
             const int t1 = in ? min(r.fresh, max(a.T - r.start, 0)) : 0;
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                if (j < t1) plan_token(a, st, r, b, j);
-                if (e0 + j < e1) plan_entry(a, st, r, b, e0 + j);
+            if (t1 > 1 || e1 - e0 > 1) {
+                const int at = atomicAdd(&n_longer, 1);                  // (they write to places of their own: their order does not matter)
+                longer[at] = r;
+                longer_row[at] = b;
             }
-            for (uint64_t more = __ballot(t1 > 2 || e1 - e0 > 2); more; more &= more - 1) {
-                const int w = __ffsll((unsigned long long)more) - 1;
-                plan_row q;
-                q.held = __shfl(r.held, w, 64);
-                q.granted = __shfl(r.granted, w, 64);
-                q.start = __shfl(r.start, w, 64);
-                q.need = __shfl(r.need, w, 64);
-                q.first = __shfl(r.first, w, 64);
-                q.back = __shfl(r.back, w, 64);
-                q.back_first = __shfl(r.back_first, w, 64);
-                const int row = b - lane + w, f0 = __shfl(e0, w, 64), f1 = __shfl(e1, w, 64), u1 = __shfl(t1, w, 64);
-                for (int i = 2 + lane; i < u1; i += 64) plan_token(a, st, q, row, i);
-                for (int j = f0 + 2 + lane; j < f1; j += 64) plan_entry(a, st, q, row, j);
+            plan_write_tokens<1>(a, st, r, b, 0, 1, min(t1, 1));
+            plan_write_entries<1>(a, st, r, b, e0, 1, min(e1, e0 + 1));
+            __syncthreads();
+            // a wave per row, or several if there are fewer rows than waves
+            const int rows_left = n_longer, share = max(1, PLAN_THREADS / 64 / max(rows_left, 1)), step = 64 * share;
+            for (int i = wave / share; i < rows_left && wave / share * share + share <= PLAN_THREADS / 64; i += PLAN_THREADS / 64 / share) {
+                const plan_row q = longer[i];
+                const int row = longer_row[i], f0 = plan_first_entry(q, a.shift), from = 1 + wave % share * 64 + lane;
+                plan_write_tokens<8>(a, st, q, row, from, step, min(q.fresh, max(a.T - q.start, 0)));
+                plan_write_entries<8>(a, st, q, row, f0 + from, step, plan_entries(q, a.shift));
             }
         }
-        __syncthreads();                         // (the sums' places are written again)
+        __syncthreads();                         // (the sums' places and the list are written again)
+        if (tid == 0) n_longer = 0;
     }
     if (ALL) plan_behind(a, tid, PLAN_THREADS, (int)tokens);
     // the largest `taken` of all threads
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) taken = max(taken, (uint32_t)__shfl_xor(taken, o, 64));
-    if (lane == 0) sums[0][tid >> 6] = taken;
+    taken = bs_read(bs_scan(taken, [](uint32_t a, uint32_t b) { return max(a, b); }), 63);
+    if (lane == 0) sums[0][wave] = taken;
     __syncthreads();
     if (tid == 0) {
         for (int w = 1; w < PLAN_THREADS / 64; w++) taken = max(taken, sums[0][w]);
@@ -215,8 +236,8 @@ __global__ __launch_bounds__(PLAN_STRIP) void plan_write_kernel(const plan_args 
         return;
     }
     const int t1 = min(r.fresh, max(a.T - r.start, 0)), e1 = plan_entries(r, a.shift);
-    for (int i = from; i < t1; i += step) plan_token(a, st, r, b, i);
-    for (int j = plan_first_entry(r, a.shift) + from; j < e1; j += step) plan_entry(a, st, r, b, j);
+    plan_write_tokens<4>(a, st, r, b, from, step, t1);
+    plan_write_entries<4>(a, st, r, b, plan_first_entry(r, a.shift) + from, step, e1);
 }
 
 // Up to so many rows and tokens one workgroup writes everything.

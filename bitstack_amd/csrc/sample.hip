@@ -17,7 +17,7 @@
 //
 // What bounds the second one is a chain of latencies, and instructions that come from memory the first time: they are the larger part of a short call, so
 // loops over a piece's eight values stay loops there, and all kinds of rows draw in one place.
-#include "common.h"
+#include "lanes.h"
 
 namespace {
 
@@ -167,40 +167,21 @@ struct sp_rule {
     }
     __device__ __forceinline__ bool wants_sum() const { return !greedy && !by_count && (by_sum || least == 0.f); }
 };
-// the value of another lane by CTRL (0 where there is none, and in the rows of 16 that ROWS leaves out)
-template <int CTRL, int ROWS = 0xf>
-__device__ __forceinline__ uint32_t sp_lane(uint32_t v) {
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
-}
-template <int CTRL, int ROWS = 0xf>
-__device__ __forceinline__ double sp_lane(double v) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    return __builtin_bit_cast(double, (uint64_t)sp_lane<CTRL, ROWS>((uint32_t)u) | (uint64_t)sp_lane<CTRL, ROWS>((uint32_t)(u >> 32)) << 32);
-}
-__device__ __forceinline__ uint32_t sp_read(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
-__device__ __forceinline__ double sp_read(double v, int lane) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    return __builtin_bit_cast(double, (uint64_t)sp_read((uint32_t)u, lane) | (uint64_t)sp_read((uint32_t)(u >> 32), lane) << 32);
-}
-// sum over the lanes up to this one: within rows of 16 by shifts, then over the rows.  (By shuffles through LDS one of these takes 0.3 us.)
+struct sp_plus {
+    template <typename T>
+    __device__ __forceinline__ T operator()(T a, T b) const { return a + b; }
+};
+struct sp_larger {
+    __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const { return max(a, b); }
+};
+// sum over the lanes up to this one
 template <typename T>
-__device__ __forceinline__ T sp_row_scan(T v) {
-    v += sp_lane<0x111>(v);
-    v += sp_lane<0x112>(v);
-    v += sp_lane<0x114>(v);
-    return v + sp_lane<0x118>(v);
-}
+__device__ __forceinline__ T sp_scan(T v) { return bs_scan(v, sp_plus()); }
 template <typename T>
-__device__ __forceinline__ T sp_scan(T v) {
-    v = sp_row_scan(v);
-    v += sp_lane<0x142, 0xa>(v);                 // the last of rows 0 and 2 to rows 1 and 3
-    return v + sp_lane<0x143, 0xc>(v);           // the last of row 1 to rows 2 and 3
-}
-template <typename T>
-__device__ __forceinline__ T sp_wave_sum(T v) { return sp_read(sp_scan(v), 63); }
+__device__ __forceinline__ T sp_wave_sum(T v) { return bs_read(sp_scan(v), 63); }
 // sum over the lanes before this one
 template <typename T>
-__device__ __forceinline__ T sp_wave_before(T v) { return sp_lane<0x138>(sp_scan(v)); }
+__device__ __forceinline__ T sp_wave_before(T v) { return bs_lane_before(sp_scan(v)); }
 // sum over the threads of 16 waves before this one, and the whole one; `to` is free again behind the next barrier
 template <typename T>
 __device__ __forceinline__ T sp_before(T v, T *to, T &total) {
@@ -208,19 +189,12 @@ __device__ __forceinline__ T sp_before(T v, T *to, T &total) {
     const T s = sp_scan(v);
     if (lane == 63) to[wave] = s;
     __syncthreads();
-    const T waves = sp_row_scan(to[lane & 15]);
-    total = sp_read(waves, 15);
-    const T mine = sp_lane<0x138>(s);
-    return wave > 0 ? sp_read(waves, wave - 1) + mine : mine;
+    const T waves = bs_row_scan(to[lane & 15], sp_plus());
+    total = bs_read(waves, 15);
+    const T mine = bs_lane_before(s);
+    return wave > 0 ? bs_read(waves, wave - 1) + mine : mine;
 }
-__device__ __forceinline__ uint32_t sp_wave_max(uint32_t v) {       // (0 is the least)
-    v = max(v, sp_lane<0x111>(v));
-    v = max(v, sp_lane<0x112>(v));
-    v = max(v, sp_lane<0x114>(v));
-    v = max(v, sp_lane<0x118>(v));
-    v = max(v, sp_lane<0x142, 0xa>(v));
-    return sp_read(max(v, sp_lane<0x143, 0xc>(v)), 63);
-}
+__device__ __forceinline__ uint32_t sp_wave_max(uint32_t v) { return bs_read(bs_scan(v, sp_larger()), 63); }       // (0 is the least)
 
 constexpr int SP_SPAN_WAVES = 4;                 // spans of a workgroup of the first kernel
 
@@ -239,11 +213,8 @@ __global__ __launch_bounds__(SP_SPAN_WAVES * 64) void sample_spans_kernel(const 
 #pragma unroll
     for (int e = 0; e < 8; e++) most = fmaxf(most, (float)v[e]);             // (a NaN is no number's larger one)
     uint32_t quarter = (uint32_t)sp_key((half_t)most);                       // of the lanes of its row of 16 up to this one
-    quarter = max(quarter, sp_lane<0x111>(quarter));
-    quarter = max(quarter, sp_lane<0x112>(quarter));
-    quarter = max(quarter, sp_lane<0x114>(quarter));
-    quarter = max(quarter, sp_lane<0x118>(quarter));
-    const uint32_t q0 = sp_read(quarter, 15), q1 = sp_read(quarter, 31), q2 = sp_read(quarter, 47), q3 = sp_read(quarter, 63);
+    quarter = bs_row_scan(quarter, sp_larger());
+    const uint32_t q0 = bs_read(quarter, 15), q1 = bs_read(quarter, 31), q2 = bs_read(quarter, 47), q3 = bs_read(quarter, 63);
     const int top = (int)max(max(q0, q1), max(q2, q3));
     double sum = 0.0;
     if (top > SP_NONE && rule.wants_sum()) {
@@ -495,8 +466,8 @@ __global__ __launch_bounds__(SP_THREADS) void sample_rows_kernel(const sp_args a
                     const uint64_t who = __ballot(n && (by_count ? seen + n_upto >= k : sum + w_upto >= goal));
                     const int c = who ? __ffsll((unsigned long long)who) - 1 : 64;
                     if (c > 0) {
-                        seen += sp_read(n_upto, c - 1);
-                        sum += sp_read(w_upto, c - 1);
+                        seen += bs_read(n_upto, c - 1);
+                        sum += bs_read(w_upto, c - 1);
                     }
                     found = who != 0;
                     if (!found) continue;
@@ -514,12 +485,12 @@ __global__ __launch_bounds__(SP_THREADS) void sample_rows_kernel(const sp_args a
                         const double in_front = up - (double)in * each, need = by_count ? (double)(k - (upto - in)) : ceil((goal - in_front) / each);
                         const uint32_t take = need < 1.0 ? 1 : need < (double)in ? (uint32_t)need : in;
                         at_key = __builtin_amdgcn_readlane(hi - i, l);
-                        at_stay = sp_read(take, l);
-                        at_count = sp_read(upto, l);
-                        at_sum = sp_read(in_front + (double)take * each, l);
+                        at_stay = bs_read(take, l);
+                        at_count = bs_read(upto, l);
+                        at_sum = bs_read(in_front + (double)take * each, l);
                         if (reach) break;
-                        seen = sp_read(upto, 63);
-                        sum = sp_read(up, 63);
+                        seen = bs_read(upto, 63);
+                        sum = bs_read(up, 63);
                     }
                 }
                 if (found && at_key >= border) {
@@ -562,18 +533,18 @@ __global__ __launch_bounds__(SP_THREADS) void sample_rows_kernel(const sp_args a
                             at++;
                         }
                 }
-                have += sp_read(upto, 63);
+                have += bs_read(upto, 63);
             });
             if (lane == 0) wave_count[wave] = have;
             __syncthreads();
-            const uint32_t upto = sp_row_scan(wave_count[lane & 15]);
-            n = sp_read(upto, 15);
+            const uint32_t upto = bs_row_scan(wave_count[lane & 15], sp_plus());
+            n = bs_read(upto, 15);
             // thread t's token: the wave whose part of the list it lies in
             int of = 0;
             n_before = 0;
 #pragma unroll
             for (int w = 0; w < SP_WAVES - 1; w++) {
-                const uint32_t end = sp_read(upto, w);
+                const uint32_t end = bs_read(upto, w);
                 if ((uint32_t)tid >= end) {
                     of = w + 1;
                     n_before = end;

@@ -357,6 +357,9 @@ def page_plan_hip(lengths, new_tokens, block_table, free_pages, free_state, page
     `released` [B] (bool) is set its pages go back first.  Pages come from the ring free_pages [pool] with free_state = {first, count} (int32 [2]);
     a new pool is free_pages = arange(pool), free_state = [0, pool].  block_table [B, max_pages] and the ring are written in place, lengths and
     free_state too with `inplace` (else new tensors are given back).  `tokens` is the number of token rows, at least sum(new_tokens)."""
+    plan = _lib.host().page_plan(lengths, new_tokens, block_table, free_pages, free_state, page_size, tokens, released, bool(inplace))
+    if plan is not None:
+        return PagePlan._make(plan)
     dev = _lib.require_gpu(lengths, new_tokens, block_table, free_pages, free_state, released)
     B, tokens = lengths.shape[0] if lengths.dim() == 1 else -1, int(tokens)
     _vector(lengths, B, torch.int32, "lengths")
@@ -397,6 +400,8 @@ def rope_store_paged_hip(q, k, v, cos, sin, kpages, vpages, positions, slots, ou
     """RoPE on the token rows of q [T, heads * d] (in place, or into `out`; None: keys and values alone), rotated k and v [T, kv * d] to their
     slots in the pages [pool, kv, page_size, d].  positions (int32) and slots (int64) as page_plan_hip gives them; rows without a
     slot are left as they are.  q, k and v may be column slices of one wider matrix.  Returns the rotated q."""
+    if _lib.host().rope_store_paged(q, k, v, cos, sin, kpages, vpages, positions, slots, out):
+        return q if out is None else out
     dev = _lib.require_gpu(q, k, v, cos, sin, kpages, vpages, positions, slots, out)
     pool, kv, page, d, max_pos = _pages(kpages, vpages, cos, sin)
     T = k.shape[0]
@@ -423,6 +428,9 @@ def attention_paged_hip(qkv, kpages, vpages, cos, sin, block_table, lengths, slo
     """One new token per request: RoPE on q and k of qkv [B, (heads + 2 kv) * d] at position lengths[b] - 1, k and v to slots[b] of the pages
     [pool, kv, page_size, d], attention over positions 0 .. lengths[b] - 1 by block_table [B, max_pages]; returns [B, heads * d].
     lengths (int32) and slots (int64) as page_plan_hip leaves them; a request without a slot is idle and its row zeros."""
+    y = _lib.host().attention_paged(qkv, kpages, vpages, cos, sin, block_table, lengths, slots, heads, kv_heads, out)
+    if y is not None:
+        return y if out is None else out
     dev = _lib.require_gpu(qkv, kpages, vpages, cos, sin, block_table, lengths, slots, out)
     pool, kv, page, d, max_pos = _pages(kpages, vpages, cos, sin)
     B = qkv.shape[0]
@@ -450,6 +458,9 @@ def sample_hip(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=
     """The next token of every row of logits [B, V] (fp16, rows may be strided), int64 [B], drawn with the given random numbers uniform [B] of [0, 1).
     temperature, top_p, min_p (fp32 [B]) and top_k (int32 [B]) may be None: temperature 1, all tokens.  A temperature of 0 is argmax_hip.
     What stays and how it is drawn: bs_sample_f16 in include/bitstack_hip.h."""
+    y = _lib.host().sample(logits, uniform, temperature, top_k, top_p, min_p, out)
+    if y is not None:
+        return y if out is None else out
     dev = _lib.require_gpu(logits, uniform, temperature, top_k, top_p, min_p, out)
     if logits.dim() != 2:
         raise ValueError("logits must be a fp16 [B, V] tensor")
