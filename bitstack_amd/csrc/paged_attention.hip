@@ -15,15 +15,15 @@
 //
 // The split: the lengths are known on the device alone, so every workgroup works out from them what it is to do.  The first B workgroups of a unit take
 // one request each, or the first part of it; if requests are longer than C = (all tiles) / (parts that fill the chip), the next ones take
-// the further parts, in order.  Parts leave (max, sum, weighted v) in the workspace, and a second launch puts them together, in order: the
+// the further parts, in order.  (The further parts first: 172 us instead of 105 for two requests of 80000, the numbers that no part has leave gaps.)  Parts leave (max, sum, weighted v) in the workspace, and a second launch puts them together, in order: the
 // result does not depend on which came first.
 #include "common.h"
 
 namespace {
 
 constexpr int PA_TILE = 16, PA_HEADS = 16;       // positions of a tile; query heads of a unit
-constexpr int PA_PARTS = 768;                    // workgroups (over all units) that further parts may add
-constexpr int PA_LEAST = 32;                     // tiles of a part, at least
+constexpr int PA_LEAST = 8;                      // tiles of a part, at least
+constexpr int PA_WHOLE = 512;                    // tables of up to so many positions are not cut
 
 struct pa_args {
     const half_t *qkv, *cosv, *sinv;
@@ -36,9 +36,8 @@ struct pa_args {
     int ldqkv, B, heads, kv_heads, groups, per_unit, max_pos, shift, max_pages, pool, parts;
 };
 
-// positions of request b that the cache holds (without its own): 0 for a length that is none
-__device__ __forceinline__ int pa_cached(const pa_args &a, int b) {
-    const int len = a.lengths[b];
+// positions that the cache holds of a request (without its own): 0 for a length that is none
+__device__ __forceinline__ int pa_cached(const pa_args &a, int len) {
     return len > 0 && len <= a.max_pos && (int64_t)len <= (int64_t)a.max_pages << a.shift ? len - 1 : 0;
 }
 __device__ __forceinline__ int pa_tiles(int cached) { return (cached + PA_TILE - 1) / PA_TILE; }
@@ -61,7 +60,7 @@ __device__ __forceinline__ float eight_on(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x128, 0xf, 0xf, true));    // row_ror:8
 }
 
-template <int D, int HP, int WAVES>
+template <int D, int HP, int WAVES, bool STREAM>
 __global__ __launch_bounds__(WAVES * 64) void attention_paged_kernel(const pa_args a, const int32_t *__restrict__ table) {
     constexpr int THREADS = WAVES * 64, W = D / 16, NC = D / 32, D2 = D / 2;
     typedef half_t vec_t __attribute__((ext_vector_type(W)));
@@ -75,21 +74,22 @@ __global__ __launch_bounds__(WAVES * 64) void attention_paged_kernel(const pa_ar
     const int hk = unit % a.kv_heads, hg = unit / a.kv_heads, rep = a.heads / a.kv_heads;
     const int head0 = hk * rep + hg * a.per_unit, nh = min(a.per_unit, rep - hg * a.per_unit);
 
+    int b = work, part = 0;
+    const bool first_part = work < a.B;
     // ---- which request, which part of it
     int all = 0;
-    for (int i = tid; i < a.B; i += THREADS) all += pa_tiles(pa_cached(a, i));
-    int b = work, part = 0;
-    const int64_t slot0 = work < a.B ? a.slots[work] : 0;
+    for (int i = tid; i < a.B; i += THREADS) all += pa_tiles(pa_cached(a, a.lengths[i]));
+    int64_t slot = first_part ? a.slots[work] : 0;
     all = pa_sum<WAVES>(all, sums);
     const int most = max(PA_LEAST, (all + a.parts - 1) / max(a.parts, 1));
     int further = 0, place = 0;                  // further parts of this request, and the first one's number
-    if (work < a.B) further = a.parts > 0 ? pa_further(pa_tiles(pa_cached(a, work)), most) : 0;
-    if (work >= a.B || further > 0) {            // numbers of the further parts: a running sum over the requests
+    if (first_part && a.parts > 0) further = pa_further(pa_tiles(pa_cached(a, a.lengths[b])), most);
+    if (!first_part || further > 0) {            // numbers of the further parts: a running sum over the requests
         if (tid == 0) found[0] = -1;
         int before = 0;
         const int wanted = work - a.B;
         for (int i0 = 0; i0 < a.B; i0 += THREADS) {
-            const int i = i0 + tid, mine = i < a.B ? pa_further(pa_tiles(pa_cached(a, i)), most) : 0;
+            const int i = i0 + tid, mine = i < a.B ? pa_further(pa_tiles(pa_cached(a, a.lengths[i])), most) : 0;
             int s = mine;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_paged_kernel(const pa_ar
                 before += sums[w];
             }
             const int first = ahead + s - mine;
-            if (work < a.B ? i == work : wanted >= first && wanted < first + mine) {
+            if (first_part ? i == b : wanted >= first && wanted < first + mine) {
                 found[0] = i;
                 found[1] = first;
                 found[2] = mine;
@@ -117,10 +117,12 @@ __global__ __launch_bounds__(WAVES * 64) void attention_paged_kernel(const pa_ar
         b = __builtin_amdgcn_readfirstlane(found[0]);
         place = __builtin_amdgcn_readfirstlane(found[1]);
         further = __builtin_amdgcn_readfirstlane(found[2]);
-        if (work >= a.B) part = wanted - place + 1;
+        if (!first_part) {
+            part = wanted - place + 1;
+            slot = a.slots[b];
+        }
     }
     const int len = a.lengths[b];
-    const int64_t slot = work < a.B ? slot0 : a.slots[b];
     const bool live = slot >= 0 && slot < (int64_t)a.pool << a.shift && len > 0 && len <= a.max_pos && (int64_t)len <= (int64_t)a.max_pages << a.shift;
     half_t *orow = a.out + ((int64_t)b * a.heads + head0) * D;
     if (part == 0 && unit == 0 && a.parts > 0 && tid == 0) {
@@ -136,32 +138,36 @@ __global__ __launch_bounds__(WAVES * 64) void attention_paged_kernel(const pa_ar
     const int t_first = (int)((int64_t)tiles * part / parts), t_end = (int)((int64_t)tiles * (part + 1) / parts);
 
     // ---- the rows of the cache
-    const half_t *qh = a.qkv + (int64_t)b * a.ldqkv;
-    const int32_t *row = table + (int64_t)b * a.max_pages;
     const int64_t page_step = (int64_t)a.kv_heads * D << a.shift, head_at = (int64_t)hk * D << a.shift;
     half8_t k8[NC];
     vec_t v8[4];
+    const int32_t *row = table + (int64_t)b * a.max_pages;
     auto page_of = [&](int t) { return row[__builtin_amdgcn_readfirstlane((t * PA_TILE) >> a.shift)]; };
     auto good = [&](int id) { return id >= 0 && id < a.pool; };       // (positions of a page that does not exist are left out)
     auto at_row = [&](int id, int t, int r) {    // rows past the last are the last again; their scores are masked
         return (int64_t)(good(id) ? id : 0) * page_step + head_at + (int64_t)(min(t * PA_TILE + r, pos - 1) & ((1 << a.shift) - 1)) * D;
     };
+    auto fetch = [](const auto *p) {
+        if constexpr (STREAM) return __builtin_nontemporal_load(p);
+        else return *p;
+    };
     auto fetch_k = [&](int id, int t) {
         const half_t *p = a.kpages + at_row(id, t, r16) + 8 * g;
 #pragma unroll
-        for (int c = 0; c < NC; c++) k8[c] = *reinterpret_cast<const half8_t *>(p + 32 * c);
+        for (int c = 0; c < NC; c++) k8[c] = fetch(reinterpret_cast<const half8_t *>(p + 32 * c));
     };
     auto fetch_v = [&](int id, int t) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) v8[i] = *reinterpret_cast<const vec_t *>(a.vpages + at_row(id, t, 4 * g + i) + W * r16);
+        for (int i = 0; i < 4; i++) v8[i] = fetch(reinterpret_cast<const vec_t *>(a.vpages + at_row(id, t, 4 * g + i) + W * r16));
     };
-    int t = t_first + wave, id = 0, next_id = 0;
+    int t = t_first + wave;
+    int id = 0, next_id = 0;
     if (t < t_end) id = page_of(t);
     if (t + WAVES < t_end) next_id = page_of(t + WAVES);
-
-    // ---- this position's own: pairs (i, i + D / 2) of the unit's queries, of k and of v
+    // this position's own: pairs (i, i + D / 2) of the unit's queries, of k and of v
     constexpr int PAIRS = (HP + 2) * D2, EACH = (PAIRS + THREADS - 1) / THREADS;
     half_t pa[EACH], pb[EACH];
+    const half_t *qh = a.qkv + (int64_t)b * a.ldqkv;
 #pragma unroll
     for (int e = 0; e < EACH; e++) {
         const int it = tid + e * THREADS, h = it / D2, i = it % D2;
@@ -353,22 +359,24 @@ __global__ __launch_bounds__(WAVES * 64) void attention_paged_kernel(const pa_ar
     }
 }
 
-// The parts of one head put together, in order, eight of them requested at once.
-template <int D>
-__global__ __launch_bounds__(D) void attention_paged_merge_kernel(const float *__restrict__ part, const int32_t *__restrict__ heads_of, half_t *__restrict__ out,
-                                                                  int B, int heads) {
-    const int dim = threadIdx.x, b = blockIdx.x / heads, head = blockIdx.x % heads;
-    const int place = heads_of[2 * b], further = heads_of[2 * b + 1];
-    if (further == 0) return;                    // written by the first launch
-    auto from = [&](int i) { return part + ((int64_t)(i == 0 ? b : B + place + i - 1) * heads + head) * (D + 4); };
+// The parts of a head put together, in order: G threads per dimension take G runs of them, eight parts requested at once, and one puts the runs together; H heads to a workgroup.
+template <int D, int G, int H>
+__global__ __launch_bounds__(D * G * H) void attention_paged_merge_kernel(const float *__restrict__ part, const int32_t *__restrict__ heads_of, half_t *__restrict__ out,
+                                                                          int B, int heads, int groups) {
+    __shared__ float sm[H][G][D], sd[H][G][D], so[H][G][D];
+    const int dim = threadIdx.x % D, g = threadIdx.x / D % G, h = threadIdx.x / (D * G), b = blockIdx.x / groups, head = blockIdx.x % groups * H + h;
+    const int place = heads_of[2 * b], parts = heads_of[2 * b + 1] + 1;
+    if (parts == 1) return;                      // written by the first launch
+    auto from = [&](int i) { return part + ((int64_t)(i == 0 ? b : B + place + i - 1) * heads + min(head, heads - 1)) * (D + 4); };
+    const int each = (parts + G - 1) / G, i_end = min((g + 1) * each, parts);
     float mx = -INFINITY, o = 0.f, den = 0.f;
-    for (int i0 = 0; i0 <= further; i0 += 8) {
+    for (int i0 = g * each; i0 < i_end; i0 += 8) {
         float m[8], l[8], v[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float *p = from(min(i0 + j, further));
+            const float *p = from(min(i0 + j, i_end - 1));
             m[j] = p[0];
-            l[j] = i0 + j <= further ? p[1] : 0.f;
+            l[j] = i0 + j < i_end ? p[1] : 0.f;  // (0: a part that saw no position, or none)
             v[j] = p[4 + dim];
         }
         float top = mx;
@@ -385,25 +393,59 @@ __global__ __launch_bounds__(D) void attention_paged_merge_kernel(const float *_
         }
         mx = top;
     }
-    out[(int64_t)blockIdx.x * D + dim] = (half_t)(o / den);
+    if (G > 1) {
+        sm[h][g][dim] = mx;
+        sd[h][g][dim] = den;
+        so[h][g][dim] = o;
+        __syncthreads();
+        if (g > 0) return;
+#pragma unroll
+        for (int j = 1; j < G; j++) mx = fmaxf(mx, sd[h][j][dim] != 0.f ? sm[h][j][dim] : -INFINITY);
+        const float r0 = den != 0.f ? __builtin_amdgcn_exp2f(sm[h][0][dim] - mx) : 0.f;
+        o = den != 0.f ? o * r0 : 0.f;
+        den *= r0;
+#pragma unroll
+        for (int j = 1; j < G; j++) {
+            const float d = sd[h][j][dim], r = d != 0.f ? __builtin_amdgcn_exp2f(sm[h][j][dim] - mx) : 0.f;
+            o += d != 0.f ? r * so[h][j][dim] : 0.f;
+            den += r * d;
+        }
+    }
+    if (head < heads) out[((int64_t)b * heads + head) * D + dim] = (half_t)(o / den);
 }
 
 struct pa_shape {
     int rep, groups, per_unit, units, parts;
 };
-pa_shape shape_of(int heads, int kv_heads, int64_t positions) {
+pa_shape shape_of(int B, int heads, int kv_heads, int64_t positions) {
     pa_shape p;
     p.rep = heads / kv_heads;
     p.groups = (int)bs_cdiv(p.rep, PA_HEADS);
     p.per_unit = (int)bs_cdiv(p.rep, p.groups);
     p.units = kv_heads * p.groups;
-    p.parts = positions <= PA_LEAST * PA_TILE ? 0 : (int)(PA_PARTS / p.units > 1 ? PA_PARTS / p.units : 1);
+    // Workgroups that further parts add: with few first ones all together are one per CU, with more two (as many as fit beside each other), beyond that enough of them
+    // to even out unequal lengths.  (us at 256 in all / 512 in all / 768 more: 1 request of 40000, 32 heads on 8 KV heads, 35.3 / 36.7 / 41.3; 2 of 80000, 64 on 8, 107 / 112 / 112; 16 of 100 to
+    // 8000 63.1 / 57.6 / 60.8; with 256 more / 768 more 48 of 1 to 4096 89 / 75.7.)
+    const int64_t first = (int64_t)B * p.units, further = first <= 64 ? 256 - first : first <= 256 ? 512 - first : 768;
+    p.parts = positions <= PA_WHOLE ? 0 : (int)(further / p.units > 1 ? further / p.units : 1);
     return p;
 }
 
+// A cache that the last-level cache cannot hold is read past it.  (us without / with: 48 requests of 1 to 4096, 404 MB, 82.3 / 76.2; 2 of 80000, 655 MB, 132.8 / 115.6; but 8 of 2000,
+// 67 MB, over and over 22.4 / 25.5.)
+constexpr int64_t PA_STREAM = 256ll << 20;
+
 template <int D, int HP>
 int launch(const pa_args &a, const int32_t *table, int64_t workgroups, hipStream_t s) {
-    attention_paged_kernel<D, HP, HP == 16 ? 4 : 8><<<(unsigned)workgroups, (HP == 16 ? 4 : 8) * 64, 0, s>>>(a, table);
+    constexpr int WAVES = HP == 16 ? 4 : 8;
+    const bool stream = ((int64_t)a.pool << a.shift) * a.kv_heads * D * 4 >= PA_STREAM;
+    (stream ? attention_paged_kernel<D, HP, WAVES, true> : attention_paged_kernel<D, HP, WAVES, false>)<<<(unsigned)workgroups, WAVES * 64, 0, s>>>(a, table);
+    BS_LAUNCH_CHECK();
+    if (a.parts == 0) return BS_OK;
+    // few heads: the parts of each in four runs; many: several heads to a workgroup, most of which have one part
+    const bool few = (int64_t)a.B * a.heads < 1024;
+    const int groups = few ? a.heads : (a.heads + 3) / 4;
+    (few ? attention_paged_merge_kernel<D, 4, 1> : attention_paged_merge_kernel<D, 1, 4>)<<<(unsigned)((int64_t)a.B * groups), D * 4, 0, s>>>(a.part, a.heads_of, a.out, a.B, a.heads, groups);
     BS_LAUNCH_CHECK();
     return BS_OK;
 }
@@ -411,27 +453,21 @@ int launch(const pa_args &a, const int32_t *table, int64_t workgroups, hipStream
 }  // namespace
 
 int64_t bs_attention_paged_scratch(int B, int heads, int kv_heads, int head_dim, int max_pages, int page) {
-    const pa_shape p = shape_of(heads, kv_heads, (int64_t)max_pages * page);
+    const pa_shape p = shape_of(B, heads, kv_heads, (int64_t)max_pages * page);
     return p.parts ? bs_cdiv(8ll * B, 16) * 16 + (int64_t)(B + p.parts) * heads * (head_dim + 4) * 4 : 0;
 }
 
 int bs_launch_attention_paged(const half_t *qkv, int ldqkv, half_t *kpages, half_t *vpages, const half_t *cos, const half_t *sin, const int32_t *table,
                               const int32_t *lengths, const int64_t *slots, half_t *out, int B, int heads, int kv_heads, int head_dim, int max_pos,
                               int shift, int max_pages, int pool, void *workspace, hipStream_t s) {
-    const pa_shape p = shape_of(heads, kv_heads, (int64_t)max_pages << shift);
+    const pa_shape p = shape_of(B, heads, kv_heads, (int64_t)max_pages << shift);
     const int64_t workgroups = (int64_t)(B + p.parts) * p.units;
     if (workgroups > INT32_MAX) return BS_ERR_SHAPE;
     pa_args a = {qkv, cos, sin, kpages, vpages, lengths, slots, out, (int32_t *)workspace, (float *)((char *)workspace + bs_cdiv(8ll * B, 16) * 16),
                  ldqkv, B, heads, kv_heads, p.groups, p.per_unit, max_pos, shift, max_pages, pool, p.parts};
-    int st;
     if (head_dim == 128)
-        st = p.per_unit > 8 ? launch<128, 16>(a, table, workgroups, s) : p.per_unit > 4 ? launch<128, 8>(a, table, workgroups, s) : p.per_unit > 2 ? launch<128, 4>(a, table, workgroups, s)
-           : p.per_unit > 1 ? launch<128, 2>(a, table, workgroups, s) : launch<128, 1>(a, table, workgroups, s);
-    else
-        st = p.per_unit > 8 ? launch<64, 16>(a, table, workgroups, s) : p.per_unit > 4 ? launch<64, 8>(a, table, workgroups, s) : p.per_unit > 2 ? launch<64, 4>(a, table, workgroups, s)
-           : p.per_unit > 1 ? launch<64, 2>(a, table, workgroups, s) : launch<64, 1>(a, table, workgroups, s);
-    if (st != BS_OK || p.parts == 0) return st;
-    (head_dim == 128 ? attention_paged_merge_kernel<128> : attention_paged_merge_kernel<64>)<<<(unsigned)((int64_t)B * heads), head_dim, 0, s>>>(a.part, a.heads_of, out, B, heads);
-    BS_LAUNCH_CHECK();
-    return BS_OK;
+        return p.per_unit > 8 ? launch<128, 16>(a, table, workgroups, s) : p.per_unit > 4 ? launch<128, 8>(a, table, workgroups, s) : p.per_unit > 2 ? launch<128, 4>(a, table, workgroups, s)
+             : p.per_unit > 1 ? launch<128, 2>(a, table, workgroups, s) : launch<128, 1>(a, table, workgroups, s);
+    return p.per_unit > 8 ? launch<64, 16>(a, table, workgroups, s) : p.per_unit > 4 ? launch<64, 8>(a, table, workgroups, s) : p.per_unit > 2 ? launch<64, 4>(a, table, workgroups, s)
+         : p.per_unit > 1 ? launch<64, 2>(a, table, workgroups, s) : launch<64, 1>(a, table, workgroups, s);
 }
