@@ -23,7 +23,7 @@ namespace {
 
 constexpr int SP_THREADS = 1024, SP_MAX_V = 1 << 18;
 constexpr int SP_SPANS = SP_MAX_V / 512;         // spans of 64 pieces of eight values
-constexpr int SP_BINS = 32768;                   // keys that are counted at a time
+constexpr int SP_BINS = 36864;                   // keys that are counted at a time: all that 160 KB of LDS leave room for (from 12 down to -8 there are 37000)
 typedef uint16_t ushort8_t __attribute__((ext_vector_type(8)));
 typedef int16_t short8_t __attribute__((ext_vector_type(8)));
 
@@ -273,11 +273,10 @@ constexpr int SP_WAVES = SP_THREADS / 64, SP_LIST = SP_THREADS;      // (a token
 __global__ __launch_bounds__(SP_THREADS) void sample_rows_kernel(const sp_args a) {
     // tokens per key, from the highest key of the window down; then [wave][SP_LIST] keys and indexes
     extern __shared__ __attribute__((aligned(16))) uint32_t bins[];
-    static_assert(SP_BINS == 2 * SP_WAVES * SP_LIST && SP_SPANS <= SP_THREADS && SP_SPANS <= 64 * SP_WAVES, "both fit; a span per thread; a wave's spans one per lane");
-    __shared__ double table[SP_POWER_COUNT], part[SP_WAVES], chunk_sum[64], span_kept[SP_SPANS], span_before, list_w[SP_LIST];
-    __shared__ uint32_t part32[SP_WAVES], chunk_count[64], span_ties[SP_SPANS], span_left, wave_count[SP_WAVES];
+    static_assert(SP_BINS >= 2 * SP_WAVES * SP_LIST && SP_BINS <= 64 * 4096 && SP_SPANS <= SP_THREADS && SP_SPANS <= 64 * SP_WAVES, "both fit; a span per thread; a wave's spans one per lane");
+    __shared__ double table[SP_POWER_COUNT], part[SP_WAVES], chunk_sum[64], span_kept[SP_SPANS], span_before;
+    __shared__ uint32_t part32[SP_WAVES], chunk_count[64], span_ties[SP_SPANS], span_left, wave_count[SP_WAVES], listed;
     __shared__ int keys[SP_SPANS], floor_key, at_first, at_last;
-    __shared__ uint16_t list_key[SP_LIST];
     __shared__ uint2_t quarter_keys[SP_SPANS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), b = blockIdx.x;
     const sp_row row(a.logits + b * a.ld, a.V);
@@ -307,10 +306,9 @@ __global__ __launch_bounds__(SP_THREADS) void sample_rows_kernel(const sp_args a
     }
     const sp_weight weight(table, rule.scale, top);
     // The wave's spans, one after another in the order of the row, that reach a key: f(span, values), the next one's values on their way.
-    const int per_wave = (a.spans + SP_WAVES - 1) / SP_WAVES, span0 = wave * per_wave;
-    auto each_span = [&](int from, auto f) {
-        const int at = span0 + lane;
-        uint64_t left = __ballot(lane < per_wave && at < a.spans && keys[min(at, a.spans - 1)] >= from);
+    auto each_span = [&](int first, int end, int from, auto f) {
+        const int per_wave = (end - first + SP_WAVES - 1) / SP_WAVES, span0 = first + wave * per_wave, at = span0 + lane;
+        uint64_t left = __ballot(lane < per_wave && at < end && keys[min(at, a.spans - 1)] >= from);
         if (!left) return;
         int s = span0 + __ffsll((unsigned long long)left) - 1;
         half8_t v = row.values(s * 64 + lane);
@@ -350,7 +348,9 @@ __global__ __launch_bounds__(SP_THREADS) void sample_rows_kernel(const sp_args a
         sums_are_there = !rule.by_sum;
     }
     const bool few = rule.by_count && rule.k <= 4 * a.spans;
-    int from = SP_NONE + 1;                      // no key below it is kept
+    uint32_t counted = 0, border_ties = 0;       // tokens down to the border and with its key, and the weights that stay, where they have been counted
+    double counted_sum = 0.0;
+    int from = SP_NONE + 1, first = 0, end = a.spans;          // no key below it is kept; the spans that are summed
     if (!sums_are_there) {
         int least = top == SP_INFINITE ? top : SP_NONE + 1;              // the lowest key that min-p leaves
         if (rule.least > 0.f) {
@@ -406,7 +406,6 @@ __global__ __launch_bounds__(SP_THREADS) void sample_rows_kernel(const sp_args a
         if (!few || !rule.by_sum) from = max(from, least);
 
         // ---- the border of top-k and top-p by counting, where no list can be made: top-p leaves no bound on the tokens, nor does a large k
-        uint32_t counted = 0;                    // tokens down to the border, where they have been counted
         auto count = [&]() {
             // no border is below the key at which all tokens together would have less than top-p leaves
             double total = 0.0;
@@ -415,7 +414,7 @@ __global__ __launch_bounds__(SP_THREADS) void sample_rows_kernel(const sp_args a
             int held = 0;                        // highest key of the window that the bins hold
             double limit = total, at_sum = 0.0;  // the sum that top-k leaves; up to what was found,
             int at_key = 0;                      // the key that was,
-            uint32_t at_stay = 0, at_count = 0;  // and how many tokens with it stay, and how many there are down to it
+            uint32_t at_stay = 0, at_count = 0, at_ties = 0;     // how many tokens with it stay, how many there are down to it and with it
             // Twice: the first key at which the count reaches k, and the one at which the sum reaches the goal.  Every wave looks for them by itself.
 #pragma unroll 1
             for (int turn = rule.by_count ? 0 : 1; turn < (rule.by_sum ? 2 : 1); turn++) {
@@ -433,7 +432,7 @@ __global__ __launch_bounds__(SP_THREADS) void sample_rows_kernel(const sp_args a
                         __syncthreads();         // (the last window's bins are read no more)
                         for (int i = tid; i < chunks * (chunk / 4); i += SP_THREADS) reinterpret_cast<uint4_t *>(bins)[i] = (uint4_t)0u;
                         __syncthreads();
-                        each_span(lo, [&](int, const half8_t v) {
+                        each_span(0, a.spans, lo, [&](int, const half8_t v) {
                             const ushort8_t down = (uint16_t)hi - sp_keys(v);
 #pragma unroll
                             for (int e = 0; e < 8; e++)
@@ -487,6 +486,7 @@ __global__ __launch_bounds__(SP_THREADS) void sample_rows_kernel(const sp_args a
                         at_key = __builtin_amdgcn_readlane(hi - i, l);
                         at_stay = bs_read(take, l);
                         at_count = bs_read(upto, l);
+                        at_ties = bs_read(in, l);
                         at_sum = bs_read(in_front + (double)take * each, l);
                         if (reach) break;
                         seen = bs_read(upto, 63);
@@ -497,6 +497,8 @@ __global__ __launch_bounds__(SP_THREADS) void sample_rows_kernel(const sp_args a
                     stay = border > SP_NONE && at_key == border ? min(stay, at_stay) : at_stay;
                     border = at_key;
                     counted = at_count;
+                    border_ties = at_ties;
+                    counted_sum = at_sum;
                 }
                 limit = found ? at_sum : sum;    // (fewer than k: all stay)
             }
@@ -511,10 +513,13 @@ __global__ __launch_bounds__(SP_THREADS) void sample_rows_kernel(const sp_args a
         for (;;) {
             if (counting) count();
             if (counted > SP_LIST) break;
+            if (tid == 0) listed = 0;
             __syncthreads();                     // (the bins are read no more)
             uint32_t *const k_list = bins + wave * SP_LIST, *const i_list = bins + (SP_WAVES + wave) * SP_LIST;
             uint32_t have = 0;
-            each_span(from, [&](int s, const half8_t v) {
+            bool full = false;                   // (too many: then nobody goes on)
+            each_span(0, a.spans, from, [&](int s, const half8_t v) {
+                if (full) return;
                 const ushort8_t key = sp_keys(v);
                 uint32_t in = 0;
 #pragma unroll
@@ -533,12 +538,16 @@ __global__ __launch_bounds__(SP_THREADS) void sample_rows_kernel(const sp_args a
                             at++;
                         }
                 }
-                have += bs_read(upto, 63);
+                const uint32_t more = bs_read(upto, 63);
+                uint32_t all = 0;
+                if (lane == 0) all = atomicAdd(&listed, more) + more;
+                full = bs_read(all, 0) > SP_LIST;
+                have += more;
             });
             if (lane == 0) wave_count[wave] = have;
             __syncthreads();
             const uint32_t upto = bs_row_scan(wave_count[lane & 15], sp_plus());
-            n = bs_read(upto, 15);
+            n = listed;
             // thread t's token: the wave whose part of the list it lies in
             int of = 0;
             n_before = 0;
@@ -556,11 +565,15 @@ __global__ __launch_bounds__(SP_THREADS) void sample_rows_kernel(const sp_args a
                 const double w = in ? weight(key) : 0.0;
                 bool stays = in;
                 if (ranked) {                    // how many are ahead of it, and their sum: 1 to 16 threads per token, each takes a part of the others
+                    double *const sums = reinterpret_cast<double *>(bins), *const list_w = sums + 2 * SP_LIST;
+                    uint32_t *const ranks = bins + 2 * SP_LIST;
+                    uint16_t *const list_key = reinterpret_cast<uint16_t *>(bins + 6 * SP_LIST);
+                    __syncthreads();             // (the waves' lists are read no more)
                     list_w[tid] = w;
                     list_key[tid] = (uint16_t)key;
                     const int groups = n <= 64 ? 16 : n <= 128 ? 8 : n <= 256 ? 4 : n <= 512 ? 2 : 1, width = SP_LIST / groups, g = tid / width, i = tid % width;
                     const int each = ((int)n + groups - 1) / groups, j1 = min((g + 1) * each, (int)n);
-                    __syncthreads();             // (and the bins are read no more)
+                    __syncthreads();
                     const int my_key = list_key[i];
                     uint32_t rank = 0;
                     double sum = 0.0;
@@ -571,8 +584,6 @@ __global__ __launch_bounds__(SP_THREADS) void sample_rows_kernel(const sp_args a
                         rank += ahead;
                         sum += ahead ? list_w[j] : 0.0;
                     }
-                    double *const sums = reinterpret_cast<double *>(bins);
-                    uint32_t *const ranks = bins + 2 * SP_LIST;
                     sums[tid] = sum;
                     ranks[tid] = rank;
                     __syncthreads();
@@ -606,54 +617,84 @@ __global__ __launch_bounds__(SP_THREADS) void sample_rows_kernel(const sp_args a
             counting = true;
         }
 
-        // ---- too many for a list: the spans' kept sums
-        __syncthreads();
-        if (tid < a.spans) {
-            span_kept[tid] = 0.0;
-            span_ties[tid] = 0;
+        // ---- too many for a list: the spans' kept sums.  Where their total is known from the counting, the spans up to the one in which the random number will fall do, or those
+        // from there on, if these are fewer: all of a span's weights (known) grow along the row nearly as the kept ones do.
+        if (rule.by_sum && !rule.by_count && border > SP_NONE && least <= border) {
+            double total;
+            const double before = sp_before(kept, part, total);
+            const int s = first_beyond(kept, before, rule.u * total), margin = a.spans / 16 + 2;
+            if (2 * s < a.spans) end = min(a.spans, s + margin);
+            else first = max(0, s - margin);
         }
-        __syncthreads();
-        each_span(from, [&](int s, const half8_t v) {
-            const ushort8_t key = sp_keys(v);
-            double w[2] = {0.0, 0.0};
-            uint32_t n = 0;
+    }
+#pragma unroll 1
+    for (;;) {
+        const bool whole = first == 0 && end == a.spans;
+        if (!sums_are_there) {
+            __syncthreads();
+            if (tid < a.spans) {
+                span_kept[tid] = 0.0;
+                span_ties[tid] = 0;
+            }
+            if (tid == 0) {
+                at_first = 0x7fffffff;
+                at_last = -1;
+            }
+            __syncthreads();
+            each_span(first, end, from, [&](int s, const half8_t v) {
+                const ushort8_t key = sp_keys(v);
+                double w[2] = {0.0, 0.0};
+                uint32_t n = 0;
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const sp_power at = weight.of(top == SP_INFINITE ? weight.largest : (double)(float)v[e]);
-                w[e & 1] = __builtin_fma(key[e] > border && key[e] >= from && key[e] <= top ? at.power : 0.0, at.p, w[e & 1]);
-                n += key[e] == border;
-            }
-            double sum = w[0] + w[1];
-            sum = sp_wave_sum(sum);
-            n = sp_wave_sum(n);
-            if (lane == 0) {
-                span_kept[s] = sum;
-                span_ties[s] = border > SP_NONE ? n : 0;
-            }
-        });
+                for (int e = 0; e < 8; e++) {
+                    const sp_power at = weight.of(top == SP_INFINITE ? weight.largest : (double)(float)v[e]);
+                    w[e & 1] = __builtin_fma(key[e] > border && key[e] >= from && key[e] <= top ? at.power : 0.0, at.p, w[e & 1]);
+                    n += key[e] == border;
+                }
+                double sum = w[0] + w[1];
+                sum = sp_wave_sum(sum);
+                n = sp_wave_sum(n);
+                if (lane == 0) {
+                    span_kept[s] = sum;
+                    span_ties[s] = border > SP_NONE ? n : 0;
+                }
+            });
+            __syncthreads();
+            kept = tid < a.spans ? span_kept[tid] : 0.0;
+            ties = tid < a.spans ? span_ties[tid] : 0;
+        }
+        // ---- the draw from the spans' sums: ties that stay are those of the first spans
+        uint32_t ties_before = 0;
+        if (border > SP_NONE) {
+            uint32_t all;
+            ties_before = sp_before(ties, part32, all);
+            if (first > 0) ties_before += border_ties - all;
+            kept += (double)(ties_before < stay ? min(ties, stay - ties_before) : 0) * (border >= from ? weight(border) : 0.0);
+        }
+        double total, before = sp_before(kept, part, total);
+        if (!whole) {
+            if (first > 0) before += counted_sum - total;
+            total = counted_sum;
+        }
+        const double goal = rule.u * total;
+        const int s = first_beyond(tid >= first && tid < end ? kept : 0.0, before, goal);
+        if (tid == s) {
+            span_before = before;
+            span_left = ties_before < stay ? stay - ties_before : 0;
+        }
+        const bool reached = at_first != 0x7fffffff;
         __syncthreads();
-        kept = tid < a.spans ? span_kept[tid] : 0.0;
-        ties = tid < a.spans ? span_ties[tid] : 0;
-    }
-
-    // ---- the draw from the spans' sums: ties that stay are those of the first spans
-    uint32_t ties_before = 0;
-    if (border > SP_NONE) {
-        uint32_t all;
-        ties_before = sp_before(ties, part32, all);
-        kept += (double)(ties_before < stay ? min(ties, stay - ties_before) : 0) * (border >= from ? weight(border) : 0.0);
-    }
-    double total;
-    const double before = sp_before(kept, part, total), goal = rule.u * total;
-    const int s = first_beyond(kept, before, goal);
-    if (tid == s) {
-        span_before = before;
-        span_left = ties_before < stay ? stay - ties_before : 0;
-    }
-    __syncthreads();
-    if (wave == 0) {
-        const int at = sp_draw(row, s, border, from, weight, span_left, span_before, goal);
-        if (tid == 0) a.out[b] = at;
+        // (not in the spans that were summed, or in front of them: then all)
+        if (!whole && (!reached || (s == first && first > 0 && span_before > goal))) {
+            first = 0;
+            end = a.spans;
+            continue;
+        }
+        if (wave == 0) {
+            const int at = sp_draw(row, s, border, from, weight, span_left, span_before, goal);
+            if (tid == 0) a.out[b] = at;
+        }
+        return;
     }
 }
 
