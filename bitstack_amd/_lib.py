@@ -75,7 +75,7 @@ SIGNATURES.update({
     "bs_attention_decode_workspace_bytes": (_L, [_I, _I, _I, _I, _I]),
     "bs_attention_decode_ws_f16": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _L, _P]),
     "bs_page_plan_workspace_bytes": (_L, [_I, _I]),
-    "bs_page_plan": (_I, [_P] * 12 + [_I, _I, _I, _I, _I, _P, _L, _P]),
+    "bs_page_plan": (_I, [_P] * 13 + [_I, _I, _I, _I, _I, _P, _L, _P]),
     "bs_rope_store_paged_f16": (_I, [_P, _I, _P, _I, _P, _P, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P]),
     "bs_attention_paged_workspace_bytes": (_L, [_I, _I, _I, _I, _I, _I]),
     "bs_attention_paged_f16": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _L, _P]),

@@ -456,8 +456,8 @@ extern "C" int64_t bs_page_plan_workspace_bytes(int B, int T) {
 
 extern "C" int bs_page_plan(const int32_t *lengths, const int32_t *new_tokens, const uint8_t *released, int32_t *block_table, int32_t *free_pages,
                             const int32_t *free_state, int32_t *lengths_out, int32_t *free_state_out, int32_t *granted, int32_t *starts,
-                            int32_t *positions, int64_t *slots, int B, int T, int page_size, int max_pages, int pool_pages, void *workspace,
-                            int64_t workspace_bytes, void *stream) {
+                            int32_t *positions, int64_t *slots, int64_t *row_slots, int B, int T, int page_size, int max_pages, int pool_pages,
+                            void *workspace, int64_t workspace_bytes, void *stream) {
     const int st = plan_shape(B, T, page_size, max_pages, pool_pages);
     if (st != BS_OK) return st;
     if (!free_pages || !free_state || !free_state_out || !starts || (T > 0 && (!positions || !slots)) ||
@@ -466,11 +466,11 @@ extern "C" int bs_page_plan(const int32_t *lengths, const int32_t *new_tokens, c
     for (const void *p : {(const void *)lengths, (const void *)new_tokens, (const void *)block_table, (const void *)free_pages, (const void *)free_state,
                           (const void *)lengths_out, (const void *)free_state_out, (const void *)granted, (const void *)starts, (const void *)positions})
         if (!bs_aligned(p, 4)) return BS_ERR_ALIGN;
-    if (!bs_aligned(slots, 8)) return BS_ERR_ALIGN;
+    if (!bs_aligned(slots, 8) || !bs_aligned(row_slots, 8)) return BS_ERR_ALIGN;
     const int64_t need = bs_page_plan_scratch(B, T);
     if (need > 0 && (!workspace || workspace_bytes < need || !bs_aligned(workspace, 16))) return BS_ERR_WORKSPACE;
     return bs_launch_page_plan(lengths, new_tokens, released, block_table, free_pages, free_state, lengths_out, free_state_out, granted, starts, positions, slots,
-                               B, T, page_shift(page_size), max_pages, pool_pages, workspace, (hipStream_t)stream);
+                               row_slots, B, T, page_shift(page_size), max_pages, pool_pages, workspace, (hipStream_t)stream);
 }
 
 extern "C" int bs_rope_store_paged_f16(void *q, int ldq, void *q_out, int ldq_out, const void *k, const void *v, int ldkv, const void *cos, const void *sin,
@@ -494,7 +494,7 @@ extern "C" int bs_rope_store_paged_f16(void *q, int ldq, void *q_out, int ldq_ou
 static int attention_paged_shape(int B, int heads, int kv_heads, int head_dim, int page_size, int max_pages) {
     return B < 0 || B > 65536 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || (head_dim != 64 && head_dim != 128) || page_shift(page_size) < 0 ||
                    max_pages < 1 || (int64_t)max_pages * page_size > INT32_MAX || (int64_t)B * ((int64_t)max_pages * page_size / 16) > INT32_MAX ||
-                   ((int64_t)heads + 2 * (int64_t)kv_heads) * head_dim > INT32_MAX || (int64_t)B * heads > INT32_MAX
+                   ((int64_t)heads + 2 * (int64_t)kv_heads) * head_dim > INT32_MAX || (int64_t)B * heads > 1 << 22
                ? BS_ERR_SHAPE
                : BS_OK;
 }
@@ -522,7 +522,9 @@ extern "C" int bs_attention_paged_f16(const void *qkv, int ldqkv, void *kpages, 
                                      (hipStream_t)stream);
 }
 
-static int sample_shape(int B, int V) { return B < 0 || B > 1 << 20 || V < 1 || V > 1 << 18 ? BS_ERR_SHAPE : BS_OK; }
+static int sample_shape(int B, int V) {
+    return B < 0 || B > 1 << 20 || V < 1 || V > 1 << 18 || (int64_t)B * ((V + 511) / 512) > 1 << 24 ? BS_ERR_SHAPE : BS_OK;
+}
 
 extern "C" int64_t bs_sample_workspace_bytes(int B, int V) {
     const int st = sample_shape(B, V);

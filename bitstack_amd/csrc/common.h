@@ -136,8 +136,8 @@ int64_t bs_attention_parts_bytes(int B, int heads, int kv_heads, int max_len);  
 // requests of unequal lengths: the plan of pages and the store to them (paged.hip), attention over them (paged_attention.hip); pages of 1 << shift positions
 int64_t bs_page_plan_scratch(int B, int T);
 int bs_launch_page_plan(const int32_t *lengths, const int32_t *fresh, const uint8_t *released, int32_t *table, int32_t *ring, const int32_t *state,
-                        int32_t *lengths_out, int32_t *state_out, int32_t *granted, int32_t *starts, int32_t *positions, int64_t *slots, int B,
-                        int T, int shift, int max_pages, int pool, void *workspace, hipStream_t s);
+                        int32_t *lengths_out, int32_t *state_out, int32_t *granted, int32_t *starts, int32_t *positions, int64_t *slots, int64_t *row_slots,
+                        int B, int T, int shift, int max_pages, int pool, void *workspace, hipStream_t s);
 int bs_launch_rope_store_paged(const half_t *q, half_t *qout, const half_t *k, const half_t *v, const half_t *cos, const half_t *sin,
                                const int32_t *positions, const int64_t *slots, half_t *kpages, half_t *vpages, int ldq, int ldqo, int ldkv, int T,
                                int heads, int kv_heads, int d, int max_pos, int shift, int pool, hipStream_t s);

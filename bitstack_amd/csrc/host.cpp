@@ -564,7 +564,7 @@ bool pages_args(PyObject *kp, PyObject *vp, PyObject *cosp, PyObject *sinp, c10:
 }
 
 // page_plan(lengths, new_tokens, block_table, free_pages, free_state, page_size, tokens, released or None, inplace)
-// -> (lengths, state, granted, starts, positions, slots), or None
+// -> (lengths, state, granted, starts, positions, slots, row_slots), or None
 PyObject *host_page_plan(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (n != 9) return PyErr_Format(PyExc_TypeError, "page_plan takes 9 arguments");
     HANDLE_TH_ERRORS
@@ -586,7 +586,7 @@ PyObject *host_page_plan(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const uint8_t *gone = released ? (const uint8_t *)released->const_data_ptr() : nullptr;
         int32_t *tp = (int32_t *)table->mutable_data_ptr(), *rp = (int32_t *)ring->mutable_data_ptr();
         const int max_pages = (int)table->size(1), pool = (int)ring->size(0);
-        at::Tensor out[6];
+        at::Tensor out[7];
         if (inplace) {
             out[0] = *lengths;
             out[1] = *state;
@@ -602,15 +602,16 @@ PyObject *host_page_plan(PyObject *, PyObject *const *a, Py_ssize_t n) {
             out[3] = new_tensor({B + 1}, at::kInt, dev);
             out[4] = new_tensor({T}, at::kInt, dev);
             out[5] = new_tensor({T}, at::kLong, dev);
+            out[6] = new_tensor({B}, at::kLong, dev);
             const Workspace ws = workspace_for(dev.index(), stream, need);
             std::lock_guard<std::mutex> launching(*ws.launching);
             return bs_page_plan(lp, fp, gone, tp, rp, sp, (int32_t *)out[0].mutable_data_ptr(), (int32_t *)out[1].mutable_data_ptr(), (int32_t *)out[2].mutable_data_ptr(),
-                                (int32_t *)out[3].mutable_data_ptr(), (int32_t *)out[4].mutable_data_ptr(), (int64_t *)out[5].mutable_data_ptr(), (int)B, (int)T, (int)page,
-                                max_pages, pool, ws.data(), ws.buffer.numel(), stream);
+                                (int32_t *)out[3].mutable_data_ptr(), (int32_t *)out[4].mutable_data_ptr(), (int64_t *)out[5].mutable_data_ptr(), (int64_t *)out[6].mutable_data_ptr(), (int)B, (int)T,
+                                (int)page, max_pages, pool, ws.data(), ws.buffer.numel(), stream);
         });
         if (st != BS_OK) return raise_status(st, "bs_page_plan");
-        PyObject *all = PyTuple_New(6);
-        for (int i = 0; all && i < 6; i++) {
+        PyObject *all = PyTuple_New(7);
+        for (int i = 0; all && i < 7; i++) {
             PyObject *t = THPVariable_Wrap(out[i]);
             if (!t) {
                 Py_DECREF(all);

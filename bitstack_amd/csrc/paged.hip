@@ -21,7 +21,7 @@ struct plan_args {
     int32_t *table, *ring;
     const int32_t *state;
     int32_t *lengths_out, *state_out, *granted, *starts, *positions;
-    int64_t *slots;
+    int64_t *slots, *row_slots;
     int B, T, shift, max_pages, pool;
 };
 // what a row has to write
@@ -93,6 +93,16 @@ __device__ __forceinline__ void plan_write_entries(const plan_args &a, const pla
             if (taken[n]) row[j] = fresh[n];
         }
     }
+}
+// the slot of a request's first token
+__device__ __forceinline__ void plan_write_row_slot(const plan_args &a, const plan_state &st, const plan_row &r, int b) {
+    int64_t slot = -1;
+    if (r.granted > 0) {
+        const int p = r.held >> a.shift, own = p - plan_pages(r.held, a.shift);
+        const int32_t id = own >= 0 ? a.ring[plan_wrap((uint32_t)st.head + r.first + own, a.pool)] : a.table[(int64_t)b * a.max_pages + p];
+        if (id >= 0) slot = ((int64_t)id << a.shift) + (r.held & ((1 << a.shift) - 1));
+    }
+    a.row_slots[b] = slot;
 }
 template <int N>
 __device__ __forceinline__ void plan_write_tokens(const plan_args &a, const plan_state &st, const plan_row &r, int b, int from, int step, int end) {
@@ -187,6 +197,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(const plan_args
                 longer_row[at] = b;
             }
             plan_write_tokens<1>(a, st, r, b, 0, 1, min(t1, 1));
+            if (in && a.row_slots) plan_write_row_slot(a, st, r, b);
             plan_write_entries<1>(a, st, r, b, e0, 1, min(e1, e0 + 1));
             __syncthreads();
             // a wave per row, or several if there are fewer rows than waves
@@ -236,6 +247,7 @@ __global__ __launch_bounds__(PLAN_STRIP) void plan_write_kernel(const plan_args 
         return;
     }
     const int t1 = min(r.fresh, max(a.T - r.start, 0)), e1 = plan_entries(r, a.shift);
+    if (from == 0 && a.row_slots) plan_write_row_slot(a, st, r, b);
     plan_write_tokens<4>(a, st, r, b, from, step, t1);
     plan_write_entries<4>(a, st, r, b, plan_first_entry(r, a.shift) + from, step, e1);
 }
@@ -301,9 +313,9 @@ __global__ __launch_bounds__(THREADS) void rope_store_paged_kernel(const half_t 
 int64_t bs_page_plan_scratch(int B, int T) { return plan_few(B, T) ? 0 : (int64_t)(B + 1) * sizeof(plan_row); }
 
 int bs_launch_page_plan(const int32_t *lengths, const int32_t *fresh, const uint8_t *released, int32_t *table, int32_t *ring, const int32_t *state,
-                        int32_t *lengths_out, int32_t *state_out, int32_t *granted, int32_t *starts, int32_t *positions, int64_t *slots, int B,
-                        int T, int shift, int max_pages, int pool, void *workspace, hipStream_t s) {
-    const plan_args a = {lengths, fresh, released, table, ring, state, lengths_out, state_out, granted, starts, positions, slots, B, T, shift, max_pages, pool};
+                        int32_t *lengths_out, int32_t *state_out, int32_t *granted, int32_t *starts, int32_t *positions, int64_t *slots, int64_t *row_slots,
+                        int B, int T, int shift, int max_pages, int pool, void *workspace, hipStream_t s) {
+    const plan_args a = {lengths, fresh, released, table, ring, state, lengths_out, state_out, granted, starts, positions, slots, row_slots, B, T, shift, max_pages, pool};
     if (plan_few(B, T)) {
         page_plan_kernel<true><<<1, PLAN_THREADS, 0, s>>>(a, nullptr);
     } else {
@@ -325,8 +337,10 @@ int bs_launch_rope_store_paged(const half_t *q, half_t *qout, const half_t *k, c
     for (const void *p : {(const void *)q, (const void *)qout, (const void *)k, (const void *)v, (const void *)cos, (const void *)sin, (const void *)kpages, (const void *)vpages})
         wide = wide && bs_aligned(p, 16);
     auto *kernel = wide ? rope_store_paged_kernel<8> : rope_store_paged_kernel<1>;
-    kernel<<<T, THREADS, 0, s>>>(q, qout, k, v, cos, sin, positions, slots, kpages, vpages, ldq, ldqo, ldkv, heads, kv_heads, d, max_pos, shift,
-                                 (int64_t)pool << shift);
-    BS_LAUNCH_CHECK();
+    for (int64_t t = 0; t < T; t += 1 << 23) {   // (a grid holds 2^32 threads along x)
+        kernel<<<(unsigned)(T - t < 1 << 23 ? T - t : 1 << 23), THREADS, 0, s>>>(q + t * ldq, qout + t * ldqo, k + t * ldkv, v + t * ldkv, cos, sin, positions + t, slots + t, kpages,
+                                                                                vpages, ldq, ldqo, ldkv, heads, kv_heads, d, max_pos, shift, (int64_t)pool << shift);
+        BS_LAUNCH_CHECK();
+    }
     return BS_OK;
 }

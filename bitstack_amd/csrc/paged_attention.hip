@@ -461,8 +461,7 @@ int bs_launch_attention_paged(const half_t *qkv, int ldqkv, half_t *kpages, half
                               const int32_t *lengths, const int64_t *slots, half_t *out, int B, int heads, int kv_heads, int head_dim, int max_pos,
                               int shift, int max_pages, int pool, void *workspace, hipStream_t s) {
     const pa_shape p = shape_of(B, heads, kv_heads, (int64_t)max_pages << shift);
-    const int64_t workgroups = (int64_t)(B + p.parts) * p.units;
-    if (workgroups > INT32_MAX) return BS_ERR_SHAPE;
+    const int64_t workgroups = (int64_t)(B + p.parts) * p.units;          // (at most 2^22 and the parts: 2^32 threads hold them)
     pa_args a = {qkv, cos, sin, kpages, vpages, lengths, slots, out, (int32_t *)workspace, (float *)((char *)workspace + bs_cdiv(8ll * B, 16) * 16),
                  ldqkv, B, heads, kv_heads, p.groups, p.per_unit, max_pos, shift, max_pages, pool, p.parts};
     if (head_dim == 128)

@@ -343,13 +343,15 @@ def _vector(t, n, dtype, name):
 
 class PagePlan(NamedTuple):
     """What page_plan_hip gives: positions per request and the ring's {first, count} afterwards, tokens that got slots [B], first
-    token row of every request [B + 1], position (int32) and slot (int64) of every token row, -1 without one."""
+    token row of every request [B + 1], position (int32) and slot (int64) of every token row, slot of every request's first token [B];
+    -1 without one."""
     lengths: torch.Tensor
     state: torch.Tensor
     granted: torch.Tensor
     starts: torch.Tensor
     positions: torch.Tensor
     slots: torch.Tensor
+    row_slots: torch.Tensor
 
 
 def page_plan_hip(lengths, new_tokens, block_table, free_pages, free_state, page_size, tokens, released=None, inplace=False):
@@ -377,7 +379,8 @@ def page_plan_hip(lengths, new_tokens, block_table, free_pages, free_state, page
         _lib.check(need, "bs_page_plan_workspace_bytes")
     i32 = dict(dtype=torch.int32, device=dev)
     plan = PagePlan(lengths if inplace else torch.empty(B, **i32), free_state if inplace else torch.empty(2, **i32), torch.empty(B, **i32),
-                    torch.empty(B + 1, **i32), torch.empty(tokens, **i32), torch.empty(tokens, dtype=torch.int64, device=dev))
+                    torch.empty(B + 1, **i32), torch.empty(tokens, **i32), torch.empty(tokens, dtype=torch.int64, device=dev),
+                    torch.empty(B, dtype=torch.int64, device=dev))
     with torch.cuda.device(dev), _lib.scratch(dev, need) as ws:
         _lib.check(_lib.lib().bs_page_plan(_lib.ptr(lengths), _lib.ptr(new_tokens), _lib.ptr(released), _lib.ptr(block_table), _lib.ptr(free_pages),
                                            _lib.ptr(free_state), *(_lib.ptr(t) for t in plan), B, tokens, int(page_size), block_table.shape[1],
@@ -427,7 +430,7 @@ def rope_store_paged_hip(q, k, v, cos, sin, kpages, vpages, positions, slots, ou
 def attention_paged_hip(qkv, kpages, vpages, cos, sin, block_table, lengths, slots, heads, kv_heads, out=None):
     """One new token per request: RoPE on q and k of qkv [B, (heads + 2 kv) * d] at position lengths[b] - 1, k and v to slots[b] of the pages
     [pool, kv, page_size, d], attention over positions 0 .. lengths[b] - 1 by block_table [B, max_pages]; returns [B, heads * d].
-    lengths (int32) and slots (int64) as page_plan_hip leaves them; a request without a slot is idle and its row zeros."""
+    lengths (int32) and slots (int64) are page_plan_hip's lengths and row_slots; a request without a slot is idle and its row zeros."""
     y = _lib.host().attention_paged(qkv, kpages, vpages, cos, sin, block_table, lengths, slots, heads, kv_heads, out)
     if y is not None:
         return y if out is None else out

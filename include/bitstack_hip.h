@@ -451,6 +451,9 @@ int bs_argmax_advance_f16(const void *x, int64_t *out, int64_t *pos, int B, int 
  *                   new_tokens, refused ones counted; at most T + 1)
  *   positions [T], slots [T]   of every token row; -1 where a request was
  *                   refused, and behind the last token
+ *   row_slots [B]   slot of every request's first token, -1 without one: the
+ *                   slots of a decode step whose rows are the requests, idle ones
+ *                   among them (may be NULL)
  * Pages that go back in a call are not taken in the same one.  Negative lengths
  * and counts are taken as 0, lengths beyond the row as a full one, a free_state
  * that no ring has as an empty ring.  Deterministic.  Many tokens need scratch
@@ -460,8 +463,8 @@ int bs_argmax_advance_f16(const void *x, int64_t *out, int64_t *pos, int B, int 
 int64_t bs_page_plan_workspace_bytes(int B, int T);
 int bs_page_plan(const int32_t *lengths, const int32_t *new_tokens, const uint8_t *released, int32_t *block_table, int32_t *free_pages,
                  const int32_t *free_state, int32_t *lengths_out, int32_t *free_state_out, int32_t *granted, int32_t *starts,
-                 int32_t *positions, int64_t *slots, int B, int T, int page_size, int max_pages, int pool_pages, void *workspace,
-                 int64_t workspace_bytes, void *stream);
+                 int32_t *positions, int64_t *slots, int64_t *row_slots, int B, int T, int page_size, int max_pages, int pool_pages,
+                 void *workspace, int64_t workspace_bytes, void *stream);
 
 /*
  * The prompts' keys and values to their pages: for every token row t with a slot,
@@ -484,12 +487,13 @@ int bs_rope_store_paged_f16(void *q, int ldq, void *q_out, int ldq_out, const vo
  * bs_attention_decode_f16, but over the pages.  lengths[b] counts the new position
  * (what bs_page_plan has left there): q and k of qkv [B, (heads + 2 kv_heads) *
  * head_dim] (rows ldqkv halves apart) are rotated by lengths[b] - 1, k and v stored at
- * slots[b], and out[B, heads * head_dim] = softmax(q k^T / sqrt(head_dim)) v over
+ * slots[b] (bs_page_plan's row_slots), and out[B, heads * head_dim] = softmax(q k^T / sqrt(head_dim)) v over
  * positions 0 .. lengths[b] - 1.  A row without a slot (negative, or one that
  * does not exist), or with a length below 1, beyond its table's row or beyond
  * max_pos, is idle: zeros, nothing stored.  Positions whose table entry is no page
  * are left out.  Requests may share pages that none of them writes.  Any heads per
- * KV head, head_dim 64 or 128; B <= 65536 and B * max_pages * page_size < 2^35.
+ * KV head, head_dim 64 or 128; B <= 65536, B * heads <= 2^22 and B * max_pages *
+ * page_size < 2^35.  Slots must differ.
  * Long requests are cut into parts by what the lengths are at the call, and summed
  * in order: deterministic.  Scratch: bs_attention_paged_workspace_bytes, 16-byte
  * aligned (0: none; negative: an error status).
@@ -501,7 +505,7 @@ int bs_attention_paged_f16(const void *qkv, int ldqkv, void *kpages, void *vpage
 
 /*
  * The next token of each of B rows of logits (fp16, rows ld values apart, V <=
- * 2^18, B <= 2^20), drawn with the random number uniform[b] of [0, 1) that the caller gives.
+ * 2^18, B <= 2^20, B * V <= 2^33), drawn with the random number uniform[b] of [0, 1) that the caller gives.
  * With w_i = exp((x_i - max) / temperature[b]):
  *   top_k[b]   the k largest stay (among equals the lowest indexes); <= 0: all
  *   top_p[b]   of those, from the largest down (among equals the lowest index

@@ -43,6 +43,8 @@ def call(lengths, new, table, ring, state, gone, page, tokens, inplace=False):
     assert (plan.lengths is args[0]) == inplace and (plan.state is args[4]) == inplace
     if not inplace:
         assert args[0].tolist() == list(lengths) and args[4].tolist() == list(state)
+    # a request's own slot is that of its first token
+    assert plan.row_slots.tolist() == [plan.slots.tolist()[s] if g else -1 for s, g in zip(plan.starts.tolist(), plan.granted.tolist())]
     return args[2].tolist(), args[3].tolist(), plan.lengths.tolist(), tuple(plan.state.tolist()), plan.granted.tolist(), plan.starts.tolist(), plan.positions.tolist(), plan.slots.tolist()
 
 

@@ -25,7 +25,7 @@ def call(fn, spec, **changed):
     return fn(*args.values())
 
 
-PLAN = dict(lengths=ONE, new=ONE, released=NUL, table=ONE, ring=ONE, state=ONE, lengths_out=ONE, state_out=ONE, granted=ONE, starts=ONE, positions=ONE, slots=ONE,
+PLAN = dict(lengths=ONE, new=ONE, released=NUL, table=ONE, ring=ONE, state=ONE, lengths_out=ONE, state_out=ONE, granted=ONE, starts=ONE, positions=ONE, slots=ONE, row_slots=NUL,
             B=4, T=5000, page=16, max_pages=8, pool=100, ws=ONE, ws_bytes=1 << 20, stream=NUL)
 STORE = dict(q=ONE, ldq=512, q_out=NUL, ldq_out=0, k=ONE, v=ONE, ldkv=256, cos=ONE, sin=ONE, positions=ONE, slots=ONE, kpages=ONE, vpages=ONE, T=4, heads=4, kv_heads=2,
              d=128, max_pos=100, page=16, pool=100, stream=NUL)
@@ -41,7 +41,7 @@ def test_plan(L):
     for name in ("lengths", "new", "table", "ring", "state", "lengths_out", "state_out", "granted", "starts", "positions", "slots"):
         assert refused(**{name: NUL}) == NULLS, name
         assert refused(**{name: ODD}) == ALIGN, name
-    assert refused(slots=ctypes.c_void_p(4100)) == ALIGN
+    assert refused(slots=ctypes.c_void_p(4100)) == refused(row_slots=ctypes.c_void_p(4100)) == ALIGN
     for change in ({"B": -1}, {"B": 65537}, {"T": -1}, {"T": (1 << 30) + 1}, {"page": 8}, {"page": 24}, {"page": 2048}, {"page": 0}, {"page": -16}, {"max_pages": 0},
                    {"max_pages": (1 << 24) + 1}, {"pool": 0}, {"pool": 1 << 27}):
         assert refused(**change) == SHAPE, change
@@ -69,7 +69,7 @@ def test_attention(L):
         assert refused(**{name: ODD}) == ALIGN, name
     assert refused(kpages=EIGHT) == refused(vpages=EIGHT) == refused(slots=ctypes.c_void_p(4100)) == ALIGN
     for change in ({"B": -1}, {"B": 65537}, {"heads": 0}, {"kv_heads": 0}, {"heads": 5}, {"d": 96}, {"d": 32}, {"page": 48}, {"page": 8}, {"max_pages": 0}, {"max_pos": 0},
-                   {"pool": 0}, {"pool": 1 << 27}, {"ld": 1023}, {"max_pages": 1 << 27}, {"B": 65536, "max_pages": 1 << 20}):
+                   {"pool": 0}, {"pool": 1 << 27}, {"ld": 1023}, {"max_pages": 1 << 27}, {"B": 65536, "max_pages": 1 << 20}, {"B": 65536, "heads": 128, "max_pages": 4, "ld": 1 << 20}):
         assert refused(**change) == SHAPE, change
     assert refused(ws=NUL) == refused(ws_bytes=100) == refused(ws=EIGHT) == WORKSPACE
     assert refused(B=0) == 0
@@ -85,7 +85,7 @@ def test_sample(L):
     for name in ("logits", "uniform", "temperature", "top_k", "top_p", "min_p", "out"):
         assert refused(**{name: ODD}) == ALIGN, name
     assert refused(out=ctypes.c_void_p(4100)) == refused(top_k=ctypes.c_void_p(4098)) == ALIGN
-    for change in ({"B": -1}, {"B": (1 << 20) + 1}, {"V": 0}, {"V": (1 << 18) + 1}, {"ld": 999}, {"ld": -1000}):
+    for change in ({"B": -1}, {"B": (1 << 20) + 1}, {"V": 0}, {"V": (1 << 18) + 1}, {"ld": 999}, {"ld": -1000}, {"B": 1 << 20, "V": 9000, "ld": 9000}):
         assert refused(**change) == SHAPE, change
     assert refused(ws=NUL) == refused(ws_bytes=10) == refused(ws=EIGHT) == WORKSPACE
     assert L.bs_sample_workspace_bytes(4, 0) == L.bs_sample_workspace_bytes(-1, 10) == SHAPE and L.bs_sample_workspace_bytes(0, 10) == 0
