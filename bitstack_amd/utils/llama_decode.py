@@ -24,7 +24,9 @@ import torch.nn.functional as F
 from bitstack_amd import _lib
 from bitstack_amd._lib import EPI_NONE, EPI_RESIDUAL, EPI_SWIGLU
 from bitstack_amd.modules.BitStackLinear import BitStackLinear
-from bitstack_amd.utils.inference_utils import MatrixGroup, add_rmsnorm_hip, argmax_hip, attention_prefill_hip, forward_cat_hip, linear_f16_hip, plainly_called, rmsnorm_hip, rope_store_hip, silu_mul_hip
+from bitstack_amd.utils.inference_utils import (MatrixGroup, add_rmsnorm_hip, argmax_hip, attention_paged_hip, attention_prefill_hip, bitstack_forward_group_hip,
+                                                forward_cat_hip, linear_f16_hip, page_plan_hip, plainly_called, rmsnorm_hip, rope_store_hip, rope_store_paged_hip,
+                                                sample_hip, silu_mul_hip)
 
 PROJ = ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj", "self_attn.o_proj",
         "mlp.gate_proj", "mlp.up_proj", "mlp.down_proj")
@@ -128,6 +130,29 @@ def _synthetic_bitstack(m, n, blocks, k, dev, gen, name):
     mod.u = (torch.randn(blocks, m, k, device=dev, generator=gen).abs() * scale).half()
     mod.vt = (torch.randn(blocks, k, n, device=dev, generator=gen).abs() * scale).half()
     return mod
+
+
+class PagedCache:
+    """Keys and values of up to `rows` requests of unequal lengths, in pages that a decoder's layers share one table of: what prefill_paged()
+    and step_paged() work on.  Everything is on the device: plans, lengths and free pages never come to the host."""
+
+    def __init__(self, decoder, rows: int, pool_pages: int, page_size: int = 16):
+        s, dev = decoder.s, decoder.dev
+        if not 1 <= rows <= 48:
+            raise ValueError("1 to 48 rows (the grouped launches take up to 48 tokens)")
+        i32 = dict(dtype=torch.int32, device=dev)
+        self.rows, self.page_size = rows, page_size
+        self.kpages = torch.zeros(s.layers, pool_pages, s.kv_heads, page_size, s.head_dim, dtype=torch.float16, device=dev)
+        self.vpages = torch.zeros_like(self.kpages)
+        self.block_table = torch.zeros(rows, -(-decoder.max_len // page_size), **i32)
+        self.lengths = torch.zeros(rows, **i32)                            # positions held per request
+        self.free_pages = torch.arange(pool_pages, **i32)                  # a ring, and its {first, count}
+        self.free_state = torch.tensor([0, pool_pages], **i32)
+        self.token = torch.zeros(rows, dtype=torch.long, device=dev)       # next token of every request
+
+    def plan(self, new_tokens, tokens, released=None):
+        """page_plan_hip on this cache, in place."""
+        return page_plan_hip(self.lengths, new_tokens, self.block_table, self.free_pages, self.free_state, self.page_size, tokens, released=released, inplace=True)
 
 
 class SyntheticLlamaDecoder:
@@ -555,6 +580,63 @@ class SyntheticLlamaDecoder:
         self.token.copy_(self.logits.argmax(-1))
         self.pos.fill_(n)
         return full if all_logits else None
+
+    # ---- requests of unequal lengths --------------------------------------------------------------------
+    @torch.no_grad()
+    def prefill_paged(self, cache: PagedCache, row: int, prompt: torch.Tensor):
+        """A new request in row `row`: its prompt [len] in one pass, keys and values to pages (those that the row held go back
+        first).  Returns (the plan, logits [1, vocab] of the last position); plan.granted[row] is 0 where the pages were not there, and the logits
+        are of no use then.  The caller puts the first token into cache.token[row]."""
+        s, d = self.s, self.s.head_dim
+        n = prompt.numel()
+        if d != 128:
+            raise ValueError("prefill_paged needs heads of 128")
+        if n < 1 or n > self.max_len:
+            raise ValueError("prompt length must be in 1..max_len")
+        at = torch.arange(cache.rows, device=self.dev) == row
+        plan = cache.plan(n * at.int(), n, released=at)
+        x = self.embed.index_select(0, prompt.reshape(-1))
+        # the prompt attends to its own rows, which lie side by side
+        kc, vc = torch.empty(2, 1, s.kv_heads, self.max_len, d, dtype=torch.float16, device=self.dev)
+        wide = s.heads * d, s.kv_heads * d, s.kv_heads * d
+        hn = rmsnorm_hip(x, self.norm_w[0, 0], s.rms_eps)
+        for L in range(s.layers):
+            lin = self.lin[L]
+            qkv = forward_cat_hip([lin[p] for p in PROJ[:3]], hn)
+            q, k, v = qkv.split(wide, 1) if qkv is not None else (self._output(lin[p], hn) for p in PROJ[:3])
+            rope_store_paged_hip(None, k, v, self.cos, self.sin, cache.kpages[L], cache.vpages[L], plan.positions, plan.slots)
+            rope_store_hip(q, k, v, self.cos, self.sin, kc, vc, n)
+            ctx = attention_prefill_hip(q, kc, vc, n)
+            x, hn = self._sum_norm(x, self._output(lin["self_attn.o_proj"], ctx), self.norm_w[L, 1])
+            act = self._silu_mul(*(self._output(lin[p], hn) for p in PROJ[4:6]))
+            down = self._output(lin["mlp.down_proj"], act)
+            if L + 1 < s.layers:
+                x, hn = self._sum_norm(x, down, self.norm_w[L + 1, 0])
+        x, hn = self._sum_norm(x[-1:].contiguous(), down[-1:].contiguous(), self.final_norm)
+        return plan, self._head(hn)
+
+    @torch.no_grad()
+    def step_paged(self, cache: PagedCache, new_tokens=None, released=None, uniform=None, **sampling):
+        """One token for every request of the cache: cache.token at its next position.  new_tokens (int32 [rows]; None: all) is 0 for rows
+        that are idle, `released` [rows] gives the pages of finished ones back.  The next tokens, greedy or with `uniform` [rows] drawn as sample_hip
+        does with temperature, top_k, top_p, min_p, go to cache.token for requests that got a slot.  Returns the plan; self.logits holds the logits."""
+        s, eps = self.s, self.s.rms_eps
+        if self._groups is None:
+            self._build_groups()
+        if new_tokens is None:
+            new_tokens = torch.ones_like(cache.lengths)
+        plan = cache.plan(new_tokens, cache.rows, released=released)
+        x = self.embed.index_select(0, cache.token)
+        for L, grp in enumerate(self._groups):
+            qkv = bitstack_forward_group_hip(grp["qkv"], x, rms_eps=eps)
+            ctx = attention_paged_hip(qkv, cache.kpages[L], cache.vpages[L], self.cos, self.sin, cache.block_table, cache.lengths, plan.row_slots, s.heads, s.kv_heads)
+            x = bitstack_forward_group_hip(grp["o"], ctx, EPI_RESIDUAL, residual=x)
+            act = bitstack_forward_group_hip(grp["gate_up"], x, EPI_SWIGLU, rms_eps=eps)
+            x = bitstack_forward_group_hip(grp["down"], act, EPI_RESIDUAL, residual=x)
+        self.logits = self._head(rmsnorm_hip(x, self.final_norm, eps))
+        token = argmax_hip(self.logits) if uniform is None else sample_hip(self.logits, uniform, **sampling)
+        torch.where(plan.granted > 0, token, cache.token, out=cache.token)
+        return plan
 
     def prefill_positions(self, prompt: torch.Tensor, fused=False):
         """Feed a prompt token by token (the measurement is about decode).  `prompt`
