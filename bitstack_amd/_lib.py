@@ -234,14 +234,15 @@ def workspace(dev, nbytes: int):
 class scratch:
     """`with scratch(dev, nbytes) as ws:` the scratch of workspace() for one C-ABI call that keeps something there between its
     kernels: threads that share a stream share its scratch, and the interpreter lock is not held during such a call, so
-    the stream's other calls wait until the block is left."""
+    the stream's other calls wait until the block is left.  own: a call that is captured gets a buffer of its own, so that
+    graphs captured on one stream may be replayed on several at once."""
 
-    def __init__(self, dev, nbytes: int):
+    def __init__(self, dev, nbytes: int, own: bool = False):
         self.index = torch.cuda.current_device() if dev.index is None else dev.index
-        self.nbytes = int(nbytes)
+        self.nbytes, self.own = int(nbytes), bool(own)
 
     def __enter__(self):
-        ws, self.key = host().hold(self.index, self.nbytes)
+        ws, self.key = host().hold(self.index, self.nbytes, self.own)
         return ws
 
     def __exit__(self, *error):

@@ -77,6 +77,16 @@ Workspace workspace_for(int device, hipStream_t stream, int64_t bytes) {
     }
     return {t, &space.launching};
 }
+// The same for a call that a graph may hold beside others: under capture a buffer of its own, from the graph's memory.  Graphs captured on one
+// stream (torch captures on one by itself) may then be replayed on several at once.
+Workspace own_workspace_for(int device, hipStream_t stream, int64_t bytes) {
+    hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+    if (bytes == 0 || hipStreamIsCapturing(stream, &capturing) != hipSuccess || capturing == hipStreamCaptureStatusNone) return workspace_for(device, stream, bytes);
+    at::Tensor own = at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, (c10::DeviceIndex)device));
+    Scratch &s = scratch();
+    std::lock_guard<std::mutex> guard(s.lock);
+    return {own, &s.current[{device, stream}].launching};
+}
 
 // ---- arguments -----------------------------------------------------------------------------------
 const at::Tensor *tensor_arg(PyObject *o) { return THPVariable_CheckExact(o) ? &THPVariable_Unpack(o) : nullptr; }
@@ -346,14 +356,17 @@ PyObject *host_workspace(PyObject *, PyObject *const *a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// hold(device index, nbytes) -> (scratch tensor, key): as workspace(), with the stream's launches kept to this thread until let_go(key)
+// hold(device index, nbytes, own) -> (scratch tensor, key): as workspace(), with the stream's launches kept to this thread until let_go(key);
+// own: a captured call gets a buffer of its own
 PyObject *host_hold(PyObject *, PyObject *const *a, Py_ssize_t n) {
-    if (n != 2) return PyErr_Format(PyExc_TypeError, "hold takes 2 arguments");
+    if (n != 3) return PyErr_Format(PyExc_TypeError, "hold takes 3 arguments");
     HANDLE_TH_ERRORS
         int64_t dev, bytes;
         if (!int_arg(a[0], dev) || !int_arg(a[1], bytes)) return nullptr;
+        const bool own = a[2] == Py_True;
         const Workspace ws = while_others_run([&] {
-            const Workspace w = workspace_for((int)dev, c10::hip::getCurrentHIPStream((c10::DeviceIndex)dev).stream(), bytes);
+            const hipStream_t stream = c10::hip::getCurrentHIPStream((c10::DeviceIndex)dev).stream();
+            const Workspace w = own ? own_workspace_for((int)dev, stream, bytes) : workspace_for((int)dev, stream, bytes);
             w.launching->lock();
             return w;
         });
@@ -603,7 +616,7 @@ PyObject *host_page_plan(PyObject *, PyObject *const *a, Py_ssize_t n) {
             out[4] = new_tensor({T}, at::kInt, dev);
             out[5] = new_tensor({T}, at::kLong, dev);
             out[6] = new_tensor({B}, at::kLong, dev);
-            const Workspace ws = workspace_for(dev.index(), stream, need);
+            const Workspace ws = own_workspace_for(dev.index(), stream, need);
             std::lock_guard<std::mutex> launching(*ws.launching);
             return bs_page_plan(lp, fp, gone, tp, rp, sp, (int32_t *)out[0].mutable_data_ptr(), (int32_t *)out[1].mutable_data_ptr(), (int32_t *)out[2].mutable_data_ptr(),
                                 (int32_t *)out[3].mutable_data_ptr(), (int32_t *)out[4].mutable_data_ptr(), (int64_t *)out[5].mutable_data_ptr(), (int64_t *)out[6].mutable_data_ptr(), (int)B, (int)T,
@@ -684,7 +697,7 @@ PyObject *host_attention_paged(PyObject *, PyObject *const *a, Py_ssize_t n) {
             DeviceScope scope(dev);
             const hipStream_t stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
             if (!y.defined()) y = new_half({B, heads * p.d}, dev);
-            const Workspace ws = workspace_for(dev.index(), stream, need);
+            const Workspace ws = own_workspace_for(dev.index(), stream, need);
             std::lock_guard<std::mutex> launching(*ws.launching);
             return bs_attention_paged_f16(xp, (int)ld, p.k, p.v, p.cos, p.sin, tp, lp, sp, y.mutable_data_ptr(), (int)B, (int)heads, (int)kv, p.d, p.positions, p.page, max_pages,
                                           p.pool, ws.data(), ws.buffer.numel(), stream);
@@ -719,7 +732,7 @@ PyObject *host_sample(PyObject *, PyObject *const *a, Py_ssize_t n) {
             DeviceScope scope(dev);
             const hipStream_t stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
             if (!y.defined()) y = new_tensor({B}, at::kLong, dev);
-            const Workspace ws = workspace_for(dev.index(), stream, need);
+            const Workspace ws = own_workspace_for(dev.index(), stream, need);
             std::lock_guard<std::mutex> launching(*ws.launching);
             return bs_sample_f16(xp, ld, (const float *)up, (const float *)tp, (const int32_t *)kp, (const float *)pp, (const float *)mp, (int64_t *)y.mutable_data_ptr(), (int)B,
                                  (int)V, ws.data(), ws.buffer.numel(), stream);

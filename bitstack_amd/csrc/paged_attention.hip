@@ -77,13 +77,15 @@ __global__ __launch_bounds__(WAVES * 64) void attention_paged_kernel(const pa_ar
     int b = work, part = 0;
     const bool first_part = work < a.B;
     // ---- which request, which part of it
-    int all = 0;
-    for (int i = tid; i < a.B; i += THREADS) all += pa_tiles(pa_cached(a, a.lengths[i]));
     int64_t slot = first_part ? a.slots[work] : 0;
-    all = pa_sum<WAVES>(all, sums);
-    const int most = max(PA_LEAST, (all + a.parts - 1) / max(a.parts, 1));
-    int further = 0, place = 0;                  // further parts of this request, and the first one's number
-    if (first_part && a.parts > 0) further = pa_further(pa_tiles(pa_cached(a, a.lengths[b])), most);
+    int most = 0, further = 0, place = 0;        // tiles of a part at most; further parts of this request, and the first one's number
+    if (a.parts > 0) {
+        int all = 0;
+        for (int i = tid; i < a.B; i += THREADS) all += pa_tiles(pa_cached(a, a.lengths[i]));
+        all = pa_sum<WAVES>(all, sums);
+        most = max(PA_LEAST, (all + a.parts - 1) / a.parts);
+        if (first_part) further = pa_further(pa_tiles(pa_cached(a, a.lengths[b])), most);
+    }
     if (!first_part || further > 0) {            // numbers of the further parts: a running sum over the requests
         if (tid == 0) found[0] = -1;
         int before = 0;

@@ -381,7 +381,7 @@ def page_plan_hip(lengths, new_tokens, block_table, free_pages, free_state, page
     plan = PagePlan(lengths if inplace else torch.empty(B, **i32), free_state if inplace else torch.empty(2, **i32), torch.empty(B, **i32),
                     torch.empty(B + 1, **i32), torch.empty(tokens, **i32), torch.empty(tokens, dtype=torch.int64, device=dev),
                     torch.empty(B, dtype=torch.int64, device=dev))
-    with torch.cuda.device(dev), _lib.scratch(dev, need) as ws:
+    with torch.cuda.device(dev), _lib.scratch(dev, need, own=True) as ws:
         _lib.check(_lib.lib().bs_page_plan(_lib.ptr(lengths), _lib.ptr(new_tokens), _lib.ptr(released), _lib.ptr(block_table), _lib.ptr(free_pages),
                                            _lib.ptr(free_state), *(_lib.ptr(t) for t in plan), B, tokens, int(page_size), block_table.shape[1],
                                            free_pages.shape[0], _lib.ptr(ws), ws.numel(), _lib.stream_ptr(dev)), "bs_page_plan")
@@ -450,7 +450,7 @@ def attention_paged_hip(qkv, kpages, vpages, cos, sin, block_table, lengths, slo
     need = int(_lib.lib().bs_attention_paged_workspace_bytes(B, heads, kv_heads, d, page, block_table.shape[1]))
     if need < 0:
         _lib.check(need, "bs_attention_paged_workspace_bytes")
-    with torch.cuda.device(dev), _lib.scratch(dev, need) as ws:
+    with torch.cuda.device(dev), _lib.scratch(dev, need, own=True) as ws:
         _lib.check(_lib.lib().bs_attention_paged_f16(_lib.ptr(qkv), ldqkv, _lib.ptr(kpages), _lib.ptr(vpages), _lib.ptr(cos), _lib.ptr(sin), _lib.ptr(block_table),
                                                      _lib.ptr(lengths), _lib.ptr(slots), _lib.ptr(y), B, heads, kv_heads, d, max_pos, page,
                                                      block_table.shape[1], pool, _lib.ptr(ws), ws.numel(), _lib.stream_ptr(dev)), "bs_attention_paged_f16")
@@ -478,7 +478,7 @@ def sample_hip(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=
     need = int(_lib.lib().bs_sample_workspace_bytes(B, V))
     if need < 0:
         _lib.check(need, "bs_sample_workspace_bytes")
-    with torch.cuda.device(dev), _lib.scratch(dev, need) as ws:
+    with torch.cuda.device(dev), _lib.scratch(dev, need, own=True) as ws:
         _lib.check(_lib.lib().bs_sample_f16(_lib.ptr(logits), ld, _lib.ptr(uniform), _lib.ptr(temperature), _lib.ptr(top_k), _lib.ptr(top_p), _lib.ptr(min_p),
                                             _lib.ptr(y), B, V, _lib.ptr(ws), ws.numel(), _lib.stream_ptr(dev)), "bs_sample_f16")
     return y
