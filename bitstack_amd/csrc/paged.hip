@@ -252,9 +252,10 @@ __global__ __launch_bounds__(PLAN_STRIP) void plan_write_kernel(const plan_args 
     plan_write_entries<4>(a, st, r, b, plan_first_entry(r, a.shift) + from, step, e1);
 }
 
-// Up to so many rows and tokens one workgroup writes everything.
-constexpr int PLAN_FEW_TOKENS = 4096, PLAN_FEW_ROWS = 1024;
-bool plan_few(int B, int T) { return B <= PLAN_FEW_ROWS && T <= PLAN_FEW_TOKENS; }
+// One workgroup writes everything in a decode step (a token per row, and a few rows more), and where a wave is left for every row of few tokens.
+// (us, one launch / two: a token each for 48 rows 5.5 / 8.3, for 1024 5.6 / 8.3, for 4096 15.1 / 16.1; 1 row of 1024 tokens 6.4 / 8.3, 8 of 128 8.2 / 8.4; but
+// 32 of 64 11.5 / 8.2, 500 of 8 45 / 8.3, 1 of 16384 11.7 / 8.3.)
+bool plan_few(int B, int T) { return (B <= 4096 && T <= B + 64) || (B <= PLAN_THREADS / 64 && T <= 1024); }
 
 // ---- store -----------------------------------------------------------------------------------------------------------
 constexpr int THREADS = 256;
@@ -321,8 +322,8 @@ int bs_launch_page_plan(const int32_t *lengths, const int32_t *fresh, const uint
     } else {
         page_plan_kernel<false><<<1, PLAN_THREADS, 0, s>>>(a, (plan_row *)workspace);
         BS_LAUNCH_CHECK();
-        // strips enough for one long row, few for many rows
-        const int64_t strips = bs_cdiv(T, (int64_t)PLAN_STRIP * (B < 64 ? 1 : 16));
+        // (16 strips of a row to a workgroup, were all tokens one row's.  One: 500 rows of 60 tokens 33.6 us instead of 8.4; a row of 16384 takes 8.3 to 8.4 with both.)
+        const int64_t strips = bs_cdiv(T, (int64_t)PLAN_STRIP * 16);
         plan_write_kernel<<<dim3(B + 1, (unsigned)(strips < 1 ? 1 : strips > 64 ? 64 : strips)), PLAN_STRIP, 0, s>>>(a, (const plan_row *)workspace);
     }
     BS_LAUNCH_CHECK();

@@ -22,6 +22,8 @@
 namespace {
 
 constexpr int PA_TILE = 16, PA_HEADS = 16;       // positions of a tile; query heads of a unit
+// (us with 4 waves / 8: 48 requests of 1 to 4096, 32 heads on 8, 83.9 / 72.6; 2 of 80000, 128 on 8, 128.8 / 112.0; 16 of 100 to 8000, 32 on 2, 24.0 / 23.7; 1 of 700 11.2 / 11.7)
+constexpr int WAVES = 8, THREADS = WAVES * 64;
 constexpr int PA_LEAST = 8;                      // tiles of a part, at least
 constexpr int PA_WHOLE = 512;                    // tables of up to so many positions are not cut
 
@@ -43,7 +45,6 @@ __device__ __forceinline__ int pa_cached(const pa_args &a, int len) {
 __device__ __forceinline__ int pa_tiles(int cached) { return (cached + PA_TILE - 1) / PA_TILE; }
 __device__ __forceinline__ int pa_further(int tiles, int most) { return tiles > most ? (tiles + most - 1) / most - 1 : 0; }
 
-template <int WAVES>
 __device__ __forceinline__ int pa_sum(int v, int *to) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
@@ -60,9 +61,9 @@ __device__ __forceinline__ float eight_on(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x128, 0xf, 0xf, true));    // row_ror:8
 }
 
-template <int D, int HP, int WAVES, bool STREAM>
-__global__ __launch_bounds__(WAVES * 64) void attention_paged_kernel(const pa_args a, const int32_t *__restrict__ table) {
-    constexpr int THREADS = WAVES * 64, W = D / 16, NC = D / 32, D2 = D / 2;
+template <int D, int HP, bool STREAM>
+__global__ __launch_bounds__(THREADS) void attention_paged_kernel(const pa_args a, const int32_t *__restrict__ table) {
+    constexpr int W = D / 16, NC = D / 32, D2 = D / 2;
     typedef half_t vec_t __attribute__((ext_vector_type(W)));
     __shared__ __attribute__((aligned(16))) half_t qrot[2][HP][D];             // rotated queries, first and second terms
     __shared__ __attribute__((aligned(16))) half_t knew[D], vnew[D];           // this position's rotated k and v
@@ -82,7 +83,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_paged_kernel(const pa_ar
     if (a.parts > 0) {
         int all = 0;
         for (int i = tid; i < a.B; i += THREADS) all += pa_tiles(pa_cached(a, a.lengths[i]));
-        all = pa_sum<WAVES>(all, sums);
+        all = pa_sum(all, sums);
         most = max(PA_LEAST, (all + a.parts - 1) / a.parts);
         if (first_part) further = pa_further(pa_tiles(pa_cached(a, a.lengths[b])), most);
     }
@@ -439,13 +440,13 @@ constexpr int64_t PA_STREAM = 256ll << 20;
 
 template <int D, int HP>
 int launch(const pa_args &a, const int32_t *table, int64_t workgroups, hipStream_t s) {
-    constexpr int WAVES = HP == 16 ? 4 : 8;
     const bool stream = ((int64_t)a.pool << a.shift) * a.kv_heads * D * 4 >= PA_STREAM;
-    (stream ? attention_paged_kernel<D, HP, WAVES, true> : attention_paged_kernel<D, HP, WAVES, false>)<<<(unsigned)workgroups, WAVES * 64, 0, s>>>(a, table);
+    (stream ? attention_paged_kernel<D, HP, true> : attention_paged_kernel<D, HP, false>)<<<(unsigned)workgroups, THREADS, 0, s>>>(a, table);
     BS_LAUNCH_CHECK();
     if (a.parts == 0) return BS_OK;
-    // few heads: the parts of each in four runs; many: several heads to a workgroup, most of which have one part
-    const bool few = (int64_t)a.B * a.heads < 1024;
+    // Few heads: the parts of each in four runs; many: several heads to a workgroup, most of which have one part.  (us, runs / heads: 1 request of 8000, 32 heads, 14.7 / 16.6; 2 of
+    // 80000, 64 heads, 107.9 / 108.4; 8 of up to 8000, 32 heads, 33.5 / 33.1; 48 of up to 4096 88.0 / 85.5.)
+    const bool few = (int64_t)a.B * a.heads < 256;
     const int groups = few ? a.heads : (a.heads + 3) / 4;
     (few ? attention_paged_merge_kernel<D, 4, 1> : attention_paged_merge_kernel<D, 1, 4>)<<<(unsigned)((int64_t)a.B * groups), D * 4, 0, s>>>(a.part, a.heads_of, a.out, a.B, a.heads, groups);
     BS_LAUNCH_CHECK();

@@ -57,10 +57,11 @@ def check(case, page, pad=0, tokens=None, inplace=False):
     return got
 
 
-# rows, page, entries of a row, most new tokens, padding, released: one workgroup and (more than 4096 tokens or 1024 rows) two launches
+# rows, page, entries of a row, most new tokens, padding, released: one workgroup (about a token per row, or few tokens) and two launches
 SIZES = [(1, 16, 1, 1, 0, False), (1, 16, 9, 100, 3, False), (2, 1024, 3, 900, 0, True), (63, 16, 40, 1, 0, True), (64, 32, 17, 70, 11, True), (65, 64, 5, 3, 0, False),
          (300, 16, 70, 5, 100, True), (1000, 128, 3, 2, 0, True), (1024, 16, 4, 4, 0, True), (1025, 16, 4, 4, 7, True), (2500, 32, 6, 2, 0, True), (1, 16, 800, 12000, 5, False),
-         (3, 256, 40, 9000, 0, True), (100, 16, 130, 2000, 777, True)]
+         (3, 256, 40, 9000, 0, True), (100, 16, 130, 2000, 777, True),
+         (16, 16, 9, 120, 0, True), (17, 16, 9, 40, 0, True), (3000, 16, 4, 1, 0, True), (4096, 16, 3, 1, 64, True), (5000, 64, 3, 1, 0, True)]
 
 
 @pytest.mark.parametrize("B,page,max_pages,new_hi,pad,released", SIZES)
