@@ -94,15 +94,19 @@ __device__ __forceinline__ void plan_write_entries(const plan_args &a, const pla
         }
     }
 }
-// the slot of a request's first token
-__device__ __forceinline__ void plan_write_row_slot(const plan_args &a, const plan_state &st, const plan_row &r, int b) {
+// a request's first token (if its row is one of the output's), and its slot for the request
+__device__ __forceinline__ void plan_write_first(const plan_args &a, const plan_state &st, const plan_row &r, int b) {
     int64_t slot = -1;
     if (r.granted > 0) {
         const int p = r.held >> a.shift, own = p - plan_pages(r.held, a.shift);
         const int32_t id = own >= 0 ? a.ring[plan_wrap((uint32_t)st.head + r.first + own, a.pool)] : a.table[(int64_t)b * a.max_pages + p];
         if (id >= 0) slot = ((int64_t)id << a.shift) + (r.held & ((1 << a.shift) - 1));
     }
-    a.row_slots[b] = slot;
+    if (r.fresh > 0 && r.start < a.T) {
+        a.slots[r.start] = slot;
+        a.positions[r.start] = r.granted > 0 ? r.held : -1;
+    }
+    if (a.row_slots) a.row_slots[b] = slot;
 }
 template <int N>
 __device__ __forceinline__ void plan_write_tokens(const plan_args &a, const plan_state &st, const plan_row &r, int b, int from, int step, int end) {
@@ -196,8 +200,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(const plan_args
                 longer[at] = r;
                 longer_row[at] = b;
             }
-            plan_write_tokens<1>(a, st, r, b, 0, 1, min(t1, 1));
-            if (in && a.row_slots) plan_write_row_slot(a, st, r, b);
+            if (in) plan_write_first(a, st, r, b);
             plan_write_entries<1>(a, st, r, b, e0, 1, min(e1, e0 + 1));
             __syncthreads();
             // a wave per row, or several if there are fewer rows than waves
@@ -247,8 +250,8 @@ __global__ __launch_bounds__(PLAN_STRIP) void plan_write_kernel(const plan_args 
         return;
     }
     const int t1 = min(r.fresh, max(a.T - r.start, 0)), e1 = plan_entries(r, a.shift);
-    if (from == 0 && a.row_slots) plan_write_row_slot(a, st, r, b);
-    plan_write_tokens<4>(a, st, r, b, from, step, t1);
+    if (from == 0) plan_write_first(a, st, r, b);
+    plan_write_tokens<4>(a, st, r, b, from > 0 ? from : step, step, t1);
     plan_write_entries<4>(a, st, r, b, plan_first_entry(r, a.shift) + from, step, e1);
 }
 

@@ -75,7 +75,7 @@ def sample(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         return int(order[0])
     with np.errstate(invalid="ignore"):
         w = np.where(x == top, 1.0, np.exp((x - top) / np.float64(np.float32(temperature))))
-    w[x == -np.inf] = 0.0
+    w[(x == -np.inf) | (w < 1e-300)] = 0.0
     if top == np.inf:
         w[x != top] = 0.0
     keep = np.zeros(len(x), bool)

@@ -120,6 +120,19 @@ def test_rows_anywhere(ahead, ld):
     check(x, numbers(5, ahead + 1), top_k=[20] * 5, top_p=[0.8] * 5)
 
 
+@pytest.mark.parametrize("temperature", [1e-30, 1e-4, 2e-3, 0.01, 0.1, 30.0, 1e30])
+@pytest.mark.parametrize("size", [0.01, 3.0, 4000.0])
+def test_weights_of_all_sizes(temperature, size):
+    """Many tokens are kept, of which few, or all, weigh something: temperatures and values from one end to the other, with the least random numbers too."""
+    B, V = 6, 9000
+    x = (torch.randn(B, V, device="cuda", generator=torch.Generator(device="cuda").manual_seed(9)) * size).half()
+    x[4] = -x[4].abs()
+    u = [0.0, 1e-9, 0.3, 0.7, 0.0, 1.0 - 2.0 ** -24]
+    for settings in (dict(top_k=3000), dict(top_p=0.999), dict(top_k=5000, top_p=0.99), dict(min_p=1e-30), {}):
+        print(f"sample temperature={temperature} size={size} {settings}", flush=True)
+        check(x, u, temperature=[temperature] * B, **{k: [v] * B for k, v in settings.items()})
+
+
 def test_frequencies():
     """20000 draws of one row of 16 values: each count within six standard deviations of its weight's."""
     row = rows(1, 16, 2, 1.0)
