@@ -423,7 +423,9 @@ struct pa_shape {
 pa_shape shape_of(int B, int heads, int kv_heads, int64_t positions) {
     pa_shape p;
     p.rep = heads / kv_heads;
-    p.groups = (int)bs_cdiv(p.rep, PA_HEADS);
+    // One head to a unit where that leaves at most a workgroup per CU and nothing is cut: heads that share rows then read them again from the L2, side by side.  (us, heads together / one by
+    // one: 1 request of 385, 32 heads on 8, 8.7 / 8.3, 64 on 8 9.8 / 8.2; 8 of 300 to 500, 32 on 8, 9.7 / 9.5; but 32 of 10 to 500 12.3 / 24.0.)
+    p.groups = positions <= PA_WHOLE && (int64_t)B * heads <= 256 ? p.rep : (int)bs_cdiv(p.rep, PA_HEADS);
     p.per_unit = (int)bs_cdiv(p.rep, p.groups);
     p.units = kv_heads * p.groups;
     // Workgroups that further parts add: with few first ones all together are one per CU, with more two (as many as fit beside each other), beyond that enough of them

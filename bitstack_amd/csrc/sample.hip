@@ -367,14 +367,30 @@ __global__ __launch_bounds__(SP_THREADS) void sample_rows_kernel(const sp_args a
         kept = mine > SP_NONE ? my_sum * weight(mine) : 0.0;
         sums_are_there = !rule.by_sum;
     }
-    const bool few = rule.by_count && rule.k <= 4 * a.spans;
+    // A small k is found in a list of the values from the k-th largest of some disjoint parts' largest on: the quarters of the spans, or, in short rows, what a thread reads.  At least
+    // twice as many parts as k: then about 0.7 values per part are in the list.  (us, so / with as many parts as k, and counting where they are fewer: 11 rows of 3693, k to 100 with top-p, 15.1 / 33.0; 49 of 10338
+    // 16.8 / 38.7; 49 of 3000, k alone, 14.8 / 20.9; 48 of 32000 with top-p 16.1 both.)
+    const int pieces = (a.V + 7) / 8;
+    const bool quarters_do = rule.k <= 2 * a.spans, few = rule.by_count && (quarters_do || rule.k <= min(256, min(pieces, SP_THREADS) / 2));
     uint32_t counted = 0, border_ties = 0;       // tokens down to the border and with its key, and the weights that stay, where they have been counted
     double counted_sum = 0.0;
     int from = SP_NONE + 1, first = 0, end = a.spans;          // no key below it is kept; the spans that are summed
     if (!sums_are_there) {
         // the lowest key that min-p leaves
         const int least = rule.least > 0.f ? key_from((double)rule.least, log2f(rule.least)) : top == SP_INFINITE ? top : SP_NONE + 1;
-        if (few) {                               // the k-th largest of the largest keys of every 128 values, or of the spans, bit by bit
+        if (few) {                               // the k-th largest of the largest keys of every 128 values, of the spans, or of the threads, bit by bit
+            uint16_t *const thread_key = reinterpret_cast<uint16_t *>(bins);
+            if (!quarters_do) {
+                float most = -INFINITY;
+#pragma unroll 1
+                for (int i = tid; i < pieces; i += SP_THREADS) {
+                    const half8_t v = row.values(i);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) most = fmaxf(most, (float)v[e]);             // (a NaN is no number's larger one)
+                }
+                thread_key[tid] = (uint16_t)sp_key((half_t)most);
+                __syncthreads();
+            }
             if (wave == 0) {
                 const uint16_t *all = reinterpret_cast<const uint16_t *>(quarter_keys);
                 int kth = 0;
@@ -391,8 +407,9 @@ __global__ __launch_bounds__(SP_THREADS) void sample_rows_kernel(const sp_args a
                     }
                 };
                 auto quarter_at = [&](int i) { return i < 4 * a.spans ? (int)all[i] : 0; };
-                if (4 * a.spans <= 256) search(sp_count<4>(), quarter_at);
-                else if (rule.k <= a.spans) search(sp_count<SP_SPANS / 64>(), [&](int i) { return i < a.spans ? keys[i] : 0; });
+                if (!quarters_do) search(sp_count<SP_WAVES>(), [&](int i) { return (int)thread_key[i]; });
+                else if (4 * a.spans <= 256) search(sp_count<4>(), quarter_at);
+                else if (2 * rule.k <= a.spans) search(sp_count<SP_SPANS / 64>(), [&](int i) { return i < a.spans ? keys[i] : 0; });
                 else search(sp_count<4 * SP_SPANS / 64>(), quarter_at);
                 floor_key = max(SP_NONE + 1, kth);
             }

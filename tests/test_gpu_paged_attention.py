@@ -111,6 +111,12 @@ def test_groups_of_heads(heads, kv, d):
     check(heads, kv, d, 32, [1, 40, 700, 0, 1111], seed=kv)
 
 
+@pytest.mark.parametrize("heads,kv", [(1, 1), (3, 1), (8, 8), (14, 2), (17, 1), (40, 2), (64, 8)])
+@pytest.mark.parametrize("rows", [1, 4, 20])
+def test_groups_of_heads_in_short_tables(heads, kv, rows):
+    check(heads, kv, 128, 16, [(500, 1, 40, 0, 333)[b % 5] + b // 5 for b in range(rows)], seed=rows)
+
+
 # one long request, long and short ones together, many (more than one workgroup has threads), very many short ones
 @pytest.mark.parametrize("heads,kv,d,page,lengths", [
     (32, 8, 128, 16, [385]), (32, 8, 128, 16, [5000]), (64, 8, 128, 256, [20000, 3]), (8, 8, 64, 32, [33000]), (4, 1, 128, 128, [1, 70000, 700]),

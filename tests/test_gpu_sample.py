@@ -144,6 +144,17 @@ def test_frequencies():
     assert bool(((count - n * p).abs() <= 6 * (n * p * (1 - p)).sqrt()).all())
 
 
+@pytest.mark.parametrize("V", [17, 600, 1025, 4000, 10338, 50257])
+def test_top_k_at_the_ends_of_its_ways(V):
+    """k around twice the spans, half the pieces of eight values, and the sizes of the lists."""
+    spans, pieces = -(-V // 512), -(-V // 8)
+    ks = sorted({k for n in (1, spans // 2, spans, 2 * spans, pieces // 2, 256, 512, 1024) for k in (n - 1, n, n + 1) if 1 <= k <= V})
+    x = rows(len(ks), V, V)
+    check(x, numbers(len(ks), 3), top_k=ks, temperature=[1.5] * len(ks))
+    check(x, numbers(len(ks), 4), top_k=ks, top_p=[0.97] * len(ks))
+    check(x.round(), numbers(len(ks), 5), top_k=ks, top_p=[0.9] * len(ks), temperature=[3.0] * len(ks))
+
+
 @pytest.mark.parametrize("V", [3000, 33000])
 def test_settings_together(V):
     """min-p drops tokens that top-p's sum still counts: every pair of settings, and all of them, with k below and above what a list holds."""
