@@ -15,7 +15,9 @@
 //   sample_rows_kernel     a row per workgroup: the largest; without top-k and top-p the span in which the random number falls, from the sums alone; otherwise the
 //                          border, then the kept weights of the spans that reach it
 //
-// What bounds the second one is a chain of latencies, and instructions that come from memory the first time: they are the larger part of a short call, so
+// What bounds the first is its 64-bit operations where sums are wanted (200 rows of 50257: 12.3 us, 89 % of the vector units' cycles; 20 MB), otherwise the launch (2.5 us for a row of 32000).
+// What bounds the second one is a chain of latencies (11 us for a row of 32000 with k 50 and top-p, 17 for top-p alone, 44 where it leaves most of 128256 tokens: counting 9,
+// the keys' sums 10, the spans' 16), and instructions that come from memory the first time: they are the larger part of a short call, so
 // loops over a piece's eight values stay loops there, and all kinds of rows draw in one place.
 #include "lanes.h"
 
