@@ -593,6 +593,8 @@ class SyntheticLlamaDecoder:
             raise ValueError("prefill_paged needs heads of 128")
         if n < 1 or n > self.max_len:
             raise ValueError("prompt length must be in 1..max_len")
+        if not 0 <= row < cache.rows:
+            raise ValueError(f"the cache has rows 0..{cache.rows - 1}")
         at = torch.arange(cache.rows, device=self.dev) == row
         plan = cache.plan(n * at.int(), n, released=at)
         x = self.embed.index_select(0, prompt.reshape(-1))
@@ -619,12 +621,16 @@ class SyntheticLlamaDecoder:
     def step_paged(self, cache: PagedCache, new_tokens=None, released=None, uniform=None, **sampling):
         """One token for every request of the cache: cache.token at its next position.  new_tokens (int32 [rows]; None: all) is 0 for rows
         that are idle, `released` [rows] gives the pages of finished ones back.  The next tokens, greedy or with `uniform` [rows] drawn as sample_hip
-        does with temperature, top_k, top_p, min_p, go to cache.token for requests that got a slot.  Returns the plan; self.logits holds the logits."""
+        does with temperature, top_k, top_p, min_p, go to cache.token for requests that got a slot: not those at max_len, or without a page (plan.granted).
+        Returns the plan; self.logits holds the logits."""
         s, eps = self.s, self.s.rms_eps
         if self._groups is None:
             self._build_groups()
         if new_tokens is None:
             new_tokens = torch.ones_like(cache.lengths)
+        if self.max_len % cache.page_size:                                 # (the last page has room for more than the RoPE tables)
+            room = cache.lengths < self.max_len
+            new_tokens = new_tokens * (room if released is None else room | released.bool())
         plan = cache.plan(new_tokens, cache.rows, released=released)
         x = self.embed.index_select(0, cache.token)
         for L, grp in enumerate(self._groups):

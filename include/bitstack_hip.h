@@ -454,7 +454,8 @@ int bs_argmax_advance_f16(const void *x, int64_t *out, int64_t *pos, int B, int 
  *   row_slots [B]   slot of every request's first token, -1 without one: the
  *                   slots of a decode step whose rows are the requests, idle ones
  *                   among them (may be NULL)
- * Pages that go back in a call are not taken in the same one.  Negative lengths
+ * Pages that go back in a call are not taken in the same one; all of a released
+ * row's go back, so a row that names pages of another must not be released.  Negative lengths
  * and counts are taken as 0, lengths beyond the row as a full one, a free_state
  * that no ring has as an empty ring.  Deterministic.  Many tokens need scratch
  * (bs_page_plan_workspace_bytes, 16-byte aligned; 0: none).  At most 65536

@@ -131,6 +131,29 @@ def test_a_pool_that_runs_out():
     assert cache.lengths.tolist() == [17, 0]               # three pages are needed, one is free
 
 
+@pytest.mark.parametrize("max_len", [40, 48])
+def test_up_to_the_last_position(max_len):
+    """A request goes to the end of the RoPE tables, inside a page or at its end, and stays there; one that is given back there starts anew."""
+    dec, alone = decoder(max_len=max_len), decoder(max_len=max_len)
+    cache = PagedCache(dec, 2, 8)
+    _, logits = dec.prefill_paged(cache, 1, prompt(max_len - 2, 3))
+    alone.prefill(prompt(max_len - 2, 3))
+    cache.token[1] = logits.argmax()
+    live = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    for i in range(4):
+        token = int(cache.token[1])
+        plan = dec.step_paged(cache, live)
+        assert plan.granted.tolist() == [0, int(i < 2)] and int(cache.lengths[1]) == min(max_len, max_len - 1 + i)
+        if i < 2:
+            alone.token.fill_(token)
+            alone.step_fused()
+            assert near(dec.logits[1], alone.logits[0])
+        else:
+            assert int(cache.token[1]) == token
+    plan = dec.step_paged(cache, live, released=live.bool())
+    assert plan.granted.tolist() == [0, 1] and int(cache.lengths[1]) == 1
+
+
 def test_a_captured_step():
     """step_paged() captured once and replayed: each replay is the eager step, across page ends and beside eager work."""
     eager, captured = decoder(), decoder()
@@ -179,6 +202,9 @@ def test_refusals():
         dec.prefill_paged(cache, 0, prompt(257, 0))
     with pytest.raises(ValueError):
         dec.prefill_paged(cache, 0, prompt(0, 0))
+    for row in (-1, 2):
+        with pytest.raises(ValueError, match="rows"):
+            dec.prefill_paged(cache, row, prompt(3, 0))
     with pytest.raises(RuntimeError):
         dec.step_paged(PagedCache(dec, 2, 8, page_size=24))
     narrow = SyntheticLlamaDecoder(LlamaShape(layers=1, hidden=256, intermediate=512, heads=4, kv_heads=2, vocab=1000), CONFIG, 64, "cuda")
