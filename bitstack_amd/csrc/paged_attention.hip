@@ -28,8 +28,6 @@ namespace {
 constexpr int PA_TILE = 16, PA_HEADS = 16;       // positions of a tile; query heads of a unit
 // (us with 4 waves / 8: 48 requests of 1 to 4096, 32 heads on 8, 83.9 / 72.6; 2 of 80000, 128 on 8, 128.8 / 112.0; 16 of 100 to 8000, 32 on 2, 24.0 / 23.7; 1 of 700 11.2 / 11.7)
 constexpr int WAVES = 8, THREADS = WAVES * 64;
-constexpr int PA_LEAST = 8;                      // tiles of a part, at least
-constexpr int PA_WHOLE = 512;                    // tables of up to so many positions are not cut
 
 struct pa_args {
     const half_t *qkv, *cosv, *sinv;
@@ -39,7 +37,7 @@ struct pa_args {
     half_t *out;
     int32_t *heads_of;                           // workspace: {first further part, further parts} of every request
     float *part;                                 // ... and what the parts leave
-    int ldqkv, B, heads, kv_heads, groups, per_unit, max_pos, shift, max_pages, pool, parts;
+    int ldqkv, B, heads, kv_heads, groups, per_unit, max_pos, shift, max_pages, pool, parts, least;
 };
 
 // positions that the cache holds of a request (without its own): 0 for a length that is none
@@ -88,7 +86,7 @@ __global__ __launch_bounds__(THREADS) void attention_paged_kernel(const pa_args 
         int all = 0;
         for (int i = tid; i < a.B; i += THREADS) all += pa_tiles(pa_cached(a, a.lengths[i]));
         all = pa_sum(all, sums);
-        most = max(PA_LEAST, (all + a.parts - 1) / a.parts);
+        most = max(a.least, (all + a.parts - 1) / a.parts);
         if (first_part) further = pa_further(pa_tiles(pa_cached(a, a.lengths[b])), most);
     }
     if (!first_part || further > 0) {            // numbers of the further parts: a running sum over the requests
@@ -422,21 +420,27 @@ __global__ __launch_bounds__(D * G * H) void attention_paged_merge_kernel(const 
 }
 
 struct pa_shape {
-    int rep, groups, per_unit, units, parts;
+    int rep, groups, per_unit, units, parts, least;        // (least: tiles of a part)
 };
 pa_shape shape_of(int B, int heads, int kv_heads, int64_t positions) {
     pa_shape p;
     p.rep = heads / kv_heads;
+    // Tables that are not cut: a few workgroups' to 768 positions, more ones' to 1024.  (us, cut / whole: 1 request of 700, 32 heads on 8, 11.8 / 10.9, of 900 11.8 / 12.7; 16 of up to 800 15.0 / 12.6, 16 of up to
+    // 1500 18.3 / 20.0; 48 of up to 1000 29.2 / 23.5, one of 1000 among 47 of 100 15.3 / 14.7, up to 1500 38.6 / 39.0; 256 of up to 1000 101.7 / 97.1.)
+    const int64_t together = (int64_t)B * kv_heads * bs_cdiv(p.rep, PA_HEADS);
+    const bool whole = positions <= (together <= 64 ? 768 : 1024);
     // One head to a unit where that leaves at most a workgroup per CU and nothing is cut: heads that share rows then read them again from the L2, side by side.  (us, heads together / one by
     // one: 1 request of 385, 32 heads on 8, 8.7 / 8.3, 64 on 8 9.8 / 8.2; 8 of 300 to 500, 32 on 8, 9.7 / 9.5; but 32 of 10 to 500 12.3 / 24.0.)
-    p.groups = positions <= PA_WHOLE && (int64_t)B * heads <= 256 ? p.rep : (int)bs_cdiv(p.rep, PA_HEADS);
+    p.groups = whole && (int64_t)B * heads <= 256 ? p.rep : (int)bs_cdiv(p.rep, PA_HEADS);
     p.per_unit = (int)bs_cdiv(p.rep, p.groups);
     p.units = kv_heads * p.groups;
     // Workgroups that further parts add: with few first ones all together are one per CU, with more two (as many as fit beside each other), beyond that enough of them
     // to even out unequal lengths.  (us at 256 in all / 512 in all / 768 more: 1 request of 40000, 32 heads on 8 KV heads, 35.3 / 36.7 / 41.3; 2 of 80000, 64 on 8, 107 / 112 / 112; 16 of 100 to
     // 8000 63.1 / 57.6 / 60.8; with 256 more / 768 more 48 of 1 to 4096 89 / 75.7.)
     const int64_t first = (int64_t)B * p.units, further = first <= 64 ? 256 - first : first <= 256 ? 512 - first : 768;
-    p.parts = positions <= PA_WHOLE ? 0 : (int)(further / p.units > 1 ? further / p.units : 1);
+    p.parts = whole ? 0 : (int)(further / p.units > 1 ? further / p.units : 1);
+    // Shorter parts where few workgroups leave room: 4 tiles instead of 8 12.0 us -> 11.3 for 1 request of 1000; but 47 of 100 and one of 1000 15.3 -> 21.5.
+    p.least = first <= 64 ? 4 : 8;
     return p;
 }
 
@@ -472,7 +476,7 @@ int bs_launch_attention_paged(const half_t *qkv, int ldqkv, half_t *kpages, half
     const pa_shape p = shape_of(B, heads, kv_heads, (int64_t)max_pages << shift);
     const int64_t workgroups = (int64_t)(B + p.parts) * p.units;          // (at most 2^22 and the parts: 2^32 threads hold them)
     pa_args a = {qkv, cos, sin, kpages, vpages, lengths, slots, out, (int32_t *)workspace, (float *)((char *)workspace + bs_cdiv(8ll * B, 16) * 16),
-                 ldqkv, B, heads, kv_heads, p.groups, p.per_unit, max_pos, shift, max_pages, pool, p.parts};
+                 ldqkv, B, heads, kv_heads, p.groups, p.per_unit, max_pos, shift, max_pages, pool, p.parts, p.least};
     if (head_dim == 128)
         return p.per_unit > 8 ? launch<128, 16>(a, table, workgroups, s) : p.per_unit > 4 ? launch<128, 8>(a, table, workgroups, s) : p.per_unit > 2 ? launch<128, 4>(a, table, workgroups, s)
              : p.per_unit > 1 ? launch<128, 2>(a, table, workgroups, s) : launch<128, 1>(a, table, workgroups, s);

@@ -101,8 +101,17 @@ EDGES = [1, 2, 0, 15, 16, 17, 18, 31, 33, 64, 127, 129, 130, 255, 257, 511, 513,
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("page", [16, 64, 1024])
 @pytest.mark.parametrize("turned", [False, True])
-def test_lengths_at_the_ends_of_tiles_and_pages(d, page, turned):
-    check(8, 2, d, page, EDGES, turned=turned, idle=(5, 9))
+@pytest.mark.parametrize("cut", [False, True])
+def test_lengths_at_the_ends_of_tiles_and_pages(d, page, turned, cut):
+    """Short tables are not cut, longer ones are, whatever the lengths."""
+    check(8, 2, d, page, EDGES, turned=turned, idle=(5, 9), max_pages=1 + 1024 // page if cut else None)
+
+
+@pytest.mark.parametrize("heads,kv", [(8, 8), (6, 2), (12, 1), (32, 4), (20, 1)])
+@pytest.mark.parametrize("longest", [767, 768, 769, 1023, 1024, 1025])
+@pytest.mark.parametrize("rows", [1, 3, 40])
+def test_tables_around_the_longest_that_are_not_cut(heads, kv, longest, rows):
+    check(heads, kv, 128, 16, [longest if b == 0 else (37 * b) % longest for b in range(rows)], seed=rows)
 
 
 @pytest.mark.parametrize("heads,kv", [(1, 1), (2, 1), (3, 1), (5, 1), (8, 8), (6, 2), (14, 2), (16, 1), (17, 1), (32, 1), (40, 2), (99, 3), (64, 8)])
