@@ -722,8 +722,8 @@ __global__ __launch_bounds__(SP_THREADS) void sample_rows_kernel(const sp_args a
         }
         const bool reached = at_first != 0x7fffffff;
         __syncthreads();
-        // (not in the spans that were summed, or in front of them: then all)
-        if (!whole && (!reached || (s == first && first > 0 && span_before > goal))) {
+        // (not in the spans that were summed, or in front of the first of them that has a kept token: then all)
+        if (!whole && (!reached || (first > 0 && span_before > goal))) {
             first = 0;
             end = a.spans;
             continue;
