@@ -6,8 +6,9 @@
 //                                       in two fp16 terms too.  Up to eight heads leave columns free: those are the second terms', and a
 //                                       score is the sum of two lanes; with more heads it is a product of its own.  (Rounded to fp16 the query alone put the
 //                                       result's error against 64 bits from 2.0e-4, the rounding of the result, to 3.4e-4.)
-//   output  O[dim, head] += V^T P       16x16x32, four positions twice: P is split into two fp16 terms, p = hi + lo to 2^-22, and the eight
-//                                       k slots of a lane hold {hi, lo} against {v, v}: the weights keep the precision of fp32 numbers
+//   output  O[dim, head] += V^T P       16x16x32, four positions twice: P is split into two fp16 terms and the eight k slots of a lane hold {hi, lo}
+//                                       against {v, v}.  The largest weight goes in as 2^15, as far up as fp16 lets it: p = hi + lo to 2^-22 of itself down to weights
+//                                       of 2^-18 of the largest, below that to 2^-40 of the largest (as 1 it would be 2^-25: a weight of e^-16 was off by 6 %)
 // A lane of the scores holds positions 4 (l / 16) + i of head l % 16, which is what the second product wants of P; V needs no transposition
 // either: a lane loads dimensions W r .. W r + W - 1 (r = l % 16, W = D / 16) of its four positions, and product j takes element j of each, so that its
 // row r is dimension W r + j.  Maximum, sum and output are fp32, in base 2; K of the next tile of 16 positions is requested behind the scores, V behind the
@@ -26,6 +27,7 @@
 namespace {
 
 constexpr int PA_TILE = 16, PA_HEADS = 16;       // positions of a tile; query heads of a unit
+constexpr float PA_UP = 32768.f;                 // what the weights are multiplied by on their way into fp16
 // (us with 4 waves / 8: 48 requests of 1 to 4096, 32 heads on 8, 83.9 / 72.6; 2 of 80000, 128 on 8, 128.8 / 112.0; 16 of 100 to 8000, 32 on 2, 24.0 / 23.7; 1 of 700 11.2 / 11.7)
 constexpr int WAVES = 8, THREADS = WAVES * 64;
 
@@ -255,8 +257,8 @@ __global__ __launch_bounds__(THREADS) void attention_paged_kernel(const pa_args 
         for (int i = 0; i < 4; i++) {
             p[i] = __builtin_amdgcn_exp2f(p[i] - mn);
             sum += p[i];
-            p8[i] = (half_t)p[i];
-            p8[i + 4] = (half_t)(p[i] - (float)p8[i]);
+            p8[i] = (half_t)(p[i] * PA_UP);
+            p8[i + 4] = (half_t)__builtin_fmaf(p[i], PA_UP, -(float)p8[i]);
         }
         l = l * r + sum;
         if (__any(r != 1.f)) {
@@ -338,7 +340,7 @@ __global__ __launch_bounds__(THREADS) void attention_paged_kernel(const pa_args 
         for (int i = 0; i < 4; i++)              // row 4 g + i of product j is dimension W (4 g + i) + j
 #pragma unroll
             for (int j = 0; j < W; j += 4)
-                *reinterpret_cast<float4_t *>(&wacc[r16][wave][W * (4 * g + i) + j]) = (float4_t){acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]};
+                *reinterpret_cast<float4_t *>(&wacc[r16][wave][W * (4 * g + i) + j]) = (float4_t){acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]} * (1.f / PA_UP);
     }
     __syncthreads();
     const int64_t mine = ((int64_t)(part == 0 ? b : a.B + place + part - 1) * a.kv_heads + hk) * rep + hg * a.per_unit;

@@ -1,0 +1,46 @@
+"""attention_paged_hip at the ends of the numbers: weights far below the largest.
+
+Bounds as in test_gpu_paged_attention.py, but for what the second fp16 term of a weight cuts off: the largest weight is held as 2^15, and half of the smallest
+step of fp16, 2^-25, is then 2^-40 of it per position."""
+import pytest
+import torch
+
+import paged_oracle as oracle
+from test_gpu_paged_attention import Case
+
+pytestmark = pytest.mark.gpu
+
+def rows_of(c, b):
+    """(keys, values) of request b in 64 bits, the step's own among them; its queries."""
+    n = int(c.lengths[b])
+    x = c.qkv[b].view(-1, c.d)
+    q, own = oracle.rotate(x[:c.heads], c.cos[n - 1], c.sin[n - 1]), oracle.rotate(x[c.heads:c.heads + c.kv], c.cos[n - 1], c.sin[n - 1])
+    keys, values = (torch.cat([t[r] for r in c.rows[b]], 1).transpose(0, 1)[:n - 1].double() for t in (c.kpages, c.vpages))
+    return torch.cat([keys, own[None]]), torch.cat([values, x[None, c.heads + c.kv:].double()]), q
+
+
+def near(c, out, b, want, spread, size, lost):
+    e = 2.0 ** -16 * size + 2.0 ** -20
+    bound = 2.0 ** -11 * want.abs() + 2.0 ** -25 + (2 * e + 2.0 ** -14) * spread + lost * 2.0 ** -15      # (`lost` is 2^-25 per position)
+    off = (out[b].view(c.heads, c.d).double() - want).abs()
+    assert bool((off <= bound).all()), (b, float((off / bound).max()))
+
+
+@pytest.mark.parametrize("heads,kv,d", [(8, 2, 128), (4, 4, 64), (16, 1, 128), (20, 1, 64), (1, 1, 128)])
+@pytest.mark.parametrize("n", [600, 5000, 40000])
+@pytest.mark.parametrize("ahead", [9.0, 14.0, 16.0, 18.0, 22.0])
+@pytest.mark.parametrize("sinks", [1, 8])
+def test_small_weights_are_not_lost(heads, kv, d, n, ahead, sinks):
+    """One position far ahead whose v is 0 (or one in each of the first eight tiles), all others small and alike: the result is the small ones' alone."""
+    print(f"sinks heads={heads} kv={kv} d={d} n={n} ahead={ahead} sinks={sinks}", flush=True)
+    c = Case(heads, kv, d, 16, [n], filler=0.0)
+    g = torch.Generator(device="cuda").manual_seed(n)
+    c.qkv.zero_()
+    c.qkv[:, :heads * d].view(1, heads, d)[:, :, 0] = 8.0
+    c.kpages.zero_()
+    c.vpages.copy_(0.5 + torch.rand(c.vpages.shape, device="cuda", generator=g))
+    for t in range(sinks):
+        c.kpages[c.rows[0][t], :, 0, 0] = ahead * d ** 0.5 / 8.0
+        c.vpages[c.rows[0][t], :, 0] = 0.0
+    keys, values, q = rows_of(c, 0)
+    near(c, c.run(), 0, *oracle.attend(q, keys, values, kv))
