@@ -523,7 +523,7 @@ extern "C" int bs_attention_paged_f16(const void *qkv, int ldqkv, void *kpages, 
 }
 
 static int sample_shape(int B, int V) {
-    return B < 0 || B > 1 << 20 || V < 1 || V > 1 << 18 || (int64_t)B * ((V + 511) / 512) > 1 << 24 ? BS_ERR_SHAPE : BS_OK;
+    return B < 0 || B > 1 << 20 || V < 1 || V > 1 << 18 || (int64_t)B * V > 1ll << 33 ? BS_ERR_SHAPE : BS_OK;
 }
 
 extern "C" int64_t bs_sample_workspace_bytes(int B, int V) {

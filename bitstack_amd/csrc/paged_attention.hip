@@ -3,9 +3,10 @@
 //
 // A unit is the up to 16 query heads of one KV head that share its rows: they are the columns of both products, so K and V are read once.
 //   scores  S[position, head] = K q     16x16x32, K rows as loaded (a lane: position l % 16, dimensions 32 c + 8 (l / 16) ..); the rotated query
-//                                       in two fp16 terms too.  Up to eight heads leave columns free: those are the second terms', and a
-//                                       score is the sum of two lanes; with more heads it is a product of its own.  (Rounded to fp16 the query alone put the
-//                                       result's error against 64 bits from 2.0e-4, the rounding of the result, to 3.4e-4.)
+//                                       in two fp16 terms too, x / 2 = hi + lo / 2^11: half of it, as a rotation goes up to sqrt(2) times the largest fp16 number, and the rest
+//                                       enlarged, so that it is one of fp16's full numbers whatever x is (2^-22 of x).  Up to eight heads leave columns free: those are the second
+//                                       terms', and a score is the sum of two lanes; with more heads it is a product of its own.  (Rounded to fp16 the query alone put
+//                                       the result's error against 64 bits from 2.0e-4, the rounding of the result, to 3.4e-4.)
 //   output  O[dim, head] += V^T P       16x16x32, four positions twice: P is split into two fp16 terms and the eight k slots of a lane hold {hi, lo}
 //                                       against {v, v}.  The largest weight goes in as 2^15, as far up as fp16 lets it: p = hi + lo to 2^-22 of itself down to weights
 //                                       of 2^-18 of the largest, below that to 2^-40 of the largest (as 1 it would be 2^-25: a weight of e^-16 was off by 6 %)
@@ -27,7 +28,7 @@
 namespace {
 
 constexpr int PA_TILE = 16, PA_HEADS = 16;       // positions of a tile; query heads of a unit
-constexpr float PA_UP = 32768.f;                 // what the weights are multiplied by on their way into fp16
+constexpr float PA_UP = 32768.f, PA_REST = 2048.f;         // what the weights, and the second terms of the queries, are multiplied by on their way into fp16
 // (us with 4 waves / 8: 48 requests of 1 to 4096, 32 heads on 8, 83.9 / 72.6; 2 of 80000, 128 on 8, 128.8 / 112.0; 16 of 100 to 8000, 32 on 2, 24.0 / 23.7; 1 of 700 11.2 / 11.7)
 constexpr int WAVES = 8, THREADS = WAVES * 64;
 
@@ -195,12 +196,15 @@ __global__ __launch_bounds__(THREADS) void attention_paged_kernel(const pa_args 
         if (h < HP + 1) {
             const float c = (float)a.cosv[(int64_t)pos * D2 + i], sn = (float)a.sinv[(int64_t)pos * D2 + i];
             const float x = (float)pa[e] * c - (float)pb[e] * sn, y = (float)pb[e] * c + (float)pa[e] * sn;
-            half_t *to = h < HP ? qrot[0][h] : knew;
-            to[i] = (half_t)x;
-            to[i + D2] = (half_t)y;
             if (h < HP) {
-                qrot[1][h][i] = (half_t)(x - (float)(half_t)x);
-                qrot[1][h][i + D2] = (half_t)(y - (float)(half_t)y);
+                const half_t x0 = (half_t)(0.5f * x), y0 = (half_t)(0.5f * y);
+                qrot[0][h][i] = x0;
+                qrot[0][h][i + D2] = y0;
+                qrot[1][h][i] = (half_t)((0.5f * x - (float)x0) * PA_REST);
+                qrot[1][h][i + D2] = (half_t)((0.5f * y - (float)y0) * PA_REST);
+            } else {
+                knew[i] = (half_t)x;
+                knew[i + D2] = (half_t)y;
             }
         } else if (h < HP + 2) {
             vnew[i] = pa[e];
@@ -223,20 +227,23 @@ __global__ __launch_bounds__(THREADS) void attention_paged_kernel(const pa_args 
 #pragma unroll
         for (int c = 0; c < NC; c++)
             q8[e][c] = column < HP ? *reinterpret_cast<const half8_t *>(&qrot[HP > 8 ? e : r16 >> 3][column < HP ? column : 0][32 * c + 8 * g]) : (half8_t)(half_t)0;
-    const float scale2 = (D == 128 ? 0.08838834764831845f : 0.125f) * 1.4426950408889634f;    // log2(e) / sqrt(D)
+    const float scale2 = (D == 128 ? 0.17677669529663689f : 0.25f) * 1.4426950408889634f;     // 2 log2(e) / sqrt(D): the queries' terms are of half of them
+    const float term = TERMS == 1 && r16 >= 8 ? scale2 / PA_REST : scale2;     // (of this lane's column)
     float m = -INFINITY, l = 0.f;                // of head l % 16; the sum over this lane's positions only
     float4_t acc[W];
 #pragma unroll
     for (int j = 0; j < W; j++) acc[j] = (float4_t)0.f;
-    auto scores = [&]() {
-        float4_t s = (float4_t)0.f;
+    auto scores = [&]() {                        // log2(e) / sqrt(D) q k
+        float4_t s = (float4_t)0.f, rest = (float4_t)0.f;
 #pragma unroll
-        for (int e = 0; e < TERMS; e++)
+        for (int c = 0; c < NC; c++) {
+            s = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8[c], q8[0][c], s, 0, 0, 0);
+            if (TERMS == 2) rest = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8[c], q8[TERMS - 1][c], rest, 0, 0, 0);
+        }
 #pragma unroll
-            for (int c = 0; c < NC; c++) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8[c], q8[e][c], s, 0, 0, 0);
-        if (TERMS == 1) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) s[i] += eight_on(s[i]);
+        for (int i = 0; i < 4; i++) {
+            const float one = s[i] * term;
+            s[i] = TERMS == 1 ? one + eight_on(one) : __builtin_fmaf(rest[i], scale2 / PA_REST, one);
         }
         return s;
     };
@@ -244,7 +251,7 @@ __global__ __launch_bounds__(THREADS) void attention_paged_kernel(const pa_args 
         float p[4], mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            p[i] = 4 * g + i < valid ? s[i] * scale2 : -INFINITY;
+            p[i] = 4 * g + i < valid ? s[i] : -INFINITY;
             mx = fmaxf(mx, p[i]);
         }
         mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
@@ -311,7 +318,7 @@ __global__ __launch_bounds__(THREADS) void attention_paged_kernel(const pa_args 
             auto add = [&](const float4_t s, int valid) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float w = __shfl(__builtin_amdgcn_exp2f(s[i] * scale2 - m), (lane & 48) | h, 64);
+                    const float w = __shfl(__builtin_amdgcn_exp2f(s[i] - m), (lane & 48) | h, 64);
 #pragma unroll
                     for (int e = 0; e < W; e++)
                         if (4 * g + i < valid) o[e] += w * (float)v8[i][e];

@@ -495,8 +495,8 @@ int bs_rope_store_paged_f16(void *q, int ldq, void *q_out, int ldq_out, const vo
  * are left out.  Requests may share pages that none of them writes.  Any heads per
  * KV head, head_dim 64 or 128; B <= 65536, B * heads <= 2^22 and B * max_pages *
  * page_size < 2^35.  Slots must differ; out must not overlap qkv.
- * Rotation, scores, maximum and sums in fp32; products of fp16 terms that hold a weight to
- * 2^-22, or 2^-40 of the largest.
+ * Rotation, scores, maximum and sums in fp32; products of fp16 terms that hold the rotated
+ * query to 2^-22 and a weight to 2^-22, or 2^-40 of the largest.
  * Long requests are cut into parts by what the lengths are at the call, and summed
  * in order: deterministic.  Scratch: bs_attention_paged_workspace_bytes, 16-byte
  * aligned (0: none; negative: an error status).

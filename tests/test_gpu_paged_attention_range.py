@@ -1,4 +1,4 @@
-"""attention_paged_hip at the ends of the numbers: weights far below the largest.
+"""attention_paged_hip at the ends of the numbers: weights far below the largest, queries beyond fp16 after their rotation.
 
 Bounds as in test_gpu_paged_attention.py, but for what the second fp16 term of a weight cuts off: the largest weight is held as 2^15, and half of the smallest
 step of fp16, 2^-25, is then 2^-40 of it per position."""
@@ -9,6 +9,9 @@ import paged_oracle as oracle
 from test_gpu_paged_attention import Case
 
 pytestmark = pytest.mark.gpu
+
+GROUPS = [(1, 1), (2, 1), (4, 1), (8, 1), (12, 1), (20, 1), (6, 2)]
+
 
 def rows_of(c, b):
     """(keys, values) of request b in 64 bits, the step's own among them; its queries."""
@@ -44,3 +47,25 @@ def test_small_weights_are_not_lost(heads, kv, d, n, ahead, sinks):
         c.vpages[c.rows[0][t], :, 0] = 0.0
     keys, values, q = rows_of(c, 0)
     near(c, c.run(), 0, *oracle.attend(q, keys, values, kv))
+
+
+@pytest.mark.parametrize("heads,kv", GROUPS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("longest", [500, 3000])
+def test_queries_beyond_fp16(heads, kv, d, longest):
+    """Two halves of 60000 rotated by an eighth of a turn are 0 and 84853: finite, as their scores are; and queries near the smallest fp16 numbers with large keys."""
+    for scale, key in ((60000.0, 2e-4), (1e-5, 3e4)):
+        c = Case(heads, kv, d, 16, [longest, 17, 1], filler=0.0)
+        g = torch.Generator(device="cuda").manual_seed(longest + heads)
+        c.cos.fill_(0.5 ** 0.5)
+        c.sin.fill_(0.5 ** 0.5)
+        q = torch.randn(3, heads, d, device="cuda", generator=g).clamp(-1, 1) * scale
+        q[:, 0] = scale * (torch.rand(3, d, device="cuda", generator=g) < 0.5)
+        c.qkv[:, :heads * d] = q.view(3, -1).half()
+        c.qkv[:, heads * d:(heads + kv) * d] = 0.0                        # (its own key is not rounded)
+        c.kpages.copy_(torch.randn(c.kpages.shape, device="cuda", generator=g).clamp(-2, 2) * key)
+        assert scale < 1 or float(oracle.rotate(q[0], c.cos[0], c.sin[0]).abs().max()) > 65504
+        out = c.run()
+        for b in range(3):
+            keys, values, q64 = rows_of(c, b)
+            near(c, out, b, *oracle.attend(q64, keys, values, kv))
