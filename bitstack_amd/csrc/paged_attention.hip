@@ -308,33 +308,62 @@ __global__ __launch_bounds__(THREADS) void attention_paged_kernel(const pa_args 
 #pragma unroll
     for (int j = 0; j < W; j++) sum += (acc[j][0] + acc[j][1]) + (acc[j][2] + acc[j][3]);
     if (__builtin_expect(__any(sum != sum), 0)) {
-        // An infinite v: times a second term of zero or below it, or a masked weight, it is NaN in the output product.  The wave's
-        // positions once more, head by head, each weight as one fp32 number: a lane owns dimensions W r16 .. W r16 + W - 1.
+        // An infinite k or v: times a second term of zero or of the other sign, or a masked weight, it is NaN in the products, and so is the weight of a score of -inf next to
+        // a maximum of -inf.  The wave's positions twice more (maximum, then sums), head by head, query and weights as one fp32 number each: a lane has the score of position
+        // r16, dimensions 32 c + 8 g .., and owns dimensions W r16 .. W r16 + W - 1 of the output.  A score of -inf weighs nothing, one of +inf or NaN makes its head NaN.
 #pragma unroll 1
-        for (int h = 0; h < HP; h++) {
-            float o[W];
-#pragma unroll
-            for (int e = 0; e < W; e++) o[e] = 0.f;
-            auto add = [&](const float4_t s, int valid) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float w = __shfl(__builtin_amdgcn_exp2f(s[i] - m), (lane & 48) | h, 64);
-#pragma unroll
-                    for (int e = 0; e < W; e++)
-                        if (4 * g + i < valid) o[e] += w * (float)v8[i][e];
+        for (int h = 0; h < nh; h++) {
+            auto each_tile = [&](auto f) {
+#pragma unroll 1
+                for (t = t_first + wave; t < t_end; t += WAVES) {
+                    id = page_of(t);
+                    if (!good(id)) continue;
+                    fetch_k(id, t);
+                    fetch_v(id, t);
+                    f(pos - t * PA_TILE);
+                }
+                if (own) {
+                    take_own();
+                    f(1);
                 }
             };
-            for (t = t_first + wave; t < t_end; t += WAVES) {
-                id = page_of(t);
-                if (!good(id)) continue;
-                fetch_k(id, t);
-                fetch_v(id, t);
-                add(scores(), pos - t * PA_TILE);
-            }
-            if (own) {
-                take_own();
-                add(scores(), 1);
-            }
+            auto score = [&]() {
+                float d = 0.f;
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    const half8_t q0 = *reinterpret_cast<const half8_t *>(&qrot[0][h][32 * c + 8 * g]), q1 = *reinterpret_cast<const half8_t *>(&qrot[1][h][32 * c + 8 * g]);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) d = __builtin_fmaf(__builtin_fmaf((float)q1[e], 1.f / PA_REST, (float)q0[e]), (float)k8[c][e], d);
+                    __builtin_amdgcn_sched_barrier(0);       // (all pieces side by side take registers, and with heads of 64 a workgroup per CU: 85 instead of 78)
+                }
+                d += __shfl_xor(d, 16, 64);
+                d += __shfl_xor(d, 32, 64);
+                return d * scale2;
+            };
+            float top = -INFINITY, sum_w = 0.f, o[W];
+            each_tile([&](int valid) {
+                const float s = score();
+                if (r16 < valid) top = fmaxf(top, s);
+            });
+#pragma unroll
+            for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+            const float from = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int e = 0; e < W; e++) o[e] = 0.f;
+            each_tile([&](int valid) {
+                const float w = r16 < valid ? __builtin_amdgcn_exp2f(score() - from) : 0.f;
+                sum_w += w;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float wi = __shfl(w, 4 * g + i, 64);
+#pragma unroll
+                    for (int e = 0; e < W; e++)
+                        if (4 * g + i < valid) o[e] += wi * (float)v8[i][e];
+                }
+            });
+#pragma unroll
+            for (int x = 1; x < 16; x <<= 1) sum_w += __shfl_xor(sum_w, x, 64);
+            if (lane == 0) { wm[h][wave] = top; wl[h][wave] = sum_w; }
 #pragma unroll
             for (int e = 0; e < W; e++) {
                 o[e] += __shfl_xor(o[e], 16, 64);

@@ -496,7 +496,8 @@ int bs_rope_store_paged_f16(void *q, int ldq, void *q_out, int ldq_out, const vo
  * KV head, head_dim 64 or 128; B <= 65536, B * heads <= 2^22 and B * max_pages *
  * page_size < 2^35.  Slots must differ; out must not overlap qkv.
  * Rotation, scores, maximum and sums in fp32; products of fp16 terms that hold the rotated
- * query to 2^-22 and a weight to 2^-22, or 2^-40 of the largest.
+ * query to 2^-22 and a weight to 2^-22, or 2^-40 of the largest.  A score of -inf (an
+ * infinite key's) weighs nothing, one of +inf or NaN makes its head's output NaN.
  * Long requests are cut into parts by what the lengths are at the call, and summed
  * in order: deterministic.  Scratch: bs_attention_paged_workspace_bytes, 16-byte
  * aligned (0: none; negative: an error status).

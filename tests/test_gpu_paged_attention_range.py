@@ -1,4 +1,4 @@
-"""attention_paged_hip at the ends of the numbers: weights far below the largest, queries beyond fp16 after their rotation.
+"""attention_paged_hip at the ends of the numbers: weights far below the largest, queries beyond fp16 after their rotation, infinite keys.
 
 Bounds as in test_gpu_paged_attention.py, but for what the second fp16 term of a weight cuts off: the largest weight is held as 2^15, and half of the smallest
 step of fp16, 2^-25, is then 2^-40 of it per position."""
@@ -69,3 +69,45 @@ def test_queries_beyond_fp16(heads, kv, d, longest):
         for b in range(3):
             keys, values, q64 = rows_of(c, b)
             near(c, out, b, *oracle.attend(q64, keys, values, kv))
+
+
+def without_weight(c, b, out):
+    """Request b against the definition where keys hold infinities: a score of -inf is a weight of 0, one of +inf or NaN makes its head NaN."""
+    keys, values, q = rows_of(c, b)
+    rep, seen = c.heads // c.kv, set()
+    for h in range(c.heads):
+        hk, got = h // rep, out[b].view(c.heads, c.d)[h]
+        s = (keys[:, hk] * q[h]).sum(1)
+        if bool(torch.isnan(s).any()) or float(s.max()) == float("inf"):
+            assert bool(torch.isnan(got).all()), (b, h)
+            seen.add("nan")
+            continue
+        stays = s > -float("inf")
+        want, spread, size, lost = oracle.attend(q[h:h + 1], keys[stays][:, hk:hk + 1], values[stays][:, hk:hk + 1], 1)
+        bound = 2.0 ** -11 * want.abs() + 2.0 ** -25 + (2 * (2.0 ** -16 * size + 2.0 ** -20) + 2.0 ** -14) * spread + lost
+        assert bool(((got.double() - want[0]).abs() <= bound[0]).all()), (b, h)
+        seen.add("number")
+    return seen
+
+
+@pytest.mark.parametrize("heads,kv", GROUPS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("longest", [300, 2500])
+def test_infinite_keys(heads, kv, d, longest):
+    """Single keys, all keys of a tile, those of a wave's every tile, and all but the step's own; the sign of a query's element decides what an infinite one does to its head."""
+    inf = float("inf")
+    c = Case(heads, kv, d, 16, [longest, 40, 129, 40, longest, 40], filler=0.0, spare=1)
+    c.qkv[:, :heads * d].view(6, heads, d)[:, :, 3].abs_().clamp_(min=0.25)        # one way for all heads ...
+    c.qkv[:, :heads * d].view(6, heads, d)[4, ::2, 3] *= -1.0                     # ... but for these: their rows are NaN
+    c.kpages[c.rows[0][0], :, 2, 3] = -inf
+    c.kpages[c.rows[0][longest // 32], :, 7, 3] = -inf
+    c.kpages[c.rows[1][0], :, :, 3] = -inf
+    for p in c.rows[2]:
+        c.kpages[p, :, :, 3] = -inf
+    c.kpages[c.rows[3][1], :, 4, 3] = float("nan")
+    c.kpages[c.rows[4][5], :, 9, 3] = -inf
+    c.kpages[c.rows[5][2], :, 7, 3] = -inf                                        # (position 39 is the step's own: nobody reads what was there)
+    out = c.run()
+    assert without_weight(c, 0, out) == {"number"} and without_weight(c, 1, out) == {"number"} and without_weight(c, 2, out) == {"number"}
+    assert without_weight(c, 3, out) == {"nan"} and without_weight(c, 5, out) == {"number"}
+    assert without_weight(c, 4, out) == ({"number", "nan"} if heads > 1 else {"nan"})
