@@ -619,15 +619,15 @@ class SyntheticLlamaDecoder:
 
     @torch.no_grad()
     def step_paged(self, cache: PagedCache, new_tokens=None, released=None, uniform=None, **sampling):
-        """One token for every request of the cache: cache.token at its next position.  new_tokens (int32 [rows]; None: all) is 0 for rows
-        that are idle, `released` [rows] gives the pages of finished ones back.  The next tokens, greedy or with `uniform` [rows] drawn as sample_hip
+        """One token for every request of the cache: cache.token at its next position.  new_tokens (int32 [rows]; None: 1 for all but the
+        released) is 0 for rows that are idle, `released` [rows] gives the pages of finished ones back.  The next tokens, greedy or with `uniform` [rows] drawn as sample_hip
         does with temperature, top_k, top_p, min_p, go to cache.token for requests that got a slot: not those at max_len, or without a page (plan.granted).
         Returns the plan; self.logits holds the logits."""
         s, eps = self.s, self.s.rms_eps
         if self._groups is None:
             self._build_groups()
         if new_tokens is None:
-            new_tokens = torch.ones_like(cache.lengths)
+            new_tokens = torch.ones_like(cache.lengths) if released is None else (~released.bool()).int()
         if self.max_len % cache.page_size:                                 # (the last page has room for more than the RoPE tables)
             room = cache.lengths < self.max_len
             new_tokens = new_tokens * (room if released is None else room | released.bool())

@@ -1,0 +1,34 @@
+"""step_paged() and prefill_paged() as a serving loop calls them: rows that are given back without a count of new tokens."""
+import pytest
+import torch
+
+from bitstack_amd.utils.llama_decode import PROJ, LlamaShape, PagedCache, SyntheticLlamaDecoder
+
+CONFIG = {f"layer.{L}.{p}": 2 for L in range(2) for p in PROJ}
+
+
+def decoder(vocab=1000, max_len=256):
+    return SyntheticLlamaDecoder(LlamaShape(layers=2, hidden=512, intermediate=1024, heads=4, kv_heads=2, vocab=vocab), CONFIG, max_len, "cuda", seed=5)
+
+
+def admit(dec, cache, *lengths):
+    for row, n in enumerate(lengths):
+        _, logits = dec.prefill_paged(cache, row, torch.randint(0, dec.s.vocab, (n,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(row)))
+        cache.token[row] = logits.argmax()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_len", [256, 250])
+@pytest.mark.parametrize("dtype", [torch.bool, torch.uint8])
+def test_released_rows_take_no_new_token(max_len, dtype):
+    """Without new_tokens: a row that gives its pages back is idle from then on, all others go on."""
+    dec = decoder(max_len=max_len)
+    cache = PagedCache(dec, 3, 40)
+    admit(dec, cache, 20, 33, 16)
+    tokens = cache.token.tolist()
+    plan = dec.step_paged(cache, released=torch.tensor([0, 1, 0], device="cuda").to(dtype))
+    assert plan.granted.tolist() == [1, 0, 1] and cache.lengths.tolist() == [21, 0, 17] and plan.row_slots.tolist()[1] == -1
+    assert cache.token.tolist()[1] == tokens[1]
+    assert cache.free_state.tolist()[1] == 40 - 2 - 2
+    plan = dec.step_paged(cache, torch.tensor([1, 1, 0], dtype=torch.int32, device="cuda"), released=torch.tensor([0, 0, 1], device="cuda").to(dtype))
+    assert plan.granted.tolist() == [1, 1, 0] and cache.lengths.tolist() == [22, 1, 0]
