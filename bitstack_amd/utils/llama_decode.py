@@ -640,7 +640,13 @@ class SyntheticLlamaDecoder:
             act = bitstack_forward_group_hip(grp["gate_up"], x, EPI_SWIGLU, rms_eps=eps)
             x = bitstack_forward_group_hip(grp["down"], act, EPI_RESIDUAL, residual=x)
         self.logits = self._head(rmsnorm_hip(x, self.final_norm, eps))
-        token = argmax_hip(self.logits) if uniform is None else sample_hip(self.logits, uniform, **sampling)
+        if uniform is not None:
+            token = sample_hip(self.logits, uniform, **sampling)
+        elif cache.rows == 1 or self.logits.shape[1] % 8 == 0:
+            token = argmax_hip(self.logits)
+        else:                                                              # (rows that do not start on 16 bytes)
+            zeros = torch.zeros(cache.rows, device=self.dev)
+            token = sample_hip(self.logits, zeros, temperature=zeros)
         torch.where(plan.granted > 0, token, cache.token, out=cache.token)
         return plan
 

@@ -1,4 +1,4 @@
-"""step_paged() and prefill_paged() as a serving loop calls them: rows that are given back without a count of new tokens."""
+"""step_paged() and prefill_paged() as a serving loop calls them: rows that are given back without a count of new tokens, vocabularies of any size."""
 import pytest
 import torch
 
@@ -32,3 +32,15 @@ def test_released_rows_take_no_new_token(max_len, dtype):
     assert cache.free_state.tolist()[1] == 40 - 2 - 2
     plan = dec.step_paged(cache, torch.tensor([1, 1, 0], dtype=torch.int32, device="cuda"), released=torch.tensor([0, 0, 1], device="cuda").to(dtype))
     assert plan.granted.tolist() == [1, 1, 0] and cache.lengths.tolist() == [22, 1, 0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [1003, 1002, 1004, 1000])
+@pytest.mark.parametrize("rows", [1, 3, 9])
+def test_greedy_with_any_vocabulary(vocab, rows):
+    dec = decoder(vocab)
+    cache = PagedCache(dec, rows, 40)
+    admit(dec, cache, *(5 + 7 * b for b in range(rows)))
+    for _ in range(3):
+        dec.step_paged(cache)
+        assert cache.token.tolist() == dec.logits.argmax(-1).tolist()
