@@ -623,6 +623,8 @@ class SyntheticLlamaDecoder:
         released) is 0 for rows that are idle, `released` [rows] gives the pages of finished ones back.  The next tokens, greedy or with `uniform` [rows] drawn as sample_hip
         does with temperature, top_k, top_p, min_p, go to cache.token for requests that got a slot: not those at max_len, or without a page (plan.granted).
         Returns the plan; self.logits holds the logits."""
+        if uniform is None and any(v is not None for v in sampling.values()):
+            raise ValueError("temperature, top_k, top_p and min_p need the random numbers `uniform`; without them the step is greedy")
         s, eps = self.s, self.s.rms_eps
         if self._groups is None:
             self._build_groups()

@@ -44,3 +44,11 @@ def test_greedy_with_any_vocabulary(vocab, rows):
     for _ in range(3):
         dec.step_paged(cache)
         assert cache.token.tolist() == dec.logits.argmax(-1).tolist()
+
+
+def test_settings_without_random_numbers_are_refused():
+    """Greedy steps have no use for them: refused before anything is changed."""
+    dec = SyntheticLlamaDecoder.__new__(SyntheticLlamaDecoder)
+    for settings in (dict(temperature=1.0), dict(top_k=4), dict(top_p=None, min_p=0.1)):
+        with pytest.raises(ValueError, match="uniform"):
+            dec.step_paged(None, **settings)
