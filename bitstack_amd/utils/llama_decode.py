@@ -599,7 +599,8 @@ class SyntheticLlamaDecoder:
         plan = cache.plan(n * at.int(), n, released=at)
         x = self.embed.index_select(0, prompt.reshape(-1))
         # the prompt attends to its own rows, which lie side by side
-        kc, vc = torch.empty(2, 1, s.kv_heads, self.max_len, d, dtype=torch.float16, device=self.dev)
+        kc, vc = torch.empty(2, 1, s.kv_heads, n, d, dtype=torch.float16, device=self.dev)
+        cos, sin = self.cos[:n], self.sin[:n]
         wide = s.heads * d, s.kv_heads * d, s.kv_heads * d
         hn = rmsnorm_hip(x, self.norm_w[0, 0], s.rms_eps)
         for L in range(s.layers):
@@ -607,7 +608,7 @@ class SyntheticLlamaDecoder:
             qkv = forward_cat_hip([lin[p] for p in PROJ[:3]], hn)
             q, k, v = qkv.split(wide, 1) if qkv is not None else (self._output(lin[p], hn) for p in PROJ[:3])
             rope_store_paged_hip(None, k, v, self.cos, self.sin, cache.kpages[L], cache.vpages[L], plan.positions, plan.slots)
-            rope_store_hip(q, k, v, self.cos, self.sin, kc, vc, n)
+            rope_store_hip(q, k, v, cos, sin, kc, vc, n)
             ctx = attention_prefill_hip(q, kc, vc, n)
             x, hn = self._sum_norm(x, self._output(lin["self_attn.o_proj"], ctx), self.norm_w[L, 1])
             act = self._silu_mul(*(self._output(lin[p], hn) for p in PROJ[4:6]))

@@ -1,4 +1,5 @@
-"""step_paged() and prefill_paged() as a serving loop calls them: rows that are given back without a count of new tokens, vocabularies of any size."""
+"""step_paged() and prefill_paged() as a serving loop calls them: rows that are given back without a count of new tokens, vocabularies of any size, prompts in a
+decoder with room for long ones."""
 import pytest
 import torch
 
@@ -44,6 +45,22 @@ def test_greedy_with_any_vocabulary(vocab, rows):
     for _ in range(3):
         dec.step_paged(cache)
         assert cache.token.tolist() == dec.logits.argmax(-1).tolist()
+
+
+@pytest.mark.gpu
+def test_a_prompt_takes_memory_by_its_length():
+    """A short prompt of a decoder with room for 64 times as many positions allocates no more than one without."""
+    peaks = []
+    for max_len in (256, 16384):
+        dec = decoder(max_len=max_len)
+        cache = PagedCache(dec, 1, 16)
+        admit(dec, cache, 100)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        admit(dec, cache, 100)
+        peaks.append(torch.cuda.max_memory_allocated() - before)
+    assert peaks[1] <= peaks[0] + (1 << 20), peaks
 
 
 def test_settings_without_random_numbers_are_refused():
