@@ -1,4 +1,5 @@
-"""attention_paged_hip at the ends of the numbers: weights far below the largest, queries beyond fp16 after their rotation, infinite keys.
+"""attention_paged_hip at the ends of the numbers: weights far below the largest, queries beyond fp16 after their rotation, infinite keys and values, and the
+builds for large pools.
 
 Bounds as in test_gpu_paged_attention.py, but for what the second fp16 term of a weight cuts off: the largest weight is held as 2^15, and half of the smallest
 step of fp16, 2^-25, is then 2^-40 of it per position."""
@@ -111,3 +112,54 @@ def test_infinite_keys(heads, kv, d, longest):
     assert without_weight(c, 0, out) == {"number"} and without_weight(c, 1, out) == {"number"} and without_weight(c, 2, out) == {"number"}
     assert without_weight(c, 3, out) == {"nan"} and without_weight(c, 5, out) == {"number"}
     assert without_weight(c, 4, out) == ({"number", "nan"} if heads > 1 else {"nan"})
+
+
+@pytest.mark.parametrize("heads,kv", GROUPS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_infinite_values_in_cut_requests(heads, kv, d):
+    """A v of infinity in a request that is cut, and in one that is not beside it: infinity in its dimension for the heads that share it, all else as without it."""
+    inf = float("inf")
+    c = Case(heads, kv, d, 16, [4000, 700, 30], filler=0.0)
+    plain = c.run()
+    for b, p, at, dim, v in ((0, 3, 5, 17, inf), (0, 240, 2, 60, -inf), (1, 20, 0, 1, inf), (2, 0, 15, 33, -inf)):
+        c.vpages[c.rows[b][p], 0, at, dim] = v
+    out, rep = c.run().view(3, heads, d), heads // kv
+    for b, dim, v in ((0, 17, inf), (0, 60, -inf), (1, 1, inf), (2, 33, -inf)):
+        assert bool((out[b, :rep, dim] == v).all()), (b, dim)
+        out[b, :rep, dim] = plain.view(3, heads, d)[b, :rep, dim]
+    # the repeated sums are fp32 in another order, where a wave takes them: 2^-14 of the weights' sum of |v|, and a rounding to fp16
+    assert bool(((out.double() - plain.view(3, heads, d).double()).abs() <= 2.0 ** -10 * plain.view(3, heads, d).double().abs() + 2.0 ** -12).all())
+
+
+@pytest.mark.parametrize("heads,kv", GROUPS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lengths", [[300, 0, 1, 47], [3000, 20, 1025]])
+def test_large_pools(heads, kv, d, lengths):
+    """Pools from 256 MiB on are read past the last-level cache: the same bits as from a small pool, nothing read of what nobody has written."""
+    c = Case(heads, kv, d, 64, lengths, turned=True)
+    before = c.kpages.clone(), c.vpages.clone()
+    small = c.run()
+    c.check(small, before)
+    pool = -(-2 ** 28 // (64 * kv * d * 4))
+    order = torch.randperm(pool, device="cuda", generator=torch.Generator(device="cuda").manual_seed(d))[:c.pool]
+    big = torch.full((2, pool, kv, 64, d), float("nan"), device="cuda", dtype=torch.float16)
+    big[0, order], big[1, order] = before
+    kpages = c.kpages
+    c.kpages, c.vpages = big[0], big[1]
+    c.table = torch.where(c.table >= 0, order[c.table.clamp(min=0).long()].int(), c.table)
+    c.slots = torch.where(c.slots >= 0, order[c.slots.clamp(min=0) // 64] * 64 + c.slots % 64, c.slots)
+    assert torch.equal(c.run().view(torch.int16), small.view(torch.int16))
+    assert torch.equal(big[0, order].view(torch.int16), kpages.view(torch.int16))
+
+
+def test_a_length_beyond_the_tables_row():
+    """... is idle by that alone: the RoPE tables go further."""
+    c = Case(8, 2, 128, 16, [100, 1000, 100])
+    c.cos, c.sin = torch.ones(2000, 64, device="cuda", dtype=torch.float16), torch.zeros(2000, 64, device="cuda", dtype=torch.float16)
+    before = c.kpages.clone(), c.vpages.clone()
+    c.lengths[0] = 63 * 16 + 1
+    out = c.run()
+    assert bool((out[0] == 0).all()) and bool((out[1:] != 0).any(1).all())
+    for pages, old in ((c.kpages, before[0]), (c.vpages, before[1])):
+        p, o = c.rows[0][99 // 16], 99 % 16
+        assert torch.equal(pages[p, :, o].view(torch.int16), old[p, :, o].view(torch.int16))
