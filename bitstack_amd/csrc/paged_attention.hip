@@ -476,7 +476,7 @@ pa_shape shape_of(int B, int heads, int kv_heads, int64_t positions) {
     // to even out unequal lengths.  (us at 256 in all / 512 in all / 768 more: 1 request of 40000, 32 heads on 8 KV heads, 35.3 / 36.7 / 41.3; 2 of 80000, 64 on 8, 107 / 112 / 112; 16 of 100 to
     // 8000 63.1 / 57.6 / 60.8; with 256 more / 768 more 48 of 1 to 4096 89 / 75.7.)
     const int64_t first = (int64_t)B * p.units, further = first <= 64 ? 256 - first : first <= 256 ? 512 - first : 768;
-    p.parts = whole ? 0 : (int)(further / p.units > 1 ? further / p.units : 1);
+    p.parts = whole ? 0 : (int)(further / p.units);        // (0 for more than 768 units, which are enough by themselves: nothing is cut, and the grid holds 2^22 of them)
     // Shorter parts where few workgroups leave room: 4 tiles instead of 8 12.0 us -> 11.3 for 1 request of 1000; but 47 of 100 and one of 1000 15.3 -> 21.5.
     p.least = first <= 64 ? 4 : 8;
     return p;
@@ -512,7 +512,7 @@ int bs_launch_attention_paged(const half_t *qkv, int ldqkv, half_t *kpages, half
                               const int32_t *lengths, const int64_t *slots, half_t *out, int B, int heads, int kv_heads, int head_dim, int max_pos,
                               int shift, int max_pages, int pool, void *workspace, hipStream_t s) {
     const pa_shape p = shape_of(B, heads, kv_heads, (int64_t)max_pages << shift);
-    const int64_t workgroups = (int64_t)(B + p.parts) * p.units;          // (at most 2^22 and the parts: 2^32 threads hold them)
+    const int64_t workgroups = (int64_t)(B + p.parts) * p.units;          // (at most 2^22 and 768: 2^32 threads hold them)
     pa_args a = {qkv, cos, sin, kpages, vpages, lengths, slots, out, (int32_t *)workspace, (float *)((char *)workspace + bs_cdiv(8ll * B, 16) * 16),
                  ldqkv, B, heads, kv_heads, p.groups, p.per_unit, max_pos, shift, max_pages, pool, p.parts, p.least};
     if (head_dim == 128)
