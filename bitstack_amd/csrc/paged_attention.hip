@@ -20,9 +20,10 @@
 // the further parts, in order.  (The further parts first: 172 us instead of 105 for two requests of 80000, the numbers that no part has leave gaps.)  Parts leave (max, sum, weighted v)
 // in the workspace, and a second launch puts them together, in order: the result does not depend on which came first.
 //
-// What bounds it is the cache's bytes, at up to 6.4 TB/s (a kernel that only reads): 2 requests of 60001 and 99991, 64 heads on 8 of 128, 655 MB, 105 us and 4.8 for the parts = 6.2 TB/s; 48 of 1 to 4096, 32 on 8, 404 MB, 74 and
-// 4.7 (5.5: unequal lengths, 51 % of the waves' time is waiting for memory, 33 % for the turn to issue); 200 of 100 to 1500, 16 on 16 of 64, 658 MB, 120 (5.5: for one head in use the vector units are busy 47 % with
-// rotating, splitting and folding).  Short requests wait for their chain: 8.3 us for one of 385, 5.3 for one of 20.
+// What bounds it is the cache's bytes, at up to 6.4 TB/s (a kernel that only reads): 2 requests of 60001 and 99991, 64 heads on 8 of 128, 655 MB, 105 us and 4.7 for the parts = 6.2 TB/s; 48 of 1 to 4096, 32 on 8, 404 MB, 74 and
+// 4.7 (5.5: unequal lengths, 51 % of the waves' time is waiting for memory, 32 % for the turn to issue); 200 of 100 to 1500, 16 on 16 of 64, 658 MB, 119 (5.5: for one head in use the vector units are busy 48 % with
+// rotating, splitting and folding).  Short requests wait for their chain: one of 385, 32 heads on 8, 8.1 us and one of 20 5.1 in a table that is not cut; in a longer one, as a server's is, the second launch is
+// there too, and heads stay together: 10.7 and 7.4.
 #include "common.h"
 
 namespace {
@@ -469,6 +470,7 @@ pa_shape shape_of(int B, int heads, int kv_heads, int64_t positions) {
     const bool whole = positions <= (together <= 64 ? 768 : 1024);
     // One head to a unit where that leaves at most a workgroup per CU and nothing is cut: heads that share rows then read them again from the L2, side by side.  (us, heads together / one by
     // one: 1 request of 385, 32 heads on 8, 8.7 / 8.3, 64 on 8 9.8 / 8.2; 8 of 300 to 500, 32 on 8, 9.7 / 9.5; but 32 of 10 to 500 12.3 / 24.0.)
+    // The rules go by the table's width, as the host does not know the lengths: requests of up to 1000 positions in tables of 8192 pay the second launch (48 of them 28.5 us instead of 21.0).
     p.groups = whole && (int64_t)B * heads <= 256 ? p.rep : (int)bs_cdiv(p.rep, PA_HEADS);
     p.per_unit = (int)bs_cdiv(p.rep, p.groups);
     p.units = kv_heads * p.groups;
@@ -483,7 +485,8 @@ pa_shape shape_of(int B, int heads, int kv_heads, int64_t positions) {
 }
 
 // A cache that the last-level cache cannot hold is read past it.  (us without / with: 48 requests of 1 to 4096, 404 MB, 82.3 / 76.2; 2 of 80000, 655 MB, 132.8 / 115.6; but 8 of 2000,
-// 67 MB, over and over 22.4 / 25.5.)
+// 67 MB, over and over 22.4 / 25.5, and 48 of up to 1000, 96 MB of a pool of 1 GiB, 21.0 / 25.3.  The rule goes by the pool, as the host does not know the lengths: a step's layers together read more than
+// the pages of one, which are gone from the cache when the next step comes to them.)
 constexpr int64_t PA_STREAM = 256ll << 20;
 
 template <int D, int HP>

@@ -1,6 +1,7 @@
 // The next token of every row from its logits, with temperature, top-k, top-p and min-p, from a random number that is given.
 //
-//   w_i = exp((x_i - max) / T)                     in 64 bits: a random number next to a border of a large vocabulary is decided by 1e-9 of the sum
+//   w_i = exp((x_i - max) / T)                     to 3e-13 of itself, summed in 64 bits: a random number next to a border of a large vocabulary is decided by 1e-9 of the sum.  (Four terms of
+//                                                  a series, 1.4e-13, twice where a weight is a product of two; a fifth would cost every weight an operation more, for borders 1e-12 away)
 //   top-k   the k largest; among equals the lowest indexes
 //   top-p   of those, in the same order, the ones whose larger ones sum to less than p times the sum
 //   min-p   of those, the ones with w_i >= min-p (the largest weight is 1)

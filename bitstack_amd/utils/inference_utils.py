@@ -430,7 +430,8 @@ def rope_store_paged_hip(q, k, v, cos, sin, kpages, vpages, positions, slots, ou
 def attention_paged_hip(qkv, kpages, vpages, cos, sin, block_table, lengths, slots, heads, kv_heads, out=None):
     """One new token per request: RoPE on q and k of qkv [B, (heads + 2 kv) * d] at position lengths[b] - 1, k and v to slots[b] of the pages
     [pool, kv, page_size, d], attention over positions 0 .. lengths[b] - 1 by block_table [B, max_pages]; returns [B, heads * d].
-    lengths (int32) and slots (int64) are page_plan_hip's lengths and row_slots; a request without a slot is idle and its row zeros."""
+    lengths (int32) and slots (int64) are page_plan_hip's lengths and row_slots; a request without a slot is idle and its row zeros.  A score of -inf weighs
+    nothing, one of +inf or NaN makes its head's output NaN."""
     y = _lib.host().attention_paged(qkv, kpages, vpages, cos, sin, block_table, lengths, slots, heads, kv_heads, out)
     if y is not None:
         return y if out is None else out

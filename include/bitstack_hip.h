@@ -519,7 +519,9 @@ int bs_attention_paged_f16(const void *qkv, int ldqkv, void *kpages, void *vpage
  *              <= 0: all; the largest always stays
  *   out[b]     the lowest index whose sum of kept weights up to it is more than
  *              uniform[b] times the sum of all kept
- * Weights and sums are those of 64 bits; a weight below 1e-300 is none.  A temperature that is not above 0:
+ * Weights are held to 3e-13 of themselves and summed in 64 bits: where a random number, top_p or
+ * min_p lies within 1e-12 of the sum from a border, the token may be the one on its other side.  A
+ * weight below 1e-300 is none.  A temperature that is not above 0:
  * bs_argmax_f16.  The four may be NULL: temperature 1, no top_k, top_p, min_p.  NaN
  * and -inf have no weight; a row without any: 0.  A random number outside [0, 1)
  * is taken as the nearest inside, NaN as 0.  Deterministic.  Scratch:
