@@ -81,6 +81,14 @@ SIGNATURES.update({
     "bs_attention_paged_f16": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _L, _P]),
     "bs_sample_workspace_bytes": (_L, [_I, _I]),
     "bs_sample_f16": (_I, [_P, _L, _P, _P, _P, _P, _P, _P, _I, _I, _P, _L, _P]),
+    "bs_tree_plan": (_I, [_P] * 6 + [_I, _I, _P]),
+    "bs_attention_tree_workspace_bytes": (_L, [_I] * 8),
+    "bs_attention_tree_f16": (_I, [_P, _I] + [_P] * 8 + [_I] * 9 + [_P, _L, _P]),
+    "bs_tree_accept_workspace_bytes": (_L, [_I]),
+    "bs_tree_accept_f16": (_I, [_P] * 17 + [_I] * 9 + [_P, _L, _P]),
+    "bs_page_fork_workspace_bytes": (_L, [_I, _I, _I]),
+    "bs_page_fork_f16": (_I, [_P] * 11 + [_I] * 7 + [_P, _L, _P]),
+    "bs_logits_adjust_f16": (_I, [_P, _L, _P, _L, _P, _P, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _P, _I, _P, _I, _I, _I, _P]),
 })
 EPI_NONE, EPI_RESIDUAL, EPI_SWIGLU = 0, 1, 2
 

@@ -2,6 +2,7 @@
 #include "common.h"
 
 #include <algorithm>
+#include <initializer_list>
 #include <mutex>
 
 extern "C" int bs_version(void) { return BS_VERSION_NUMBER; }
@@ -541,4 +542,119 @@ extern "C" int bs_sample_f16(const void *logits, int64_t ld, const float *unifor
         return BS_ERR_ALIGN;
     if (!workspace || workspace_bytes < bs_sample_scratch(B, V) || !bs_aligned(workspace, 16)) return BS_ERR_WORKSPACE;
     return bs_launch_sample((const half_t *)logits, ld, uniform, temperature, top_k, top_p, min_p, out, B, V, workspace, (hipStream_t)stream);
+}
+
+// ---- drafted tokens, forked rows, settings on logits -----------------------------------------------
+static bool all_aligned(std::initializer_list<const void *> pointers, uintptr_t to) {
+    for (const void *p : pointers)
+        if (!bs_aligned(p, to)) return false;
+    return true;
+}
+static bool any_null(std::initializer_list<const void *> pointers) {
+    for (const void *p : pointers)
+        if (!p) return true;
+    return false;
+}
+
+extern "C" int bs_tree_plan(const int32_t *parents, const int32_t *lengths, const int32_t *granted, const int32_t *starts, int32_t *positions, int64_t *masks, int B, int T,
+                            void *stream) {
+    if (B < 0 || B > 65536 || T < 0 || T > 1 << 30) return BS_ERR_SHAPE;
+    if (T == 0) return BS_OK;
+    if (any_null({parents, positions, masks}) || (B > 0 && any_null({lengths, granted, starts}))) return BS_ERR_NULL;
+    if (!all_aligned({parents, lengths, granted, starts, positions}, 4) || !bs_aligned(masks, 8)) return BS_ERR_ALIGN;
+    return bs_launch_tree_plan(parents, lengths, granted, starts, positions, masks, B, T, (hipStream_t)stream);
+}
+
+static int attention_tree_shape(int B, int T, int nodes, int heads, int kv_heads, int head_dim, int page_size, int max_pages) {
+    return attention_paged_shape(B, heads, kv_heads, head_dim, page_size, max_pages) != BS_OK || T < 0 || (int64_t)T * heads > 1 << 22 || nodes < 1 || nodes > 64
+               ? BS_ERR_SHAPE
+               : BS_OK;
+}
+
+extern "C" int64_t bs_attention_tree_workspace_bytes(int B, int T, int nodes, int heads, int kv_heads, int head_dim, int page_size, int max_pages) {
+    const int st = attention_tree_shape(B, T, nodes, heads, kv_heads, head_dim, page_size, max_pages);
+    return st != BS_OK ? st : B == 0 || T == 0 ? 0 : bs_attention_tree_scratch(B, T, nodes, heads, kv_heads, head_dim, max_pages, page_size);
+}
+
+extern "C" int bs_attention_tree_f16(const void *q, int ldq, const void *kpages, const void *vpages, const int32_t *block_table, const int32_t *lengths,
+                                     const int32_t *granted, const int32_t *starts, const int64_t *masks, void *out, int B, int T, int nodes, int heads, int kv_heads,
+                                     int head_dim, int page_size, int max_pages, int pool_pages, void *workspace, int64_t workspace_bytes, void *stream) {
+    const int st = attention_tree_shape(B, T, nodes, heads, kv_heads, head_dim, page_size, max_pages);
+    if (st != BS_OK) return st;
+    if (!pool_fits(pool_pages, page_size) || ldq < (int64_t)heads * head_dim) return BS_ERR_SHAPE;
+    if (T == 0) return BS_OK;
+    if (any_null({q, out, masks}) || (B > 0 && any_null({kpages, vpages, block_table, lengths, granted, starts}))) return BS_ERR_NULL;
+    if (!all_aligned({q, out}, 2) || !all_aligned({kpages, vpages}, 16) || !all_aligned({block_table, lengths, granted, starts}, 4) || !bs_aligned(masks, 8))
+        return BS_ERR_ALIGN;
+    const int64_t need = B == 0 ? 0 : bs_attention_tree_scratch(B, T, nodes, heads, kv_heads, head_dim, max_pages, page_size);
+    if (need > 0 && (!workspace || workspace_bytes < need || !bs_aligned(workspace, 16))) return BS_ERR_WORKSPACE;
+    return bs_launch_attention_tree((const half_t *)q, ldq, (const half_t *)kpages, (const half_t *)vpages, block_table, lengths, granted, starts, masks, (half_t *)out, B,
+                                    T, nodes, heads, kv_heads, head_dim, page_shift(page_size), max_pages, pool_pages, workspace, (hipStream_t)stream);
+}
+
+// a cache whose pieces of a row, in all layers, 32 bits count
+static int layers_shape(int B, int layers, int kv_heads, int head_dim, int page_size, int max_pages, int pool_pages) {
+    return B < 0 || B > 65536 || layers < 1 || kv_heads < 1 || head_dim < 8 || head_dim % 8 != 0 || kv_heads > 1 << 20 || head_dim > 1 << 20 ||
+                   (int64_t)kv_heads * head_dim >= 1 << 28 || layers * ((int64_t)kv_heads * head_dim) >= 1 << 28 || page_shift(page_size) < 0 || max_pages < 1 ||
+                   max_pages > 1 << 24 || (int64_t)B * max_pages > INT32_MAX || !pool_fits(pool_pages, page_size)
+               ? BS_ERR_SHAPE
+               : BS_OK;
+}
+
+extern "C" int64_t bs_tree_accept_workspace_bytes(int B) { return B < 0 || B > 65536 ? BS_ERR_SHAPE : bs_tree_accept_scratch(B); }
+
+extern "C" int bs_tree_accept_f16(const int64_t *tokens, const int32_t *parents, const int64_t *targets, const int64_t *slots, const int32_t *lengths, const int32_t *granted,
+                                  const int32_t *starts, const int32_t *block_table, int32_t *free_pages, const int32_t *free_state, void *kpages, void *vpages,
+                                  int32_t *lengths_out, int32_t *free_state_out, int32_t *accepted, int32_t *path, int64_t *token, int B, int T, int nodes, int layers,
+                                  int kv_heads, int head_dim, int page_size, int max_pages, int pool_pages, void *workspace, int64_t workspace_bytes, void *stream) {
+    const int st = layers_shape(B, layers, kv_heads, head_dim, page_size, max_pages, pool_pages);
+    if (st != BS_OK) return st;
+    if (T < 0 || T > 1 << 30 || nodes < 1 || nodes > 64) return BS_ERR_SHAPE;
+    if (any_null({free_pages, free_state, free_state_out}) || (T > 0 && any_null({tokens, parents, targets, slots})) ||
+        (B > 0 && any_null({lengths, granted, starts, block_table, kpages, vpages, lengths_out, accepted, path, token})))
+        return BS_ERR_NULL;
+    if (!all_aligned({parents, lengths, granted, starts, block_table, free_pages, free_state, lengths_out, free_state_out, accepted, path}, 4) ||
+        !all_aligned({tokens, targets, slots, token}, 8) || !all_aligned({kpages, vpages}, 16))
+        return BS_ERR_ALIGN;
+    if (B > 0 && (!workspace || workspace_bytes < bs_tree_accept_scratch(B) || !bs_aligned(workspace, 16))) return BS_ERR_WORKSPACE;
+    return bs_launch_tree_accept(tokens, parents, targets, slots, lengths, granted, starts, block_table, free_pages, free_state, (half_t *)kpages, (half_t *)vpages,
+                                 lengths_out, free_state_out, accepted, path, token, B, T, nodes, layers, kv_heads, head_dim, page_shift(page_size), max_pages, pool_pages,
+                                 workspace, (hipStream_t)stream);
+}
+
+extern "C" int64_t bs_page_fork_workspace_bytes(int B, int max_pages, int pool_pages) {
+    return B < 0 || B > 65536 || max_pages < 1 || max_pages > 1 << 24 || (int64_t)B * max_pages > INT32_MAX || pool_pages < 1 ? BS_ERR_SHAPE
+                                                                                                                   : bs_page_fork_scratch(B, max_pages, pool_pages);
+}
+
+extern "C" int bs_page_fork_f16(const int32_t *source, const int32_t *lengths, int32_t *block_table, int32_t *free_pages, const int32_t *free_state, int32_t *shares,
+                                void *kpages, void *vpages, int32_t *lengths_out, int32_t *free_state_out, int32_t *granted, int B, int layers, int kv_heads, int head_dim,
+                                int page_size, int max_pages, int pool_pages, void *workspace, int64_t workspace_bytes, void *stream) {
+    const int st = layers_shape(B, layers, kv_heads, head_dim, page_size, max_pages, pool_pages);
+    if (st != BS_OK) return st;
+    if (any_null({free_pages, free_state, free_state_out}) || (B > 0 && any_null({source, lengths, block_table, shares, kpages, vpages, lengths_out, granted})))
+        return BS_ERR_NULL;
+    if (!all_aligned({source, lengths, block_table, free_pages, free_state, shares, lengths_out, free_state_out, granted}, 4) || !all_aligned({kpages, vpages}, 16))
+        return BS_ERR_ALIGN;
+    if (!workspace || workspace_bytes < bs_page_fork_scratch(B, max_pages, pool_pages) || !bs_aligned(workspace, 16)) return BS_ERR_WORKSPACE;
+    return bs_launch_page_fork(source, lengths, block_table, free_pages, free_state, shares, (half_t *)kpages, (half_t *)vpages, lengths_out, free_state_out, granted, B,
+                               layers, kv_heads, head_dim, page_shift(page_size), max_pages, pool_pages, workspace, (hipStream_t)stream);
+}
+
+extern "C" int bs_logits_adjust_f16(const void *logits, int64_t ld, void *out, int64_t ld_out, const int32_t *requests, const int32_t *history, int history_width,
+                                    const int32_t *history_lengths, const int32_t *prompt_lengths, const float *repetition, const float *frequency, const float *presence,
+                                    const int32_t *drafted, int drafted_width, const int32_t *bias_tokens, const float *bias, int biases, const int32_t *allowed, int masks,
+                                    const int32_t *allowed_rows, int R, int V, int B, void *stream) {
+    if (sample_shape(R, V) != BS_OK || B < 0 || (R > 1 && (ld < V || ld_out < V)) || history_width < 0 || drafted_width < 0 || biases < 0 || masks < 0 ||
+        (history_lengths && !history) || (prompt_lengths && !history) || (bias_tokens != nullptr) != (bias != nullptr) || (allowed_rows && !allowed) ||
+        (allowed && !allowed_rows && masks < R) || (logits == out && ld != ld_out && R > 1) ||
+        (!requests && B < R && (history || drafted || bias || repetition || frequency || presence)))
+        return BS_ERR_SHAPE;
+    if (R == 0) return BS_OK;
+    if (!logits || !out) return BS_ERR_NULL;
+    if (!all_aligned({logits, out}, 2) || !all_aligned({requests, history, history_lengths, prompt_lengths, repetition, frequency, presence, drafted, bias_tokens, bias, allowed,
+                                                        allowed_rows}, 4))
+        return BS_ERR_ALIGN;
+    return bs_launch_logits_adjust((const half_t *)logits, ld, (half_t *)out, ld_out, requests, history, history_lengths, prompt_lengths, repetition, frequency, presence,
+                                   drafted, bias_tokens, bias, allowed, allowed_rows, R, V, B, history_width, drafted_width, biases, masks, (hipStream_t)stream);
 }

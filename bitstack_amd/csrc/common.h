@@ -149,3 +149,25 @@ int bs_launch_attention_paged(const half_t *qkv, int ldqkv, half_t *kpages, half
 int64_t bs_sample_scratch(int B, int V);
 int bs_launch_sample(const half_t *logits, int64_t ld, const float *uniform, const float *temperature, const int32_t *top_k, const float *top_p,
                      const float *min_p, int64_t *out, int B, int V, void *workspace, hipStream_t s);
+// drafted tokens as a tree per request: masks, positions and acceptance (tree.hip), attention (tree_attention.hip)
+int bs_launch_tree_plan(const int32_t *parents, const int32_t *lengths, const int32_t *granted, const int32_t *starts, int32_t *positions, int64_t *masks, int B, int T,
+                        hipStream_t s);
+int64_t bs_tree_accept_scratch(int B);
+int bs_launch_tree_accept(const int64_t *tokens, const int32_t *parents, const int64_t *targets, const int64_t *slots, const int32_t *lengths, const int32_t *granted,
+                          const int32_t *starts, const int32_t *table, int32_t *ring, const int32_t *state, half_t *kpages, half_t *vpages, int32_t *lengths_out,
+                          int32_t *state_out, int32_t *accepted, int32_t *path, int64_t *token, int B, int T, int nodes, int layers, int kv_heads, int head_dim, int shift,
+                          int max_pages, int pool, void *workspace, hipStream_t s);
+int64_t bs_attention_tree_scratch(int B, int T, int nodes, int heads, int kv_heads, int head_dim, int max_pages, int page);
+int bs_launch_attention_tree(const half_t *q, int ldq, const half_t *kpages, const half_t *vpages, const int32_t *table, const int32_t *lengths, const int32_t *granted,
+                             const int32_t *starts, const int64_t *masks, half_t *out, int B, int T, int nodes, int heads, int kv_heads, int head_dim, int shift, int max_pages,
+                             int pool, void *workspace, hipStream_t s);
+// rows of a paged cache become copies of other rows (fork.hip)
+int64_t bs_page_fork_scratch(int B, int max_pages, int pool);
+int bs_launch_page_fork(const int32_t *source, const int32_t *lengths, int32_t *table, int32_t *ring, const int32_t *state, int32_t *shares, half_t *kpages, half_t *vpages,
+                        int32_t *lengths_out, int32_t *state_out, int32_t *granted, int B, int layers, int kv_heads, int head_dim, int shift, int max_pages, int pool,
+                        void *workspace, hipStream_t s);
+// penalties, biases and grammar masks on logits (logits.hip)
+int bs_launch_logits_adjust(const half_t *logits, int64_t ld, half_t *out, int64_t ld_out, const int32_t *requests, const int32_t *history, const int32_t *history_lengths,
+                            const int32_t *prompt_lengths, const float *repetition, const float *frequency, const float *presence, const int32_t *drafted,
+                            const int32_t *bias_tokens, const float *bias, const int32_t *allowed, const int32_t *allowed_rows, int rows, int V, int B, int most, int path,
+                            int biases, int masks, hipStream_t s);

@@ -742,10 +742,275 @@ PyObject *host_sample(PyObject *, PyObject *const *a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- drafted tokens, forked rows, settings on logits -----------------------------------------------
+PyObject *tuple_of(const at::Tensor *t, int n) {
+    PyObject *all = PyTuple_New(n);
+    for (int i = 0; all && i < n; i++) {
+        PyObject *o = THPVariable_Wrap(t[i]);
+        if (!o) {
+            Py_DECREF(all);
+            return nullptr;
+        }
+        PyTuple_SET_ITEM(all, i, o);
+    }
+    return all;
+}
+// lengths [B], granted [B], starts [B + 1]
+struct Trees {
+    int64_t B;
+    int32_t *lengths;
+    const int32_t *granted, *starts;
+};
+bool trees_args(PyObject *lp, PyObject *gp, PyObject *sp, Trees &t) {
+    const at::Tensor *lengths = tensor_arg(lp), *granted = tensor_arg(gp), *starts = tensor_arg(sp);
+    if (!lengths || !granted || !starts || !lengths->is_cuda() || lengths->dim() != 1) return false;
+    const c10::Device dev = lengths->device();
+    t.B = lengths->size(0);
+    if (t.B >= INT32_MAX || !vector(*lengths, t.B, at::kInt, dev) || !vector(*granted, t.B, at::kInt, dev) || !vector(*starts, t.B + 1, at::kInt, dev)) return false;
+    t.lengths = (int32_t *)lengths->mutable_data_ptr();
+    t.granted = (const int32_t *)granted->const_data_ptr();
+    t.starts = (const int32_t *)starts->const_data_ptr();
+    return true;
+}
+// a cache in pages, of one layer or of all
+struct Layers {
+    int layers, pool, kv, page, d;
+    void *k, *v;
+};
+bool layers_args(PyObject *kp, PyObject *vp, c10::Device dev, Layers &p) {
+    const at::Tensor *k = tensor_arg(kp), *v = tensor_arg(vp);
+    if (!k || !v || !plain(*k, at::kHalf, dev) || !plain(*v, at::kHalf, dev) || (k->dim() != 4 && k->dim() != 5) || k->sizes() != v->sizes()) return false;
+    for (int64_t n : k->sizes())
+        if (n < 1 || n >= INT32_MAX) return false;
+    p = {k->dim() == 5 ? (int)k->size(0) : 1, (int)k->size(-4), (int)k->size(-3), (int)k->size(-2), (int)k->size(-1), k->mutable_data_ptr(), v->mutable_data_ptr()};
+    return true;
+}
+bool table_arg(PyObject *o, int64_t B, c10::Device dev, int32_t *&p, int &max_pages) {
+    const at::Tensor *t = tensor_arg(o);
+    if (!t || !plain(*t, at::kInt, dev) || t->dim() != 2 || t->size(0) != B || t->size(1) >= INT32_MAX) return false;
+    p = (int32_t *)t->mutable_data_ptr();
+    max_pages = (int)t->size(1);
+    return true;
+}
+bool vector_arg(PyObject *o, int64_t n, at::ScalarType type, c10::Device dev, void *&p) {
+    const at::Tensor *t = tensor_arg(o);
+    if (!t || !vector(*t, n, type, dev)) return false;
+    p = t->mutable_data_ptr();
+    return true;
+}
+
+// tree_plan(parents, lengths, granted, starts) -> (positions, masks), or None
+PyObject *host_tree_plan(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 4) return PyErr_Format(PyExc_TypeError, "tree_plan takes 4 arguments");
+    HANDLE_TH_ERRORS
+        const at::Tensor *parents = tensor_arg(a[0]);
+        Trees t;
+        if (!parents || !parents->is_cuda() || parents->dim() != 1 || !trees_args(a[1], a[2], a[3], t)) Py_RETURN_NONE;
+        const c10::Device dev = parents->device();
+        const int64_t T = parents->size(0);
+        if (T >= INT32_MAX || !plain(*parents, at::kInt, dev) || tensor_arg(a[1])->device() != dev) Py_RETURN_NONE;
+        const int32_t *pp = (const int32_t *)parents->const_data_ptr();
+        at::Tensor out[2];
+        const int st = while_others_run([&] {
+            DeviceScope scope(dev);
+            out[0] = new_tensor({T}, at::kInt, dev);
+            out[1] = new_tensor({T}, at::kLong, dev);
+            return bs_tree_plan(pp, t.lengths, t.granted, t.starts, (int32_t *)out[0].mutable_data_ptr(), (int64_t *)out[1].mutable_data_ptr(), (int)t.B, (int)T,
+                                c10::hip::getCurrentHIPStream(dev.index()).stream());
+        });
+        if (st != BS_OK) return raise_status(st, "bs_tree_plan");
+        return tuple_of(out, 2);
+    END_HANDLE_TH_ERRORS
+}
+
+// attention_tree(q, kpages, vpages, block_table, lengths, granted, starts, masks, nodes, out or None) -> out, or None
+PyObject *host_attention_tree(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 10) return PyErr_Format(PyExc_TypeError, "attention_tree takes 10 arguments");
+    HANDLE_TH_ERRORS
+        const at::Tensor *q = tensor_arg(a[0]), *out;
+        int64_t nodes, ld;
+        if (!int_arg(a[8], nodes)) return nullptr;
+        Trees t;
+        Layers p;
+        int32_t *table;
+        int max_pages;
+        void *masks;
+        if (!q || !optional_arg(a[9], out) || !q->is_cuda() || q->dim() != 2 || !trees_args(a[4], a[5], a[6], t)) Py_RETURN_NONE;
+        const c10::Device dev = q->device();
+        const int64_t T = q->size(0), width = q->size(1);
+        if (tensor_arg(a[4])->device() != dev || !layers_args(a[1], a[2], dev, p) || tensor_arg(a[1])->dim() != 4 || !table_arg(a[3], t.B, dev, table, max_pages) || T >= INT32_MAX ||
+            width == 0 || width % p.d != 0 || !matrix_rows(*q, T, width, dev, ld) || !vector_arg(a[7], T, at::kLong, dev, masks) || nodes < 1 || nodes > 64 ||
+            (out && (!plain(*out, at::kHalf, dev) || out->numel() != T * width)))
+            Py_RETURN_NONE;
+        const int heads = (int)(width / p.d);
+        const int64_t need = bs_attention_tree_workspace_bytes((int)t.B, (int)T, (int)nodes, heads, p.kv, p.d, p.page, max_pages);
+        if (need < 0) Py_RETURN_NONE;
+        const void *xp = q->const_data_ptr();
+        at::Tensor y;
+        if (out) y = *out;
+        const int st = while_others_run([&] {
+            DeviceScope scope(dev);
+            const hipStream_t stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+            if (!y.defined()) y = new_half({T, width}, dev);
+            const Workspace ws = own_workspace_for(dev.index(), stream, need);
+            std::lock_guard<std::mutex> launching(*ws.launching);
+            return bs_attention_tree_f16(xp, (int)ld, p.k, p.v, table, t.lengths, t.granted, t.starts, (const int64_t *)masks, y.mutable_data_ptr(), (int)t.B, (int)T, (int)nodes,
+                                         heads, p.kv, p.d, p.page, max_pages, p.pool, ws.data(), ws.buffer.numel(), stream);
+        });
+        if (st != BS_OK) return raise_status(st, "bs_attention_tree_f16");
+        return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
+// tree_accept(tokens, parents, targets, slots, lengths, granted, starts, block_table, free_pages, free_state, kpages, vpages, nodes, inplace)
+// -> (lengths, state, accepted, path, token), or None
+PyObject *host_tree_accept(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 14) return PyErr_Format(PyExc_TypeError, "tree_accept takes 14 arguments");
+    HANDLE_TH_ERRORS
+        const at::Tensor *parents = tensor_arg(a[1]), *ring = tensor_arg(a[8]);
+        int64_t nodes;
+        if (!int_arg(a[12], nodes)) return nullptr;
+        Trees t;
+        Layers p;
+        int32_t *table;
+        int max_pages;
+        void *tokens, *targets, *slots, *state;
+        if (!parents || !ring || !parents->is_cuda() || parents->dim() != 1 || !trees_args(a[4], a[5], a[6], t)) Py_RETURN_NONE;
+        const c10::Device dev = parents->device();
+        const int64_t T = parents->size(0);
+        if (tensor_arg(a[4])->device() != dev || T >= INT32_MAX || !plain(*parents, at::kInt, dev) || !vector_arg(a[0], T, at::kLong, dev, tokens) ||
+            !vector_arg(a[2], T, at::kLong, dev, targets) || !vector_arg(a[3], T, at::kLong, dev, slots) || !table_arg(a[7], t.B, dev, table, max_pages) ||
+            !layers_args(a[10], a[11], dev, p) || !vector(*ring, p.pool, at::kInt, dev) || !vector_arg(a[9], 2, at::kInt, dev, state) || nodes < 1 || nodes > 64)
+            Py_RETURN_NONE;
+        const int64_t need = bs_tree_accept_workspace_bytes((int)t.B);
+        if (need < 0) Py_RETURN_NONE;
+        const int32_t *pp = (const int32_t *)parents->const_data_ptr();
+        int32_t *rp = (int32_t *)ring->mutable_data_ptr();
+        const bool inplace = a[13] == Py_True;
+        at::Tensor out[5];
+        if (inplace) {
+            out[0] = *tensor_arg(a[4]);
+            out[1] = *tensor_arg(a[9]);
+        }
+        const int st = while_others_run([&] {
+            DeviceScope scope(dev);
+            const hipStream_t stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+            if (!inplace) {
+                out[0] = new_tensor({t.B}, at::kInt, dev);
+                out[1] = new_tensor({2}, at::kInt, dev);
+            }
+            out[2] = new_tensor({t.B}, at::kInt, dev);
+            out[3] = new_tensor({t.B, nodes}, at::kInt, dev);
+            out[4] = new_tensor({t.B}, at::kLong, dev);
+            const Workspace ws = own_workspace_for(dev.index(), stream, need);
+            std::lock_guard<std::mutex> launching(*ws.launching);
+            return bs_tree_accept_f16((const int64_t *)tokens, pp, (const int64_t *)targets, (const int64_t *)slots, t.lengths, t.granted, t.starts, table, rp,
+                                      (const int32_t *)state, p.k, p.v, (int32_t *)out[0].mutable_data_ptr(), (int32_t *)out[1].mutable_data_ptr(),
+                                      (int32_t *)out[2].mutable_data_ptr(), (int32_t *)out[3].mutable_data_ptr(), (int64_t *)out[4].mutable_data_ptr(), (int)t.B, (int)T,
+                                      (int)nodes, p.layers, p.kv, p.d, p.page, max_pages, p.pool, ws.data(), ws.buffer.numel(), stream);
+        });
+        if (st != BS_OK) return raise_status(st, "bs_tree_accept_f16");
+        return tuple_of(out, 5);
+    END_HANDLE_TH_ERRORS
+}
+
+// page_fork(source, lengths, block_table, free_pages, free_state, shares, kpages, vpages, inplace) -> (lengths, state, granted), or None
+PyObject *host_page_fork(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 9) return PyErr_Format(PyExc_TypeError, "page_fork takes 9 arguments");
+    HANDLE_TH_ERRORS
+        const at::Tensor *lengths = tensor_arg(a[1]);
+        Layers p;
+        int32_t *table;
+        int max_pages;
+        void *source, *held, *ring, *state, *shares;
+        if (!lengths || !lengths->is_cuda() || lengths->dim() != 1 || lengths->size(0) >= INT32_MAX) Py_RETURN_NONE;
+        const c10::Device dev = lengths->device();
+        const int64_t B = lengths->size(0);
+        if (!vector_arg(a[0], B, at::kInt, dev, source) || !vector_arg(a[1], B, at::kInt, dev, held) || !table_arg(a[2], B, dev, table, max_pages) ||
+            !layers_args(a[6], a[7], dev, p) || !vector_arg(a[3], p.pool, at::kInt, dev, ring) || !vector_arg(a[4], 2, at::kInt, dev, state) ||
+            !vector_arg(a[5], p.pool, at::kInt, dev, shares))
+            Py_RETURN_NONE;
+        const int64_t need = bs_page_fork_workspace_bytes((int)B, max_pages, p.pool);
+        if (need < 0) Py_RETURN_NONE;
+        const bool inplace = a[8] == Py_True;
+        at::Tensor out[3];
+        if (inplace) {
+            out[0] = *lengths;
+            out[1] = *tensor_arg(a[4]);
+        }
+        const int st = while_others_run([&] {
+            DeviceScope scope(dev);
+            const hipStream_t stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+            if (!inplace) {
+                out[0] = new_tensor({B}, at::kInt, dev);
+                out[1] = new_tensor({2}, at::kInt, dev);
+            }
+            out[2] = new_tensor({B}, at::kInt, dev);
+            const Workspace ws = own_workspace_for(dev.index(), stream, need);
+            std::lock_guard<std::mutex> launching(*ws.launching);
+            return bs_page_fork_f16((const int32_t *)source, (const int32_t *)held, table, (int32_t *)ring, (const int32_t *)state, (int32_t *)shares, p.k, p.v,
+                                    (int32_t *)out[0].mutable_data_ptr(), (int32_t *)out[1].mutable_data_ptr(), (int32_t *)out[2].mutable_data_ptr(), (int)B, p.layers, p.kv, p.d,
+                                    p.page, max_pages, p.pool, ws.data(), ws.buffer.numel(), stream);
+        });
+        if (st != BS_OK) return raise_status(st, "bs_page_fork_f16");
+        return tuple_of(out, 3);
+    END_HANDLE_TH_ERRORS
+}
+
+// logits_adjust(logits, history, history_lengths, prompt_lengths, repetition, frequency, presence, drafted, requests, bias_tokens, bias, allowed, allowed_rows, out; all
+// but the first or None) -> True, or None
+PyObject *host_logits_adjust(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 14) return PyErr_Format(PyExc_TypeError, "logits_adjust takes 14 arguments");
+    HANDLE_TH_ERRORS
+        const at::Tensor *x = tensor_arg(a[0]), *t[13];
+        if (!x || !x->is_cuda() || x->dim() != 2) Py_RETURN_NONE;
+        for (int i = 0; i < 13; i++)
+            if (!optional_arg(a[i + 1], t[i])) Py_RETURN_NONE;
+        const at::Tensor *history = t[0], *drafted = t[6], *requests = t[7], *tokens = t[8], *bias = t[9], *allowed = t[10], *states = t[11], *out = t[12];
+        const c10::Device dev = x->device();
+        const int64_t R = x->size(0), V = x->size(1);
+        int64_t ld, ldo, B = -1;
+        if (R >= INT32_MAX || V >= INT32_MAX || !matrix_rows(*x, R, V, dev, ld)) Py_RETURN_NONE;
+        ldo = ld;
+        if (out && !matrix_rows(*out, R, V, dev, ldo)) Py_RETURN_NONE;
+        // what there is one of for every request, and whether it is a vector
+        for (int i : {0, 1, 2, 3, 4, 5, 8, 9}) {
+            if (!t[i]) continue;
+            const bool wide = i == 0 || i >= 8, real = i == 9 || (i >= 3 && i <= 5);
+            if (t[i]->dim() != (wide ? 2 : 1) || !plain(*t[i], real ? at::kFloat : at::kInt, dev)) Py_RETURN_NONE;
+            if (B < 0) B = t[i]->size(0);
+            if (t[i]->size(0) != B || (wide && t[i]->size(1) >= INT32_MAX)) Py_RETURN_NONE;
+        }
+        if (B < 0) B = R;
+        if (B >= INT32_MAX || (!history && (t[1] || t[2])) || (!history && !drafted && (t[3] || t[4] || t[5])) || !tokens != !bias || (bias && bias->sizes() != tokens->sizes()) ||
+            (!allowed && states) || (drafted && (drafted->dim() != 2 || drafted->size(0) != R || drafted->size(1) >= INT32_MAX || !plain(*drafted, at::kInt, dev))) ||
+            (requests ? !vector(*requests, R, at::kInt, dev) : B != R) ||
+            (allowed && (allowed->dim() != 2 || allowed->size(1) != (V + 31) / 32 || allowed->size(0) >= INT32_MAX || !plain(*allowed, at::kInt, dev) ||
+                         (states ? !vector(*states, R, at::kInt, dev) : allowed->size(0) != R))))
+            Py_RETURN_NONE;
+        auto ints = [](const at::Tensor *v) { return v ? (const int32_t *)v->const_data_ptr() : nullptr; };
+        auto reals = [](const at::Tensor *v) { return v ? (const float *)v->const_data_ptr() : nullptr; };
+        auto width = [](const at::Tensor *v) { return v ? (int)v->size(1) : 0; };
+        const void *xp = x->const_data_ptr();
+        void *yp = (out ? out : x)->mutable_data_ptr();
+        const int32_t *hp = ints(history), *hl = ints(t[1]), *pl = ints(t[2]), *dp = ints(drafted), *qp = ints(requests), *tp = ints(tokens), *ap = ints(allowed), *sp = ints(states);
+        const float *rp = reals(t[3]), *fp = reals(t[4]), *ep = reals(t[5]), *bp = reals(bias);
+        const int masks = allowed ? (int)allowed->size(0) : 0, wide[3] = {width(history), width(drafted), width(bias)};
+        const int st = while_others_run([&] {
+            DeviceScope scope(dev);
+            return bs_logits_adjust_f16(xp, ld, yp, ldo, qp, hp, wide[0], hl, pl, rp, fp, ep, dp, wide[1], tp, bp, wide[2], ap, masks, sp, (int)R, (int)V, (int)B,
+                                        c10::hip::getCurrentHIPStream(dev.index()).stream());
+        });
+        if (st != BS_OK) return raise_status(st, "bs_logits_adjust_f16");
+        Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
 #define HOST_METHOD(name) {#name, (PyCFunction)(void (*)(void))host_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {HOST_METHOD(forward), HOST_METHOD(rebuild), HOST_METHOD(unpack), HOST_METHOD(rebuild_from_sign), HOST_METHOD(linear), HOST_METHOD(forward_cat), HOST_METHOD(workspace),
                          HOST_METHOD(hold), HOST_METHOD(let_go), HOST_METHOD(argmax), HOST_METHOD(make_steps), HOST_METHOD(run_steps),
-                         HOST_METHOD(page_plan), HOST_METHOD(rope_store_paged), HOST_METHOD(attention_paged), HOST_METHOD(sample), {nullptr, nullptr, 0, nullptr}};
+                         HOST_METHOD(page_plan), HOST_METHOD(rope_store_paged), HOST_METHOD(attention_paged), HOST_METHOD(sample),
+                         HOST_METHOD(tree_plan), HOST_METHOD(attention_tree), HOST_METHOD(tree_accept), HOST_METHOD(page_fork), HOST_METHOD(logits_adjust), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Native host path over libbitstack_hip.so.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -1,6 +1,7 @@
 // A key-value cache in pages, for requests of unequal lengths: which pages a step's tokens take (page_plan_kernel), and the prompts'
 // keys and values on their way into them (rope_store_paged_kernel).
 #include "lanes.h"
+#include "pages.h"
 
 namespace {
 
@@ -53,19 +54,6 @@ __device__ __forceinline__ uint32_t plan_scan(uint32_t v, uint32_t cap, uint32_t
     if ((threadIdx.x & 63) == 63) waves[threadIdx.x >> 6] = s;
     return s;
 }
-
-__device__ __forceinline__ int plan_pages(int n, int shift) { return n > 0 ? ((n - 1) >> shift) + 1 : 0; }
-__device__ __forceinline__ int plan_wrap(uint32_t i, int pool) { return i >= (uint32_t)pool ? (int)(i - pool) : (int)i; }   // i < 2 * pool
-
-struct plan_state {
-    int head, count, tail;                       // (a state that no ring can have is an empty ring)
-    __device__ __forceinline__ plan_state(const int32_t *p, int pool) {
-        head = p[0];
-        count = p[1];
-        if (head < 0 || head >= pool || count < 0 || count > pool) head = count = 0;
-        tail = plan_wrap((uint32_t)head + count, pool);
-    }
-};
 
 // The entries of a row that change, first <= j < end: pages that go back are read before new ones take their place, by the same thread.  Several at a time: a
 // load that stands behind another entry's store waits for nothing but it.

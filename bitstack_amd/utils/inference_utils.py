@@ -485,6 +485,209 @@ def sample_hip(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=
     return y
 
 
+# ---- drafted tokens: a tree per request; forked rows; settings on logits -----------------------------------------------------
+class TreePlan(NamedTuple):
+    """What tree_plan_hip gives for every token row: the position that it is rotated by (int32, -1 for rows that are no node), and the
+    nodes of its request that it attends to (int64, bit i for node i)."""
+    positions: torch.Tensor
+    masks: torch.Tensor
+
+
+class TreeAccept(NamedTuple):
+    """What tree_accept_hip gives: positions per request and the ring's {first, count} afterwards, how many nodes were accepted [B], which
+    [B, nodes] (-1 behind them), and the token that each request goes on with (int64 [B], -1 without nodes)."""
+    lengths: torch.Tensor
+    state: torch.Tensor
+    accepted: torch.Tensor
+    path: torch.Tensor
+    token: torch.Tensor
+
+
+class PageFork(NamedTuple):
+    """What page_fork_hip gives: positions per row and the ring's {first, count} afterwards, 1 or 0 for every row (0: no page was there, it stays)."""
+    lengths: torch.Tensor
+    state: torch.Tensor
+    granted: torch.Tensor
+
+
+def _table(t, B):
+    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != B or not t.is_contiguous():
+        raise ValueError(f"block_table must be a contiguous int32 tensor [{B}, max_pages], got {t.dtype} {tuple(t.shape)}")
+
+
+def _trees(lengths, granted, starts):
+    B = lengths.shape[0] if lengths.dim() == 1 else -1
+    _vector(lengths, B, torch.int32, "lengths")
+    _vector(granted, B, torch.int32, "granted")
+    _vector(starts, B + 1, torch.int32, "starts")
+    return B
+
+
+def _layers(kpages, vpages, pool):
+    """(layers, kv_heads, page_size, head_dim) of a cache in pages, of one layer or of all."""
+    for t in (kpages, vpages):
+        if t.dtype != torch.float16 or t.dim() not in (4, 5) or t.shape != kpages.shape or not t.is_contiguous():
+            raise ValueError("kpages and vpages must be contiguous fp16 tensors [layers, pool, kv_heads, page_size, head_dim] (or without layers) of one shape")
+    if kpages.shape[-4] != pool:
+        raise ValueError(f"free_pages must hold a number for each of the {kpages.shape[-4]} pages, got {pool}")
+    return (kpages.shape[0] if kpages.dim() == 5 else 1, *kpages.shape[-3:])
+
+
+def tree_plan_hip(parents, lengths, granted, starts):
+    """Positions and masks of the drafted tokens, once per step.  Request b's tokens are rows starts[b] .. of parents [T] (int32): the first is the one that it goes
+    on with, each other names its parent's number among them, a smaller one than its own (-1: none).  lengths, granted, starts: page_plan_hip's for a step of that many tokens
+    per request, at most 64."""
+    plan = _lib.host().tree_plan(parents, lengths, granted, starts)
+    if plan is not None:
+        return TreePlan._make(plan)
+    dev = _lib.require_gpu(parents, lengths, granted, starts)
+    B, T = _trees(lengths, granted, starts), parents.shape[0] if parents.dim() == 1 else -1
+    _vector(parents, T, torch.int32, "parents")
+    plan = TreePlan(torch.empty(T, dtype=torch.int32, device=dev), torch.empty(T, dtype=torch.int64, device=dev))
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().bs_tree_plan(_lib.ptr(parents), _lib.ptr(lengths), _lib.ptr(granted), _lib.ptr(starts), _lib.ptr(plan.positions), _lib.ptr(plan.masks), B, T,
+                                           _lib.stream_ptr(dev)), "bs_tree_plan")
+    return plan
+
+
+def attention_tree_hip(q, kpages, vpages, block_table, lengths, granted, starts, masks, nodes=64, out=None):
+    """Attention of drafted tokens: q [T, heads * d] rotated (rows may be strided), their keys and values stored (rope_store_paged_hip with tree_plan_hip's positions does both),
+    over the positions that each request held in the pages [pool, kv, page_size, d] and the nodes that masks [T] names.  lengths, granted, starts as in tree_plan_hip;
+    `nodes` is the largest number of them that a request has (up to 64; one with more is left out).  Returns [T, heads * d], zeros in rows that are no node."""
+    y = _lib.host().attention_tree(q, kpages, vpages, block_table, lengths, granted, starts, masks, nodes, out)
+    if y is not None:
+        return y if out is None else out
+    dev = _lib.require_gpu(q, kpages, vpages, block_table, lengths, granted, starts, masks, out)
+    B, nodes = _trees(lengths, granted, starts), int(nodes)
+    pool, kv, page, d = kpages.shape if kpages.dim() == 4 else (-1, -1, -1, -1)
+    _layers(kpages, vpages, pool)
+    _table(block_table, B)
+    if q.dim() != 2 or q.shape[1] % d or q.shape[1] == 0:
+        raise ValueError("q must hold whole heads")
+    T, heads = q.shape[0], q.shape[1] // d
+    ldq = _rows(q, (T, heads * d))
+    _vector(masks, T, torch.int64, "masks")
+    y = out if out is not None else torch.empty((T, heads * d), dtype=torch.float16, device=dev)
+    if y.dtype != torch.float16 or not y.is_contiguous() or y.numel() != T * heads * d:
+        raise ValueError("out must be a contiguous fp16 [T, heads * head_dim] tensor")
+    need = int(_lib.lib().bs_attention_tree_workspace_bytes(B, T, nodes, heads, kv, d, page, block_table.shape[1]))
+    if need < 0:
+        _lib.check(need, "bs_attention_tree_workspace_bytes")
+    with torch.cuda.device(dev), _lib.scratch(dev, need, own=True) as ws:
+        _lib.check(_lib.lib().bs_attention_tree_f16(_lib.ptr(q), ldq, _lib.ptr(kpages), _lib.ptr(vpages), _lib.ptr(block_table), _lib.ptr(lengths), _lib.ptr(granted),
+                                                    _lib.ptr(starts), _lib.ptr(masks), _lib.ptr(y), B, T, nodes, heads, kv, d, page, block_table.shape[1], pool, _lib.ptr(ws),
+                                                    ws.numel(), _lib.stream_ptr(dev)), "bs_attention_tree_f16")
+    return y
+
+
+def tree_accept_hip(tokens, parents, targets, slots, lengths, granted, starts, block_table, free_pages, free_state, kpages, vpages, nodes=64, inplace=False):
+    """What the model accepts of drafted trees: from every request's first node on the child whose token (tokens [T], int64) is the target (targets [T], int64: what the
+    model gives behind each node) of the node that is reached.  The accepted nodes' keys and values move to the places behind the held positions, in all layers of
+    kpages, vpages ([layers, pool, kv, page_size, d], or without layers), and the pages behind them go back to the ring.  slots, lengths, granted, starts and the ring are
+    page_plan_hip's, parents and nodes as in tree_plan_hip and attention_tree_hip.  The ring is written in place, lengths and free_state too with `inplace`."""
+    done = _lib.host().tree_accept(tokens, parents, targets, slots, lengths, granted, starts, block_table, free_pages, free_state, kpages, vpages, nodes, bool(inplace))
+    if done is not None:
+        return TreeAccept._make(done)
+    dev = _lib.require_gpu(tokens, parents, targets, slots, lengths, granted, starts, block_table, free_pages, free_state, kpages, vpages)
+    B, T, nodes = _trees(lengths, granted, starts), parents.shape[0] if parents.dim() == 1 else -1, int(nodes)
+    for name, t, dtype in (("tokens", tokens, torch.int64), ("parents", parents, torch.int32), ("targets", targets, torch.int64), ("slots", slots, torch.int64)):
+        _vector(t, T, dtype, name)
+    _vector(free_pages, free_pages.numel(), torch.int32, "free_pages")
+    _vector(free_state, 2, torch.int32, "free_state")
+    _table(block_table, B)
+    layers, kv, page, d = _layers(kpages, vpages, free_pages.shape[0])
+    if not 1 <= nodes <= 64:
+        raise ValueError("nodes must be 1 to 64")
+    need = int(_lib.lib().bs_tree_accept_workspace_bytes(B))
+    if need < 0:
+        _lib.check(need, "bs_tree_accept_workspace_bytes")
+    i32 = dict(dtype=torch.int32, device=dev)
+    done = TreeAccept(lengths if inplace else torch.empty(B, **i32), free_state if inplace else torch.empty(2, **i32), torch.empty(B, **i32), torch.empty(B, nodes, **i32),
+                      torch.empty(B, dtype=torch.int64, device=dev))
+    with torch.cuda.device(dev), _lib.scratch(dev, need, own=True) as ws:
+        _lib.check(_lib.lib().bs_tree_accept_f16(*(_lib.ptr(t) for t in (tokens, parents, targets, slots, lengths, granted, starts, block_table, free_pages, free_state, kpages,
+                                                                         vpages, *done)), B, T, nodes, layers, kv, d, page, block_table.shape[1], free_pages.shape[0],
+                                                 _lib.ptr(ws), ws.numel(), _lib.stream_ptr(dev)), "bs_tree_accept_f16")
+    return done
+
+
+def page_fork_hip(source, lengths, block_table, free_pages, free_state, shares, kpages, vpages, inplace=False):
+    """Rows of a paged cache become copies of other rows: row b what row source[b] (int32 [B]) was, -1 empty, its own number the row that it is.  Whole pages are shared
+    (shares [pool], int32, zeros in a new pool: holders less one), a last page that is not full is copied in all layers of kpages, vpages ([layers, pool, kv, page_size, d], or
+    without layers) to a new one; pages that nobody holds any more go back to the ring.  Rows that share pages must not be released by page_plan_hip.
+    block_table, the ring and shares are written in place, lengths and free_state too with `inplace`."""
+    done = _lib.host().page_fork(source, lengths, block_table, free_pages, free_state, shares, kpages, vpages, bool(inplace))
+    if done is not None:
+        return PageFork._make(done)
+    dev = _lib.require_gpu(source, lengths, block_table, free_pages, free_state, shares, kpages, vpages)
+    B = lengths.shape[0] if lengths.dim() == 1 else -1
+    _vector(lengths, B, torch.int32, "lengths")
+    _vector(source, B, torch.int32, "source")
+    _vector(free_pages, free_pages.numel(), torch.int32, "free_pages")
+    _vector(shares, free_pages.numel(), torch.int32, "shares")
+    _vector(free_state, 2, torch.int32, "free_state")
+    _table(block_table, B)
+    layers, kv, page, d = _layers(kpages, vpages, free_pages.shape[0])
+    need = int(_lib.lib().bs_page_fork_workspace_bytes(B, block_table.shape[1], free_pages.shape[0]))
+    if need < 0:
+        _lib.check(need, "bs_page_fork_workspace_bytes")
+    i32 = dict(dtype=torch.int32, device=dev)
+    done = PageFork(lengths if inplace else torch.empty(B, **i32), free_state if inplace else torch.empty(2, **i32), torch.empty(B, **i32))
+    with torch.cuda.device(dev), _lib.scratch(dev, need, own=True) as ws:
+        _lib.check(_lib.lib().bs_page_fork_f16(*(_lib.ptr(t) for t in (source, lengths, block_table, free_pages, free_state, shares, kpages, vpages, *done)), B, layers, kv, d,
+                                               page, block_table.shape[1], free_pages.shape[0], _lib.ptr(ws), ws.numel(), _lib.stream_ptr(dev)), "bs_page_fork_f16")
+    return done
+
+
+def _given(t, shape, dtype, name):
+    """A contiguous tensor of that type and shape (None: any size), or None."""
+    if t is not None and (t.dtype != dtype or t.dim() != len(shape) or any(want is not None and want != got for want, got in zip(shape, t.shape)) or not t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor {list(shape)}, got {t.dtype} {tuple(t.shape)}")
+
+
+def logits_adjust_hip(logits, history=None, history_lengths=None, prompt_lengths=None, repetition=None, frequency=None, presence=None, drafted=None, requests=None,
+                      bias_tokens=None, bias=None, allowed=None, allowed_rows=None, out=None):
+    """Penalties, biases and grammar masks on logits [R, V] (fp16, rows may be strided), in place or into `out`; returns what was written.  Row r belongs to request requests[r]
+    (int32; None: r).  history [B, n] (int32) are the requests' tokens, history_lengths and prompt_lengths [B] how many of them there are and belong to the prompt, drafted [R, m]
+    more tokens of single rows (-1: none); repetition, frequency and presence [B] (fp32) are the penalties.  bias [B, k] (fp32) is added for bias_tokens [B, k] (int32, -1:
+    none).  allowed [masks, ceil(V / 32)] (int32) has a bit for each token, allowed_rows [R] (int32; None: r) says which mask a row uses (-1: none).  What is computed, in
+    which order: bs_logits_adjust_f16 in include/bitstack_hip.h."""
+    y = _lib.host().logits_adjust(logits, history, history_lengths, prompt_lengths, repetition, frequency, presence, drafted, requests, bias_tokens, bias, allowed, allowed_rows,
+                                  out)
+    if y:
+        return logits if out is None else out
+    dev = _lib.require_gpu(logits, history, history_lengths, prompt_lengths, repetition, frequency, presence, drafted, requests, bias_tokens, bias, allowed, allowed_rows, out)
+    if logits.dim() != 2:
+        raise ValueError("logits must be a fp16 [R, V] tensor")
+    R, V = logits.shape
+    ld = _rows(logits, (R, V))
+    y = logits if out is None else out
+    ldo = _rows(y, (R, V))
+    if (history is None and (history_lengths is not None or prompt_lengths is not None)) or (bias is None) != (bias_tokens is None) or (allowed is None and allowed_rows is not None):
+        raise ValueError("history_lengths and prompt_lengths go with history, bias with bias_tokens, allowed_rows with allowed")
+    if history is None and drafted is None and any(t is not None for t in (repetition, frequency, presence)):
+        raise ValueError("penalties need history or drafted tokens")
+    per_request = [t.shape[0] for t in (history, history_lengths, prompt_lengths, repetition, frequency, presence, bias_tokens, bias) if t is not None]
+    B = per_request[0] if per_request else R
+    i32, f32 = torch.int32, torch.float32
+    for t, shape, dtype, name in ((history, (B, None), i32, "history"), (history_lengths, (B,), i32, "history_lengths"), (prompt_lengths, (B,), i32, "prompt_lengths"),
+                                  (repetition, (B,), f32, "repetition"), (frequency, (B,), f32, "frequency"), (presence, (B,), f32, "presence"),
+                                  (drafted, (R, None), i32, "drafted"), (requests, (R,), i32, "requests"), (bias_tokens, (B, None), i32, "bias_tokens"),
+                                  (bias, (B, None), f32, "bias"), (allowed, (None, (V + 31) // 32), i32, "allowed"), (allowed_rows, (R,), i32, "allowed_rows")):
+        _given(t, shape, dtype, name)
+    if bias is not None and bias.shape != bias_tokens.shape:
+        raise ValueError("bias must have the shape of bias_tokens")
+    if (requests is None and B != R) or (allowed is not None and allowed_rows is None and allowed.shape[0] != R):
+        raise ValueError(f"without requests and allowed_rows there must be one request and one mask for each of the {R} rows")
+    width = lambda t: 0 if t is None else t.shape[1]                       # noqa: E731
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().bs_logits_adjust_f16(_lib.ptr(logits), ld, _lib.ptr(y), ldo, _lib.ptr(requests), _lib.ptr(history), width(history), _lib.ptr(history_lengths),
+                                                   _lib.ptr(prompt_lengths), _lib.ptr(repetition), _lib.ptr(frequency), _lib.ptr(presence), _lib.ptr(drafted), width(drafted),
+                                                   _lib.ptr(bias_tokens), _lib.ptr(bias), width(bias), _lib.ptr(allowed), 0 if allowed is None else allowed.shape[0],
+                                                   _lib.ptr(allowed_rows), R, V, B, _lib.stream_ptr(dev)), "bs_logits_adjust_f16")
+    return y
+
+
 def linear_f16_hip(x, w, bias=None):
     """F.linear on the library's own MFMA kernel (fp16 in, fp32 accumulate)."""
     y = _lib.host().linear(x, w, bias)

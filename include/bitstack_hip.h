@@ -532,6 +532,96 @@ int64_t bs_sample_workspace_bytes(int B, int V);
 int bs_sample_f16(const void *logits, int64_t ld, const float *uniform, const float *temperature, const int32_t *top_k, const float *top_p,
                   const float *min_p, int64_t *out, int B, int V, void *workspace, int64_t workspace_bytes, void *stream);
 
+/*
+ * ---- drafted tokens: a tree per request -----------------------------------
+ * A step may take several tokens of a request: node 0 is the one that it goes on
+ * with, the others are drafts, each a continuation of its parent.  Node j of
+ * request b is token row starts[b] + j, parents[row] < j the number of its parent in
+ * the tree (another number: none, a root of its own); lengths, granted and starts are what
+ * bs_page_plan has left for a step of that many tokens: request b held lengths[b] -
+ * granted[b] positions and has granted[b] nodes (0: refused, or idle).  starts must not
+ * decrease.  At most 64 nodes, and as many as `nodes` says where it is given; a request with
+ * more, or with more than its token rows or its length, has none.  No counterpart in the reference.
+ *
+ * bs_tree_plan, once per step: positions[T], the positions held plus the node's depth,
+ * which its query and key are rotated by (bs_rope_store_paged_f16 with these and the plan's
+ * slots), and masks[T], whose bit i says that node i is the node itself or one of its ancestors.  -1 and
+ * 0 for rows that are no node.
+ */
+int bs_tree_plan(const int32_t *parents, const int32_t *lengths, const int32_t *granted, const int32_t *starts, int32_t *positions, int64_t *masks,
+                 int B, int T, void *stream);
+
+/*
+ * Attention of the nodes, their keys and values being stored: out[T, heads * head_dim] =
+ * softmax(q k^T / sqrt(head_dim)) v over the positions that the request held and those of
+ * its nodes that masks[t] names (any mask, not only a tree's; bits of no node are ignored).  q [T, heads * head_dim] is
+ * rotated (rows ldq halves apart).  Position p of request b, nodes behind the held ones, is at row p of its pages.  Rows that are no node, and rows
+ * that nothing is left for, are zeros.  Positions whose table entry is no page are left out.  What is masked or left out has no
+ * influence, whatever stands there.  head_dim 64 or 128; B <= 65536, T * heads <= 2^22, B * heads <= 2^22 and B *
+ * max_pages * page_size < 2^35.  out must not overlap q.
+ * Scores, maximum and sums in fp32, the weights in fp16 for the product with v, the largest as 2^15.  A score of -inf weighs nothing, one of
+ * +inf or NaN makes its row of its head NaN.  Deterministic.  Scratch: bs_attention_tree_workspace_bytes, 16-byte aligned (0: none; negative: an error status).
+ */
+int64_t bs_attention_tree_workspace_bytes(int B, int T, int nodes, int heads, int kv_heads, int head_dim, int page_size, int max_pages);
+int bs_attention_tree_f16(const void *q, int ldq, const void *kpages, const void *vpages, const int32_t *block_table, const int32_t *lengths, const int32_t *granted,
+                          const int32_t *starts, const int64_t *masks, void *out, int B, int T, int nodes, int heads, int kv_heads, int head_dim, int page_size,
+                          int max_pages, int pool_pages, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * What the model accepts of the trees: targets[T] is the token that it gives behind every
+ * node (drawn or greedy).  From node 0 on, the child (the lowest one) whose tokens[row]
+ * is the target of the node that is reached, until there is none.
+ *   path [B, nodes]   the nodes on the way, -1 behind them; accepted [B] their number (0 for a request without nodes)
+ *   token [B]         the target of the last one, the token that the request goes on with (-1 without nodes)
+ *   lengths_out [B]   positions held and accepted; may be lengths
+ * The keys and values of node path[i] move to slots[starts[b] + i], in all `layers` of kpages and vpages [layers,
+ * pool_pages, kv_heads, page_size, head_dim] (head_dim a multiple of 8).  Pages behind the last
+ * position go back behind the ring's end, in order of the requests (no other row may hold them); the block table is left alone.  Nothing moves from or to a slot that does
+ * not exist.  Slots must differ.  B * max_pages < 2^31, layers * kv_heads * head_dim < 2^28.  Scratch: bs_tree_accept_workspace_bytes, 16-byte aligned.
+ */
+int64_t bs_tree_accept_workspace_bytes(int B);
+int bs_tree_accept_f16(const int64_t *tokens, const int32_t *parents, const int64_t *targets, const int64_t *slots, const int32_t *lengths, const int32_t *granted,
+                       const int32_t *starts, const int32_t *block_table, int32_t *free_pages, const int32_t *free_state, void *kpages, void *vpages,
+                       int32_t *lengths_out, int32_t *free_state_out, int32_t *accepted, int32_t *path, int64_t *token, int B, int T, int nodes, int layers, int kv_heads,
+                       int head_dim, int page_size, int max_pages, int pool_pages, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Rows become copies of rows: row b what row source[b] was before the call, all at once
+ * (continuations of one prompt, beams that change places); source[b] == -1 empties it, its own
+ * number, or one that no row has, leaves it.  Whole pages are shared: shares[p] (pool_pages numbers, 0 in a
+ * new pool) is the number of rows that hold page p, less one.  A last page that is not full is copied, in all `layers`, to a new page from the ring; requests
+ * are granted in order: the first row that finds no page, and all later ones that need one, stay as they are (granted[b] 0, else 1).
+ * What a row held it gives up; a page whose last holder has left it goes back behind the ring's end, in order of the rows that
+ * gave it up first.  Pages that go back in a call are not taken in the same one.  Entries of the table behind a row's pages are left alone.
+ * Rows that share pages are given back here and not by bs_page_plan's `released`.  lengths_out and free_state_out may be
+ * lengths and free_state.  Deterministic.  B * max_pages < 2^31, layers * kv_heads * head_dim < 2^28, head_dim a multiple of 8.
+ * Scratch: bs_page_fork_workspace_bytes (negative: an error status), 16-byte aligned.  No counterpart in the reference.
+ */
+int64_t bs_page_fork_workspace_bytes(int B, int max_pages, int pool_pages);
+int bs_page_fork_f16(const int32_t *source, const int32_t *lengths, int32_t *block_table, int32_t *free_pages, const int32_t *free_state, int32_t *shares, void *kpages,
+                     void *vpages, int32_t *lengths_out, int32_t *free_state_out, int32_t *granted, int B, int layers, int kv_heads, int head_dim, int page_size,
+                     int max_pages, int pool_pages, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Settings on R rows of logits (fp16, rows ld and ld_out values apart; out may be logits with the same ld), in fp32, rounded
+ * once.  Row r belongs to request requests[r] of B (NULL: row r to request r, R <= B; a number that
+ * no request has: neither penalties nor biases).  In this order:
+ *   penalties   history [B, history_width] are the request's tokens, the first history_lengths[b] of them, the first prompt_lengths[b] its prompt;
+ *               drafted [R, drafted_width] more tokens of the row alone (of its path in a tree).  A token
+ *               that occurs: x / repetition[b] where x > 0, else x * repetition[b].  One that
+ *               occurs n > 0 times behind the prompt: x - frequency[b] * n - presence[b]
+ *   bias        x + bias[b, i] for the tokens bias_tokens[b, i]; of several entries for a token the last
+ *   allowed     [masks, ceil(V / 32)] words of 32 tokens, the lowest bit first; row r uses mask
+ *               allowed_rows[r] (NULL: mask r; a number that no mask has: none); -inf where the bit is 0
+ * Any of them may be NULL: history_lengths the whole width, prompt_lengths 0, repetition 1 (also where it is not above 0),
+ * frequency and presence 0.  Tokens outside 0 .. V - 1 are none.  Finite logits stay finite up to here, at most 65504, unless a bias is infinite; settings other
+ * than biases must be finite.  R <= 2^20, V <= 2^18, R * V <= 2^33.  No counterpart in the reference.
+ */
+int bs_logits_adjust_f16(const void *logits, int64_t ld, void *out, int64_t ld_out, const int32_t *requests, const int32_t *history, int history_width,
+                         const int32_t *history_lengths, const int32_t *prompt_lengths, const float *repetition, const float *frequency, const float *presence,
+                         const int32_t *drafted, int drafted_width, const int32_t *bias_tokens, const float *bias, int biases, const int32_t *allowed, int masks,
+                         const int32_t *allowed_rows, int R, int V, int B, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
