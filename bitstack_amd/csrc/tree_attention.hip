@@ -2,27 +2,27 @@
 // behind them, that masks[t] names.
 //
 // The rows of a KV head of a request are its nodes' queries of that head's group, the head fastest: nodes * group of them, which all read the same K and V.  A workgroup takes up to 16 QT WR of
-// them, the columns of both products, and walks the positions in stages of 64, which come to LDS straight from the pages (no registers), one stage ahead, one barrier per stage.
-// WR waves take 16 QT rows each, WP waves share the positions of a stage; what these leave is put together in LDS at the end.
+// them, the columns of both products, 16 QT to a wave, and walks the positions in stages of 32, which come to LDS straight from the pages (no registers), up to three stages ahead, one barrier per stage.
 //   scores  S[position, row] = K q      16x16x32; the 16-byte pieces of K's rows are XOR-ed with the row's number, so that 16 rows of one piece lie in different banks
 //   output  O[dim, row] += V^T P        16x16x32; a lane of the scores holds four positions of a row in each of two tiles of 16, which are the eight k slots of this product, and V
 //                                       is used as it lies: product j takes element j of the W = D / 16 dimensions that a lane reads
+// The scores of a stage are computed one stage ahead, beside the softmax of the one before it: the matrix unit runs while the vector unit issues.
 // Maximum, sum and output are fp32, in base 2.  The weights are rounded to fp16 for the second product (the queries are given in fp16), the largest as 2^15, so that one of
 // 2^-40 of the largest is still held; their sum is that of the fp32 weights.
 //
 // What a row does not see has a weight of zero, but zero times an infinity is NaN: in the stages with nodes V is looked through, and infinities and NaN, if any, are taken out of the
 // product.  Rows that see them, or whose result is not finite for another reason, are computed again, each by a wave, in fp32.
 //
-// The split: as the lengths are known on the device alone, every workgroup works out from them what it is to do.  The first B workgroups of a unit (row tile, KV head) take one request each, or the
-// first part of it; requests longer than C = (all stages) / (further parts) are cut, and the next workgroups take the further parts, in order.  Parts leave
-// (max, sum, weighted v) in the workspace, and a second launch puts them together, in order: the result does not depend on which came first.
-#include "common.h"
+// The split: as the lengths are known on the device alone, every workgroup works out from them what it is to do.  The stages of all requests, one after another, are dealt to G workgroups of a unit
+// (KV head, or row tile of one) in equal shares; a share may end in the middle of a request, and hold several.  What is not a whole request's leaves (max, sum, weighted v) in
+// the workspace, and a second launch puts the parts together, in order: the result does not depend on which came first.
+#include "lanes.h"
 
 #include <type_traits>
 
 namespace {
 
-constexpr int TA_P = 64;                         // positions of a stage
+constexpr int TA_P = 32;                         // positions of a stage; LDS holds four
 constexpr float TA_LOW = -1e30f;                 // a maximum before the first score (finite scores are above it)
 constexpr float TA_UP = 15.f;                    // log2 of the largest weight
 
@@ -31,13 +31,15 @@ struct ta_args {
     const int32_t *table, *lengths, *granted, *starts;
     const int64_t *masks;
     half_t *out;
-    int32_t *parts_of;                           // workspace: {first further part, further parts} of every token row
-    float *part;                                 // ... and what the parts leave: [token row or (further part, node)][head][max, sum, pad, pad, weighted v]
-    int ldq, B, T, nodes, heads, kv_heads, row_tiles, shift, max_pages, pool, parts, least;
+    int32_t *before;                             // workspace: stages of the requests before each one, and of all
+    float *part;                                 // ... and what parts leave: [share, first or last][node][head][max, sum, pad, pad, weighted v]
+    float per_rep;                               // 1 / (heads per KV head)
+    int ldq, B, T, nodes, heads, kv_heads, row_tiles, shift, max_pages, pool, shares, least;      // (shares 0: a workgroup of a unit takes one request)
 };
 
 struct ta_request {
     int start, end, n, len;                      // token rows, nodes (0: idle), positions with the nodes
+    __device__ __forceinline__ ta_request() {}
     __device__ __forceinline__ ta_request(const ta_args &a, int b) {
         start = min(max(a.starts[b], 0), a.T);
         end = min(max(a.starts[b + 1], start), a.T);
@@ -47,7 +49,15 @@ struct ta_request {
     }
     __device__ __forceinline__ int stages() const { return (len + TA_P - 1) / TA_P; }
 };
-__device__ __forceinline__ int ta_further(int stages, int most) { return stages > most ? (stages + most - 1) / most - 1 : 0; }
+// node of a row: row / rep, at most 64
+__device__ __forceinline__ int ta_node(int row, int rep, float per_rep) {
+    const int node = (int)((float)row * per_rep), rest = row - node * rep;
+    return rest < 0 ? node - 1 : rest >= rep ? node + 1 : node;
+}
+// share g of `sum` stages dealt to `shares`: where it begins; and whose stage x is
+__device__ __forceinline__ int ta_begins(int g, int sum, int shares) { return (int)((int64_t)g * sum / shares); }
+__device__ __forceinline__ int ta_whose(int x, int sum, int shares) { return (int)((((int64_t)x + 1) * shares - 1) / sum); }
+__device__ __forceinline__ int ta_shares(const ta_args &a, int sum) { return min(a.shares, (sum + a.least - 1) / a.least); }
 
 // the larger of v here and in the lane whose number differs by W (16 or 32), or (SUM) both together
 template <int W, bool SUM = false>
@@ -60,339 +70,147 @@ __device__ __forceinline__ float across(float v) {
 
 typedef __attribute__((address_space(3))) void *ta_lds;
 
-template <int D, int QT, int WR, int WP>
-__global__ __launch_bounds__(WR *WP * 64, WR *WP == 2 ? 1 : 2) void attention_tree_kernel(const ta_args a) {
-    constexpr int W = D / 16, NC = D / 32, WAVES = WR * WP, THREADS = WAVES * 64, ROWS = 16 * QT * WR;
-    constexpr int A = TA_P / 16 / WP;            // tiles of 16 positions that a wave takes of a stage
-    constexpr int LINES = D / 32;                // requests of 1 KB for a tile of 16 rows
-    constexpr int TILES = TA_P / 16 / WAVES;     // tiles that a wave requests of a stage: 1 or 2, of K and of V
-    typedef half_t vec_t __attribute__((ext_vector_type(W)));
-    // (an array per operand and stage: the compiler then knows that a request for one does not touch the others)
-    __shared__ __attribute__((aligned(1024))) half_t sk0[TA_P * D], sk1[TA_P * D], sv0[TA_P * D], sv1[TA_P * D];
-    __shared__ float wm[WP][ROWS], wl[WP][ROWS];
-    __shared__ int sums[WAVES], found[4], again[ROWS], odd_held;
-    __shared__ uint32_t odd_nodes[2];            // positions where something in v is infinite or NaN
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
-    const int wr = wave / WP, wp = wave % WP;
-    const int units = a.kv_heads * a.row_tiles, unit = blockIdx.x % units, work = blockIdx.x / units;
-    const int hk = unit % a.kv_heads, row0 = unit / a.kv_heads * ROWS, rep = a.heads / a.kv_heads;
-
-    // ---- which request, which part of it
-    int b = work, part = 0, most = 0, further = 0, place = 0;          // stages of a part at most; further parts of this request, and the first one's number
-    const bool first_part = work < a.B;
-    if (a.parts > 0) {
-        int all = 0;
-        for (int i = tid; i < a.B; i += THREADS) all += ta_request(a, i).stages();
+// What a workgroup is at: stages st .. st_end - 1 of request b, whose stages have the numbers from `before` on.
+struct ta_work {
+    int g, at, end;                              // its share, stages still to do
+    int b, before, st, st_end, slot;             // slot: of a part; -1: the whole request
+    ta_request rq;
+    __device__ __forceinline__ void take(int first) {
+        const int stages = rq.stages();
+        st = at - before;
+        st_end = min(stages, st + end - at);
+        slot = st == 0 && st_end == stages ? -1 : 2 * g + (at != first);
+        at += st_end - st;
+    }
+};
+__device__ __forceinline__ ta_request ta_uniform(const ta_request &r, int lane) {
+    ta_request u;
+    u.start = (int)bs_read((uint32_t)r.start, lane);
+    u.end = (int)bs_read((uint32_t)r.end, lane);
+    u.n = (int)bs_read((uint32_t)r.n, lane);
+    u.len = (int)bs_read((uint32_t)r.len, lane);
+    return u;
+}
+// The next request of the share (up to 64 requests: the first one too): false where there is none.  Up to 64 requests every wave finds it by itself, a lane a request.
+template <bool FIRST>
+__device__ __forceinline__ bool ta_next_of_few(const ta_args &a, ta_work &w, int &first) {
+    const int lane = threadIdx.x & 63;
+    const ta_request r(a, min(lane, a.B - 1));
+    const int stages = lane < a.B ? r.stages() : 0, upto = (int)bs_scan((uint32_t)stages, [](uint32_t x, uint32_t y) { return x + y; });
+    if (FIRST) {
+        const int sum = (int)bs_read((uint32_t)upto, 63), shares = ta_shares(a, sum);
+        if (blockIdx.x == 0 && threadIdx.x == 0) a.before[a.B] = sum;
+        if (w.g >= shares) return false;
+        w.at = first = ta_begins(w.g, sum, shares);
+        w.end = ta_begins(w.g + 1, sum, shares);
+    }
+    if (w.at >= w.end) return false;
+    w.b = __builtin_ctzll(__ballot(w.at >= upto - stages && w.at < upto));
+    w.before = (int)bs_read((uint32_t)(upto - stages), w.b);
+    w.rq = ta_uniform(r, w.b);
+    w.take(first);
+    return true;
+}
+// More: the workgroup looks for the first one together, and goes on from there.
+template <int WAVES>
+__device__ __forceinline__ bool ta_first_of_many(const ta_args &a, ta_work &w, int &first) {
+    __shared__ int sums[WAVES], found[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), THREADS = WAVES * 64;
+    auto plus = [](uint32_t x, uint32_t y) { return x + y; };
+    uint32_t all = 0;
+    for (int i = tid; i < a.B; i += THREADS) all += ta_request(a, i).stages();
+    all = bs_read(bs_scan(all, plus), 63);
+    if (lane == 0) sums[wave] = (int)all;
+    __syncthreads();
+    int sum = 0;
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) all += __shfl_xor(all, o, 64);
-        if (lane == 0) sums[wave] = all;
+    for (int v = 0; v < WAVES; v++) sum += sums[v];
+    const int shares = ta_shares(a, sum);
+    if (blockIdx.x == 0 && tid == 0) a.before[a.B] = sum;
+    if (w.g >= shares) return false;
+    w.at = first = ta_begins(w.g, sum, shares);
+    w.end = ta_begins(w.g + 1, sum, shares);
+    if (w.at >= w.end) return false;
+    int before = 0;
+    for (int i0 = 0; i0 < a.B && before <= w.at; i0 += THREADS) {
+        const int i = i0 + tid, mine = i < a.B ? ta_request(a, i).stages() : 0, upto = (int)bs_scan((uint32_t)mine, plus);
         __syncthreads();
-        all = 0;
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) all += sums[w];
-        most = max(a.least, (all + a.parts - 1) / a.parts);
-        if (first_part) further = ta_further(ta_request(a, b).stages(), most);
-    }
-    if (!first_part || further > 0) {            // numbers of the further parts: a running sum over the requests
-        if (tid == 0) found[0] = -1;
-        int before = 0;
-        const int wanted = work - a.B;
-        for (int i0 = 0; i0 < a.B; i0 += THREADS) {
-            const int i = i0 + tid, mine = i < a.B ? ta_further(ta_request(a, i).stages(), most) : 0;
-            int s = mine;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int below = __shfl_up(s, o, 64);
-                if (lane >= o) s += below;
-            }
-            __syncthreads();
-            if (lane == 63) sums[wave] = s;
-            __syncthreads();
-            int ahead = before;
-#pragma unroll
-            for (int w = 0; w < WAVES; w++) {
-                if (w < wave) ahead += sums[w];
-                before += sums[w];
-            }
-            const int first = ahead + s - mine;
-            if (first_part ? i == b : wanted >= first && wanted < first + mine) {
-                found[0] = i;
-                found[1] = first;
-                found[2] = mine;
-            }
-        }
+        if (lane == 63) sums[wave] = upto;
         __syncthreads();
-        if (found[0] < 0) return;                // no such part
-        b = __builtin_amdgcn_readfirstlane(found[0]);
-        place = __builtin_amdgcn_readfirstlane(found[1]);
-        further = __builtin_amdgcn_readfirstlane(found[2]);
-        if (!first_part) part = wanted - place + 1;
-    }
-    const ta_request rq(a, b);
-    const int64_t orow = (int64_t)a.heads * D;
-    if (part == 0 && unit == 0) {                // rows that are no node: zeros; this request's, and some of those behind the last request's
-        auto idle = [&](int t) {
-            for (int i = tid; i < orow; i += THREADS) a.out[t * orow + i] = (half_t)0;
-            if (a.parts > 0 && tid < 2) a.parts_of[2 * t + tid] = 0;
-        };
-        for (int t = rq.start + rq.n; t < rq.end; t++) idle(t);
-        const int last = min(max(a.starts[a.B], 0), a.T), first = min(max(a.starts[0], 0), a.T);
-        for (int t = last + b; t < a.T; t += a.B) idle(t);
-        for (int t = b; t < first; t += a.B) idle(t);
-        if (a.parts > 0)
-            for (int j = tid; j < rq.n; j += THREADS) {
-                a.parts_of[2 * (rq.start + j)] = place;
-                a.parts_of[2 * (rq.start + j) + 1] = further;
-            }
-    }
-    const int all_rows = rq.n * rep;
-    if (row0 >= all_rows) return;
-    const int held = rq.len - rq.n, stages = rq.stages(), parts = further + 1;
-    const int st_first = (int)((int64_t)stages * part / parts), st_end = (int)((int64_t)stages * (part + 1) / parts);
-
-    // ---- the rows of the cache
-    const int64_t page_step = (int64_t)a.kv_heads * D << a.shift, head_at = (int64_t)hk * D << a.shift;
-    const int32_t *ids = a.table + (int64_t)b * a.max_pages;
-    const int last_tile = (rq.len - 1) / 16;
-    // the pages of a stage's tiles (those behind the last tile are the last again), and which of them exist; ones that do not are read as another of the stage
-    struct stage_pages { int id[4]; };
-    auto pages_of = [&](int st) {
-        stage_pages p;
+        int from = before + upto - mine;
 #pragma unroll
-        for (int i = 0; i < 4; i++) p.id[i] = ids[(min(4 * st + i, last_tile) * 16) >> a.shift];
-        return p;
-    };
-    auto good = [&](int id) { return id >= 0 && id < a.pool; };
-    // lane -> row of a tile and piece of it, for the requests of 1 KB, and where they lie: K's pieces XOR-ed with the row (D == 64: two rows to a line of 256 bytes; V's rows change places in it by turns)
-    auto request = [&](auto stage, int st, const stage_pages &p) {
-        half_t *const k_to = decltype(stage)::value ? sk1 : sk0, *const v_to = decltype(stage)::value ? sv1 : sv0;
-        int other = 0;
-#pragma unroll
-        for (int i = 3; i >= 0; i--) other = good(p.id[i]) ? p.id[i] : other;
-#pragma unroll
-        for (int i = 0; i < TILES; i++) {
-            const int tile = wave * TILES + i;
-            int id = p.id[0];
-#pragma unroll
-            for (int e = 1; e < 4; e++) id = tile == e ? p.id[e] : id;
-            id = good(id) ? id : other;
-            const int pos = min(4 * st + tile, last_tile) * 16, rows = rq.len - pos;       // rows of the tile that are there (the last one again behind them)
-            const int64_t at = (int64_t)id * page_step + head_at + (int64_t)(pos & ((1 << a.shift) - 1)) * D;
-            const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void *)(a.kpages + at), 0, -1, 0x00020000);
-            const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void *)(a.vpages + at), 0, -1, 0x00020000);
-#pragma unroll
-            for (int j = 0; j < LINES; j++) {
-                const int line = 4 * j + g;
-                const int krow = D == 128 ? line : 2 * line + (r16 >> 3), piece = D == 128 ? r16 ^ line : (r16 & 7) ^ (line & 7);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (ta_lds)(k_to + tile * 16 * D + j * 512), 16, min(krow, rows - 1) * (D * 2) + 16 * piece, 0, 0, 0);
-            }
-#pragma unroll
-            for (int j = 0; j < LINES; j++) {
-                const int line = 4 * j + g;
-                const int vrow = D == 128 ? line : 2 * line + ((r16 >> 3) ^ (line >> 1 & 1)), piece = D == 128 ? r16 : r16 & 7;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (ta_lds)(v_to + tile * 16 * D + j * 512), 16, min(vrow, rows - 1) * (D * 2) + 16 * piece, 0, 0, 0);
-            }
+        for (int v = 0; v < WAVES; v++) {
+            if (v < wave) from += sums[v];
+            before += sums[v];
         }
-    };
-    auto k_at = [](int row, int piece) { return D == 128 ? row * D + 8 * (piece ^ (row & 15)) : (row >> 1) * 128 + 64 * (row & 1) + 8 * (piece ^ (row >> 1 & 7)); };
-    auto v_at = [](int row) { return D == 128 ? row * D : (row >> 1) * 128 + 64 * ((row ^ row >> 2) & 1); };
-
-    if (tid < 2) odd_nodes[tid] = 0;             // (behind a barrier of the first stage when it is next written)
-    if (tid == 2) odd_held = 0;
-    stage_pages now = pages_of(st_first), next = pages_of(min(st_first + 1, st_end - 1));
-    request(std::integral_constant<int, 0>{}, st_first, now);
-
-    // ---- the rows of q
-    const bool mine = row0 + 16 * QT * wr < all_rows;
-    half8_t q8[QT][NC];
-    uint64_t mask[QT];
-#pragma unroll
-    for (int t = 0; t < QT; t++) {
-        const int row = min(row0 + 16 * (QT * wr + t) + r16, all_rows - 1), node = row / rep;
-        const half_t *p = a.q + (int64_t)(rq.start + node) * a.ldq + (hk * rep + row - node * rep) * D + 8 * g;
-        if (((uintptr_t)a.q | (uintptr_t)(2 * a.ldq)) % 16 == 0) {
-#pragma unroll
-            for (int c = 0; c < NC; c++) q8[t][c] = *reinterpret_cast<const half8_t *>(p + 32 * c);
-        } else {
-#pragma unroll
-            for (int c = 0; c < NC; c++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) q8[t][c][e] = p[32 * c + e];
-        }
-        mask[t] = (uint64_t)a.masks[rq.start + node] & (rq.n < 64 ? (1ull << rq.n) - 1 : ~0ull);
-    }
-
-    const float scale2 = (D == 128 ? 0.08838834764831845f : 0.125f) * 1.4426950408889634f;    // log2(e) / sqrt(D)
-    float m[QT], l[QT];                          // of row r16 of a tile; l over this lane's positions only
-    float4_t acc[QT][W];
-#pragma unroll
-    for (int t = 0; t < QT; t++) {
-        m[t] = TA_LOW;
-        l[t] = 0.f;
-#pragma unroll
-        for (int j = 0; j < W; j++) acc[t][j] = (float4_t)0.f;
-    }
-    // infinities and NaN in a stage's v become zeros, and their positions are noted
-    auto clean = [&](half_t *sv, int st) {
-#pragma unroll 1
-        for (int i = tid; i < TA_P * D / 8; i += THREADS) {
-            half8_t v = *reinterpret_cast<const half8_t *>(sv + 8 * i);
-            bool odd = false;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const bool fine = (__builtin_bit_cast(uint16_t, (half_t)v[e]) & 0x7c00u) != 0x7c00u;
-                odd = odd || !fine;
-                v[e] = fine ? v[e] : (half_t)0;
-            }
-            if (!odd) continue;
-            *reinterpret_cast<half8_t *>(sv + 8 * i) = v;
-            const int line = i / 16, row = D == 128 ? line : 2 * line + ((i >> 3 & 1) ^ (line >> 1 & 1)), node = TA_P * st + row - held;
-            if (node < 0) odd_held = 1;
-            else if (node < rq.n) atomicOr(&odd_nodes[node >> 5], 1u << (node & 31));
-        }
-        __syncthreads();
-    };
-    // a stage, from LDS: scores, weights, output.  masked: some of its positions are nodes, behind the last one, or of pages that do not exist (bits of `there`: tiles that do)
-    auto step = [&](bool masked, const half_t *sk, const half_t *sv, int st, int there) __attribute__((always_inline)) {
-        float4_t s[QT][A];
-#pragma unroll
-        for (int i = 0; i < A; i++) {
-            half8_t k8[NC];
-#pragma unroll
-            for (int c = 0; c < NC; c++) k8[c] = *reinterpret_cast<const half8_t *>(sk + k_at(16 * (A * wp + i) + r16, 4 * c + g));
-#pragma unroll
-            for (int t = 0; t < QT; t++) s[t][i] = (float4_t)0.f;
-#pragma unroll
-            for (int c = 0; c < NC; c++)
-#pragma unroll
-                for (int t = 0; t < QT; t++) s[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8[c], q8[t][c], s[t][i], 0, 0, 0);
-        }
-        vec_t v8[8];
-        auto fetch_v = [&](int h) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) v8[i] = *reinterpret_cast<const vec_t *>(sv + v_at(16 * (A * wp + 2 * h + (i >> 2)) + 4 * g + (i & 3)) + W * r16);
-        };
-        fetch_v(0);                              // (arrives during the softmax)
-        __builtin_amdgcn_sched_barrier(0);
-        if (masked) {
-#pragma unroll
-            for (int i = 0; i < A; i++) {
-                const int node = TA_P * st + 16 * (A * wp + i) + 4 * g - held;             // (below 0: a position that the request held)
-#pragma unroll
-                for (int t = 0; t < QT; t++) {
-                    uint32_t seen = node >= 64 ? 0 : node >= 0 ? (uint32_t)(mask[t] >> node) : node <= -4 ? 15 : (uint32_t)mask[t] << -node | ((1u << -node) - 1);
-                    if (!(there >> (A * wp + i) & 1)) seen = 0;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) s[t][i][e] = seen >> e & 1 ? s[t][i][e] : -INFINITY;
-                }
-            }
-        }
-        float r[QT];
-        half8_t p8[A / 2][QT];
-#pragma unroll
-        for (int t = 0; t < QT; t++) {
-            float mx = s[t][0][0];
-#pragma unroll
-            for (int i = 1; i < 4 * A; i++) mx = fmaxf(mx, s[t][i >> 2][i & 3]);
-            mx = across<32>(across<16>(mx));
-            const float mn = fmaxf(m[t], mx * scale2), from = mn - TA_UP;
-            r[t] = __builtin_amdgcn_exp2f(m[t] - mn);
-            m[t] = mn;
-            float sum[2] = {0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < 4 * A; i++) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i >> 2][i & 3], scale2, -from));
-                sum[i & 1] += p;
-                p8[i >> 3][t][i & 7] = (half_t)p;
-            }
-            l[t] = l[t] * r[t] + (sum[0] + sum[1]);
-        }
-        if (__any(r[0] != 1.f || r[QT - 1] != 1.f)) {
-#pragma unroll
-            for (int t = 0; t < QT; t++)
-#pragma unroll
-                for (int j = 0; j < W; j++) acc[t][j] *= r[t];
-        }
-#pragma unroll
-        for (int h = 0; h < A / 2; h++) {
-#pragma unroll
-            for (int j = 0; j < W; j++) {
-                const half8_t v = {v8[0][j], v8[1][j], v8[2][j], v8[3][j], v8[4][j], v8[5][j], v8[6][j], v8[7][j]};
-#pragma unroll
-                for (int t = 0; t < QT; t++) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p8[h][t], acc[t][j], 0, 0, 0);
-            }
-            if (h + 1 < A / 2) fetch_v(h + 1);
-        }
-    };
-    auto walk = [&](auto stage, int st) __attribute__((always_inline)) {
-        // this wave's requests for the stage have landed; behind the barrier everybody's have, and nobody reads the other stage any more
-        __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));
-        __builtin_amdgcn_sched_barrier(0);
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
-        int there = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) there |= (int)good(now.id[i]) << i;
-        if (st + 1 < st_end) {
-            request(std::integral_constant<int, 1 - decltype(stage)::value>{}, st + 1, next);
-            now = next;
-            next = pages_of(min(st + 2, st_end - 1));
-        }
-        half_t *const sk = decltype(stage)::value ? sk1 : sk0, *const sv = decltype(stage)::value ? sv1 : sv0;
-        const bool masked = TA_P * (st + 1) > held || there != 15;
-        if (masked) clean(sv, st);
-        if (mine) step(masked, sk, sv, st, there);
-    };
-    for (int st = st_first; st < st_end; st += 2) {
-        walk(std::integral_constant<int, 0>{}, st);
-        if (st + 1 < st_end) walk(std::integral_constant<int, 1>{}, st + 1);
-    }
-
-    // ---- what the waves have: rows that are NaN are computed again, the others put together
-    for (int i = tid; i < ROWS; i += THREADS) again[i] = 0;
-    __syncthreads();                             // (nobody reads a stage any more: the weighted v take their place)
-    auto wo_at = [&](int w, int row) -> float * {                          // [WP][ROWS][D] over the four arrays
-        constexpr int PER = TA_P / 2;            // rows of an array
-        const int i = w * ROWS + row, array = i / PER;
-        return reinterpret_cast<float *>(array == 0 ? sk0 : array == 1 ? sk1 : array == 2 ? sv0 : sv1) + (i - array * PER) * D;
-    };
-    static_assert(WP * ROWS <= 4 * (TA_P / 2), "what the waves leave must fit the stages");
-    if (mine) {
-#pragma unroll
-        for (int t = 0; t < QT; t++) {
-            const int row = 16 * (QT * wr + t) + r16;
-            l[t] = across<32, true>(across<16, true>(l[t]));
-            if (g == 0) {
-                wm[wp][row] = m[t];
-                wl[wp][row] = l[t];
-            }
-            float sum = l[t];
-#pragma unroll
-            for (int j = 0; j < W; j++) sum += (acc[t][j][0] - acc[t][j][0]) + (acc[t][j][1] - acc[t][j][1]) + (acc[t][j][2] - acc[t][j][2]) + (acc[t][j][3] - acc[t][j][3]);
-            // NaN, or an infinity; a position that it sees had one
-            if (sum != sum || odd_held != 0 || (mask[t] & ((uint64_t)odd_nodes[1] << 32 | odd_nodes[0])) != 0) again[row] = 1;
-#pragma unroll
-            for (int i = 0; i < 4; i++)          // row 4 g + i of product j is dimension W (4 g + i) + j
-#pragma unroll
-                for (int j = 0; j < W; j += 4)
-                    *reinterpret_cast<float4_t *>(wo_at(wp, row) + W * (4 * g + i) + j) = (float4_t){acc[t][j][i], acc[t][j + 1][i], acc[t][j + 2][i], acc[t][j + 3][i]};
+        if (w.at >= from && w.at < from + mine) {
+            found[0] = i;
+            found[1] = from;
         }
     }
     __syncthreads();
-    const int rows = min(ROWS, all_rows - row0);
-    for (int row = wave; row < rows; row += WAVES) {
-        if (__builtin_expect(__builtin_amdgcn_readfirstlane(again[row]) == 0, 1)) continue;
-        // One row by one wave: the largest score first, then the sums.  A lane has a position's score, and owns dimensions EACH lane .. of the output.
-        constexpr int EACH = D / 64;
-        const int node = (row0 + row) / rep, p_end = min(st_end * TA_P, rq.len);
-        const half_t *qr = a.q + (int64_t)(rq.start + node) * a.ldq + (hk * rep + row0 + row - node * rep) * D;
+    w.b = __builtin_amdgcn_readfirstlane(found[0]);
+    w.before = __builtin_amdgcn_readfirstlane(found[1]);
+    w.rq = ta_uniform(ta_request(a, w.b), 0);
+    w.take(first);
+    return true;
+}
+template <int WAVES>
+__device__ __forceinline__ bool ta_first(const ta_args &a, int g, ta_work &w, int &first) {
+    w.g = g;
+    if (a.shares == 0) {                         // one request
+        w.b = g;
+        w.rq = ta_uniform(ta_request(a, g), 0);
+        w.before = w.at = first = 0;
+        w.end = w.rq.stages();
+        if (w.end == 0) return false;
+        w.take(first);
+        return true;
+    }
+    return a.B <= 64 ? ta_next_of_few<true>(a, w, first) : ta_first_of_many<WAVES>(a, w, first);
+}
+__device__ __forceinline__ bool ta_next(const ta_args &a, ta_work &w, int &first) {
+    if (w.at >= w.end) return false;
+    if (a.B <= 64) return ta_next_of_few<false>(a, w, first);
+    do {
+        w.before += w.rq.stages();
+        w.rq = ta_uniform(ta_request(a, ++w.b), 0);
+    } while (w.rq.n == 0);
+    w.take(first);
+    return true;
+}
+// rows that are no node are zeros: those of every request that is this workgroup's to see to, and some of those of no request
+template <int THREADS>
+__device__ __forceinline__ void ta_idle(const ta_args &a, int g, int of, int D) {
+    const int64_t orow = (int64_t)a.heads * D;
+    auto idle = [&](int t) {
+        for (int64_t i = threadIdx.x; i < orow; i += THREADS) a.out[t * orow + i] = (half_t)0;
+    };
+    for (int b = g; b < a.B; b += of) {
+        const ta_request r(a, b);
+        for (int t = r.start + r.n; t < r.end; t++) idle(t);
+    }
+    const int last = min(max(a.starts[a.B], 0), a.T), first = min(max(a.starts[0], 0), a.T);
+    for (int t = last + g; t < a.T; t += of) idle(t);
+    for (int t = g; t < first; t += of) idle(t);
+}
+// what a part leaves of a node's head
+__device__ __forceinline__ float *ta_part_row(const ta_args &a, int slot, int node, int head, int D) {
+    return a.part + (((int64_t)slot * a.nodes + node) * a.heads + head) * (D + 4);
+}
+// One row by one wave, in fp32, over positions p_first .. p_end - 1: the largest score first, then the sums.  A lane has a position's score, and owns dimensions D / 64 * lane .. of the output.
+template <int D>
+struct ta_again {
+    float top, sum, o[D / 64];
+    __device__ __forceinline__ ta_again(const ta_args &a, const ta_request &rq, const int32_t *ids, int node, int head, int hk, int p_first, int p_end, float scale2) {
+        constexpr int PER = D / 64;
+        const int lane = threadIdx.x & 63, held = rq.len - rq.n;
+        const half_t *qr = a.q + (int64_t)(rq.start + node) * a.ldq + head * D;
         const uint64_t sees = (uint64_t)a.masks[rq.start + node];
         auto where = [&](int p) {                // halves in front of position p; -1: not seen, or not there
             if (p >= p_end || (p >= held && !(sees >> (p - held) & 1))) return (int64_t)-1;
             const int id = ids[p >> a.shift];
-            return good(id) ? (int64_t)id * page_step + head_at + (int64_t)(p & ((1 << a.shift) - 1)) * D : (int64_t)-1;
+            return id >= 0 && id < a.pool ? ((((int64_t)id * a.kv_heads + hk) << a.shift) + (p & ((1 << a.shift) - 1))) * D : (int64_t)-1;
         };
         auto score = [&](int64_t at) {
             if (at < 0) return -INFINITY;
@@ -405,97 +223,702 @@ __global__ __launch_bounds__(WR *WP * 64, WR *WP == 2 ? 1 : 2) void attention_tr
             }
             return d * scale2;
         };
-        float top = -INFINITY, sum = 0.f, o[EACH] = {};
-        for (int p0 = st_first * TA_P; p0 < p_end; p0 += 64) top = fmaxf(top, score(where(p0 + lane)));
+        top = -INFINITY;
+        sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < PER; e++) o[e] = 0.f;
+        for (int p0 = p_first; p0 < p_end; p0 += 64) top = fmaxf(top, score(where(p0 + lane)));
 #pragma unroll
         for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
         const float from = top == -INFINITY ? 0.f : top;
-        for (int p0 = st_first * TA_P; p0 < p_end; p0 += 64) {
+        for (int p0 = p_first; p0 < p_end; p0 += 64) {
             const int64_t at = where(p0 + lane);
-            const float w = __builtin_amdgcn_exp2f(score(at) - from + TA_UP);      // (a score of -inf weighs nothing; one of +inf, or NaN, is NaN)
-            sum += w;
+            const float weight = __builtin_amdgcn_exp2f(score(at) - from + TA_UP);       // (a score of -inf weighs nothing; one of +inf, or NaN, is NaN)
+            sum += weight;
 #pragma unroll 1
             for (int i = 0; i < 64; i++) {
                 const int64_t ai = __shfl(at, i, 64);
-                const float wi = __shfl(w, i, 64);
+                const float wi = __shfl(weight, i, 64);
                 if (ai < 0 || wi == 0.f) continue;
 #pragma unroll
-                for (int e = 0; e < EACH; e++) o[e] = __builtin_fmaf(wi, (float)a.vpages[ai + EACH * lane + e], o[e]);
+                for (int e = 0; e < PER; e++) o[e] = __builtin_fmaf(wi, (float)a.vpages[ai + PER * lane + e], o[e]);
             }
         }
 #pragma unroll
         for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x, 64);
-        if (lane == 0) {
-#pragma unroll
-            for (int w = 0; w < WP; w++) {
-                wm[w][row] = w == 0 ? (top == -INFINITY ? TA_LOW : top) : TA_LOW;
-                wl[w][row] = w == 0 ? sum : 0.f;
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < EACH; e++) wo_at(0, row)[EACH * lane + e] = o[e];
+        top = top == -INFINITY ? TA_LOW : top;
     }
-    __syncthreads();
-    for (int it = tid; it < rows * (D / 4); it += THREADS) {
-        const int row = it / (D / 4), dim = it % (D / 4) * 4, all_row = row0 + row, node = all_row / rep, head = hk * rep + all_row - node * rep;
-        float mx = wm[0][row];
+};
+constexpr __device__ float ta_scale(int D) { return (D == 128 ? 0.08838834764831845f : 0.125f) * 1.4426950408889634f; }       // log2(e) / sqrt(D)
+
+// The pages of 64 tiles of 16 positions at a time, a lane a tile: two of each of 32 stages, which are `step` apart (tiles behind the last one are the last again).  A page that does not exist is
+// read as the other of its stage; `gone`: tiles of such.
+struct ta_pages {
+    const int32_t *ids;
+    int last_tile, shift, pool, step, raw, id;
+    uint64_t gone;
+    __device__ __forceinline__ bool good(int i) const { return i >= 0 && i < pool; }
+    __device__ __forceinline__ void load(int st) {
+        const int lane = threadIdx.x & 63;
+        raw = ids[(min(2 * st + 2 * step * (lane >> 1) + (lane & 1), last_tile) * 16) >> shift];
+    }
+    __device__ __forceinline__ void take() {
+        gone = ~__ballot(good(raw));
+        const int beside = __builtin_amdgcn_update_dpp(0, raw, 0xb1, 0xf, 0xf, true);      // quad_perm 1, 0, 3, 2
+        id = good(raw) ? raw : good(beside) ? beside : 0;
+    }
+};
+
+// whether a row sees the nodes of four positions, the first of them `node` (below 0: a position that the request held); bits
+__device__ __forceinline__ uint32_t ta_seen(uint64_t mask, int node) {
+    return node >= 64 ? 0 : node >= 0 ? (uint32_t)(mask >> node) : node <= -4 ? 15 : (uint32_t)mask << -node | ((1u << -node) - 1);
+}
+
+// ---- few rows: what counts is the cache's bytes.  A wave has all 16 QT rows and every fourth stage, K and V in registers: K of its next stage is requested behind the
+// scores, V behind the output product, so that eight waves of a CU have 128 KB on their way.  What the waves have is put together in LDS.
+template <int D, int QT, bool STREAM>
+__global__ __launch_bounds__(256, 2) void attention_tree_few_kernel(const ta_args a) {
+    constexpr int W = D / 16, NC = D / 32, WAVES = 4, THREADS = WAVES * 64, ROWS = 16 * QT;
+    typedef half_t vec_t __attribute__((ext_vector_type(W)));
+    __shared__ __attribute__((aligned(16))) float wo[WAVES][ROWS][D + 4];              // (rows a sixteenth of the banks' turn apart)
+    __shared__ float wm[WAVES][ROWS], wl[WAVES][ROWS];
+    __shared__ uint64_t odd_of[WAVES];           // nodes at which something in v is infinite or NaN
+    __shared__ uint32_t bad[WAVES][ROWS];        // rows whose sums are not finite, or all, where a held position has such
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
+    const int hk = blockIdx.x % a.kv_heads, g_of = blockIdx.x / a.kv_heads, rep = a.heads / a.kv_heads;
+    const int64_t page_step = (int64_t)a.kv_heads * D << a.shift, head_at = (int64_t)hk * D << a.shift;
+    ta_work w;
+    int first;
+    for (bool more = ta_first<WAVES>(a, g_of, w, first); more; more = ta_next(a, w, first)) {
+        const ta_request &rq = w.rq;
+        const int rows = rq.n * rep, held = rq.len - rq.n, st_end = w.st_end;
+        if (hk == 0 && w.st == 0 && tid == 0 && a.shares > 0) a.before[w.b] = w.before;
+        ta_pages pg = {a.table + (int64_t)w.b * a.max_pages, (rq.len - 1) / 16, a.shift, a.pool, WAVES, 0, 0, 0};
+
+        half8_t k8[2][NC];
+        vec_t v8[8];
+        int st = w.st + wave, rel = 0;        // (rel: lane of the stage's first tile in the pages)
+        auto tile_at = [&](const half_t *of, int st, int lane_of, int i, int &rows_there) {
+            const int pos = min(2 * st + i, pg.last_tile) * 16;
+            rows_there = rq.len - pos;               // (the last one again behind them)
+            return __builtin_amdgcn_make_buffer_rsrc((void *)(of + head_at + (int64_t)(int)bs_read((uint32_t)pg.id, lane_of + i) * page_step + (pos & ((1 << a.shift) - 1)) * D), 0, -1, 0x00020000);
+        };
+        auto fetch_k = [&](int st, int lane_of) __attribute__((always_inline)) {
 #pragma unroll
-        for (int w = 1; w < WP; w++) mx = fmaxf(mx, wm[w][row]);
-        float den = 0.f;
-        float4_t o = (float4_t)0.f;
+            for (int i = 0; i < 2; i++) {
+                int there;
+                const __amdgpu_buffer_rsrc_t rsrc = tile_at(a.kpages, st, lane_of, i, there);
+                const int at = (there < 16 ? min(r16, there - 1) : r16) * (2 * D) + 16 * g;
 #pragma unroll
-        for (int w = 0; w < WP; w++) {
-            if (wl[w][row] != 0.f) {             // (0: nothing was seen)
-                const float r = wm[w][row] == mx ? 1.f : __builtin_amdgcn_exp2f(wm[w][row] - mx);
-                den += r * wl[w][row];
-                o += r * *reinterpret_cast<const float4_t *>(wo_at(w, row) + dim);
+                for (int c = 0; c < NC; c++) k8[i][c] = __builtin_bit_cast(half8_t, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at + 64 * c, 0, STREAM ? 2 : 0));
             }
+        };
+        auto fetch_v = [&](int st, int lane_of) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                int there;
+                const __amdgpu_buffer_rsrc_t rsrc = tile_at(a.vpages, st, lane_of, i, there);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int at = (there < 16 ? min(4 * g + e, there - 1) : 4 * g + e) * (2 * D) + 2 * W * r16;
+                    if constexpr (D == 128) v8[4 * i + e] = __builtin_bit_cast(vec_t, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, STREAM ? 2 : 0));
+                    else v8[4 * i + e] = __builtin_bit_cast(vec_t, __builtin_amdgcn_raw_buffer_load_b64(rsrc, at, 0, STREAM ? 2 : 0));
+                }
+            }
+        };
+        if (st < st_end) {
+            pg.load(st);
+            pg.take();
+            fetch_k(st, 0);
+            fetch_v(st, 0);
+            pg.load(st + 32 * WAVES);
         }
-        if (further > 0) {
-            const int64_t at = part == 0 ? (int64_t)(rq.start + node) * a.heads + head : ((int64_t)a.T + (int64_t)(place + part - 1) * a.nodes + node) * a.heads + head;
-            float *to = a.part + at * (D + 4);
-            *reinterpret_cast<float4_t *>(to + 4 + dim) = o;
-            if (dim == 0) {
-                to[0] = mx;
-                to[1] = den;
+
+        half8_t q8[QT][NC];
+        uint64_t mask[QT];
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+            const int row = min(16 * t + r16, rows - 1), node = ta_node(row, rep, a.per_rep);
+            const half_t *p = a.q + (int64_t)(rq.start + node) * a.ldq + (hk * rep + row - node * rep) * D + 8 * g;
+            if (((uintptr_t)a.q | (uintptr_t)(2 * a.ldq)) % 16 == 0) {
+#pragma unroll
+                for (int c = 0; c < NC; c++) q8[t][c] = *reinterpret_cast<const half8_t *>(p + 32 * c);
+            } else {
+#pragma unroll
+                for (int c = 0; c < NC; c++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) q8[t][c][e] = p[32 * c + e];
             }
-        } else {
-            half_t *to = a.out + (int64_t)(rq.start + node) * orow + (int64_t)head * D + dim;
+            mask[t] = (uint64_t)a.masks[rq.start + node] & (rq.n < 64 ? (1ull << rq.n) - 1 : ~0ull);
+        }
+        const float scale2 = ta_scale(D);
+        float m[QT], l[QT];                          // of row r16 of a tile; l over this lane's positions only
+        float4_t acc[QT][W];
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+            m[t] = TA_LOW;
+            l[t] = 0.f;
+#pragma unroll
+            for (int j = 0; j < W; j++) acc[t][j] = (float4_t)0.f;
+        }
+        bool odd_held = false;                       // (of this lane) v at a held position, or at these nodes, has an infinity or NaN
+        uint64_t odd_nodes = 0;
+        while (st < st_end) {
+            const int next = st + WAVES;
+            const int bits = (int)(pg.gone >> rel & 3);        // tiles of pages that do not exist
+            float4_t s[QT][2];
+#pragma unroll
+            for (int t = 0; t < QT; t++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) s[t][i] = (float4_t)0.f;
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int t = 0; t < QT; t++) s[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8[i][c], q8[t][c], s[t][i], 0, 0, 0);
+            rel += 2;
+            if (rel == 64) {
+                rel = 0;
+                pg.take();
+                pg.load(next + 32 * WAVES);
+            }
+            if (next < st_end) fetch_k(next, rel);
+            const bool masked = TA_P * (st + 1) > held || bits != 0;
+            if (masked) {
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int t = 0; t < QT; t++) {
+                        const uint32_t seen = bits >> i & 1 ? 0 : ta_seen(mask[t], TA_P * st + 16 * i + 4 * g - held);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) s[t][i][e] = seen >> e & 1 ? s[t][i][e] : -INFINITY;
+                    }
+            }
+            half8_t p8[QT];
+            float r[QT];
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
+                float mx = s[t][0][0];
+#pragma unroll
+                for (int i = 1; i < 8; i++) mx = fmaxf(mx, s[t][i >> 2][i & 3]);
+                mx = across<32>(across<16>(mx));
+                const float mn = fmaxf(m[t], mx * scale2), from = mn - TA_UP;
+                r[t] = __builtin_amdgcn_exp2f(m[t] - mn);
+                m[t] = mn;
+                float sum[2] = {0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i >> 2][i & 3], scale2, -from));
+                    sum[i & 1] += p;
+                    p8[t][i] = (half_t)p;
+                }
+                l[t] = l[t] * r[t] + (sum[0] + sum[1]);
+            }
+            if (masked) {                            // infinities and NaN (times zero: NaN) become zeros, and their positions are noted
+                vec_t check = (vec_t)(half_t)0;
+#pragma unroll
+                for (int i = 0; i < 8; i++) check += v8[i] * (vec_t)(half_t)0;
+                bool odd = false;
+#pragma unroll
+                for (int j = 0; j < W; j++) odd = odd || check[j] != check[j];
+                if (__builtin_expect(__any(odd), 0)) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        bool here = false;
+#pragma unroll
+                        for (int j = 0; j < W; j++) {
+                            const bool fine = (__builtin_bit_cast(uint16_t, (half_t)v8[i][j]) & 0x7c00u) != 0x7c00u;
+                            here = here || !fine;
+                            v8[i][j] = fine ? v8[i][j] : (half_t)0;
+                        }
+                        const int node = TA_P * st + 16 * (i >> 2) + 4 * g + (i & 3) - held;
+                        if (here && node < 0) odd_held = true;
+                        if (here && node >= 0 && node < rq.n) odd_nodes |= 1ull << node;
+                    }
+                }
+            }
+            if (__any(r[0] != 1.f || r[QT - 1] != 1.f)) {
+#pragma unroll
+                for (int t = 0; t < QT; t++)
+#pragma unroll
+                    for (int j = 0; j < W; j++) acc[t][j] *= r[t];
+            }
+#pragma unroll
+            for (int j = 0; j < W; j++) {
+                const half8_t v = {v8[0][j], v8[1][j], v8[2][j], v8[3][j], v8[4][j], v8[5][j], v8[6][j], v8[7][j]};
+#pragma unroll
+                for (int t = 0; t < QT; t++) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p8[t], acc[t][j], 0, 0, 0);
+            }
+            if (next < st_end) fetch_v(next, rel);
+            st = next;
+        }
+
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+            const int row = 16 * t + r16;
+            l[t] = across<32, true>(across<16, true>(l[t]));
+            if (g == 0) {
+                wm[wave][row] = m[t];
+                wl[wave][row] = l[t];
+            }
+            float sum = l[t];                        // (not finite: NaN, or an infinity)
+#pragma unroll
+            for (int j = 0; j < W; j++) sum += (acc[t][j][0] - acc[t][j][0]) + (acc[t][j][1] - acc[t][j][1]) + (acc[t][j][2] - acc[t][j][2]) + (acc[t][j][3] - acc[t][j][3]);
+            const uint64_t not_finite = __ballot(sum != sum);
+            if (g == 0) bad[wave][row] = (not_finite >> r16 | not_finite >> (r16 + 16) | not_finite >> (r16 + 32) | not_finite >> (r16 + 48)) & 1;
+#pragma unroll
+            for (int i = 0; i < 4; i++)              // row 4 g + i of product j is dimension W (4 g + i) + j
+#pragma unroll
+                for (int j = 0; j < W; j += 4)
+                    *reinterpret_cast<float4_t *>(&wo[wave][row][W * (4 * g + i) + j]) = (float4_t){acc[t][j][i], acc[t][j + 1][i], acc[t][j + 2][i], acc[t][j + 3][i]};
+        }
+        if (__builtin_expect(__any(odd_held || odd_nodes != 0), 0)) {
+            const bool held_too = __any(odd_held);
+#pragma unroll
+            for (int x = 1; x < 64; x <<= 1)
+                odd_nodes |= (uint64_t)__shfl_xor((uint32_t)(odd_nodes >> 32), x, 64) << 32 | __shfl_xor((uint32_t)odd_nodes, x, 64);
+            if (held_too) odd_nodes = ~0ull;
+            if (held_too && lane < ROWS) bad[wave][lane] = 1;
+        }
+        if (lane == 0) odd_of[wave] = odd_nodes;
+        __syncthreads();
+        // rows that are computed again: not finite in one of the waves, or with such a node in sight
+        uint32_t any = 0;
+        uint64_t odd = 0;
+#pragma unroll
+        for (int v = 0; v < WAVES; v++) {
+            any |= bad[v][lane % ROWS];
+            odd |= odd_of[v];
+        }
+        uint64_t again = __ballot(lane < rows && any != 0);
+        if (__builtin_expect(odd != 0, 0)) again |= __ballot(lane < rows && ((uint64_t)a.masks[rq.start + ta_node(min(lane, rows - 1), rep, a.per_rep)] & odd) != 0);
+        if (__builtin_expect(again != 0, 0)) {             // (the same for all waves)
+            int turn = 0;
+            for (uint64_t left = again; left != 0; left &= left - 1, turn = turn + 1 == WAVES ? 0 : turn + 1) {
+                if (turn != wave) continue;
+                const int row = __builtin_ctzll(left), node = ta_node(row, rep, a.per_rep);
+                const ta_again<D> x(a, rq, pg.ids, node, hk * rep + row - node * rep, hk, w.st * TA_P, min(st_end * TA_P, rq.len), scale2);
+                if (lane < WAVES) {
+                    wm[lane][row] = lane == 0 ? x.top : TA_LOW;
+                    wl[lane][row] = lane == 0 ? x.sum : 0.f;
+                }
+#pragma unroll
+                for (int e = 0; e < D / 64; e++) wo[0][row][D / 64 * lane + e] = x.o[e];
+            }
+            __syncthreads();
+        }
+        // the waves' put together: THREADS / ROWS threads for a row
+        constexpr int SHARE = THREADS / ROWS, PER = D / SHARE / 4;       // ... and four dimensions, PER times
+        const int row = tid / SHARE, node = ta_node(row, rep, a.per_rep), head = hk * rep + row - node * rep;
+        if (row < rows) {
+            float mx = wm[0][row], den = 0.f, r[WAVES];
+#pragma unroll
+            for (int v = 1; v < WAVES; v++) mx = fmaxf(mx, wm[v][row]);
+#pragma unroll
+            for (int v = 0; v < WAVES; v++) {
+                const float sum = wl[v][row];
+                r[v] = sum == 0.f ? 0.f : wm[v][row] == mx ? 1.f : __builtin_amdgcn_exp2f(wm[v][row] - mx);        // (0: nothing was seen)
+                den += sum == 0.f ? 0.f : r[v] * sum;
+            }
             const float inv = den != 0.f ? 1.f / den : 0.f;
+            float *const part_row = ta_part_row(a, max(w.slot, 0), node, head, D);
+            if (w.slot >= 0 && tid % SHARE == 0) {
+                part_row[0] = mx;
+                part_row[1] = den;
+            }
 #pragma unroll
-            for (int e = 0; e < 4; e++) to[e] = (half_t)(den != 0.f ? o[e] * inv : 0.f);
+            for (int i = 0; i < PER; i++) {
+                const int dim = 4 * (tid % SHARE) + 4 * SHARE * i;
+                float4_t o = (float4_t)0.f;
+#pragma unroll
+                for (int v = 0; v < WAVES; v++)
+                    if (r[v] != 0.f) o += r[v] * *reinterpret_cast<const float4_t *>(&wo[v][row][dim]);
+                if (w.slot >= 0) *reinterpret_cast<float4_t *>(part_row + 4 + dim) = o;
+                else {
+                    half4_t h;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) h[e] = (half_t)(den != 0.f ? o[e] * inv : 0.f);
+                    half_t *to = a.out + ((int64_t)(rq.start + node) * a.heads + head) * D + dim;
+                    if (((uintptr_t)a.out & 7) == 0) *reinterpret_cast<half4_t *>(to) = h;
+                    else
+#pragma unroll
+                        for (int e = 0; e < 4; e++) to[e] = h[e];
+                }
+            }
+        }
+        if (w.at < w.end) __syncthreads();       // (the next request's go to the same places)
+    }
+    if (hk == 0) ta_idle<THREADS>(a, g_of, gridDim.x / a.kv_heads, D);
+}
+
+// ---- more rows: K and V come to LDS, for the WR waves of 16 QT rows each.  Many rows: what counts are the products and the softmax, and the scores of a stage are computed one stage ahead (AHEAD).
+// Fewer: what counts are the bytes on their way, a stage more without that.  STREAM: past the last-level cache.
+template <int D, int QT, int WR, bool AHEAD, bool STREAM>
+__global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_args a) {
+    constexpr int W = D / 16, NC = D / 32, THREADS = WR * 64, ROWS = 16 * QT * WR;
+    constexpr int PIECES = D / 32;               // requests of 1 KB (four lines of 256 bytes) for a tile of 16 rows
+    constexpr int SHARE = 4 / WR;                // of a stage's four tiles (two of K, two of V) that a wave requests
+    constexpr int EACH = SHARE * PIECES;
+    typedef half_t vec_t __attribute__((ext_vector_type(W)));
+    // (an array per stage, K and then V: the compiler then knows that a request for one does not touch the others)
+    __shared__ __attribute__((aligned(1024))) half_t s0[2 * TA_P * D], s1[2 * TA_P * D], s2[2 * TA_P * D], s3[2 * TA_P * D];
+    __shared__ uint32_t odd_nodes[2];            // positions where something in v is infinite or NaN
+    __shared__ int odd_held;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
+    const int units = a.kv_heads * a.row_tiles, unit = blockIdx.x % units, work = blockIdx.x / units;
+    const int hk = unit % a.kv_heads, row0 = unit / a.kv_heads * ROWS, rep = a.heads / a.kv_heads;
+
+    const int64_t page_step = (int64_t)a.kv_heads * D << a.shift, head_at = (int64_t)hk * D << a.shift;
+    ta_work w;
+    int first;
+    for (bool more = ta_first<WR>(a, work, w, first); more; more = ta_next(a, w, first)) {
+        const ta_request &rq = w.rq;
+        if (unit == 0 && w.st == 0 && tid == 0 && a.shares > 0) a.before[w.b] = w.before;
+        const int all_rows = rq.n * rep;
+        if (row0 >= all_rows) continue;
+        const int held = rq.len - rq.n, st_first = w.st, st_end = w.st_end;
+        ta_pages pg = {a.table + (int64_t)w.b * a.max_pages, (rq.len - 1) / 16, a.shift, a.pool, 1, 0, 0, 0};
+
+        // ---- the rows of the cache
+        // lane -> row and piece of it, for the requests of 1 KB, and where they lie: K's pieces XOR-ed with the row (D == 64: two rows to a line; V's rows change places in it by turns)
+        auto stage_at = [&](auto ring) -> half_t * { return decltype(ring)::value == 0 ? s0 : decltype(ring)::value == 1 ? s1 : decltype(ring)::value == 2 ? s2 : s3; };
+        const half_t *from[SHARE];                   // K or V of this head
+#pragma unroll
+        for (int u = 0; u < SHARE; u++) {
+            const int v = (wave * SHARE + u) >> 1;
+            from[u] = (v ? a.vpages : a.kpages) + head_at;
+        }
+        int gone_of = 0;                             // two bits for each of the last stages requested, the latest lowest
+        auto request = [&](auto ring, int st) __attribute__((always_inline)) {
+            half_t *const to = stage_at(ring);
+            const int rel = 2 * (st - st_first);
+            if (rel > 0 && (rel & 63) == 0) {
+                pg.take();
+                pg.load(st + 32);
+            }
+            gone_of = gone_of << 2 | (int)(pg.gone >> (rel & 63) & 3);
+#pragma unroll
+            for (int u = 0; u < SHARE; u++) {
+                const int which = wave * SHARE + u, v = which >> 1, tile = which & 1;
+                const int id = (int)bs_read((uint32_t)pg.id, (rel & 63) + tile), pos = min(2 * st + tile, pg.last_tile) * 16;
+                const half_t *p = from[u] + (int64_t)id * page_step + (pos & ((1 << a.shift) - 1)) * D;
+                const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, -1, 0x00020000);
+                auto all = [&](auto whole) __attribute__((always_inline)) {
+                    const int rows = rq.len - pos;   // rows of the tile that are there (the last one again behind them)
+#pragma unroll
+                    for (int j = 0; j < PIECES; j++) {
+                        const int line = 4 * j + g;
+                        int row, piece;
+                        if (D == 128) {
+                            row = line;
+                            piece = v ? r16 : r16 ^ line;
+                        } else {
+                            row = 2 * line + ((r16 >> 3) ^ (v ? line >> 1 & 1 : 0));
+                            piece = (r16 & 7) ^ (v ? 0 : line & 7);
+                        }
+                        if (!decltype(whole)::value) row = min(row, rows - 1);
+                        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (ta_lds)(to + (which * PIECES + j) * 512), 16, row * (D * 2) + 16 * piece, 0, 0, STREAM ? 2 : 0);
+                    }
+                };
+                if (pos + 16 <= rq.len) all(std::true_type{});
+                else all(std::false_type{});
+            }
+        };
+        auto k_at = [](int row, int piece) { return D == 128 ? row * D + 8 * (piece ^ (row & 15)) : (row >> 1) * 128 + 64 * (row & 1) + 8 * (piece ^ (row >> 1 & 7)); };
+        auto v_at = [](int row) { return TA_P * D + (D == 128 ? row * D : (row >> 1) * 128 + 64 * ((row ^ row >> 2) & 1)); };
+
+        __syncthreads();                             // (nobody is at the request before this one any more)
+        if (tid < 2) odd_nodes[tid] = 0;             // (behind a barrier of the first stage when it is next written)
+        if (tid == 2) odd_held = 0;
+        pg.load(st_first);
+        pg.take();
+        pg.load(st_first + 32);
+        request(std::integral_constant<int, 0>{}, st_first);
+        if (st_first + 1 < st_end) request(std::integral_constant<int, 1>{}, st_first + 1);
+        else gone_of <<= 2;
+        if (st_first + 2 < st_end) request(std::integral_constant<int, 2>{}, st_first + 2);
+        else gone_of <<= 2;
+
+        // ---- the rows of q
+        const bool mine = row0 + 16 * QT * wave < all_rows;
+        half8_t q8[QT][NC];
+        uint64_t mask[QT];
+        int node_of[QT], head_of[QT];
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+            const int row = min(row0 + 16 * (QT * wave + t) + r16, all_rows - 1), node = ta_node(row, rep, a.per_rep), head = hk * rep + row - node * rep;
+            node_of[t] = node;
+            head_of[t] = head;
+            const half_t *p = a.q + (int64_t)(rq.start + node) * a.ldq + head * D + 8 * g;
+            if (((uintptr_t)a.q | (uintptr_t)(2 * a.ldq)) % 16 == 0) {
+#pragma unroll
+                for (int c = 0; c < NC; c++) q8[t][c] = *reinterpret_cast<const half8_t *>(p + 32 * c);
+            } else {
+#pragma unroll
+                for (int c = 0; c < NC; c++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) q8[t][c][e] = p[32 * c + e];
+            }
+            mask[t] = (uint64_t)a.masks[rq.start + node] & (rq.n < 64 ? (1ull << rq.n) - 1 : ~0ull);
+        }
+
+        const float scale2 = ta_scale(D);
+        float m[QT], l[QT];                          // of row r16 of a tile; l over this lane's positions only
+        float4_t acc[QT][W];
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+            m[t] = TA_LOW;
+            l[t] = 0.f;
+#pragma unroll
+            for (int j = 0; j < W; j++) acc[t][j] = (float4_t)0.f;
+        }
+        // infinities and NaN in a stage's v become zeros, and their positions are noted
+        auto clean = [&](half_t *sv, int st) {
+#pragma unroll 1
+            for (int i = tid; i < TA_P * D / 8; i += THREADS) {
+                half8_t v = *reinterpret_cast<const half8_t *>(sv + 8 * i);
+                bool odd = false;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const bool fine = (__builtin_bit_cast(uint16_t, (half_t)v[e]) & 0x7c00u) != 0x7c00u;
+                    odd = odd || !fine;
+                    v[e] = fine ? v[e] : (half_t)0;
+                }
+                if (!odd) continue;
+                *reinterpret_cast<half8_t *>(sv + 8 * i) = v;
+                const int line = i / 16, row = D == 128 ? line : 2 * line + ((i >> 3 & 1) ^ (line >> 1 & 1)), node = TA_P * st + row - held;
+                if (node < 0) odd_held = 1;
+                else if (node < rq.n) atomicOr(&odd_nodes[node >> 5], 1u << (node & 31));
+            }
+            __syncthreads();
+        };
+        auto scores = [&](const half_t *sk, float4_t (&s)[QT][2]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                half8_t k8[NC];
+#pragma unroll
+                for (int c = 0; c < NC; c++) k8[c] = *reinterpret_cast<const half8_t *>(sk + k_at(16 * i + r16, 4 * c + g));
+#pragma unroll
+                for (int t = 0; t < QT; t++) s[t][i] = (float4_t)0.f;
+#pragma unroll
+                for (int c = 0; c < NC; c++)
+#pragma unroll
+                    for (int t = 0; t < QT; t++) s[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8[c], q8[t][c], s[t][i], 0, 0, 0);
+            }
+        };
+        // some of a stage's positions are nodes, behind the last one, or of a page that does not exist (`bits`: of its tiles)
+        auto masked = [&](int st, int bits) { return TA_P * (st + 1) > held || bits != 0; };
+        auto hide = [&](int st, int bits, float4_t (&s)[QT][2]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+#pragma unroll
+                for (int t = 0; t < QT; t++) {
+                    const uint32_t seen = bits >> i & 1 ? 0 : ta_seen(mask[t], TA_P * st + 16 * i + 4 * g - held);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[t][i][e] = seen >> e & 1 ? s[t][i][e] : -INFINITY;
+                }
+            }
+        };
+        // the requests of this wave but for the last `later` stages have landed; behind the barrier everybody's have
+        auto landed = [&](auto later) {
+            constexpr int N = decltype(later)::value * EACH;
+            static_assert(N < 64, "what the counter holds");
+            __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | (N >> 4 << 14));
+        };
+        auto together = [&]() {
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        float4_t sa[QT][2], sb[QT][2];
+        // stage st: its scores are in s, the next one's go to s_next
+        auto walk = [&](auto ring, int st, float4_t (&s)[QT][2], float4_t (&s_next)[QT][2]) __attribute__((always_inline)) {
+            constexpr int R = decltype(ring)::value;
+            // behind the barrier this stage (AHEAD: the next one) is there, and nobody reads the one before this any more
+            if (!AHEAD && st + 2 < st_end) landed(std::integral_constant<int, 2>{});
+            else if (st + (AHEAD ? 2 : 1) < st_end) landed(std::integral_constant<int, 1>{});
+            else landed(std::integral_constant<int, 0>{});
+            together();
+            if (st + 3 < st_end) request(std::integral_constant<int, (R + 3) % 4>{}, st + 3);
+            else gone_of <<= 2;
+            const int bits = gone_of >> 6 & 3, bits_next = gone_of >> 4 & 3;
+            half_t *const sv = stage_at(ring);
+            if (masked(st, bits)) clean(sv + TA_P * D, st);
+            if (mine) {
+                vec_t v8[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) v8[i] = *reinterpret_cast<const vec_t *>(sv + v_at(16 * (i >> 2) + 4 * g + (i & 3)) + W * r16);
+                if (AHEAD) scores(stage_at(std::integral_constant<int, (R + 1) % 4>{}), s_next);       // (behind the last stage: of whatever is there, for nobody)
+                else {
+                    scores(sv, s);
+                    if (masked(st, bits)) hide(st, bits, s);
+                }
+                float r[QT];
+                half8_t p8[QT];
+#pragma unroll
+                for (int t = 0; t < QT; t++) {
+                    float mx = s[t][0][0];
+#pragma unroll
+                    for (int i = 1; i < 8; i++) mx = fmaxf(mx, s[t][i >> 2][i & 3]);
+                    mx = across<32>(across<16>(mx));
+                    const float mn = fmaxf(m[t], mx * scale2), from = mn - TA_UP;
+                    r[t] = __builtin_amdgcn_exp2f(m[t] - mn);
+                    m[t] = mn;
+                    float sum[2] = {0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i >> 2][i & 3], scale2, -from));
+                        sum[i & 1] += p;
+                        p8[t][i] = (half_t)p;
+                    }
+                    l[t] = l[t] * r[t] + (sum[0] + sum[1]);
+                }
+#pragma unroll
+                for (int t = 0; t < QT; t++) asm volatile("" : "+v"(p8[t]));   // (computed here, beside the products, and not behind the branch)
+                if (AHEAD) {
+#pragma unroll
+                    for (int i = 0; i < 8 * QT; i++) {
+                        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);       // a matrix instruction, then what fills its time
+                        __builtin_amdgcn_sched_group_barrier(0x402, 6, 0);
+                    }
+                }
+                if (__any(r[0] != 1.f || r[QT - 1] != 1.f)) {
+#pragma unroll
+                    for (int t = 0; t < QT; t++)
+#pragma unroll
+                        for (int j = 0; j < W; j++) acc[t][j] *= r[t];
+                }
+#pragma unroll
+                for (int j = 0; j < W; j++) {
+                    const half8_t v = {v8[0][j], v8[1][j], v8[2][j], v8[3][j], v8[4][j], v8[5][j], v8[6][j], v8[7][j]};
+#pragma unroll
+                    for (int t = 0; t < QT; t++) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p8[t], acc[t][j], 0, 0, 0);
+                }
+                if (AHEAD && st + 1 < st_end && masked(st + 1, bits_next)) hide(st + 1, bits_next, s_next);
+            }
+        };
+        if (AHEAD) {
+            if (st_first + 2 < st_end) landed(std::integral_constant<int, 2>{});
+            else if (st_first + 1 < st_end) landed(std::integral_constant<int, 1>{});
+            else landed(std::integral_constant<int, 0>{});
+            together();
+            if (mine) {
+                scores(s0, sa);
+                if (masked(st_first, gone_of >> 4 & 3)) hide(st_first, gone_of >> 4 & 3, sa);
+            }
+        }
+        for (int st = st_first; st < st_end; st += 4) {
+            walk(std::integral_constant<int, 0>{}, st, sa, sb);
+            if (st + 1 < st_end) walk(std::integral_constant<int, 1>{}, st + 1, sb, sa);
+            if (st + 2 < st_end) walk(std::integral_constant<int, 2>{}, st + 2, sa, sb);
+            if (st + 3 < st_end) walk(std::integral_constant<int, 3>{}, st + 3, sb, sa);
+        }
+        if (!mine) continue;
+
+        // ---- what the wave has: [max, sum, pad, pad, weighted v] where other workgroups have parts, else the result
+        const bool cut = w.slot >= 0;
+        uint32_t again[QT];                          // (bit r: row r of the tile is computed again)
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+            l[t] = across<32, true>(across<16, true>(l[t]));
+            const bool there = row0 + 16 * (QT * wave + t) + r16 < all_rows;
+            // NaN, or an infinity; a position that it sees had one
+            float sum = l[t];
+#pragma unroll
+            for (int j = 0; j < W; j++) sum += (acc[t][j][0] - acc[t][j][0]) + (acc[t][j][1] - acc[t][j][1]) + (acc[t][j][2] - acc[t][j][2]) + (acc[t][j][3] - acc[t][j][3]);
+            const uint64_t bad = __ballot(there && (sum != sum || odd_held != 0 || (mask[t] & ((uint64_t)odd_nodes[1] << 32 | odd_nodes[0])) != 0));
+            again[t] = (uint32_t)((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff);
+            if (!there) continue;
+            const float inv = l[t] != 0.f ? 1.f / l[t] : 0.f;              // (0: nothing was seen)
+            if (cut) {
+                float *to = ta_part_row(a, w.slot, node_of[t], head_of[t], D);
+                if (g == 0) {
+                    to[0] = m[t];
+                    to[1] = l[t];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++)          // row 4 g + i of product j is dimension W (4 g + i) + j
+#pragma unroll
+                    for (int j = 0; j < W; j += 4)
+                        *reinterpret_cast<float4_t *>(to + 4 + W * (4 * g + i) + j) = (float4_t){acc[t][j][i], acc[t][j + 1][i], acc[t][j + 2][i], acc[t][j + 3][i]};
+            } else {
+                half_t *to = a.out + ((int64_t)(rq.start + node_of[t]) * a.heads + head_of[t]) * D;
+                const bool whole = ((uintptr_t)a.out & 15) == 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    vec_t o;
+#pragma unroll
+                    for (int j = 0; j < W; j++) o[j] = (half_t)(acc[t][j][i] * inv);
+                    if (whole) *reinterpret_cast<vec_t *>(to + W * (4 * g + i)) = o;
+                    else
+#pragma unroll
+                        for (int j = 0; j < W; j++) to[W * (4 * g + i) + j] = o[j];
+                }
+            }
+        }
+        uint32_t all_again = 0;
+#pragma unroll
+        for (int t = 0; t < QT; t++) all_again |= again[t] << 16 * t;
+        all_again = __builtin_amdgcn_readfirstlane(all_again);
+#pragma unroll 1
+        while (__builtin_expect(all_again != 0, 0)) {
+            constexpr int PER = D / 64;
+            const int which = __builtin_ctz(all_again), row = row0 + 16 * QT * wave + which, node = ta_node(row, rep, a.per_rep), head = hk * rep + row - node * rep;
+            all_again &= all_again - 1;
+            const ta_again<D> x(a, rq, pg.ids, node, head, hk, st_first * TA_P, min(st_end * TA_P, rq.len), scale2);
+            const int64_t token_head = (int64_t)(rq.start + node) * a.heads + head;
+            if (cut) {
+                float *to = ta_part_row(a, w.slot, node, head, D);
+                if (lane == 0) {
+                    to[0] = x.top;
+                    to[1] = x.sum;
+                }
+#pragma unroll
+                for (int e = 0; e < PER; e++) to[4 + PER * lane + e] = x.o[e];
+            } else {
+                const float inv = x.sum != 0.f ? 1.f / x.sum : 0.f;
+#pragma unroll
+                for (int e = 0; e < PER; e++) a.out[token_head * D + PER * lane + e] = (half_t)(x.sum != 0.f ? x.o[e] * inv : 0.f);
+            }
         }
     }
+    if (unit == 0) ta_idle<THREADS>(a, work, gridDim.x / units, D);
 }
 
 // The parts of a row of a head put together, in order: D / 4 threads each.
 template <int D>
-__global__ __launch_bounds__(256) void attention_tree_merge_kernel(const float *__restrict__ part, const int32_t *__restrict__ parts_of, const int32_t *__restrict__ starts,
-                                                                  half_t *__restrict__ out, int B, int T, int nodes, int heads) {
+__global__ __launch_bounds__(256) void attention_tree_merge_kernel(const ta_args a) {
     constexpr int PER = D / 4;
     const int64_t i = (int64_t)blockIdx.x * (256 / PER) + threadIdx.x / PER;
-    const int dim = threadIdx.x % PER * 4, t = (int)(i / heads), head = (int)(i % heads);
-    if (t >= T) return;
-    const int place = parts_of[2 * t], further = parts_of[2 * t + 1];
-    if (further == 0) return;                    // written by the first launch
-    int lo = 0, hi = B;                          // the request: the first whose rows end behind t
+    const int dim = threadIdx.x % PER * 4, t = (int)(i / a.heads), head = (int)(i % a.heads);
+    if (t >= a.T) return;
+    int lo = 0, hi = a.B;                        // the request: the first whose rows end behind t
     while (lo < hi) {
         const int mid = (lo + hi) / 2;
-        if (starts[mid + 1] > t) hi = mid;
+        if (a.starts[mid + 1] > t) hi = mid;
         else lo = mid + 1;
     }
-    const int node = t - max(starts[min(lo, B - 1)], 0);
-    auto from = [&](int j) { return part + (j == 0 ? (int64_t)t * heads + head : ((int64_t)T + (int64_t)(place + j - 1) * nodes + node) * heads + head) * (D + 4); };
+    if (lo == a.B) return;
+    const ta_request rq(a, lo);
+    const int node = t - rq.start, stages = rq.stages();
+    if (node < 0 || node >= rq.n) return;        // (zeros already)
+    const int sum = a.before[a.B], shares = ta_shares(a, sum), from = a.before[lo], g0 = ta_whose(from, sum, shares), g1 = ta_whose(from + stages - 1, sum, shares);
+    if (g0 == g1) return;                        // written by the first launch
+    const int slot0 = 2 * g0 + (from != ta_begins(g0, sum, shares));
     float mx = TA_LOW, den = 0.f;
     float4_t o = (float4_t)0.f;
-    for (int j0 = 0; j0 <= further; j0 += 4) {
+    for (int j0 = g0; j0 <= g1; j0 += 4) {
         float m[4], l[4];
         float4_t v[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const float *p = from(min(j0 + j, further));
+            const int g = min(j0 + j, g1);
+            const float *p = ta_part_row(a, g == g0 ? slot0 : 2 * g, node, head, D);
             m[j] = p[0];
-            l[j] = j0 + j <= further ? p[1] : 0.f;
+            l[j] = j0 + j <= g1 ? p[1] : 0.f;
             v[j] = *reinterpret_cast<const float4_t *>(p + 4 + dim);
         }
 #pragma unroll
@@ -508,7 +931,7 @@ __global__ __launch_bounds__(256) void attention_tree_merge_kernel(const float *
             mx = top;
         }
     }
-    half_t *to = out + ((int64_t)t * heads + head) * D + dim;
+    half_t *to = a.out + ((int64_t)t * a.heads + head) * D + dim;
     const float inv = den != 0.f ? 1.f / den : 0.f;
 #pragma unroll
     for (int e = 0; e < 4; e++) to[e] = (half_t)(den != 0.f ? o[e] * inv : 0.f);
@@ -519,42 +942,42 @@ __global__ __launch_bounds__(256) void attention_tree_zero_kernel(half_t *__rest
 }
 
 struct ta_shape {
-    int qt, wr, wp, row_tiles, units, parts, least;
+    int rows, units, shares, least;              // rows of a workgroup
 };
 ta_shape shape_of(int B, int nodes, int heads, int kv_heads, int64_t positions) {
     ta_shape p;
-    const int rows = heads / kv_heads * nodes;
-    p.qt = rows <= 16 ? 1 : 2;
-    p.wr = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
-    p.wp = rows <= 64 ? 2 : 1;
-    p.row_tiles = (int)bs_cdiv(rows, 16 * p.qt * p.wr);
-    p.units = kv_heads * p.row_tiles;
-    const int64_t first = (int64_t)B * p.units, further = first <= 256 ? 512 - first : 768;
-    p.least = 4;
-    p.parts = positions <= p.least * TA_P ? 0 : (int)(further / p.units);
+    const int64_t rows = (int64_t)(heads / kv_heads) * nodes;
+    p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    p.units = kv_heads * (int)bs_cdiv(rows, p.rows);
+    p.least = 8;
+    p.shares = positions <= 256 ? 0 : 512 / p.units > 1 ? 512 / p.units : 1;
     return p;
 }
+int64_t before_bytes(int B) { return bs_cdiv(4ll * (B + 1), 16) * 16; }
+
+// A cache that the last-level cache cannot hold is read past it, where a workgroup of the unit has all of its rows.
+constexpr int64_t TA_STREAM = 256ll << 20;
 
 template <int D>
 int launch(const ta_args &a, const ta_shape &p, hipStream_t s) {
-    const unsigned grid = (unsigned)((int64_t)(a.B + p.parts) * p.units);
-    if (p.qt == 1) attention_tree_kernel<D, 1, 1, 2><<<grid, 128, 0, s>>>(a);
-    else if (p.wr == 1) attention_tree_kernel<D, 2, 1, 2><<<grid, 128, 0, s>>>(a);
-    else if (p.wr == 2) attention_tree_kernel<D, 2, 2, 2><<<grid, 256, 0, s>>>(a);
-    else attention_tree_kernel<D, 2, 4, 1><<<grid, 256, 0, s>>>(a);
+    const unsigned grid = (unsigned)((int64_t)(p.shares ? p.shares : a.B) * p.units);
+    const bool stream = ((int64_t)a.pool << a.shift) * a.kv_heads * D * 4 >= TA_STREAM;
+    if (p.rows == 16) (stream ? attention_tree_few_kernel<D, 1, true> : attention_tree_few_kernel<D, 1, false>)<<<grid, 256, 0, s>>>(a);
+    else if (p.rows == 32) (stream ? attention_tree_few_kernel<D, 2, true> : attention_tree_few_kernel<D, 2, false>)<<<grid, 256, 0, s>>>(a);
+    else if (p.rows == 64) (stream ? attention_tree_kernel<D, 1, 4, false, true> : attention_tree_kernel<D, 1, 4, false, false>)<<<grid, 256, 0, s>>>(a);
+    else attention_tree_kernel<D, 2, 4, true, false><<<grid, 256, 0, s>>>(a);
     BS_LAUNCH_CHECK();
-    if (p.parts == 0) return BS_OK;
-    attention_tree_merge_kernel<D><<<(unsigned)bs_cdiv((int64_t)a.T * a.heads, 256 / (D / 4)), 256, 0, s>>>(a.part, a.parts_of, a.starts, a.out, a.B, a.T, a.nodes, a.heads);
+    if (p.shares == 0) return BS_OK;
+    attention_tree_merge_kernel<D><<<(unsigned)bs_cdiv((int64_t)a.T * a.heads, 256 / (D / 4)), 256, 0, s>>>(a);
     BS_LAUNCH_CHECK();
     return BS_OK;
 }
-int64_t parts_of_bytes(int T) { return bs_cdiv(8ll * T, 16) * 16; }
 
 }  // namespace
 
 int64_t bs_attention_tree_scratch(int B, int T, int nodes, int heads, int kv_heads, int head_dim, int max_pages, int page) {
     const ta_shape p = shape_of(B, nodes, heads, kv_heads, (int64_t)max_pages * page);
-    return p.parts ? parts_of_bytes(T) + ((int64_t)T + (int64_t)p.parts * nodes) * heads * (head_dim + 4) * 4 : 0;
+    return p.shares ? before_bytes(B) + 2ll * p.shares * nodes * heads * (head_dim + 4) * 4 : 0;
 }
 
 int bs_launch_attention_tree(const half_t *q, int ldq, const half_t *kpages, const half_t *vpages, const int32_t *table, const int32_t *lengths, const int32_t *granted,
@@ -566,7 +989,7 @@ int bs_launch_attention_tree(const half_t *q, int ldq, const half_t *kpages, con
         return BS_OK;
     }
     const ta_shape p = shape_of(B, nodes, heads, kv_heads, (int64_t)max_pages << shift);
-    const ta_args a = {q, kpages, vpages, table, lengths, granted, starts, masks, out, (int32_t *)workspace, (float *)((char *)workspace + parts_of_bytes(T)), ldq, B, T, nodes,
-                       heads, kv_heads, p.row_tiles, shift, max_pages, pool, p.parts, p.least};
+    const ta_args a = {q, kpages, vpages, table, lengths, granted, starts, masks, out, (int32_t *)workspace, (float *)((char *)workspace + before_bytes(B)), 1.f / (float)(heads / kv_heads), ldq, B, T, nodes,
+                       heads, kv_heads, p.units / kv_heads, shift, max_pages, pool, p.shares, p.least};
     return head_dim == 128 ? launch<128>(a, p, s) : launch<64>(a, p, s);
 }
