@@ -4,8 +4,8 @@
 // The rows of a KV head of a request are its nodes' queries of that head's group, the head fastest: nodes * group of them, which all read the same K and V.  A workgroup takes up to 16 QT WR of
 // them, the columns of both products, 16 QT to a wave, and walks the positions in stages of 32, which come to LDS straight from the pages (no registers), up to three stages ahead, one barrier per stage.
 //   scores  S[position, row] = K q      16x16x32; the 16-byte pieces of K's rows are XOR-ed with the row's number, so that 16 rows of one piece lie in different banks
-//   output  O[dim, row] += V^T P        16x16x32; a lane of the scores holds four positions of a row in each of two tiles of 16, which are the eight k slots of this product, and V
-//                                       is used as it lies: product j takes element j of the W = D / 16 dimensions that a lane reads
+//   output  O[dim, row] += V^T P        16x16x32; a lane of the scores holds four positions of a row in each of two tiles of 16, which are the eight k slots of this product.  From LDS V comes
+//                                       turned, a lane a dimension; from memory it is used as it lies: product j takes element j of the W = D / 16 dimensions that a lane reads
 // The scores of a stage are computed one stage ahead, beside the softmax of the one before it: the matrix unit runs while the vector unit issues.
 // Maximum, sum and output are fp32, in base 2.  The weights are rounded to fp16 for the second product (the queries are given in fp16), the largest as 2^15, so that one of
 // 2^-40 of the largest is still held; their sum is that of the fp32 weights.
@@ -58,6 +58,12 @@ __device__ __forceinline__ int ta_node(int row, int rep, float per_rep) {
 __device__ __forceinline__ int ta_begins(int g, int sum, int shares) { return (int)((int64_t)g * sum / shares); }
 __device__ __forceinline__ int ta_whose(int x, int sum, int shares) { return (int)((((int64_t)x + 1) * shares - 1) / sum); }
 __device__ __forceinline__ int ta_shares(const ta_args &a, int sum) { return min(a.shares, (sum + a.least - 1) / a.least); }
+
+// v, of which nothing is worked out ahead of here (registers are short in the loops over the stages)
+__device__ __forceinline__ int ta_here(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
 
 // the larger of v here and in the lane whose number differs by W (16 or 32), or (SUM) both together
 template <int W, bool SUM = false>
@@ -284,12 +290,13 @@ __global__ __launch_bounds__(256, 2) void attention_tree_few_kernel(const ta_arg
     __shared__ float wm[WAVES][ROWS], wl[WAVES][ROWS];
     __shared__ uint64_t odd_of[WAVES];           // nodes at which something in v is infinite or NaN
     __shared__ uint32_t bad[WAVES][ROWS];        // rows whose sums are not finite, or all, where a held position has such
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hk = blockIdx.x % a.kv_heads, g_of = blockIdx.x / a.kv_heads, rep = a.heads / a.kv_heads;
     const int64_t page_step = (int64_t)a.kv_heads * D << a.shift, head_at = (int64_t)hk * D << a.shift;
     ta_work w;
     int first;
     for (bool more = ta_first<WAVES>(a, g_of, w, first); more; more = ta_next(a, w, first)) {
+        const int r16 = ta_here(lane) & 15, g = ta_here(lane) >> 4;
         const ta_request &rq = w.rq;
         const int rows = rq.n * rep, held = rq.len - rq.n, st_end = w.st_end;
         if (hk == 0 && w.st == 0 && tid == 0 && a.shares > 0) a.before[w.b] = w.before;
@@ -560,12 +567,11 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
     constexpr int PIECES = D / 32;               // requests of 1 KB (four lines of 256 bytes) for a tile of 16 rows
     constexpr int SHARE = 4 / WR;                // of a stage's four tiles (two of K, two of V) that a wave requests
     constexpr int EACH = SHARE * PIECES;
-    typedef half_t vec_t __attribute__((ext_vector_type(W)));
     // (an array per stage, K and then V: the compiler then knows that a request for one does not touch the others)
     __shared__ __attribute__((aligned(1024))) half_t s0[2 * TA_P * D], s1[2 * TA_P * D], s2[2 * TA_P * D], s3[2 * TA_P * D];
     __shared__ uint32_t odd_nodes[2];            // positions where something in v is infinite or NaN
     __shared__ int odd_held;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int units = a.kv_heads * a.row_tiles, unit = blockIdx.x % units, work = blockIdx.x / units;
     const int hk = unit % a.kv_heads, row0 = unit / a.kv_heads * ROWS, rep = a.heads / a.kv_heads;
 
@@ -573,6 +579,7 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
     ta_work w;
     int first;
     for (bool more = ta_first<WR>(a, work, w, first); more; more = ta_next(a, w, first)) {
+        const int r16 = ta_here(lane) & 15, g = ta_here(lane) >> 4;
         const ta_request &rq = w.rq;
         if (unit == 0 && w.st == 0 && tid == 0 && a.shares > 0) a.before[w.b] = w.before;
         const int all_rows = rq.n * rep;
@@ -581,7 +588,7 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
         ta_pages pg = {a.table + (int64_t)w.b * a.max_pages, (rq.len - 1) / 16, a.shift, a.pool, 1, 0, 0, 0};
 
         // ---- the rows of the cache
-        // lane -> row and piece of it, for the requests of 1 KB, and where they lie: K's pieces XOR-ed with the row (D == 64: two rows to a line; V's rows change places in it by turns)
+        // lane -> row and piece of it, for the requests of 1 KB, and where they lie (D == 64: two rows to a line): pieces XOR-ed with the line, V's by pairs
         auto stage_at = [&](auto ring) -> half_t * { return decltype(ring)::value == 0 ? s0 : decltype(ring)::value == 1 ? s1 : decltype(ring)::value == 2 ? s2 : s3; };
         const half_t *from[SHARE];                   // K or V of this head
 #pragma unroll
@@ -612,10 +619,10 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
                         int row, piece;
                         if (D == 128) {
                             row = line;
-                            piece = v ? r16 : r16 ^ line;
+                            piece = r16 ^ (v ? 2 * (line & 7) : line);
                         } else {
-                            row = 2 * line + ((r16 >> 3) ^ (v ? line >> 1 & 1 : 0));
-                            piece = (r16 & 7) ^ (v ? 0 : line & 7);
+                            row = 2 * line + (r16 >> 3);
+                            piece = (r16 & 7) ^ (v ? 2 * (line & 3) : line & 7);
                         }
                         if (!decltype(whole)::value) row = min(row, rows - 1);
                         __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (ta_lds)(to + (which * PIECES + j) * 512), 16, row * (D * 2) + 16 * piece, 0, 0, STREAM ? 2 : 0);
@@ -626,7 +633,8 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
             }
         };
         auto k_at = [](int row, int piece) { return D == 128 ? row * D + 8 * (piece ^ (row & 15)) : (row >> 1) * 128 + 64 * (row & 1) + 8 * (piece ^ (row >> 1 & 7)); };
-        auto v_at = [](int row) { return TA_P * D + (D == 128 ? row * D : (row >> 1) * 128 + 64 * ((row ^ row >> 2) & 1)); };
+        // 16 lanes read four rows of 16 dimensions of V, four in each lane, and get them turned: a lane a dimension.  Dimensions 16 j ..: XOR-ed with 16 j
+        const int v_row = 4 * g + (r16 >> 2), v_from = TA_P * D + (D == 128 ? v_row * D + 16 * (v_row & 7) : (v_row >> 1) * 128 + 64 * (v_row & 1) + 16 * (v_row >> 1 & 3)) + 4 * (r16 & 3);
 
         __syncthreads();                             // (nobody is at the request before this one any more)
         if (tid < 2) odd_nodes[tid] = 0;             // (behind a barrier of the first stage when it is next written)
@@ -637,8 +645,10 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
         request(std::integral_constant<int, 0>{}, st_first);
         if (st_first + 1 < st_end) request(std::integral_constant<int, 1>{}, st_first + 1);
         else gone_of <<= 2;
-        if (st_first + 2 < st_end) request(std::integral_constant<int, 2>{}, st_first + 2);
-        else gone_of <<= 2;
+        if (!AHEAD) {
+            if (st_first + 2 < st_end) request(std::integral_constant<int, 2>{}, st_first + 2);
+            else gone_of <<= 2;
+        }
 
         // ---- the rows of q
         const bool mine = row0 + 16 * QT * wave < all_rows;
@@ -687,7 +697,7 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
                 }
                 if (!odd) continue;
                 *reinterpret_cast<half8_t *>(sv + 8 * i) = v;
-                const int line = i / 16, row = D == 128 ? line : 2 * line + ((i >> 3 & 1) ^ (line >> 1 & 1)), node = TA_P * st + row - held;
+                const int line = i / 16, row = D == 128 ? line : 2 * line + (i >> 3 & 1), node = TA_P * st + row - held;
                 if (node < 0) odd_held = 1;
                 else if (node < rq.n) atomicOr(&odd_nodes[node >> 5], 1u << (node & 31));
             }
@@ -734,87 +744,119 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
             __builtin_amdgcn_sched_barrier(0);
         };
         float4_t sa[QT][2], sb[QT][2];
-        // stage st: its scores are in s, the next one's go to s_next
-        auto walk = [&](auto ring, int st, float4_t (&s)[QT][2], float4_t (&s_next)[QT][2]) __attribute__((always_inline)) {
+        half8_t p8[QT];
+        half8_t vt[W];
+        float r[QT];
+        auto values = [&](const half_t *stage) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < W; j++) {
+                typedef short short4_t __attribute__((ext_vector_type(4)));
+                typedef __attribute__((address_space(3))) short4_t *from_t;
+                const half_t *const p = stage + (v_from ^ 16 * j);
+                const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((from_t)p), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((from_t)(p + 16 * D));
+                vt[j] = __builtin_bit_cast(half8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            }
+        };
+        // the running maximum and sum, the weights, and what the older sums are to be multiplied by
+        auto softmax = [&](const float4_t (&s)[QT][2]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
+                float mx = s[t][0][0];
+#pragma unroll
+                for (int i = 1; i < 8; i++) mx = fmaxf(mx, s[t][i >> 2][i & 3]);
+                mx = across<32>(across<16>(mx));
+                const float mn = fmaxf(m[t], mx * scale2), from = mn - TA_UP;
+                r[t] = __builtin_amdgcn_exp2f(m[t] - mn);
+                m[t] = mn;
+                float sum[2] = {0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i >> 2][i & 3], scale2, -from));
+                    sum[i & 1] += p;
+                    p8[t][i] = (half_t)p;
+                }
+                l[t] = l[t] * r[t] + (sum[0] + sum[1]);
+            }
+#pragma unroll
+            for (int t = 0; t < QT; t++) asm volatile("" : "+v"(p8[t]));   // (computed here, beside the products, and not behind the branch)
+        };
+        auto output = [&]() __attribute__((always_inline)) {
+            if (__any(r[0] != 1.f || r[QT - 1] != 1.f)) {
+#pragma unroll
+                for (int t = 0; t < QT; t++)
+#pragma unroll
+                    for (int j = 0; j < W; j++) acc[t][j] *= r[t];
+            }
+#pragma unroll
+            for (int j = 0; j < W; j++) {
+#pragma unroll
+                for (int t = 0; t < QT; t++) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[j], p8[t], acc[t][j], 0, 0, 0);
+            }
+        };
+        // a stage
+        auto walk = [&](auto ring, int st) __attribute__((always_inline)) {
             constexpr int R = decltype(ring)::value;
-            // behind the barrier this stage (AHEAD: the next one) is there, and nobody reads the one before this any more
-            if (!AHEAD && st + 2 < st_end) landed(std::integral_constant<int, 2>{});
-            else if (st + (AHEAD ? 2 : 1) < st_end) landed(std::integral_constant<int, 1>{});
+            // behind the barrier this stage is there, and nobody reads the one before this any more
+            if (st + 2 < st_end) landed(std::integral_constant<int, 2>{});
+            else if (st + 1 < st_end) landed(std::integral_constant<int, 1>{});
             else landed(std::integral_constant<int, 0>{});
             together();
             if (st + 3 < st_end) request(std::integral_constant<int, (R + 3) % 4>{}, st + 3);
             else gone_of <<= 2;
-            const int bits = gone_of >> 6 & 3, bits_next = gone_of >> 4 & 3;
-            half_t *const sv = stage_at(ring);
-            if (masked(st, bits)) clean(sv + TA_P * D, st);
-            if (mine) {
-                vec_t v8[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) v8[i] = *reinterpret_cast<const vec_t *>(sv + v_at(16 * (i >> 2) + 4 * g + (i & 3)) + W * r16);
-                if (AHEAD) scores(stage_at(std::integral_constant<int, (R + 1) % 4>{}), s_next);       // (behind the last stage: of whatever is there, for nobody)
-                else {
-                    scores(sv, s);
-                    if (masked(st, bits)) hide(st, bits, s);
-                }
-                float r[QT];
-                half8_t p8[QT];
-#pragma unroll
-                for (int t = 0; t < QT; t++) {
-                    float mx = s[t][0][0];
-#pragma unroll
-                    for (int i = 1; i < 8; i++) mx = fmaxf(mx, s[t][i >> 2][i & 3]);
-                    mx = across<32>(across<16>(mx));
-                    const float mn = fmaxf(m[t], mx * scale2), from = mn - TA_UP;
-                    r[t] = __builtin_amdgcn_exp2f(m[t] - mn);
-                    m[t] = mn;
-                    float sum[2] = {0.f, 0.f};
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i >> 2][i & 3], scale2, -from));
-                        sum[i & 1] += p;
-                        p8[t][i] = (half_t)p;
-                    }
-                    l[t] = l[t] * r[t] + (sum[0] + sum[1]);
-                }
-#pragma unroll
-                for (int t = 0; t < QT; t++) asm volatile("" : "+v"(p8[t]));   // (computed here, beside the products, and not behind the branch)
-                if (AHEAD) {
-#pragma unroll
-                    for (int i = 0; i < 8 * QT; i++) {
-                        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);       // a matrix instruction, then what fills its time
-                        __builtin_amdgcn_sched_group_barrier(0x402, 6, 0);
-                    }
-                }
-                if (__any(r[0] != 1.f || r[QT - 1] != 1.f)) {
-#pragma unroll
-                    for (int t = 0; t < QT; t++)
-#pragma unroll
-                        for (int j = 0; j < W; j++) acc[t][j] *= r[t];
-                }
-#pragma unroll
-                for (int j = 0; j < W; j++) {
-                    const half8_t v = {v8[0][j], v8[1][j], v8[2][j], v8[3][j], v8[4][j], v8[5][j], v8[6][j], v8[7][j]};
-#pragma unroll
-                    for (int t = 0; t < QT; t++) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p8[t], acc[t][j], 0, 0, 0);
-                }
-                if (AHEAD && st + 1 < st_end && masked(st + 1, bits_next)) hide(st + 1, bits_next, s_next);
-            }
+            const int bits = gone_of >> 6 & 3;
+            half_t *const at = stage_at(ring);
+            if (masked(st, bits)) clean(at + TA_P * D, st);
+            if (!mine) return;
+            values(at);
+            scores(at, sa);
+            if (masked(st, bits)) hide(st, bits, sa);
+            softmax(sa);
+            output();
         };
-        if (AHEAD) {
-            if (st_first + 2 < st_end) landed(std::integral_constant<int, 2>{});
-            else if (st_first + 1 < st_end) landed(std::integral_constant<int, 1>{});
-            else landed(std::integral_constant<int, 0>{});
+        // two stages: the second one's scores beside the first one's softmax
+        auto walk_two = [&](auto ring, int st) __attribute__((always_inline)) {
+            constexpr int R = decltype(ring)::value;
+            landed(std::integral_constant<int, 0>{});
             together();
-            if (mine) {
-                scores(s0, sa);
-                if (masked(st_first, gone_of >> 4 & 3)) hide(st_first, gone_of >> 4 & 3, sa);
+#pragma unroll
+            for (int i = 2; i < 4; i++) {
+                if (st + i >= st_end) gone_of <<= 2;
+                else if (i == 2) request(std::integral_constant<int, (R + 2) % 4>{}, st + 2);
+                else request(std::integral_constant<int, (R + 3) % 4>{}, st + 3);
             }
-        }
+            const int bits = gone_of >> 6 & 3, bits_next = gone_of >> 4 & 3;
+            half_t *const at = stage_at(ring), *const at_next = stage_at(std::integral_constant<int, R + 1>{});
+            const bool two = st + 1 < st_end;
+            if (masked(st, bits)) clean(at + TA_P * D, st);
+            if (two && masked(st + 1, bits_next)) clean(at_next + TA_P * D, st + 1);
+            if (!mine) return;
+            scores(at, sa);
+            if (masked(st, bits)) hide(st, bits, sa);
+            scores(at_next, sb);                 // (behind the last stage: of whatever is there, for nobody)
+            values(at);
+            softmax(sa);
+#pragma unroll
+            for (int i = 0; i < 8 * QT; i++) {
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);           // a matrix instruction, then what fills its time
+                __builtin_amdgcn_sched_group_barrier(0x402, 6, 0);
+            }
+            output();
+            if (!two) return;
+            values(at_next);
+            if (masked(st + 1, bits_next)) hide(st + 1, bits_next, sb);
+            softmax(sb);
+            output();
+        };
         for (int st = st_first; st < st_end; st += 4) {
-            walk(std::integral_constant<int, 0>{}, st, sa, sb);
-            if (st + 1 < st_end) walk(std::integral_constant<int, 1>{}, st + 1, sb, sa);
-            if (st + 2 < st_end) walk(std::integral_constant<int, 2>{}, st + 2, sa, sb);
-            if (st + 3 < st_end) walk(std::integral_constant<int, 3>{}, st + 3, sb, sa);
+            if (AHEAD) {
+                walk_two(std::integral_constant<int, 0>{}, st);
+                if (st + 2 < st_end) walk_two(std::integral_constant<int, 2>{}, st + 2);
+            } else {
+                walk(std::integral_constant<int, 0>{}, st);
+                if (st + 1 < st_end) walk(std::integral_constant<int, 1>{}, st + 1);
+                if (st + 2 < st_end) walk(std::integral_constant<int, 2>{}, st + 2);
+                if (st + 3 < st_end) walk(std::integral_constant<int, 3>{}, st + 3);
+            }
         }
         if (!mine) continue;
 
@@ -840,22 +882,19 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
                     to[1] = l[t];
                 }
 #pragma unroll
-                for (int i = 0; i < 4; i++)          // row 4 g + i of product j is dimension W (4 g + i) + j
-#pragma unroll
-                    for (int j = 0; j < W; j += 4)
-                        *reinterpret_cast<float4_t *>(to + 4 + W * (4 * g + i) + j) = (float4_t){acc[t][j][i], acc[t][j + 1][i], acc[t][j + 2][i], acc[t][j + 3][i]};
+                for (int j = 0; j < W; j++) *reinterpret_cast<float4_t *>(to + 4 + 16 * j + 4 * g) = acc[t][j];
             } else {
                 half_t *to = a.out + ((int64_t)(rq.start + node_of[t]) * a.heads + head_of[t]) * D;
-                const bool whole = ((uintptr_t)a.out & 15) == 0;
+                const bool whole = ((uintptr_t)a.out & 7) == 0;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    vec_t o;
+                for (int j = 0; j < W; j++) {        // row 4 g + i of product j is dimension 16 j + 4 g + i
+                    half4_t o;
 #pragma unroll
-                    for (int j = 0; j < W; j++) o[j] = (half_t)(acc[t][j][i] * inv);
-                    if (whole) *reinterpret_cast<vec_t *>(to + W * (4 * g + i)) = o;
+                    for (int i = 0; i < 4; i++) o[i] = (half_t)(acc[t][j][i] * inv);
+                    if (whole) *reinterpret_cast<half4_t *>(to + 16 * j + 4 * g) = o;
                     else
 #pragma unroll
-                        for (int j = 0; j < W; j++) to[W * (4 * g + i) + j] = o[j];
+                        for (int i = 0; i < 4; i++) to[16 * j + 4 * g + i] = o[i];
                 }
             }
         }
