@@ -83,7 +83,89 @@ __global__ __launch_bounds__(THREADS) void fork_plan_kernel(const fork_args a) {
 
 __device__ __forceinline__ bool fork_page(int32_t p, int pool) { return p >= 0 && p < pool; }
 
-// Tables, shares and the ring, by one workgroup: a wave per row.
+// Tables, shares and the ring, by one workgroup: a wave per row, a lane per entry.  A page goes back when its shares fall below 0, and at the place of the first entry that gave it up: that is the
+// smallest of its givers' numbers, whatever the order of the atomics.
+// Few entries: N of a lane, which holds them from one pass to the next.  (4 rows of 19 pages: 19 us when every pass went through the tables again, with fences that write the L2 back, and 4.1 so.)
+template <int N>
+__device__ __forceinline__ void fork_few_tables(const fork_args &a) {
+    __shared__ uint32_t counts[WAVES * N], upto[WAVES * N];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), chunks = (a.max_pages + 63) / 64;
+    const plan_state st(a.state, a.pool);
+    const int taken = *a.needed, room = a.pool - st.count;
+    auto load = [](const int32_t *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    fork_row r[N];
+    int32_t gives[N], takes[N];                  // page that the entry gives up, and that it holds afterwards; -1: none
+    int at[N];                                   // its number
+#pragma unroll
+    for (int n = 0; n < N; n++) {                // (the row's chunk n % chunks, of the row's turn n / chunks)
+        const int b = wave + WAVES * (n / chunks);
+        r[n].source = b;
+        if (b < a.B) r[n] = a.rows[b];
+    }
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        const int b = wave + WAVES * (n / chunks), j = 64 * (n % chunks) + lane;
+        at[n] = b * a.max_pages + j;
+        const bool moves = b < a.B && r[n].source != b;
+        gives[n] = moves && j < r[n].gives ? a.table[(int64_t)at[n]] : -1;
+        takes[n] = moves && j < r[n].whole ? a.table[(int64_t)r[n].source * a.max_pages + j] : -1;
+    }
+#pragma unroll
+    for (int n = 0; n < N; n++)
+        if (fork_page(gives[n], a.pool)) __hip_atomic_store(a.owner + gives[n], INT32_MAX, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        if (fork_page(gives[n], a.pool)) {
+            atomicMin(a.owner + gives[n], at[n]);
+            atomicAdd(a.shares + gives[n], -1);
+        }
+        if (fork_page(takes[n], a.pool)) atomicAdd(a.shares + takes[n], 1);
+    }
+    __syncthreads();
+    uint64_t back[N];
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        const bool page = fork_page(gives[n], a.pool);
+        const int32_t owner = page ? load(a.owner + gives[n]) : -1, left = page ? load(a.shares + gives[n]) : 0;
+        back[n] = __ballot(page && owner == at[n] && left < 0);
+        // in order of the rows, and of a row's chunks
+        if (lane == 0 && n / chunks < N / chunks) counts[(wave + WAVES * (n / chunks)) * chunks + n % chunks] = __popcll(back[n]);
+    }
+    __syncthreads();
+    const int entries = WAVES * (N / chunks) * chunks;
+    if (wave == 0) {
+        uint32_t sum = 0;
+        for (int i0 = 0; i0 < entries; i0 += 64) {
+            const uint32_t v = i0 + lane < entries ? counts[i0 + lane] : 0, s = bs_scan(v, [](uint32_t x, uint32_t y) { return x + y; });
+            if (i0 + lane < entries) upto[i0 + lane] = sum + s - v;
+            sum += bs_read(s, 63);
+        }
+        if (lane == 0) {
+            a.state_out[0] = plan_wrap((uint32_t)st.head + taken, a.pool);
+            a.state_out[1] = st.count - taken + min((int)sum, room);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        const int b = wave + WAVES * (n / chunks);
+        if (b >= a.B || n / chunks >= N / chunks) continue;
+        const int place = (int)upto[b * chunks + n % chunks] + __popcll(back[n] & ((1ull << lane) - 1));
+        if (back[n] >> lane & 1) {
+            __hip_atomic_store(a.shares + gives[n], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (place < room) a.ring[plan_wrap((uint32_t)st.tail + place, a.pool)] = gives[n];            // (a full ring takes no more)
+        }
+        if (r[n].source != b) {
+            const int j = 64 * (n % chunks) + lane;
+            if (j < r[n].whole) a.table[(int64_t)at[n]] = takes[n];
+            else if (j == r[n].whole && r[n].rest > 0) a.table[(int64_t)at[n]] = r[n].fresh;
+        }
+        if (n % chunks == 0 && lane == 0) a.lengths_out[b] = r[n].length;
+    }
+}
+
+// ... and as many as there are.
 __device__ __forceinline__ void fork_tables(const fork_args &a) {
     __shared__ uint32_t waves[WAVES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -100,7 +182,6 @@ __device__ __forceinline__ void fork_tables(const fork_args &a) {
         }
         for (int j = lane; j < r.whole; j += 64) a.stage[(int64_t)entry(b, j)] = a.table[(int64_t)entry(r.source, j)];
     }
-    __threadfence();
     __syncthreads();
     for (int b = wave; b < a.B; b += WAVES) {
         const fork_row r = a.rows[b];
@@ -116,7 +197,6 @@ __device__ __forceinline__ void fork_tables(const fork_args &a) {
             if (fork_page(p, a.pool)) atomicAdd(a.shares + p, 1);
         }
     }
-    __threadfence();
     __syncthreads();
     auto goes = [&](int b, int j, const fork_row &r, int32_t &p) {
         p = j < r.gives ? a.table[(int64_t)entry(b, j)] : -1;
@@ -130,7 +210,6 @@ __device__ __forceinline__ void fork_tables(const fork_args &a) {
             for (int j0 = 0; j0 < r.gives; j0 += 64) n += __popcll(__ballot(goes(b, j0 + lane, r, p)));
         if (lane == 0) a.freed[b] = n;
     }
-    __threadfence();
     __syncthreads();
     uint32_t all = 0;
     for (int b0 = 0; b0 < a.B; b0 += THREADS) {
@@ -140,7 +219,6 @@ __device__ __forceinline__ void fork_tables(const fork_args &a) {
         if (b < a.B) a.freed[b] = (int32_t)(all + before);
         all += total;
     }
-    __threadfence();
     __syncthreads();
     for (int b = wave; b < a.B; b += WAVES) {
         const fork_row r = a.rows[b];
@@ -169,7 +247,10 @@ __device__ __forceinline__ void fork_tables(const fork_args &a) {
 
 // Workgroup 0 the tables, the others the positions of the last pages: a run (a head of a layer's keys or values) to a wave.
 __global__ __launch_bounds__(THREADS) void fork_apply_kernel(const fork_args a) {
-    if (blockIdx.x == 0) return fork_tables(a);
+    if (blockIdx.x == 0) {
+        const int entries = (a.B + WAVES - 1) / WAVES * ((a.max_pages + 63) / 64);         // of a lane
+        return entries <= 1 ? fork_few_tables<1>(a) : entries <= 4 ? fork_few_tables<4>(a) : fork_tables(a);
+    }
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int b = (blockIdx.x - 1) / a.blocks, block = (blockIdx.x - 1) - b * a.blocks;
     const fork_row r = a.rows[b];

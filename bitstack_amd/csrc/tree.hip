@@ -73,15 +73,25 @@ struct accept_args {
     int B, T, nodes, blocks, layers, kv_heads, pieces, shift, max_pages, pool;
 };
 
-__global__ __launch_bounds__(THREADS) void tree_accept_kernel(const accept_args a) {
-    const int lane = threadIdx.x & 63, b = blockIdx.x / a.blocks, block = blockIdx.x - b * a.blocks;
-    const tree_rows r(a.starts, a.granted, b, a.T, a.nodes);
-    const bool there = lane < r.nodes;
-    const int parent = there ? a.parents[r.start + lane] : -1;
-    const int64_t drafted = there ? a.tokens[r.start + lane] : 0, target = there ? a.targets[r.start + lane] : 0, slot = there ? a.slots[r.start + lane] : -1;
-    int at = -1, count = 0, mine = -1;           // (lane i: node i of the path)
-    if (r.nodes > 0) {
-        at = 0;
+// one request by one wave, a lane a node
+struct accept_path {
+    tree_rows r;
+    int parent;
+    int64_t drafted, target, slot;
+    int at, count, mine;                         // the last node of the path, nodes on it, lane i: node i of it
+    __device__ __forceinline__ accept_path(const accept_args &a, int b) : r(a.starts, a.granted, b, a.T, a.nodes) {
+        const int lane = threadIdx.x & 63;
+        const bool there = lane < r.nodes;
+        parent = there ? a.parents[r.start + lane] : -1;
+        drafted = there ? a.tokens[r.start + lane] : 0;
+        target = there ? a.targets[r.start + lane] : 0;
+        slot = there ? a.slots[r.start + lane] : -1;
+    }
+    __device__ __forceinline__ void walk() {
+        const int lane = threadIdx.x & 63;
+        at = count = 0;
+        mine = -1;
+        if (r.nodes == 0) return;
         mine = lane == 0 ? 0 : -1;
         count = 1;
         while (true) {
@@ -93,44 +103,93 @@ __global__ __launch_bounds__(THREADS) void tree_accept_kernel(const accept_args 
             count++;
         }
     }
-    if (block == 0 && threadIdx.x < 64) {
+    // what the caller gets; {first page that goes back, pages}
+    __device__ __forceinline__ int2 write(const accept_args &a, int b) const {
+        const int lane = threadIdx.x & 63;
+        const int most = (int)min((int64_t)a.max_pages << a.shift, (int64_t)INT32_MAX);
+        const int before = min(max(a.lengths[b], 0), most), given = min(max(a.granted[b], 0), before), after = before - given + min(count, given), first = plan_pages(after, a.shift);
         if (lane < a.nodes) a.path[(int64_t)b * a.nodes + lane] = mine;
         if (lane == 0) {
-            const int most = (int)min((int64_t)a.max_pages << a.shift, (int64_t)INT32_MAX);
-            const int before = min(max(a.lengths[b], 0), most), given = min(max(a.granted[b], 0), before), after = before - given + min(count, given);
-            const int first = plan_pages(after, a.shift);
-            a.back[2 * b] = first;
-            a.back[2 * b + 1] = plan_pages(before, a.shift) - first;
             a.lengths_out[b] = after;
             a.accepted[b] = count;
         }
         if (count == 0 ? lane == 0 : lane == at) a.token[b] = count == 0 ? -1 : target;
+        return {first, plan_pages(before, a.shift) - first};
     }
-    // ---- the moves: from the slot of node path[i] to that of node i
-    const int32_t to = (int32_t)(slot >= 0 && slot < (int64_t)a.pool << a.shift ? slot : -1);
-    const int32_t from = __shfl(to, max(mine, 0), 64);
-    const bool moves = lane < count && mine != lane && to >= 0 && from >= 0;
-    uint64_t left = __ballot(moves);
-    if (left == 0) return;
-    const int units = 2 * a.layers * a.kv_heads * a.pieces, mask = (1 << a.shift) - 1;
-    for (int u = block * THREADS + threadIdx.x; u < units; u += a.blocks * THREADS) {
-        const int piece = u % a.pieces, head = u / a.pieces % a.kv_heads, layer = u / (a.pieces * a.kv_heads);
-        half_t *const base = (layer & 1 ? a.vpages : a.kpages) + (layer >> 1) * a.layer + 8 * piece;
-        auto where = [&](int32_t s) { return reinterpret_cast<half8_t *>(base + ((((int64_t)(s >> a.shift) * a.kv_heads + head) << a.shift) + (s & mask)) * (8 * a.pieces)); };
-        for (uint64_t todo = left; todo != 0;) {
-            half8_t v[8];
-            uint64_t rest = todo;
+    // the moves, from the slot of node path[i] to that of node i: pieces `first`, `first` + step, ..
+    __device__ __forceinline__ void move(const accept_args &a, int first, int step) const {
+        const int lane = threadIdx.x & 63;
+        const int32_t to = (int32_t)(slot >= 0 && slot < (int64_t)a.pool << a.shift ? slot : -1), from = __shfl(to, max(mine, 0), 64);
+        const uint64_t left = __ballot(lane < count && mine != lane && to >= 0 && from >= 0);
+        if (left == 0) return;
+        const int units = 2 * a.layers * a.kv_heads * a.pieces, mask = (1 << a.shift) - 1;
+        for (int u = first; u < units; u += step) {
+            const int piece = u % a.pieces, head = u / a.pieces % a.kv_heads, layer = u / (a.pieces * a.kv_heads);
+            half_t *const base = (layer & 1 ? a.vpages : a.kpages) + (layer >> 1) * a.layer + 8 * piece;
+            auto where = [&](int32_t s) { return reinterpret_cast<half8_t *>(base + ((((int64_t)(s >> a.shift) * a.kv_heads + head) << a.shift) + (s & mask)) * (8 * a.pieces)); };
+            for (uint64_t todo = left; todo != 0;) {
+                half8_t v[8];
+                uint64_t rest = todo;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                if (rest != 0) v[i] = *where((int32_t)bs_read((uint32_t)from, __builtin_ctzll(rest)));
-                rest &= rest - 1;
-            }
+                for (int i = 0; i < 8; i++) {
+                    if (rest != 0) v[i] = *where((int32_t)bs_read((uint32_t)from, __builtin_ctzll(rest)));
+                    rest &= rest - 1;
+                }
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                if (todo != 0) *where((int32_t)bs_read((uint32_t)to, __builtin_ctzll(todo))) = v[i];
-                todo &= todo - 1;
+                for (int i = 0; i < 8; i++) {
+                    if (todo != 0) *where((int32_t)bs_read((uint32_t)to, __builtin_ctzll(todo))) = v[i];
+                    todo &= todo - 1;
+                }
             }
         }
+    }
+};
+
+// Many requests: workgroups of one request each; the ring in a launch of its own.
+__global__ __launch_bounds__(THREADS) void tree_accept_kernel(const accept_args a) {
+    const int b = blockIdx.x / a.blocks, block = blockIdx.x - b * a.blocks;
+    accept_path p(a, b);
+    p.walk();
+    if (block == 0 && threadIdx.x < 64) {
+        const int2 back = p.write(a, b);
+        if (threadIdx.x == 0) {
+            a.back[2 * b] = back.x;
+            a.back[2 * b + 1] = back.y;
+        }
+    }
+    p.move(a, block * THREADS + threadIdx.x, a.blocks * THREADS);
+}
+
+// Up to 64: one workgroup writes what the caller gets, and the ring; beside it, the others move.  (one request of 8 nodes, 32 layers of 8 heads of 128: ALONE us, with a second launch 10.3.)
+constexpr int FEW = 64, FEW_THREADS = 1024, FEW_WAVES = FEW_THREADS / 64;
+__global__ __launch_bounds__(FEW_THREADS) void tree_accept_few_kernel(const accept_args a, const int32_t *__restrict__ table, int32_t *ring, const int32_t *state, int32_t *state_out) {
+    if (blockIdx.x > 0) {
+        const int b = (blockIdx.x - 1) / a.blocks, block = (blockIdx.x - 1) - b * a.blocks;
+        accept_path p(a, b);
+        p.walk();
+        return p.move(a, block * FEW_THREADS + threadIdx.x, a.blocks * FEW_THREADS);
+    }
+    __shared__ int first[FEW], pages[FEW];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const plan_state st(state, a.pool);
+    for (int b0 = 0; b0 < a.B; b0 += FEW_WAVES) {
+        const int b = b0 + wave;
+        if (b >= a.B) break;
+        accept_path p(a, b);
+        p.walk();
+        const int2 back = p.write(a, b);
+        if (lane == 0) {
+            first[b] = back.x;
+            pages[b] = back.y;
+        }
+    }
+    __syncthreads();
+    if (wave > 0) return;
+    const int n = lane < a.B ? pages[lane] : 0, room = a.pool - st.count, upto = (int)bs_scan((uint32_t)n, [](uint32_t x, uint32_t y) { return x + y; }), sum = (int)bs_read((uint32_t)upto, 63);
+    for (int j = 0; j < n && upto - n + j < room; j++) ring[plan_wrap((uint32_t)st.tail + upto - n + j, a.pool)] = table[(int64_t)lane * a.max_pages + first[lane] + j];
+    if (lane == 0) {
+        state_out[0] = st.head;
+        state_out[1] = st.count + min(sum, room);
     }
 }
 
@@ -142,7 +201,7 @@ __global__ __launch_bounds__(BACK_THREADS) void tree_back_kernel(const int32_t *
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const plan_state st(state, pool);
     const int room = pool - st.count;
-    int sum = 0;                                 // (at most 5 pages of each of 65536 requests)
+    int sum = 0;                                 // (B * max_pages < 2^31)
     for (int b0 = 0; b0 < B; b0 += BACK_THREADS) {
         const int b = b0 + threadIdx.x, n = b < B ? back[2 * b + 1] : 0, first = b < B ? back[2 * b] : 0;
         const uint32_t upto = bs_scan((uint32_t)n, [](uint32_t x, uint32_t y) { return x + y; });
@@ -179,16 +238,18 @@ int bs_launch_tree_accept(const int64_t *tokens, const int32_t *parents, const i
                           const int32_t *starts, const int32_t *table, int32_t *ring, const int32_t *state, half_t *kpages, half_t *vpages, int32_t *lengths_out,
                           int32_t *state_out, int32_t *accepted, int32_t *path, int64_t *token, int B, int T, int nodes, int layers, int kv_heads, int head_dim, int shift,
                           int max_pages, int pool, void *workspace, hipStream_t s) {
-    if (B > 0) {
-        const int pieces = head_dim / 8;
-        const int64_t units = 2ll * layers * kv_heads * pieces;
-        const int64_t most = bs_cdiv(units, THREADS), fill = bs_cdiv(4096, B);
-        const int blocks = (int)(most < fill ? most : fill);
-        const accept_args a = {tokens, targets, slots, parents, lengths, granted, starts, kpages, vpages, lengths_out, accepted, path, token, (int32_t *)workspace,
-                               ((int64_t)pool * kv_heads << shift) * head_dim, B, T, nodes, blocks, layers, kv_heads, pieces, shift, max_pages, pool};
-        tree_accept_kernel<<<(unsigned)((int64_t)B * blocks), THREADS, 0, s>>>(a);
+    const int pieces = head_dim / 8, threads = B <= FEW ? FEW_THREADS : THREADS;
+    const int64_t most = bs_cdiv(2ll * layers * kv_heads * pieces, threads), fill = bs_cdiv(1 << 20, (int64_t)(B > 0 ? B : 1) * threads);
+    const int blocks = (int)(most < fill ? most : fill);
+    const accept_args a = {tokens, targets, slots, parents, lengths, granted, starts, kpages, vpages, lengths_out, accepted, path, token, (int32_t *)workspace,
+                           ((int64_t)pool * kv_heads << shift) * head_dim, B, T, nodes, blocks, layers, kv_heads, pieces, shift, max_pages, pool};
+    if (B <= FEW) {
+        tree_accept_few_kernel<<<(unsigned)(1 + B * blocks), FEW_THREADS, 0, s>>>(a, table, ring, state, state_out);
         BS_LAUNCH_CHECK();
+        return BS_OK;
     }
+    tree_accept_kernel<<<(unsigned)((int64_t)B * blocks), THREADS, 0, s>>>(a);
+    BS_LAUNCH_CHECK();
     tree_back_kernel<<<1, BACK_THREADS, 0, s>>>((const int32_t *)workspace, table, ring, state, state_out, B, max_pages, pool);
     BS_LAUNCH_CHECK();
     return BS_OK;

@@ -125,7 +125,7 @@ def test_many_calls_one_after_another(page, d, kv, layers):
         c.fork([rng.choice((b, b, -1, rng.randrange(B))) for b in range(B)], inplace=step % 2 == 0)
 
 
-@pytest.mark.parametrize("B,longest,wide", [(300, 60, 2), (1100, 40, 0), (70, 3000, 100), (3, 70000, 5)])
+@pytest.mark.parametrize("B,longest,wide", [(300, 60, 2), (1100, 40, 0), (70, 3000, 100), (3, 70000, 5), (16, 2900, 0), (9, 3800, 10), (64, 700, 10), (30, 1500, 20), (17, 900, 60), (40, 1900, 3)])
 def test_many_rows_and_wide_tables(B, longest, wide):
     rng = random.Random(B)
     c = Cache([rng.randrange(longest) for _ in range(B)], layers=1, kv=1, d=8, spare=B, together=tuple(range(0, B, 3)), wide=wide)
