@@ -3,7 +3,8 @@
 
 namespace {
 
-constexpr int THREADS = 512, SPAN = THREADS * 8;           // tokens of the vocabulary that a workgroup takes
+constexpr int THREADS = 512, RUN = THREADS * 8, RUNS = 2, SPAN = RUN * RUNS;          // tokens of the vocabulary that a workgroup takes: eight in a row to a thread, twice
+constexpr int BATCH = 8;                                   // tokens of the text that a thread requests at once
 constexpr uint32_t PROMPT = 1u << 31;                      // in a count: the token is in the prompt
 
 struct adjust_args {
@@ -20,91 +21,142 @@ struct adjust_args {
     int64_t mask_bytes;
 };
 
-// A workgroup counts the request's tokens of its span in LDS, and walks its logits once.
+// A workgroup counts the request's tokens of its span in LDS, and walks its logits once, which it requests before all else.  Tokens with a bias are a few of many: they are marked in a bit array, and a wave
+// that meets one looks it up in the request's list, 64 entries at a time.
+// What bounds it is the chain of a workgroup (row -> request -> text -> counts), hidden by the others of a CU, and the bytes: MEASURED
 template <bool PENALTIES, bool BIAS>
 __global__ __launch_bounds__(THREADS) void logits_adjust_kernel(const adjust_args a) {
-    __shared__ uint32_t counts[PENALTIES ? SPAN : 1], entry[BIAS ? SPAN : 1];
-    const int local = (int)(blockIdx.x / a.spans), from = (int)(blockIdx.x - (unsigned)local * a.spans) * SPAN, row = a.first + local, tid = threadIdx.x;
+    __shared__ __attribute__((aligned(16))) uint32_t counts[PENALTIES ? SPAN : 4];
+    __shared__ uint32_t marked[BIAS ? SPAN / 32 : 1];
+    const int local = (int)(blockIdx.x / a.spans), from = (int)(blockIdx.x - (unsigned)local * a.spans) * SPAN, row = a.first + local, tid = threadIdx.x, lane = tid & 63;
+    const half_t *x = a.logits + row * a.ld;
+    half_t *y = a.out + row * a.ld_out;
+    const bool whole = ((uintptr_t)x | (uintptr_t)y) % 16 == 0;
+    half8_t in[RUNS];
+#pragma unroll
+    for (int n = 0; n < RUNS; n++) {
+        const int i = from + n * RUN + 8 * tid;
+        in[n] = (half8_t)(half_t)0;
+        if (whole && i + 8 <= a.V) in[n] = *reinterpret_cast<const half8_t *>(x + i);
+        else
+            for (int e = 0; e < 8; e++)
+                if (i + e < a.V) in[n][e] = x[i + e];
+    }
+    const int state = a.allowed ? (a.allowed_rows ? a.allowed_rows[row] : row) : -1;
+    const uint8_t *allowed = state >= 0 && state < a.masks ? a.allowed + (int64_t)state * a.mask_bytes : nullptr;
+    uint32_t bits[RUNS];
+#pragma unroll
+    for (int n = 0; n < RUNS; n++) {
+        const int i = from + n * RUN + 8 * tid;
+        bits[n] = allowed && i < a.V ? allowed[i >> 3] : 0xffu;
+    }
     int b = a.requests ? a.requests[row] : row;
     const bool known = b >= 0 && b < a.B;
     b = known ? b : 0;
     float repetition = 1.f, frequency = 0.f, presence = 0.f;
-    bool counted = false, biased = false;
+    bool counted = false;
     if (PENALTIES && known) {
+        const int length = a.history_lengths ? a.history_lengths[b] : a.most, prompt = a.prompt_lengths ? a.prompt_lengths[b] : 0;
         if (a.repetition) repetition = a.repetition[b];
-        if (!(repetition > 0.f)) repetition = 1.f;
         if (a.frequency) frequency = a.frequency[b];
         if (a.presence) presence = a.presence[b];
+        if (!(repetition > 0.f)) repetition = 1.f;
         counted = repetition != 1.f || frequency != 0.f || presence != 0.f;
         if (counted) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) counts[tid + i * THREADS] = 0;
-        }
-    }
-    if (BIAS && known) {
-        biased = true;
+            for (int i = 0; i < SPAN / 4 / THREADS; i++) *reinterpret_cast<uint4_t *>(&counts[4 * (tid + i * THREADS)]) = (uint4_t)0u;
+            if (BIAS && tid < SPAN / 32) marked[tid] = 0;
+            __syncthreads();
+            const int n = min(max(length, 0), a.most);
+            const int32_t *text = a.history + (int64_t)b * a.most;
+            for (int i0 = 0; i0 < n; i0 += BATCH * THREADS) {
+                int32_t t[BATCH];
 #pragma unroll
-        for (int i = 0; i < 8; i++) entry[tid + i * THREADS] = 0;
-    }
-    if (counted || biased) __syncthreads();
-    if (counted) {
-        const int n = min(max(a.history_lengths ? a.history_lengths[b] : a.most, 0), a.most), prompt = a.prompt_lengths ? a.prompt_lengths[b] : 0;
-        const int32_t *text = a.history + (int64_t)b * a.most;
-        for (int i = tid; i < n; i += THREADS) {
-            const uint32_t t = (uint32_t)text[i] - (uint32_t)from;
-            if (t < (uint32_t)SPAN) {
-                if (i < prompt) atomicOr(&counts[t], PROMPT);
-                else atomicAdd(&counts[t], 1u);
+                for (int k = 0; k < BATCH; k++) {
+                    const int i = i0 + k * THREADS + tid;
+                    t[k] = i < n ? text[i] : -1;
+                }
+#pragma unroll
+                for (int k = 0; k < BATCH; k++) {
+                    const int i = i0 + k * THREADS + tid;
+                    const uint32_t at = (uint32_t)t[k] - (uint32_t)from;
+                    if (i >= n || at >= (uint32_t)SPAN) continue;
+                    if (i < prompt) atomicOr(&counts[at], PROMPT);
+                    else atomicAdd(&counts[at], 1u);
+                }
+            }
+            const int32_t *path = a.drafted + (int64_t)row * a.path;
+            for (int i = tid; i < a.path; i += THREADS) {
+                const uint32_t at = (uint32_t)path[i] - (uint32_t)from;
+                if (at < (uint32_t)SPAN) atomicAdd(&counts[at], 1u);
             }
         }
-        const int32_t *path = a.drafted + (int64_t)row * a.path;
-        for (int i = tid; i < a.path; i += THREADS) {
-            const uint32_t t = (uint32_t)path[i] - (uint32_t)from;
-            if (t < (uint32_t)SPAN) atomicAdd(&counts[t], 1u);
-        }
     }
+    const bool biased = BIAS && known;
+    const int32_t *tokens = a.bias_tokens + (int64_t)b * a.biases;
     if (biased) {
-        const int32_t *tokens = a.bias_tokens + (int64_t)b * a.biases;
+        if (!counted) {
+            if (tid < SPAN / 32) marked[tid] = 0;
+            __syncthreads();
+        }
         for (int i = tid; i < a.biases; i += THREADS) {
-            const uint32_t t = (uint32_t)tokens[i] - (uint32_t)from;
-            if (t < (uint32_t)SPAN) atomicMax(&entry[t], (uint32_t)i + 1);       // (the last entry of a token counts)
+            const uint32_t at = (uint32_t)tokens[i] - (uint32_t)from;
+            if (at < (uint32_t)SPAN) atomicOr(&marked[at >> 5], 1u << (at & 31));
         }
     }
     if (counted || biased) __syncthreads();
-    const int state = a.allowed ? (a.allowed_rows ? a.allowed_rows[row] : row) : -1;
-    const uint8_t *allowed = state >= 0 && state < a.masks ? a.allowed + (int64_t)state * a.mask_bytes : nullptr;
-    const half_t *x = a.logits + row * a.ld;
-    half_t *y = a.out + row * a.ld_out;
-    auto one = [&](half_t in, int t, bool fits) {          // the logit of token from + t
-        float v = (float)in;
-        bool finite = __builtin_isfinite(v);
+#pragma unroll
+    for (int n = 0; n < RUNS; n++) {
+        const int t0 = n * RUN + 8 * tid, i0 = from + t0;
+        float v[8];
+        uint32_t finite = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            v[e] = (float)in[n][e];
+            finite |= (uint32_t)__builtin_isfinite(v[e]) << e;
+        }
         if (counted) {
-            const uint32_t c = counts[t], said = c & ~PROMPT;
-            if (c != 0) v = v > 0.f ? v / repetition : v * repetition;
-            if (said != 0) v = v - frequency * (float)said - presence;
+            uint32_t c[8];
+            *reinterpret_cast<uint4_t *>(c) = *reinterpret_cast<const uint4_t *>(&counts[t0]);
+            *reinterpret_cast<uint4_t *>(c + 4) = *reinterpret_cast<const uint4_t *>(&counts[t0 + 4]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const uint32_t said = c[e] & ~PROMPT;
+                if (c[e] != 0) v[e] = v[e] > 0.f ? v[e] / repetition : v[e] * repetition;
+                if (said != 0) v[e] = v[e] - frequency * (float)said - presence;
+            }
         }
         if (biased) {
-            const uint32_t e = entry[t];
-            if (e != 0) {
-                const float w = a.bias[(int64_t)b * a.biases + e - 1];
-                v += w;
-                finite = finite && __builtin_isfinite(w);
+            uint32_t mine = marked[t0 >> 5] >> (t0 & 31) & 0xff;
+            for (uint64_t who = __ballot(mine != 0); who != 0; who = __ballot(mine != 0)) {
+                const int leader = __builtin_ctzll(who), e_of = __builtin_ctz((uint32_t)__builtin_amdgcn_readlane((int)mine, leader));
+                const int32_t token = __builtin_amdgcn_readlane(i0, leader) + e_of;
+                int last = -1;                   // (of several entries for a token the last counts)
+                for (int j0 = 0; j0 < a.biases; j0 += 64) {
+                    const uint64_t here = __ballot(j0 + lane < a.biases && tokens[j0 + lane] == token);
+                    if (here != 0) last = j0 + 63 - __builtin_clzll(here);
+                }
+                const float w = a.bias[(int64_t)b * a.biases + last];
+                const bool fine = __builtin_isfinite(w);
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (lane == leader && e == e_of) {
+                        v[e] += w;
+                        finite &= fine ? 0xffu : ~(1u << e);
+                    }
+                if (lane == leader) mine &= mine - 1;
             }
         }
-        if (finite) v = fminf(fmaxf(v, -65504.f), 65504.f);
-        return fits ? (half_t)v : (half_t)-INFINITY;
-    };
-    const int t0 = 8 * tid, i0 = from + t0;
-    if (i0 >= a.V) return;
-    const uint32_t bits = allowed ? allowed[i0 >> 3] : 0xffu;
-    if (((uintptr_t)x | (uintptr_t)y) % 16 == 0 && i0 + 8 <= a.V) {
-        const half8_t in = *reinterpret_cast<const half8_t *>(x + i0);
         half8_t o;
 #pragma unroll
-        for (int e = 0; e < 8; e++) o[e] = one(in[e], t0 + e, bits >> e & 1);
-        *reinterpret_cast<half8_t *>(y + i0) = o;
-    } else {
-        for (int e = 0; e < 8 && i0 + e < a.V; e++) y[i0 + e] = one(x[i0 + e], t0 + e, bits >> e & 1);
+        for (int e = 0; e < 8; e++) {
+            if (finite >> e & 1) v[e] = fminf(fmaxf(v[e], -65504.f), 65504.f);
+            o[e] = bits[n] >> e & 1 ? (half_t)v[e] : (half_t)-INFINITY;
+        }
+        if (whole && i0 + 8 <= a.V) *reinterpret_cast<half8_t *>(y + i0) = o;
+        else
+            for (int e = 0; e < 8; e++)
+                if (i0 + e < a.V) y[i0 + e] = o[e];
     }
 }
 
