@@ -24,9 +24,9 @@ import torch.nn.functional as F
 from bitstack_amd import _lib
 from bitstack_amd._lib import EPI_NONE, EPI_RESIDUAL, EPI_SWIGLU
 from bitstack_amd.modules.BitStackLinear import BitStackLinear
-from bitstack_amd.utils.inference_utils import (MatrixGroup, add_rmsnorm_hip, argmax_hip, attention_paged_hip, attention_prefill_hip, bitstack_forward_group_hip,
-                                                forward_cat_hip, linear_f16_hip, page_plan_hip, plainly_called, rmsnorm_hip, rope_store_hip, rope_store_paged_hip,
-                                                sample_hip, silu_mul_hip)
+from bitstack_amd.utils.inference_utils import (MatrixGroup, add_rmsnorm_hip, argmax_hip, attention_paged_hip, attention_prefill_hip, attention_tree_hip,
+                                                bitstack_forward_group_hip, forward_cat_hip, linear_f16_hip, logits_adjust_hip, page_fork_hip, page_plan_hip, plainly_called,
+                                                rmsnorm_hip, rope_store_hip, rope_store_paged_hip, sample_hip, silu_mul_hip, tree_accept_hip, tree_plan_hip)
 
 PROJ = ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj", "self_attn.o_proj",
         "mlp.gate_proj", "mlp.up_proj", "mlp.down_proj")
@@ -133,10 +133,11 @@ def _synthetic_bitstack(m, n, blocks, k, dev, gen, name):
 
 
 class PagedCache:
-    """Keys and values of up to `rows` requests of unequal lengths, in pages that a decoder's layers share one table of: what prefill_paged()
-    and step_paged() work on.  Everything is on the device: plans, lengths and free pages never come to the host."""
+    """Keys and values of up to `rows` requests of unequal lengths, in pages that a decoder's layers share one table of: what prefill_paged(),
+    step_paged() and step_tree() work on.  Everything is on the device: plans, lengths and free pages never come to the host.  With `forks` rows may
+    become copies of other rows (fork()), which share pages."""
 
-    def __init__(self, decoder, rows: int, pool_pages: int, page_size: int = 16):
+    def __init__(self, decoder, rows: int, pool_pages: int, page_size: int = 16, forks: bool = False):
         s, dev = decoder.s, decoder.dev
         if not 1 <= rows <= 48:
             raise ValueError("1 to 48 rows (the grouped launches take up to 48 tokens)")
@@ -149,10 +150,29 @@ class PagedCache:
         self.free_pages = torch.arange(pool_pages, **i32)                  # a ring, and its {first, count}
         self.free_state = torch.tensor([0, pool_pages], **i32)
         self.token = torch.zeros(rows, dtype=torch.long, device=dev)       # next token of every request
+        self.shares = torch.zeros(pool_pages, **i32) if forks else None    # rows that hold a page, less one
 
     def plan(self, new_tokens, tokens, released=None):
         """page_plan_hip on this cache, in place."""
+        if self.shares is not None and released is not None:              # (pages of such a row may be others' too)
+            self._fork(torch.where(released.bool(), -1, torch.arange(self.rows, dtype=torch.int32, device=released.device)))
+            released = None
         return page_plan_hip(self.lengths, new_tokens, self.block_table, self.free_pages, self.free_state, self.page_size, tokens, released=released, inplace=True)
+
+
+    def _fork(self, source):
+        return page_fork_hip(source, self.lengths, self.block_table, self.free_pages, self.free_state, self.shares, self.kpages, self.vpages, inplace=True)
+
+    @torch.no_grad()
+    def fork(self, source):
+        """Row b becomes what row source[b] (int32 [rows]) is, its next token too: page_fork_hip on this cache.  -1 empties a row, its own number leaves it.  Returns
+        page_fork_hip's answer: granted is 0 for rows that stay, as no page was there."""
+        if self.shares is None:
+            raise ValueError("a cache whose rows are forked is made with forks=True")
+        done = self._fork(source)
+        moved = (done.granted > 0) & (source >= 0) & (source < self.rows)
+        self.token.copy_(torch.where(moved, self.token[source.clamp(0, self.rows - 1).long()], self.token))
+        return done
 
 
 class SyntheticLlamaDecoder:
@@ -619,13 +639,12 @@ class SyntheticLlamaDecoder:
         return plan, self._head(hn)
 
     @torch.no_grad()
-    def step_paged(self, cache: PagedCache, new_tokens=None, released=None, uniform=None, **sampling):
+    def step_paged(self, cache: PagedCache, new_tokens=None, released=None, uniform=None, adjust=None, **sampling):
         """One token for every request of the cache: cache.token at its next position.  new_tokens (int32 [rows]; None: 1 for all but the
         released) is 0 for rows that are idle, `released` [rows] gives the pages of finished ones back.  The next tokens, greedy or with `uniform` [rows] drawn as sample_hip
         does with temperature, top_k, top_p, min_p, go to cache.token for requests that got a slot: not those at max_len, or without a page (plan.granted).
-        Returns the plan; self.logits holds the logits."""
-        if uniform is None and any(v is not None for v in sampling.values()):
-            raise ValueError("temperature, top_k, top_p and min_p need the random numbers `uniform`; without them the step is greedy")
+        `adjust`: logits_adjust_hip's settings, for the logits in front of that (history with cache.token in it).  Returns the plan; self.logits holds the logits."""
+        self._check_sampling(uniform, sampling)
         s, eps = self.s, self.s.rms_eps
         if self._groups is None:
             self._build_groups()
@@ -643,15 +662,81 @@ class SyntheticLlamaDecoder:
             act = bitstack_forward_group_hip(grp["gate_up"], x, EPI_SWIGLU, rms_eps=eps)
             x = bitstack_forward_group_hip(grp["down"], act, EPI_RESIDUAL, residual=x)
         self.logits = self._head(rmsnorm_hip(x, self.final_norm, eps))
-        if uniform is not None:
-            token = sample_hip(self.logits, uniform, **sampling)
-        elif cache.rows == 1 or self.logits.shape[1] % 8 == 0:
-            token = argmax_hip(self.logits)
-        else:                                                              # (rows that do not start on 16 bytes)
-            zeros = torch.zeros(cache.rows, device=self.dev)
-            token = sample_hip(self.logits, zeros, temperature=zeros)
+        if adjust:
+            logits_adjust_hip(self.logits, **adjust)
+        token = self._choose(uniform, **sampling)
         torch.where(plan.granted > 0, token, cache.token, out=cache.token)
         return plan
+
+    @staticmethod
+    def _check_sampling(uniform, sampling):
+        if uniform is None and any(v is not None for v in sampling.values()):
+            raise ValueError("temperature, top_k, top_p and min_p need the random numbers `uniform`; without them the step is greedy")
+
+    def _choose(self, uniform, **sampling):
+        """The token of every row of the logits, greedy or drawn."""
+        if uniform is not None:
+            return sample_hip(self.logits, uniform, **sampling)
+        if self.logits.shape[0] == 1 or self.logits.shape[1] % 8 == 0:
+            return argmax_hip(self.logits)
+        zeros = torch.zeros(self.logits.shape[0], device=self.dev)        # (rows that do not start on 16 bytes)
+        return sample_hip(self.logits, zeros, temperature=zeros)
+
+    @torch.no_grad()
+    def step_tree(self, cache: PagedCache, tokens, parents, new_tokens, nodes=64, released=None, uniform=None, adjust=None, **sampling):
+        """Several drafted tokens per request in one step, of which as many are kept as the model would have given one by one.  Request b's new_tokens[b] (int32 [rows], up to
+        `nodes`; 0: idle) tokens are the next rows of tokens [T] (int64) and parents [T] (int32: a number among the request's own, smaller than the token's; -1 for the first): its first
+        one is its cache.token, whatever `tokens` says, the others are drafts, each behind its parent.  The model's token behind each is greedy, or drawn with uniform [T] and the
+        requests' temperature, top_k, top_p, min_p [rows]; `adjust`: logits_adjust_hip's settings per request and allowed_rows per token (history with cache.token in it, the drafts are added).
+        Keys and values of what is accepted stay in the cache, and cache.token is the model's token behind it.  Returns (plan, tree_accept_hip's answer, the tokens): request b's new
+        tokens are tokens[plan.starts[b] + path[b, 1:accepted[b]]] and its cache.token."""
+        self._check_sampling(uniform, sampling)
+        s, d, eps, T = self.s, self.s.head_dim, self.s.rms_eps, tokens.shape[0]
+        if self.max_len % cache.page_size:
+            raise ValueError("step_tree needs max_len to be whole pages")
+        if not 1 <= nodes <= 64 or T < 1:
+            raise ValueError("1 to 64 nodes per request, and a token at least")
+        plan = cache.plan(new_tokens, T, released=released)
+        tree = tree_plan_hip(parents, cache.lengths, plan.granted, plan.starts)
+        ids = torch.cat([tokens, tokens[:1]])                             # (one more, for requests without a token)
+        ids.scatter_(0, torch.where((new_tokens > 0) & (plan.starts[:-1] < T), plan.starts[:-1], T).long(), cache.token)
+        ids = ids[:T]
+        request = torch.searchsorted(plan.starts[1:].contiguous(), torch.arange(T, dtype=torch.int32, device=self.dev), right=True).clamp(max=cache.rows - 1)
+        x = self.embed.index_select(0, ids)
+        wide = s.heads * d, s.kv_heads * d, s.kv_heads * d
+        few = T <= 48                                                     # (what the grouped launches take)
+        if few and self._groups is None:
+            self._build_groups()
+        hn = None if few else rmsnorm_hip(x, self.norm_w[0, 0], eps)
+        for L in range(s.layers):
+            lin = self.lin[L]
+            if few:
+                qkv = bitstack_forward_group_hip(self._groups[L]["qkv"], x, rms_eps=eps)
+            else:
+                qkv = forward_cat_hip([lin[p] for p in PROJ[:3]], hn)
+            q, k, v = qkv.split(wide, 1) if qkv is not None else (self._output(lin[p], hn) for p in PROJ[:3])
+            rope_store_paged_hip(q, k, v, self.cos, self.sin, cache.kpages[L], cache.vpages[L], tree.positions, plan.slots)
+            ctx = attention_tree_hip(q, cache.kpages[L], cache.vpages[L], cache.block_table, cache.lengths, plan.granted, plan.starts, tree.masks, nodes)
+            if few:
+                x = bitstack_forward_group_hip(self._groups[L]["o"], ctx, EPI_RESIDUAL, residual=x)
+                act = bitstack_forward_group_hip(self._groups[L]["gate_up"], x, EPI_SWIGLU, rms_eps=eps)
+                x = bitstack_forward_group_hip(self._groups[L]["down"], act, EPI_RESIDUAL, residual=x)
+            else:
+                x, hn = self._sum_norm(x, self._output(lin["self_attn.o_proj"], ctx), self.norm_w[L, 1])
+                act = self._silu_mul(*(self._output(lin[p], hn) for p in PROJ[4:6]))
+                x, hn = self._sum_norm(x, self._output(lin["mlp.down_proj"], act), self.norm_w[L + 1, 0] if L + 1 < s.layers else self.final_norm)
+        self.logits = self._head(rmsnorm_hip(x, self.final_norm, eps) if few else hn)
+        if adjust:
+            if adjust.get("history") is not None and nodes > 1:           # what a token has in front of it in its tree, the first one's is in the history
+                other = torch.arange(1, nodes, device=self.dev)
+                drafted = ids[(plan.starts[request].long()[:, None] + other).clamp(max=T - 1)]
+                adjust = {**adjust, "drafted": torch.where((tree.masks[:, None] >> other & 1) == 1, drafted, -1).int()}
+            logits_adjust_hip(self.logits, requests=request.int(), **adjust)
+        targets = self._choose(uniform, **{name: None if t is None else t[request] for name, t in sampling.items()})
+        done = tree_accept_hip(ids, parents, targets, plan.slots, cache.lengths, plan.granted, plan.starts, cache.block_table, cache.free_pages, cache.free_state, cache.kpages,
+                               cache.vpages, nodes, inplace=True)
+        torch.where(done.accepted > 0, done.token, cache.token, out=cache.token)
+        return plan, done, ids
 
     def prefill_positions(self, prompt: torch.Tensor, fused=False):
         """Feed a prompt token by token (the measurement is about decode).  `prompt`
