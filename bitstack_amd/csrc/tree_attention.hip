@@ -74,6 +74,17 @@ __device__ __forceinline__ float across(float v) {
     return SUM ? __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b) : fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
 }
 
+// the largest of all lanes' v, or (SUM) their sum
+template <bool SUM>
+__device__ __forceinline__ float ta_all(float v) {
+    auto both = [&](uint32_t other) { v = SUM ? v + __builtin_bit_cast(float, other) : fmaxf(v, __builtin_bit_cast(float, other)); };
+    both(bs_lane<0xb1>(__builtin_bit_cast(uint32_t, v)));        // quad_perm 1, 0, 3, 2
+    both(bs_lane<0x4e>(__builtin_bit_cast(uint32_t, v)));        // quad_perm 2, 3, 0, 1
+    both(bs_lane<0x141>(__builtin_bit_cast(uint32_t, v)));       // 8 lanes mirrored, then 16
+    both(bs_lane<0x140>(__builtin_bit_cast(uint32_t, v)));
+    return across<32, SUM>(across<16, SUM>(v));
+}
+
 typedef __attribute__((address_space(3))) void *ta_lds;
 
 // What a workgroup is at: stages st .. st_end - 1 of request b, whose stages have the numbers from `before` on.
@@ -100,7 +111,7 @@ __device__ __forceinline__ ta_request ta_uniform(const ta_request &r, int lane) 
 // The next request of the share (up to 64 requests: the first one too): false where there is none.  Up to 64 requests every wave finds it by itself, a lane a request.
 template <bool FIRST>
 __device__ __forceinline__ bool ta_next_of_few(const ta_args &a, ta_work &w, int &first) {
-    const int lane = threadIdx.x & 63;
+    const int lane = ta_here(threadIdx.x & 63);
     const ta_request r(a, min(lane, a.B - 1));
     const int stages = lane < a.B ? r.stages() : 0, upto = (int)bs_scan((uint32_t)stages, [](uint32_t x, uint32_t y) { return x + y; });
     if (FIRST) {
@@ -210,7 +221,7 @@ struct ta_again {
     float top, sum, o[D / 64];
     __device__ __forceinline__ ta_again(const ta_args &a, const ta_request &rq, const int32_t *ids, int node, int head, int hk, int p_first, int p_end, float scale2) {
         constexpr int PER = D / 64;
-        const int lane = threadIdx.x & 63, held = rq.len - rq.n;
+        const int lane = ta_here(threadIdx.x & 63), held = rq.len - rq.n;
         const half_t *qr = a.q + (int64_t)(rq.start + node) * a.ldq + head * D;
         const uint64_t sees = (uint64_t)a.masks[rq.start + node];
         auto where = [&](int p) {                // halves in front of position p; -1: not seen, or not there
@@ -234,8 +245,7 @@ struct ta_again {
 #pragma unroll
         for (int e = 0; e < PER; e++) o[e] = 0.f;
         for (int p0 = p_first; p0 < p_end; p0 += 64) top = fmaxf(top, score(where(p0 + lane)));
-#pragma unroll
-        for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+        top = ta_all<false>(top);
         const float from = top == -INFINITY ? 0.f : top;
         for (int p0 = p_first; p0 < p_end; p0 += 64) {
             const int64_t at = where(p0 + lane);
@@ -243,15 +253,14 @@ struct ta_again {
             sum += weight;
 #pragma unroll 1
             for (int i = 0; i < 64; i++) {
-                const int64_t ai = __shfl(at, i, 64);
-                const float wi = __shfl(weight, i, 64);
+                const int64_t ai = (int64_t)((uint64_t)bs_read((uint32_t)((uint64_t)at >> 32), i) << 32 | bs_read((uint32_t)at, i));
+                const float wi = __builtin_bit_cast(float, bs_read(__builtin_bit_cast(uint32_t, weight), i));
                 if (ai < 0 || wi == 0.f) continue;
 #pragma unroll
                 for (int e = 0; e < PER; e++) o[e] = __builtin_fmaf(wi, (float)a.vpages[ai + PER * lane + e], o[e]);
             }
         }
-#pragma unroll
-        for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x, 64);
+        sum = ta_all<true>(sum);
         top = top == -INFINITY ? TA_LOW : top;
     }
 };
@@ -556,7 +565,7 @@ __global__ __launch_bounds__(256, 2) void attention_tree_few_kernel(const ta_arg
         }
         if (w.at < w.end) __syncthreads();       // (the next request's go to the same places)
     }
-    if (hk == 0) ta_idle<THREADS>(a, g_of, gridDim.x / a.kv_heads, D);
+    if (hk == 0) ta_idle<THREADS>(a, g_of, a.shares ? a.shares : a.B, D);
 }
 
 // ---- more rows: K and V come to LDS, for the WR waves of 16 QT rows each.  Many rows: what counts are the products and the softmax, and the scores of a stage are computed one stage ahead (AHEAD).
@@ -653,13 +662,11 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
         // ---- the rows of q
         const bool mine = row0 + 16 * QT * wave < all_rows;
         half8_t q8[QT][NC];
-        uint64_t mask[QT];
-        int node_of[QT], head_of[QT];
+        auto sees = [&](int node) { return (uint64_t)a.masks[rq.start + node] & (rq.n < 64 ? (1ull << rq.n) - 1 : ~0ull); };
+        uint64_t mask[QT];                           // (AHEAD: read again where they are needed, registers are short)
 #pragma unroll
         for (int t = 0; t < QT; t++) {
             const int row = min(row0 + 16 * (QT * wave + t) + r16, all_rows - 1), node = ta_node(row, rep, a.per_rep), head = hk * rep + row - node * rep;
-            node_of[t] = node;
-            head_of[t] = head;
             const half_t *p = a.q + (int64_t)(rq.start + node) * a.ldq + head * D + 8 * g;
             if (((uintptr_t)a.q | (uintptr_t)(2 * a.ldq)) % 16 == 0) {
 #pragma unroll
@@ -670,7 +677,7 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
 #pragma unroll
                     for (int e = 0; e < 8; e++) q8[t][c][e] = p[32 * c + e];
             }
-            mask[t] = (uint64_t)a.masks[rq.start + node] & (rq.n < 64 ? (1ull << rq.n) - 1 : ~0ull);
+            if (!AHEAD) mask[t] = sees(node);
         }
 
         const float scale2 = ta_scale(D);
@@ -720,6 +727,10 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
         // some of a stage's positions are nodes, behind the last one, or of a page that does not exist (`bits`: of its tiles)
         auto masked = [&](int st, int bits) { return TA_P * (st + 1) > held || bits != 0; };
         auto hide = [&](int st, int bits, float4_t (&s)[QT][2]) __attribute__((always_inline)) {
+            if (AHEAD) {
+#pragma unroll
+                for (int t = 0; t < QT; t++) mask[t] = sees(ta_node(min(row0 + 16 * (QT * wave + t) + (ta_here(lane) & 15), all_rows - 1), rep, a.per_rep));
+            }
 #pragma unroll
             for (int i = 0; i < 2; i++) {
 #pragma unroll
@@ -866,17 +877,19 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
 #pragma unroll
         for (int t = 0; t < QT; t++) {
             l[t] = across<32, true>(across<16, true>(l[t]));
-            const bool there = row0 + 16 * (QT * wave + t) + r16 < all_rows;
+            const int at = row0 + 16 * (QT * wave + t) + (ta_here(lane) & 15), row = min(at, all_rows - 1), node = ta_node(row, rep, a.per_rep), head = hk * rep + row - node * rep;
+            const bool there = at < all_rows;
+            const uint64_t seen = AHEAD ? sees(node) : mask[t];
             // NaN, or an infinity; a position that it sees had one
             float sum = l[t];
 #pragma unroll
             for (int j = 0; j < W; j++) sum += (acc[t][j][0] - acc[t][j][0]) + (acc[t][j][1] - acc[t][j][1]) + (acc[t][j][2] - acc[t][j][2]) + (acc[t][j][3] - acc[t][j][3]);
-            const uint64_t bad = __ballot(there && (sum != sum || odd_held != 0 || (mask[t] & ((uint64_t)odd_nodes[1] << 32 | odd_nodes[0])) != 0));
+            const uint64_t bad = __ballot(there && (sum != sum || odd_held != 0 || (seen & ((uint64_t)odd_nodes[1] << 32 | odd_nodes[0])) != 0));
             again[t] = (uint32_t)((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff);
             if (!there) continue;
             const float inv = l[t] != 0.f ? 1.f / l[t] : 0.f;              // (0: nothing was seen)
             if (cut) {
-                float *to = ta_part_row(a, w.slot, node_of[t], head_of[t], D);
+                float *to = ta_part_row(a, w.slot, node, head, D);
                 if (g == 0) {
                     to[0] = m[t];
                     to[1] = l[t];
@@ -884,7 +897,7 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
 #pragma unroll
                 for (int j = 0; j < W; j++) *reinterpret_cast<float4_t *>(to + 4 + 16 * j + 4 * g) = acc[t][j];
             } else {
-                half_t *to = a.out + ((int64_t)(rq.start + node_of[t]) * a.heads + head_of[t]) * D;
+                half_t *to = a.out + ((int64_t)(rq.start + node) * a.heads + head) * D;
                 const bool whole = ((uintptr_t)a.out & 7) == 0;
 #pragma unroll
                 for (int j = 0; j < W; j++) {        // row 4 g + i of product j is dimension 16 j + 4 g + i
@@ -916,15 +929,15 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
                     to[1] = x.sum;
                 }
 #pragma unroll
-                for (int e = 0; e < PER; e++) to[4 + PER * lane + e] = x.o[e];
+                for (int e = 0; e < PER; e++) to[4 + PER * ta_here(lane) + e] = x.o[e];
             } else {
                 const float inv = x.sum != 0.f ? 1.f / x.sum : 0.f;
 #pragma unroll
-                for (int e = 0; e < PER; e++) a.out[token_head * D + PER * lane + e] = (half_t)(x.sum != 0.f ? x.o[e] * inv : 0.f);
+                for (int e = 0; e < PER; e++) a.out[token_head * D + PER * ta_here(lane) + e] = (half_t)(x.sum != 0.f ? x.o[e] * inv : 0.f);
             }
         }
     }
-    if (unit == 0) ta_idle<THREADS>(a, work, gridDim.x / units, D);
+    if (unit == 0) ta_idle<THREADS>(a, work, a.shares ? a.shares : a.B, D);
 }
 
 // The parts of a row of a head put together, in order: D / 4 threads each.
