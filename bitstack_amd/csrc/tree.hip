@@ -160,7 +160,7 @@ __global__ __launch_bounds__(THREADS) void tree_accept_kernel(const accept_args 
     p.move(a, block * THREADS + threadIdx.x, a.blocks * THREADS);
 }
 
-// Up to 64: one workgroup writes what the caller gets, and the ring; beside it, the others move.  (one request of 8 nodes, 32 layers of 8 heads of 128: ALONE us, with a second launch 10.3.)
+// Up to 64: one workgroup writes what the caller gets, and the ring; beside it, the others move.  (one request of 8 nodes, 32 layers of 8 heads of 128: 7.2 us, with a second launch 10.3.)
 constexpr int FEW = 64, FEW_THREADS = 1024, FEW_WAVES = FEW_THREADS / 64;
 __global__ __launch_bounds__(FEW_THREADS) void tree_accept_few_kernel(const accept_args a, const int32_t *__restrict__ table, int32_t *ring, const int32_t *state, int32_t *state_out) {
     if (blockIdx.x > 0) {

@@ -31,10 +31,10 @@ struct ta_args {
     const int32_t *table, *lengths, *granted, *starts;
     const int64_t *masks;
     half_t *out;
-    int32_t *before;                             // workspace: stages of the requests before each one, and of all
+    int32_t *before;                             // workspace: stages of the requests before each one, (or parts); of all, shares, stages of a part
     float *part;                                 // ... and what parts leave: [share, first or last][node][head][max, sum, pad, pad, weighted v]
-    float per_rep;                               // 1 / (heads per KV head)
-    int ldq, B, T, nodes, heads, kv_heads, row_tiles, shift, max_pages, pool, shares, least;      // (shares 0: a workgroup of a unit takes one request)
+    float per_rep, part_cost;                    // 1 / (heads per KV head); what a part of all units costs, in stages
+    int ldq, B, T, nodes, heads, kv_heads, row_tiles, shift, max_pages, pool, shares, more;      // (shares 0: a workgroup of a unit takes one request)
 };
 
 struct ta_request {
@@ -57,7 +57,9 @@ __device__ __forceinline__ int ta_node(int row, int rep, float per_rep) {
 // share g of `sum` stages dealt to `shares`: where it begins; and whose stage x is
 __device__ __forceinline__ int ta_begins(int g, int sum, int shares) { return (int)((int64_t)g * sum / shares); }
 __device__ __forceinline__ int ta_whose(int x, int sum, int shares) { return (int)((((int64_t)x + 1) * shares - 1) / sum); }
-__device__ __forceinline__ int ta_shares(const ta_args &a, int sum) { return min(a.shares, (sum + a.least - 1) / a.least); }
+// parts of a request that has `stages`, none of more than `per`; where part i of n begins
+__device__ __forceinline__ int ta_parts(int stages, int per) { return (int)((uint32_t)(stages + per - 1) / (uint32_t)per); }
+__device__ __forceinline__ int ta_cut(int i, int stages, int n) { return (int)((int64_t)i * stages / n); }
 
 // v, of which nothing is worked out ahead of here (registers are short in the loops over the stages)
 __device__ __forceinline__ int ta_here(int v) {
@@ -87,10 +89,10 @@ __device__ __forceinline__ float ta_all(float v) {
 
 typedef __attribute__((address_space(3))) void *ta_lds;
 
-// What a workgroup is at: stages st .. st_end - 1 of request b, whose stages have the numbers from `before` on.
+// What a workgroup is at: stages st .. st_end - 1 of request b.
 struct ta_work {
     int g, at, end;                              // its share, stages still to do
-    int b, before, st, st_end, slot;             // slot: of a part; -1: the whole request
+    int b, before, st, st_end, slot;             // before: stages (or parts) of the requests in front of b; slot: of a part; -1: the whole request
     ta_request rq;
     __device__ __forceinline__ void take(int first) {
         const int stages = rq.stages();
@@ -98,6 +100,13 @@ struct ta_work {
         st_end = min(stages, st + end - at);
         slot = st == 0 && st_end == stages ? -1 : 2 * g + (at != first);
         at += st_end - st;
+    }
+    __device__ __forceinline__ void take_part(int per) {
+        const int stages = rq.stages(), n = ta_parts(stages, per);
+        st = ta_cut(g - before, stages, n);
+        st_end = ta_cut(g - before + 1, stages, n);
+        slot = n == 1 ? -1 : 2 * g;
+        at = end = 0;
     }
 };
 __device__ __forceinline__ ta_request ta_uniform(const ta_request &r, int lane) {
@@ -108,59 +117,140 @@ __device__ __forceinline__ ta_request ta_uniform(const ta_request &r, int lane) 
     u.len = (int)bs_read((uint32_t)r.len, lane);
     return u;
 }
+// How the stages of all requests, `sum`, are dealt to a.shares workgroups of a unit.
+// Equal shares keep the workgroups busy to the end whatever the lengths are, but one may hold the end of a request and the beginning of another: each costs its chain of latencies (lengths, pages, K, what it
+// leaves), 4 us, and is a part.  Each request's own parts, one to a workgroup, have one chain, but may be unequal.  They are taken where they fit and none has `more` stages more than an equal share (16
+// up to 32 rows, whose stages take 0.3 us, else 32).  us, equal shares / own parts: 5 requests of up to 1000 with 8 nodes 19 / 14, 16 of up to 250 24 / 14, 64 of up to 1000 with 32 nodes 78 / 62, and
+// at a limit of 32 where 16 stands 32 requests of up to 4000 with 4 nodes 58 / 65.
+// A part has at least 4 stages; more where the longest request would be in many, which the second launch takes eight at a time (8 nodes, one request of 4000: 8 stages 16.6, 4 stages 20.1); and more
+// where all of them are many: what all units leave of one costs part_cost stages, so that parts of sqrt(part_cost sum) stages cost as much as they have (16 requests of 390: whole 15, in four 25).
+struct ta_deal {
+    int sum, shares, per;                        // per: stages of a part at most; 0: equal shares
+    // live: requests that have stages; longest: the most of one; count(per): parts of all requests
+    template <typename C>
+    __device__ __forceinline__ ta_deal(const ta_args &a, int sum, int live, int longest, C count) : sum(sum) {
+        const int even = (int)((uint32_t)(sum + a.shares - 1) / (uint32_t)a.shares), least = max(4, (int)__builtin_amdgcn_sqrtf(fmaxf(0.25f * (float)longest, a.part_cost * (float)sum)));
+        per = 0;
+        shares = a.shares;
+        if (live <= a.shares) {
+            const int room = a.shares - live;    // (a request has less than one part more than its stages / per)
+            per = max(even, least);
+            int n = count(per);
+            if (n > a.shares) {
+                per = room > 0 ? min(longest, max(least, (int)((uint32_t)(sum + room - 1) / (uint32_t)room))) : longest;
+                if (per > even + a.more) per = 0;
+                else n = count(per);
+            }
+            if (per) shares = n;
+        }
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            a.before[a.B] = sum;
+            a.before[a.B + 1] = shares;
+            a.before[a.B + 2] = per;
+        }
+    }
+};
 // The next request of the share (up to 64 requests: the first one too): false where there is none.  Up to 64 requests every wave finds it by itself, a lane a request.
 template <bool FIRST>
 __device__ __forceinline__ bool ta_next_of_few(const ta_args &a, ta_work &w, int &first) {
     const int lane = ta_here(threadIdx.x & 63);
     const ta_request r(a, min(lane, a.B - 1));
-    const int stages = lane < a.B ? r.stages() : 0, upto = (int)bs_scan((uint32_t)stages, [](uint32_t x, uint32_t y) { return x + y; });
+    auto plus = [](uint32_t x, uint32_t y) { return x + y; };
+    const int stages = lane < a.B ? r.stages() : 0;
+    int upto = (int)bs_scan((uint32_t)stages, plus), mine = stages, x = w.at, per = 0;
     if (FIRST) {
-        const int sum = (int)bs_read((uint32_t)upto, 63), shares = ta_shares(a, sum);
-        if (blockIdx.x == 0 && threadIdx.x == 0) a.before[a.B] = sum;
-        if (w.g >= shares) return false;
-        w.at = first = ta_begins(w.g, sum, shares);
-        w.end = ta_begins(w.g + 1, sum, shares);
+        const int longest = (int)bs_read(bs_scan((uint32_t)stages, [](uint32_t x, uint32_t y) { return max(x, y); }), 63);
+        int parts = 0, parts_upto = 0;
+        const ta_deal d(a, (int)bs_read((uint32_t)upto, 63), __popcll(__ballot(stages > 0)), longest, [&](int per) {
+            parts = ta_parts(stages, per);
+            parts_upto = (int)bs_scan((uint32_t)parts, plus);
+            return (int)bs_read((uint32_t)parts_upto, 63);
+        });
+        if (w.g >= d.shares) return false;
+        per = d.per;
+        if (per) {
+            x = w.g;
+            mine = parts;
+            upto = parts_upto;
+        } else {
+            x = w.at = first = ta_begins(w.g, d.sum, d.shares);
+            w.end = ta_begins(w.g + 1, d.sum, d.shares);
+        }
     }
-    if (w.at >= w.end) return false;
-    w.b = __builtin_ctzll(__ballot(w.at >= upto - stages && w.at < upto));
-    w.before = (int)bs_read((uint32_t)(upto - stages), w.b);
+    if (per == 0 && w.at >= w.end) return false;
+    w.b = __builtin_ctzll(__ballot(x >= upto - mine && x < upto));
+    w.before = (int)bs_read((uint32_t)(upto - mine), w.b);
     w.rq = ta_uniform(r, w.b);
-    w.take(first);
+    if (per) w.take_part(per);
+    else w.take(first);
     return true;
 }
 // More: the workgroup looks for the first one together, and goes on from there.
 template <int WAVES>
 __device__ __forceinline__ bool ta_first_of_many(const ta_args &a, ta_work &w, int &first) {
-    __shared__ int sums[WAVES], found[2];
+    __shared__ int sums[3][WAVES], found[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), THREADS = WAVES * 64;
     auto plus = [](uint32_t x, uint32_t y) { return x + y; };
-    uint32_t all = 0;
-    for (int i = tid; i < a.B; i += THREADS) all += ta_request(a, i).stages();
-    all = bs_read(bs_scan(all, plus), 63);
-    if (lane == 0) sums[wave] = (int)all;
+    auto larger = [](uint32_t x, uint32_t y) { return max(x, y); };
+    const int stages0 = tid < a.B ? ta_request(a, tid).stages() : 0;
+    auto each = [&](auto f) {
+        f(stages0);
+        for (int i = tid + THREADS; i < a.B; i += THREADS) f(ta_request(a, i).stages());
+    };
+    uint32_t sum_of = 0, live_of = 0, longest_of = 0;
+    each([&](int n) {
+        sum_of += n;
+        live_of += n > 0;
+        longest_of = max(longest_of, (uint32_t)n);
+    });
+    sum_of = bs_read(bs_scan(sum_of, plus), 63);
+    live_of = bs_read(bs_scan(live_of, plus), 63);
+    longest_of = bs_read(bs_scan(longest_of, larger), 63);
+    if (lane == 0) {
+        sums[0][wave] = (int)sum_of;
+        sums[1][wave] = (int)live_of;
+        sums[2][wave] = (int)longest_of;
+    }
     __syncthreads();
-    int sum = 0;
+    int sum = 0, live = 0, longest = 0;
 #pragma unroll
-    for (int v = 0; v < WAVES; v++) sum += sums[v];
-    const int shares = ta_shares(a, sum);
-    if (blockIdx.x == 0 && tid == 0) a.before[a.B] = sum;
-    if (w.g >= shares) return false;
-    w.at = first = ta_begins(w.g, sum, shares);
-    w.end = ta_begins(w.g + 1, sum, shares);
-    if (w.at >= w.end) return false;
-    int before = 0;
-    for (int i0 = 0; i0 < a.B && before <= w.at; i0 += THREADS) {
-        const int i = i0 + tid, mine = i < a.B ? ta_request(a, i).stages() : 0, upto = (int)bs_scan((uint32_t)mine, plus);
+    for (int v = 0; v < WAVES; v++) {
+        sum += sums[0][v];
+        live += sums[1][v];
+        longest = max(longest, sums[2][v]);
+    }
+    const ta_deal d(a, sum, live, longest, [&](int per) {
+        uint32_t parts = 0;
+        each([&](int n) { parts += ta_parts(n, per); });
+        parts = bs_read(bs_scan(parts, plus), 63);
         __syncthreads();
-        if (lane == 63) sums[wave] = upto;
+        if (lane == 0) sums[0][wave] = (int)parts;
+        __syncthreads();
+        int n = 0;
+#pragma unroll
+        for (int v = 0; v < WAVES; v++) n += sums[0][v];
+        return n;
+    });
+    if (w.g >= d.shares) return false;
+    const int x = d.per ? w.g : ta_begins(w.g, sum, d.shares);
+    if (d.per == 0) {
+        w.at = first = x;
+        w.end = ta_begins(w.g + 1, sum, d.shares);
+        if (w.at >= w.end) return false;
+    }
+    int before = 0;
+    for (int i0 = 0; i0 < a.B && before <= x; i0 += THREADS) {
+        const int i = i0 + tid, stages = i0 == 0 ? stages0 : i < a.B ? ta_request(a, i).stages() : 0, mine = d.per ? ta_parts(stages, d.per) : stages, upto = (int)bs_scan((uint32_t)mine, plus);
+        __syncthreads();
+        if (lane == 63) sums[0][wave] = upto;
         __syncthreads();
         int from = before + upto - mine;
 #pragma unroll
         for (int v = 0; v < WAVES; v++) {
-            if (v < wave) from += sums[v];
-            before += sums[v];
+            if (v < wave) from += sums[0][v];
+            before += sums[0][v];
         }
-        if (w.at >= from && w.at < from + mine) {
+        if (x >= from && x < from + mine) {
             found[0] = i;
             found[1] = from;
         }
@@ -169,7 +259,8 @@ __device__ __forceinline__ bool ta_first_of_many(const ta_args &a, ta_work &w, i
     w.b = __builtin_amdgcn_readfirstlane(found[0]);
     w.before = __builtin_amdgcn_readfirstlane(found[1]);
     w.rq = ta_uniform(ta_request(a, w.b), 0);
-    w.take(first);
+    if (d.per) w.take_part(d.per);
+    else w.take(first);
     return true;
 }
 template <int WAVES>
@@ -943,7 +1034,7 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
 // The parts of a row of a head put together, in order: D / 4 threads each.
 template <int D>
 __global__ __launch_bounds__(256) void attention_tree_merge_kernel(const ta_args a) {
-    constexpr int PER = D / 4;
+    constexpr int PER = D / 4, BATCH = 8;        // parts that are requested at once
     const int64_t i = (int64_t)blockIdx.x * (256 / PER) + threadIdx.x / PER;
     const int dim = threadIdx.x % PER * 4, t = (int)(i / a.heads), head = (int)(i % a.heads);
     if (t >= a.T) return;
@@ -957,16 +1048,17 @@ __global__ __launch_bounds__(256) void attention_tree_merge_kernel(const ta_args
     const ta_request rq(a, lo);
     const int node = t - rq.start, stages = rq.stages();
     if (node < 0 || node >= rq.n) return;        // (zeros already)
-    const int sum = a.before[a.B], shares = ta_shares(a, sum), from = a.before[lo], g0 = ta_whose(from, sum, shares), g1 = ta_whose(from + stages - 1, sum, shares);
+    const int sum = a.before[a.B], shares = a.before[a.B + 1], per = a.before[a.B + 2], from = a.before[lo];
+    const int g0 = per ? from : ta_whose(from, sum, shares), g1 = per ? from + ta_parts(stages, per) - 1 : ta_whose(from + stages - 1, sum, shares);
     if (g0 == g1) return;                        // written by the first launch
-    const int slot0 = 2 * g0 + (from != ta_begins(g0, sum, shares));
+    const int slot0 = 2 * g0 + (per == 0 && from != ta_begins(g0, sum, shares));
     float mx = TA_LOW, den = 0.f;
     float4_t o = (float4_t)0.f;
-    for (int j0 = g0; j0 <= g1; j0 += 4) {
-        float m[4], l[4];
-        float4_t v[4];
+    for (int j0 = g0; j0 <= g1; j0 += BATCH) {
+        float m[BATCH], l[BATCH];
+        float4_t v[BATCH];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < BATCH; j++) {
             const int g = min(j0 + j, g1);
             const float *p = ta_part_row(a, g == g0 ? slot0 : 2 * g, node, head, D);
             m[j] = p[0];
@@ -974,7 +1066,7 @@ __global__ __launch_bounds__(256) void attention_tree_merge_kernel(const ta_args
             v[j] = *reinterpret_cast<const float4_t *>(p + 4 + dim);
         }
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < BATCH; j++) {
             if (l[j] == 0.f) continue;           // (nothing was seen, or no part)
             const float top = fmaxf(mx, m[j]), r0 = mx == top ? 1.f : __builtin_amdgcn_exp2f(mx - top), r = m[j] == top ? 1.f : __builtin_amdgcn_exp2f(m[j] - top);
             den = den * r0 + r * l[j];
@@ -994,18 +1086,17 @@ __global__ __launch_bounds__(256) void attention_tree_zero_kernel(half_t *__rest
 }
 
 struct ta_shape {
-    int rows, units, shares, least;              // rows of a workgroup
+    int rows, units, shares;                     // rows of a workgroup
 };
 ta_shape shape_of(int B, int nodes, int heads, int kv_heads, int64_t positions) {
     ta_shape p;
     const int64_t rows = (int64_t)(heads / kv_heads) * nodes;
     p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
     p.units = kv_heads * (int)bs_cdiv(rows, p.rows);
-    p.least = 8;
-    p.shares = positions <= 256 ? 0 : 512 / p.units > 1 ? 512 / p.units : 1;
+    p.shares = positions <= 512 ? 0 : 512 / p.units > 1 ? 512 / p.units : 1;
     return p;
 }
-int64_t before_bytes(int B) { return bs_cdiv(4ll * (B + 1), 16) * 16; }
+int64_t before_bytes(int B) { return bs_cdiv(4ll * (B + 3), 16) * 16; }
 
 // A cache that the last-level cache cannot hold is read past it, where a workgroup of the unit has all of its rows.
 constexpr int64_t TA_STREAM = 256ll << 20;
@@ -1041,7 +1132,7 @@ int bs_launch_attention_tree(const half_t *q, int ldq, const half_t *kpages, con
         return BS_OK;
     }
     const ta_shape p = shape_of(B, nodes, heads, kv_heads, (int64_t)max_pages << shift);
-    const ta_args a = {q, kpages, vpages, table, lengths, granted, starts, masks, out, (int32_t *)workspace, (float *)((char *)workspace + before_bytes(B)), 1.f / (float)(heads / kv_heads), ldq, B, T, nodes,
-                       heads, kv_heads, p.units / kv_heads, shift, max_pages, pool, p.shares, p.least};
+    const ta_args a = {q, kpages, vpages, table, lengths, granted, starts, masks, out, (int32_t *)workspace, (float *)((char *)workspace + before_bytes(B)), 1.f / (float)(heads / kv_heads), (float)p.units / (p.rows == 16 ? 32.f : 16.f), ldq, B, T, nodes,
+                       heads, kv_heads, p.units / kv_heads, shift, max_pages, pool, p.shares, p.rows <= 32 ? 16 : 32};
     return head_dim == 128 ? launch<128>(a, p, s) : launch<64>(a, p, s);
 }
