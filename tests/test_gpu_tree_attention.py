@@ -260,3 +260,12 @@ def test_no_rows():
     assert c.run().shape == (0, 256)
     c = Case(4, 2, 64, 16, [20], [0], nodes=4, pad=5)
     assert bool((c.run() == 0).all())
+
+
+@pytest.mark.parametrize("kv,counts", [(8, 4), (16, 8), (16, 16), (16, 32)])
+@pytest.mark.parametrize("held", [
+    [400] * 10, [100, 7000] + [3] * 30, [900 - 60 * i for i in range(14)], [300] * 31 + [301], [700 * (i % 3) for i in range(60)], [1100] + [0] * 63, [40] * 65, [25 * (i % 40) for i in range(90)],
+    [(37 * i) % 1500 for i in range(33)], [5] * 300 + [2500]])
+def test_how_requests_are_dealt(kv, counts, held):
+    """Few and many requests to a workgroup, alike and not: whole ones, own parts, equal shares."""
+    Case(2 * kv, kv, 64, 16, held, [1 + (counts + i) % counts if i % 7 else 0 for i in range(len(held))], nodes=2 * counts if counts < 32 else 64, kind="chain").check()
