@@ -1031,20 +1031,19 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
     if (unit == 0) ta_idle<THREADS>(a, work, a.shares ? a.shares : a.B, D);
 }
 
-// The parts of a row of a head put together, in order: D / 4 threads each.
+// The parts of a row of a head put together, in order: D / 4 threads each, a workgroup a token's row.  What it takes is a chain of latencies: the request, looked for by 64 lanes at once, its lengths, the parts.
 template <int D>
 __global__ __launch_bounds__(256) void attention_tree_merge_kernel(const ta_args a) {
-    constexpr int PER = D / 4, BATCH = 8;        // parts that are requested at once
-    const int64_t i = (int64_t)blockIdx.x * (256 / PER) + threadIdx.x / PER;
-    const int dim = threadIdx.x % PER * 4, t = (int)(i / a.heads), head = (int)(i % a.heads);
-    if (t >= a.T) return;
+    constexpr int PER = D / 4, HEADS = 256 / PER, BATCH = 8;             // parts that are requested at once
+    const int groups = (a.heads + HEADS - 1) / HEADS, t = blockIdx.x / groups, head = (blockIdx.x - t * groups) * HEADS + threadIdx.x / PER, dim = threadIdx.x % PER * 4, lane = threadIdx.x & 63;
     int lo = 0, hi = a.B;                        // the request: the first whose rows end behind t
     while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (a.starts[mid + 1] > t) hi = mid;
-        else lo = mid + 1;
+        const int step = (hi - lo + 63) / 64, at = min(lo + step * (lane + 1), hi) - 1;        // the last request of the lane's part
+        const int behind = __builtin_popcountll(__ballot(a.starts[at + 1] <= t)), first = min(lo + step * behind, hi);
+        if (first < hi) hi = min(first + step, hi) - 1;
+        lo = first;
     }
-    if (lo == a.B) return;
+    if (lo >= a.B || head >= a.heads) return;
     const ta_request rq(a, lo);
     const int node = t - rq.start, stages = rq.stages();
     if (node < 0 || node >= rq.n) return;        // (zeros already)
@@ -1111,7 +1110,7 @@ int launch(const ta_args &a, const ta_shape &p, hipStream_t s) {
     else attention_tree_kernel<D, 2, 4, true, false><<<grid, 256, 0, s>>>(a);
     BS_LAUNCH_CHECK();
     if (p.shares == 0) return BS_OK;
-    attention_tree_merge_kernel<D><<<(unsigned)bs_cdiv((int64_t)a.T * a.heads, 256 / (D / 4)), 256, 0, s>>>(a);
+    attention_tree_merge_kernel<D><<<(unsigned)((int64_t)a.T * bs_cdiv(a.heads, 256 / (D / 4))), 256, 0, s>>>(a);
     BS_LAUNCH_CHECK();
     return BS_OK;
 }
