@@ -21,10 +21,13 @@ struct adjust_args {
     int64_t mask_bytes;
 };
 
-// A workgroup counts the request's tokens of its span in LDS, and walks its logits once, which it requests before all else.  Tokens with a bias are a few of many: they are marked in a bit array, and a wave
-// that meets one looks it up in the request's list, 64 entries at a time.
-// What bounds it is the chain of a workgroup (row -> request -> text -> counts), hidden by the others of a CU, and the bytes: 384 rows of 128256 with texts of 3000, 197 MB and the texts from the L2,
-// 60 us (a copy of as much 40); one row 5.8 (a launch).  One eight per thread 76, four 65, 256 threads 69, 1024 77: more workgroups read the text more often, larger ones leave a CU fewer to hide it.
+// A workgroup counts the request's tokens of its span in LDS.  Its logits, which it requests before all else, go out as they came (bits, not values) but for those that are not allowed and those with a
+// count or a bias, which are a few of many: a lane takes one of its eight after the other.  Tokens with a bias are marked in a bit array, and the whole wave looks one up in the request's list, 64
+// entries at a time.
+// What bounds it is the chain of a workgroup (row -> request -> text -> counts -> out), which the others of a CU hide in part: 384 rows of 128256 with texts of 3000, 197 MB of logits and the texts from the
+// L2, 61 us (with texts of 500 49; a copy of as much 40), 200 rows of 50000 17, one row 5.9 (a launch).  Every logit computed, as if it had a count, takes 90 % of the vector units: 54 and 19 where this takes
+// 49 and 17, but 10 instead of 13 for 32 rows of 32000 with texts of 20000.  In spans of half as many logits 80, of twice as many 67; 256 threads 71, 1024 58, but 200 rows then 20 (fewer at once).
+// Rows one after another in a workgroup, the next one's logits requested ahead and a request's counts kept: 91, on registers for half as many workgroups.
 template <bool PENALTIES, bool BIAS>
 __global__ __launch_bounds__(THREADS) void logits_adjust_kernel(const adjust_args a) {
     __shared__ __attribute__((aligned(16))) uint32_t counts[PENALTIES ? SPAN : 4];
@@ -33,15 +36,17 @@ __global__ __launch_bounds__(THREADS) void logits_adjust_kernel(const adjust_arg
     const half_t *x = a.logits + row * a.ld;
     half_t *y = a.out + row * a.ld_out;
     const bool whole = ((uintptr_t)x | (uintptr_t)y) % 16 == 0;
-    half8_t in[RUNS];
+    uint4_t in[RUNS];                            // eight halves
 #pragma unroll
     for (int n = 0; n < RUNS; n++) {
         const int i = from + n * RUN + 8 * tid;
-        in[n] = (half8_t)(half_t)0;
-        if (whole && i + 8 <= a.V) in[n] = *reinterpret_cast<const half8_t *>(x + i);
-        else
+        if (whole && i + 8 <= a.V) in[n] = *reinterpret_cast<const uint4_t *>(x + i);
+        else {
+            half8_t v = (half8_t)(half_t)0;
             for (int e = 0; e < 8; e++)
-                if (i + e < a.V) in[n][e] = x[i + e];
+                if (i + e < a.V) v[e] = x[i + e];
+            in[n] = __builtin_bit_cast(uint4_t, v);
+        }
     }
     const int state = a.allowed ? (a.allowed_rows ? a.allowed_rows[row] : row) : -1;
     const uint8_t *allowed = state >= 0 && state < a.masks ? a.allowed + (int64_t)state * a.mask_bytes : nullptr;
@@ -56,6 +61,7 @@ __global__ __launch_bounds__(THREADS) void logits_adjust_kernel(const adjust_arg
     b = known ? b : 0;
     float repetition = 1.f, frequency = 0.f, presence = 0.f;
     bool counted = false;
+    const bool biased = BIAS && known;
     if (PENALTIES && known) {
         const int length = a.history_lengths ? a.history_lengths[b] : a.most, prompt = a.prompt_lengths ? a.prompt_lengths[b] : 0;
         if (a.repetition) repetition = a.repetition[b];
@@ -64,9 +70,9 @@ __global__ __launch_bounds__(THREADS) void logits_adjust_kernel(const adjust_arg
         if (!(repetition > 0.f)) repetition = 1.f;
         counted = repetition != 1.f || frequency != 0.f || presence != 0.f;
         if (counted) {
+            if (BIAS && tid < SPAN / 32) marked[tid] = 0;
 #pragma unroll
             for (int i = 0; i < SPAN / 4 / THREADS; i++) *reinterpret_cast<uint4_t *>(&counts[4 * (tid + i * THREADS)]) = (uint4_t)0u;
-            if (BIAS && tid < SPAN / 32) marked[tid] = 0;
             __syncthreads();
             const int n = min(max(length, 0), a.most);
             const int32_t *text = a.history + (int64_t)b * a.most;
@@ -93,7 +99,6 @@ __global__ __launch_bounds__(THREADS) void logits_adjust_kernel(const adjust_arg
             }
         }
     }
-    const bool biased = BIAS && known;
     const int32_t *tokens = a.bias_tokens + (int64_t)b * a.biases;
     if (biased) {
         if (!counted) {
@@ -109,55 +114,67 @@ __global__ __launch_bounds__(THREADS) void logits_adjust_kernel(const adjust_arg
 #pragma unroll
     for (int n = 0; n < RUNS; n++) {
         const int t0 = n * RUN + 8 * tid, i0 = from + t0;
-        float v[8];
-        uint32_t finite = 0;
+        uint4_t o = in[n];
+        if (counted || biased) {
+            const uint32_t with_bias = biased ? marked[t0 >> 5] >> (t0 & 31) & 0xff : 0;
+            uint32_t todo = with_bias;
+            if (counted) {
+                const uint4_t lo = *reinterpret_cast<const uint4_t *>(&counts[t0]), hi = *reinterpret_cast<const uint4_t *>(&counts[t0 + 4]);
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            v[e] = (float)in[n][e];
-            finite |= (uint32_t)__builtin_isfinite(v[e]) << e;
-        }
-        if (counted) {
-            uint32_t c[8];
-            *reinterpret_cast<uint4_t *>(c) = *reinterpret_cast<const uint4_t *>(&counts[t0]);
-            *reinterpret_cast<uint4_t *>(c + 4) = *reinterpret_cast<const uint4_t *>(&counts[t0 + 4]);
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const uint32_t said = c[e] & ~PROMPT;
-                if (c[e] != 0) v[e] = v[e] > 0.f ? v[e] / repetition : v[e] * repetition;
-                if (said != 0) v[e] = v[e] - frequency * (float)said - presence;
+                for (int e = 0; e < 4; e++) todo |= (lo[e] != 0 ? 1u << e : 0) | (hi[e] != 0 ? 16u << e : 0);
             }
-        }
-        if (biased) {
-            uint32_t mine = marked[t0 >> 5] >> (t0 & 31) & 0xff;
-            for (uint64_t who = __ballot(mine != 0); who != 0; who = __ballot(mine != 0)) {
-                const int leader = __builtin_ctzll(who), e_of = __builtin_ctz((uint32_t)__builtin_amdgcn_readlane((int)mine, leader));
-                const int32_t token = __builtin_amdgcn_readlane(i0, leader) + e_of;
-                int last = -1;                   // (of several entries for a token the last counts)
-                for (int j0 = 0; j0 < a.biases; j0 += 64) {
-                    const uint64_t here = __ballot(j0 + lane < a.biases && tokens[j0 + lane] == token);
-                    if (here != 0) last = j0 + 63 - __builtin_clzll(here);
+            while (__any(todo != 0)) {           // (all lanes: some may have none left)
+                const int e = todo != 0 ? __builtin_ctz(todo) : 0;
+                const uint32_t pair = e < 4 ? (e < 2 ? o[0] : o[1]) : (e < 6 ? o[2] : o[3]);
+                float v = (float)__builtin_bit_cast(half_t, (uint16_t)(pair >> 16 * (e & 1)));
+                bool finite = __builtin_isfinite(v);
+                if (counted) {
+                    const uint32_t c = counts[t0 + e], said = c & ~PROMPT;
+                    if (c != 0) v = v > 0.f ? v / repetition : v * repetition;
+                    if (said != 0) v = v - frequency * (float)said - presence;
                 }
-                const float w = a.bias[(int64_t)b * a.biases + last];
-                const bool fine = __builtin_isfinite(w);
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (lane == leader && e == e_of) {
-                        v[e] += w;
-                        finite &= fine ? 0xffu : ~(1u << e);
+                if (biased) {
+                    const bool mine = todo != 0 && (with_bias >> e & 1);
+                    for (uint64_t who = __ballot(mine); who != 0; who &= who - 1) {
+                        const int leader = __builtin_ctzll(who);
+                        const int32_t token = __builtin_amdgcn_readlane(i0 + e, leader);
+                        int last = -1;           // (of several entries for a token the last counts)
+                        for (int j0 = 0; j0 < a.biases; j0 += 64) {
+                            const uint64_t here = __ballot(j0 + lane < a.biases && tokens[j0 + lane] == token);
+                            if (here != 0) last = j0 + 63 - __builtin_clzll(here);
+                        }
+                        const float w = a.bias[(int64_t)b * a.biases + last];
+                        if (lane == leader) {
+                            v += w;
+                            finite = finite && __builtin_isfinite(w);
+                        }
                     }
-                if (lane == leader) mine &= mine - 1;
+                }
+                if (finite) v = fminf(fmaxf(v, -65504.f), 65504.f);
+                const uint32_t half = __builtin_bit_cast(uint16_t, (half_t)v), keep = e & 1 ? 0xffffu : 0xffff0000u, put = half << 16 * (e & 1);
+                if (todo != 0) {
+                    o[0] = e >> 1 == 0 ? (o[0] & keep) | put : o[0];
+                    o[1] = e >> 1 == 1 ? (o[1] & keep) | put : o[1];
+                    o[2] = e >> 1 == 2 ? (o[2] & keep) | put : o[2];
+                    o[3] = e >> 1 == 3 ? (o[3] & keep) | put : o[3];
+                }
+                todo &= todo - 1;
             }
         }
-        half8_t o;
+        if (allowed) {
+            constexpr uint32_t LOW = 0xfc00u;    // -inf
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            if (finite >> e & 1) v[e] = fminf(fmaxf(v[e], -65504.f), 65504.f);
-            o[e] = bits[n] >> e & 1 ? (half_t)v[e] : (half_t)-INFINITY;
+            for (int d = 0; d < 4; d++) {
+                const uint32_t lo = bits[n] >> 2 * d & 1 ? o[d] : LOW, hi = bits[n] >> (2 * d + 1) & 1 ? o[d] : LOW << 16;
+                o[d] = (lo & 0xffffu) | (hi & 0xffff0000u);
+            }
         }
-        if (whole && i0 + 8 <= a.V) *reinterpret_cast<half8_t *>(y + i0) = o;
-        else
+        if (whole && i0 + 8 <= a.V) *reinterpret_cast<uint4_t *>(y + i0) = o;
+        else {
+            const half8_t h = __builtin_bit_cast(half8_t, o);
             for (int e = 0; e < 8; e++)
-                if (i0 + e < a.V) y[i0 + e] = o[e];
+                if (i0 + e < a.V) y[i0 + e] = h[e];
+        }
     }
 }
 
