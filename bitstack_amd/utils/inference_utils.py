@@ -553,7 +553,7 @@ def tree_plan_hip(parents, lengths, granted, starts):
 def attention_tree_hip(q, kpages, vpages, block_table, lengths, granted, starts, masks, nodes=64, out=None):
     """Attention of drafted tokens: q [T, heads * d] rotated (rows may be strided), their keys and values stored (rope_store_paged_hip with tree_plan_hip's positions does both),
     over the positions that each request held in the pages [pool, kv, page_size, d] and the nodes that masks [T] names.  lengths, granted, starts as in tree_plan_hip;
-    `nodes` is the largest number of them that a request has (up to 64; one with more is left out).  Returns [T, heads * d], zeros in rows that are no node."""
+    `nodes` is the largest number of them that a request has (up to 64; one with more is left out).  Returns [T, heads * d], zeros in rows that are no node; out must not be q's memory."""
     y = _lib.host().attention_tree(q, kpages, vpages, block_table, lengths, granted, starts, masks, nodes, out)
     if y is not None:
         return y if out is None else out

@@ -94,7 +94,7 @@ def test_adjust(L):
     for name in ("logits", "out", "requests", "history", "history_lengths", "prompt_lengths", "repetition", "frequency", "presence", "drafted", "bias_tokens", "bias", "allowed", "allowed_rows"):
         assert refused(**{name: ODD}) == ALIGN, name
     assert refused(history=TWO) == refused(bias=TWO) == ALIGN
-    for change in ({"R": -1}, {"R": (1 << 20) + 1}, {"V": 0}, {"V": (1 << 18) + 1}, {"ld": 999}, {"ld_out": 999}, {"B": -1}, {"width": -1}, {"drafted_width": -1}, {"biases": -1}, {"masks": -1},
+    for change in ({"R": -1}, {"R": (1 << 20) + 1}, {"V": 0}, {"V": (1 << 18) + 1}, {"ld": 999}, {"ld_out": 999}, {"B": -1}, {"width": -1}, {"drafted_width": -1}, {"biases": -1}, {"masks": -1}, {"width": (1 << 30) + 1}, {"drafted_width": (1 << 31) - 1}, {"biases": (1 << 31) - 1},
                    {"history": NUL}, {"bias": NUL}, {"bias_tokens": NUL}, {"allowed": NUL}, {"allowed_rows": NUL}, {"requests": NUL}, {"ld_out": 1001}, {"R": 1 << 20, "V": 9000, "ld": 9000, "ld_out": 9000}):
         assert refused(**change) == SHAPE, change
     assert refused(R=0) == 0
