@@ -1,21 +1,23 @@
 // Attention of drafted tokens over the paged cache: out[t] = softmax(q[t] k^T / sqrt(D)) v over the positions that the request held and those nodes of its tree, stored
 // behind them, that masks[t] names.
 //
-// The rows of a KV head of a request are its nodes' queries of that head's group, the head fastest: nodes * group of them, which all read the same K and V.  A workgroup takes up to 16 QT WR of
-// them, the columns of both products, 16 QT to a wave, and walks the positions in stages of 32, which come to LDS straight from the pages (no registers), up to three stages ahead, one barrier per stage.
-//   scores  S[position, row] = K q      16x16x32; the 16-byte pieces of K's rows are XOR-ed with the row's number, so that 16 rows of one piece lie in different banks
-//   output  O[dim, row] += V^T P        16x16x32; a lane of the scores holds four positions of a row in each of two tiles of 16, which are the eight k slots of this product.  From LDS V comes
-//                                       turned, a lane a dimension; from memory it is used as it lies: product j takes element j of the W = D / 16 dimensions that a lane reads
-// The scores of a stage are computed one stage ahead, beside the softmax of the one before it: the matrix unit runs while the vector unit issues.
+// The rows of a KV head of a request are its nodes' queries of that head's group, the head fastest: nodes * group of them, which all read the same K and V.  A workgroup takes 16, 32, 64 or 128 of them, the
+// columns of both products, and walks the positions in stages of 32.
+//   scores  S[position, row] = K q      16x16x32
+//   output  O[dim, row] += V^T P        16x16x32; a lane of the scores holds four positions of a row in each of two tiles of 16, which are the eight k slots of this product
+// Up to 32 rows a wave takes every fourth stage with K and V in registers; beyond, every wave has 16 or 32 rows, and the stages come to LDS straight from the pages (no registers).
 // Maximum, sum and output are fp32, in base 2.  The weights are rounded to fp16 for the second product (the queries are given in fp16), the largest as 2^15, so that one of
 // 2^-40 of the largest is still held; their sum is that of the fp32 weights.
 //
 // What a row does not see has a weight of zero, but zero times an infinity is NaN: in the stages with nodes V is looked through, and infinities and NaN, if any, are taken out of the
 // product.  Rows that see them, or whose result is not finite for another reason, are computed again, each by a wave, in fp32.
 //
-// The split: as the lengths are known on the device alone, every workgroup works out from them what it is to do.  The stages of all requests, one after another, are dealt to G workgroups of a unit
-// (KV head, or row tile of one) in equal shares; a share may end in the middle of a request, and hold several.  What is not a whole request's leaves (max, sum, weighted v) in
+// The split: as the lengths are known on the device alone, every workgroup works out from them what it is to do (ta_deal).  What is not a whole request's leaves (max, sum, weighted v) in
 // the workspace, and a second launch puts the parts together, in order: the result does not depend on which came first.
+//
+// What bounds it: up to 64 rows the cache's bytes (64 requests of 4096, 32 heads on 8: 4 nodes 176 us, 8 nodes 183, 16 nodes 209, 6.1 to 5.1 TB/s; 200 of 100 to 1500, 16 on 16 of 64, 123 us, 5.3 TB/s; 48 of
+// up to 4096 with 1 to 16 nodes 89, 4.5 TB/s and the second launch's 7); with 128 what is issued (2 documents of 80000 with trees of 64, 64 heads on 8: 0.336 TFLOP in 445 us, 0.75 PFLOP/s where a large matrix
+// product reaches 1.2; the matrix unit is busy a third of the time, the vector unit half: two exponentials, maxima and roundings per 512 flops); one short request is the chain of latencies (12 us).
 #include "lanes.h"
 
 #include <type_traits>
@@ -380,7 +382,7 @@ __device__ __forceinline__ uint32_t ta_seen(uint64_t mask, int node) {
     return node >= 64 ? 0 : node >= 0 ? (uint32_t)(mask >> node) : node <= -4 ? 15 : (uint32_t)mask << -node | ((1u << -node) - 1);
 }
 
-// ---- few rows: what counts is the cache's bytes.  A wave has all 16 QT rows and every fourth stage, K and V in registers: K of its next stage is requested behind the
+// ---- few rows: what counts is the cache's bytes on their way.  A wave has all 16 QT rows and every fourth stage, K and V in registers: K of its next stage is requested behind the
 // scores, V behind the output product, so that eight waves of a CU have 128 KB on their way.  What the waves have is put together in LDS.
 template <int D, int QT, bool STREAM>
 __global__ __launch_bounds__(256, 2) void attention_tree_few_kernel(const ta_args a) {
@@ -1090,14 +1092,19 @@ struct ta_shape {
 ta_shape shape_of(int B, int nodes, int heads, int kv_heads, int64_t positions) {
     ta_shape p;
     const int64_t rows = (int64_t)(heads / kv_heads) * nodes;
+    // As many rows as there are, up to 128: K and V are read once for each tile of them.  (33 to 64 rows with K and V in registers, four tiles of columns to a wave: 118 us instead of 93 for 48 requests of up to
+    // 4096 with 16 nodes; 64 rows to a wave, 256 to a workgroup: 796 instead of 524 for 2 of 80000 with trees of 64, the sums no longer fit the registers.)
     p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
     p.units = kv_heads * (int)bs_cdiv(rows, p.rows);
+    // Two workgroups to a CU (768 of them in all: 243 us, 1024 219, 512 201 for 64 requests of 4096).  Tables of up to 512 positions, 16 stages, are not cut: the second launch costs 2.5 us and parts their
+    // traffic (us, uncut / cut: one of 390 with 8 nodes 11.9 / 12.1, 16 of 390 12.4 / 16.8, 64 of 390 26 / 30; with 32 nodes 21 / 16, 22 / 28, 35 / 45).
     p.shares = positions <= 512 ? 0 : 512 / p.units > 1 ? 512 / p.units : 1;
     return p;
 }
 int64_t before_bytes(int B) { return bs_cdiv(4ll * (B + 3), 16) * 16; }
 
-// A cache that the last-level cache cannot hold is read past it, where a workgroup of the unit has all of its rows.
+// A cache that the last-level cache cannot hold is read past it, where a workgroup of the unit has all of its rows (64 requests of 4096, 4 nodes 203 -> 188 us, 8 nodes 214 -> 205).  Where several read the
+// same positions the second one finds them there (32 nodes: 252, past it 323).
 constexpr int64_t TA_STREAM = 256ll << 20;
 
 template <int D>

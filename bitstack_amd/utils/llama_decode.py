@@ -159,7 +159,6 @@ class PagedCache:
             released = None
         return page_plan_hip(self.lengths, new_tokens, self.block_table, self.free_pages, self.free_state, self.page_size, tokens, released=released, inplace=True)
 
-
     def _fork(self, source):
         return page_fork_hip(source, self.lengths, self.block_table, self.free_pages, self.free_state, self.shares, self.kpages, self.vpages, inplace=True)
 
@@ -686,7 +685,7 @@ class SyntheticLlamaDecoder:
     def step_tree(self, cache: PagedCache, tokens, parents, new_tokens, nodes=64, released=None, uniform=None, adjust=None, **sampling):
         """Several drafted tokens per request in one step, of which as many are kept as the model would have given one by one.  Request b's new_tokens[b] (int32 [rows], up to
         `nodes`; 0: idle) tokens are the next rows of tokens [T] (int64) and parents [T] (int32: a number among the request's own, smaller than the token's; -1 for the first): its first
-        one is its cache.token, whatever `tokens` says, the others are drafts, each behind its parent.  The model's token behind each is greedy, or drawn with uniform [T] and the
+        one is its cache.token, whatever `tokens` says, the others are drafts, each behind its parent (numbers outside the vocabulary, also in rows of no request, are none).  The model's token behind each is greedy, or drawn with uniform [T] and the
         requests' temperature, top_k, top_p, min_p [rows]; `adjust`: logits_adjust_hip's settings per request and allowed_rows per token (history with cache.token in it, the drafts are added).
         Keys and values of what is accepted stay in the cache, and cache.token is the model's token behind it.  Returns (plan, tree_accept_hip's answer, the tokens): request b's new
         tokens are tokens[plan.starts[b] + path[b, 1:accepted[b]]] and its cache.token."""
@@ -702,7 +701,7 @@ class SyntheticLlamaDecoder:
         ids.scatter_(0, torch.where((new_tokens > 0) & (plan.starts[:-1] < T), plan.starts[:-1], T).long(), cache.token)
         ids = ids[:T]
         request = torch.searchsorted(plan.starts[1:].contiguous(), torch.arange(T, dtype=torch.int32, device=self.dev), right=True).clamp(max=cache.rows - 1)
-        x = self.embed.index_select(0, ids)
+        x = self.embed.index_select(0, ids.clamp(0, s.vocab - 1))         # (drafts that are no tokens are embedded as some, and never accepted)
         wide = s.heads * d, s.kv_heads * d, s.kv_heads * d
         few = T <= 48                                                     # (what the grouped launches take)
         if few and self._groups is None:

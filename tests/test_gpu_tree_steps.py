@@ -254,3 +254,28 @@ def test_a_request_ends_at_the_last_position():
     t, p, way = drafts(one, int(cache.token[0]), random.Random(1), 3, 0)
     plan, done, _ = dec.step_tree(cache, i64(t), i32(p), i32([4]))
     assert plan.granted.tolist() == [4] and int(cache.lengths[0]) == 60 + int(done.accepted[0]) <= 64
+
+
+@pytest.mark.parametrize("nodes", [4, 30])
+def test_drafts_and_padding_that_are_no_tokens(nodes):
+    """Rows of no request, and drafts, whose numbers are outside the vocabulary: the others' results are those with any token there, and such drafts are not accepted."""
+    results = []
+    for filler in (0, -1, 1 << 40):
+        dec = decoder()
+        cache = PagedCache(dec, 3, 60)
+        for row in (0, 2):
+            dec.prefill_paged(cache, row, prompt(20 + row, row))
+        cache.token.copy_(i64([7, 8, 9]))
+        T = 2 * nodes + 5
+        tokens = torch.full((T,), filler, device="cuda")
+        tokens[:2] = i64([7, 11])
+        tokens[nodes] = 9
+        parents = torch.arange(T, dtype=torch.int32, device="cuda") - 1
+        parents[nodes:] -= nodes
+        plan, done, ids = dec.step_tree(cache, tokens, parents, i32([nodes, 0, nodes]), nodes=nodes)
+        assert plan.granted.tolist() == [nodes, 0, nodes]
+        if filler:
+            assert int(done.accepted[0]) <= 2 and int(done.accepted[2]) == 1
+        results.append((dec.logits[:2].clone(), dec.logits[nodes].clone()))
+    for got in results[1:]:
+        assert torch.equal(got[0], results[0][0]) and torch.equal(got[1], results[0][1])
