@@ -296,11 +296,11 @@ __device__ __forceinline__ void ta_idle(const ta_args &a, int g, int of, int D) 
     auto idle = [&](int t) {
         for (int64_t i = threadIdx.x; i < orow; i += THREADS) a.out[t * orow + i] = (half_t)0;
     };
+    const int last = min(max(a.starts[a.B], 0), a.T), first = min(max(a.starts[0], 0), a.T);
     for (int b = g; b < a.B; b += of) {
         const ta_request r(a, b);
         for (int t = r.start + r.n; t < r.end; t++) idle(t);
     }
-    const int last = min(max(a.starts[a.B], 0), a.T), first = min(max(a.starts[0], 0), a.T);
     for (int t = last + g; t < a.T; t += of) idle(t);
     for (int t = g; t < first; t += of) idle(t);
 }
@@ -621,14 +621,33 @@ __global__ __launch_bounds__(256, 2) void attention_tree_few_kernel(const ta_arg
         constexpr int SHARE = THREADS / ROWS, PER = D / SHARE / 4;       // ... and four dimensions, PER times
         const int row = tid / SHARE, node = ta_node(row, rep, a.per_rep), head = hk * rep + row - node * rep;
         if (row < rows) {
-            float mx = wm[0][row], den = 0.f, r[WAVES];
-#pragma unroll
-            for (int v = 1; v < WAVES; v++) mx = fmaxf(mx, wm[v][row]);
+            // (all of it is read at once, and nothing behind a branch: a wait for each took 1.5 us)
+            float4_t x[PER][WAVES];
+            float tops[WAVES], sums[WAVES], r[WAVES], den = 0.f;
 #pragma unroll
             for (int v = 0; v < WAVES; v++) {
-                const float sum = wl[v][row];
-                r[v] = sum == 0.f ? 0.f : wm[v][row] == mx ? 1.f : __builtin_amdgcn_exp2f(wm[v][row] - mx);        // (0: nothing was seen)
-                den += sum == 0.f ? 0.f : r[v] * sum;
+                tops[v] = wm[v][row];
+                sums[v] = wl[v][row];
+            }
+#pragma unroll
+            for (int i = 0; i < PER; i++)
+#pragma unroll
+                for (int v = 0; v < WAVES; v++) x[i][v] = *reinterpret_cast<const float4_t *>(&wo[v][row][4 * (tid % SHARE) + 4 * SHARE * i]);
+#pragma unroll
+            for (int v = 0; v < WAVES; v++) asm volatile("" : "+v"(tops[v]), "+v"(sums[v]));
+#pragma unroll
+            for (int i = 0; i < PER; i++)
+#pragma unroll
+                for (int v = 0; v < WAVES; v++) asm volatile("" : "+v"(x[i][v]));
+            float mx = tops[0];
+#pragma unroll
+            for (int v = 1; v < WAVES; v++) mx = fmaxf(mx, tops[v]);
+#pragma unroll
+            for (int v = 0; v < WAVES; v++) {
+                float less = __builtin_amdgcn_exp2f(tops[v] - mx);
+                asm volatile("" : "+v"(less));
+                r[v] = sums[v] == 0.f ? 0.f : tops[v] == mx ? 1.f : less;           // (0: nothing was seen)
+                den += sums[v] == 0.f ? 0.f : r[v] * sums[v];
             }
             const float inv = den != 0.f ? 1.f / den : 0.f;
             float *const part_row = ta_part_row(a, max(w.slot, 0), node, head, D);
@@ -642,7 +661,8 @@ __global__ __launch_bounds__(256, 2) void attention_tree_few_kernel(const ta_arg
                 float4_t o = (float4_t)0.f;
 #pragma unroll
                 for (int v = 0; v < WAVES; v++)
-                    if (r[v] != 0.f) o += r[v] * *reinterpret_cast<const float4_t *>(&wo[v][row][dim]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[e] += r[v] != 0.f ? r[v] * x[i][v][e] : 0.f;
                 if (w.slot >= 0) *reinterpret_cast<float4_t *>(part_row + 4 + dim) = o;
                 else {
                     half4_t h;
