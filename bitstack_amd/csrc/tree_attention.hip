@@ -15,9 +15,9 @@
 // The split: as the lengths are known on the device alone, every workgroup works out from them what it is to do (ta_deal).  What is not a whole request's leaves (max, sum, weighted v) in
 // the workspace, and a second launch puts the parts together, in order: the result does not depend on which came first.
 //
-// What bounds it: up to 64 rows the cache's bytes (64 requests of 4096, 32 heads on 8: 4 nodes 176 us, 8 nodes 183, 16 nodes 209, 6.1 to 5.1 TB/s; 200 of 100 to 1500, 16 on 16 of 64, 123 us, 5.3 TB/s; 48 of
-// up to 4096 with 1 to 16 nodes 89, 4.5 TB/s and the second launch's 7); with 128 what is issued (2 documents of 80000 with trees of 64, 64 heads on 8: 0.336 TFLOP in 445 us, 0.75 PFLOP/s where a large matrix
-// product reaches 1.2; the matrix unit is busy a third of the time, the vector unit half: two exponentials, maxima and roundings per 512 flops); one short request is the chain of latencies (12 us).
+// What bounds it: up to 64 rows the cache's bytes (64 requests of 4096, 32 heads on 8: 4 nodes 176 us, 8 nodes 183, 16 nodes 209, 6.1 to 5.1 TB/s; 200 of 100 to 1500, 16 on 16 of 64, 123 us, 5.4 TB/s; 48 of
+// up to 4096 with 1 to 16 nodes 90, 4.5 TB/s and the second launch's 7); with 128 what is issued (2 documents of 80000 with trees of 64, 64 heads on 8: 0.336 TFLOP in 440 us, 0.76 PFLOP/s where a large matrix
+// product reaches 1.2; the matrix unit is busy a third of the time, the vector unit half: two exponentials, maxima and roundings per 512 flops); one short request is the chain of latencies (11.5 us).
 #include "lanes.h"
 
 #include <type_traits>
