@@ -647,7 +647,7 @@ extern "C" int bs_logits_adjust_f16(const void *logits, int64_t ld, void *out, i
                                     const int32_t *allowed_rows, int R, int V, int B, void *stream) {
     if (sample_shape(R, V) != BS_OK || B < 0 || (R > 1 && (ld < V || ld_out < V)) || history_width < 0 || drafted_width < 0 || biases < 0 || masks < 0 ||
         history_width > 1 << 30 || drafted_width > 1 << 30 || biases > 1 << 30 ||
-        (history_lengths && !history) || (prompt_lengths && !history) || (bias_tokens != nullptr) != (bias != nullptr) || (allowed_rows && !allowed) ||
+        ((history_lengths || prompt_lengths) && !history && history_width > 0) || (bias_tokens != nullptr) != (bias != nullptr) || (allowed_rows && !allowed && masks > 0) ||
         (allowed && !allowed_rows && masks < R) || (logits == out && ld != ld_out && R > 1) ||
         (!requests && B < R && (history || drafted || bias || repetition || frequency || presence)))
         return BS_ERR_SHAPE;

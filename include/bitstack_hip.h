@@ -613,7 +613,7 @@ int bs_page_fork_f16(const int32_t *source, const int32_t *lengths, int32_t *blo
  *   bias        x + bias[b, i] for the tokens bias_tokens[b, i]; of several entries for a token the last
  *   allowed     [masks, ceil(V / 32)] words of 32 tokens, the lowest bit first; row r uses mask
  *               allowed_rows[r] (NULL: mask r; a number that no mask has: none); -inf where the bit is 0
- * Any of them may be NULL: history_lengths the whole width, prompt_lengths 0, repetition 1 (also where it is not above 0),
+ * Any of them may be NULL, or have no width: history_lengths the whole width, prompt_lengths 0, repetition 1 (also where it is not above 0),
  * frequency and presence 0.  Tokens outside 0 .. V - 1 are none.  Finite logits stay finite up to here, at most 65504, unless a bias is infinite; settings other
  * than biases must be finite.  R <= 2^20, V <= 2^18, R * V <= 2^33, widths and biases <= 2^30.  No counterpart in the reference.
  */

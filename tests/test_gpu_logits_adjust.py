@@ -186,3 +186,21 @@ def test_untouched_logits_keep_their_bits():
 
 def test_no_rows():
     assert IU.logits_adjust_hip(torch.zeros(0, 50, dtype=torch.float16, device="cuda")).shape == (0, 50)
+
+
+def test_settings_of_no_width():
+    """A text of no tokens, no drafted ones, no biases and no masks change nothing, beside others that do."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(3, 5000, dtype=torch.float16, device="cuda", generator=g)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    nothing = dict(history=torch.zeros(3, 0, **i32), history_lengths=torch.zeros(3, **i32), prompt_lengths=torch.zeros(3, **i32), repetition=torch.full((3,), 2.0, device="cuda"),
+                   drafted=torch.zeros(3, 0, **i32), bias_tokens=torch.zeros(3, 0, **i32), bias=torch.zeros(3, 0, device="cuda"), allowed=torch.zeros(0, 157, **i32), allowed_rows=torch.full((3,), -1, **i32))
+    for requests in (None, torch.tensor([2, 0, -1], **i32)):
+        assert torch.equal(IU.logits_adjust_hip(x, out=torch.empty_like(x), requests=requests, **nothing), x)
+    drafted = torch.tensor([[4], [-1], [4999]], **i32)
+    y = IU.logits_adjust_hip(x, out=torch.empty_like(x), **{**nothing, "drafted": drafted})
+    want = x.clone()
+    for row, token in ((0, 4), (2, 4999)):
+        v = x[row, token].double()
+        want[row, token] = v / 2 if v > 0 else v * 2
+    assert torch.equal(y, want)
