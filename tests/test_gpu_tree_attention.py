@@ -246,6 +246,8 @@ def test_pages_beyond_32_bits():
             c.rows[0][i] = to
     c.table = [c.rows[0]]
     c.check()
+    del c, t
+    torch.cuda.empty_cache()
 
 
 def test_the_same_bits_again():

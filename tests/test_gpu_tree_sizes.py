@@ -17,13 +17,18 @@ def i64(v):
     return torch.tensor(v, dtype=torch.int64, device="cuda")
 
 
+@pytest.fixture(scope="module", autouse=True)
+def memory_goes_back():
+    """(What later tests keep would else be cut from these tensors' memory, which then stays.)"""
+    yield
+    torch.cuda.empty_cache()
+
+
 @pytest.fixture(scope="module")
 def caches():
     pages = torch.zeros(2, LAYERS, POOL, KV, PAGE, D, dtype=torch.float16, device="cuda")
     assert pages[0, 0].numel() > 2 ** 31
     yield pages
-    del pages
-    torch.cuda.empty_cache()
 
 
 def fill(caches, used):
