@@ -761,6 +761,7 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
         __syncthreads();                             // (nobody is at the request before this one any more)
         if (tid < 2) odd_nodes[tid] = 0;             // (behind a barrier of the first stage when it is next written)
         if (tid == 2) odd_held = 0;
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");    // (the loop's barriers alone wait for no LDS write)
         pg.load(st_first);
         pg.take();
         pg.load(st_first + 32);
