@@ -6,8 +6,9 @@
 //   scores  S[position, row] = K q      16x16x32
 //   output  O[dim, row] += V^T P        16x16x32; a lane of the scores holds four positions of a row in each of two tiles of 16, which are the eight k slots of this product
 // Up to 32 rows a wave takes every fourth stage with K and V in registers; beyond, every wave has 16 or 32 rows, and the stages come to LDS straight from the pages (no registers).
-// Maximum, sum and output are fp32, in base 2.  The weights are rounded to fp16 for the second product (the queries are given in fp16), the largest as 2^15, so that one of
-// 2^-40 of the largest is still held; their sum is that of the fp32 weights.
+// Maximum, sum and output are fp32, in base 2.  The weights enter the second product as two fp16 terms, p = hi + lo, the largest as 2^15: held to 2^-22 of themselves down to 2^-18 of the
+// largest, below that to 2^-40 of the largest.  (hi alone: an error against 64 bits of 2.2 to 2.7e-4 where the result's rounding is 2.1e-4, and where many weights are rounded up values of 65504
+// everywhere became infinities, as the sum below the line is that of the fp32 weights.  Up to 64 rows the second term's products cost nothing that shows, 128 rows 545 us instead of 441 for 2 documents of 80000.)
 //
 // What a row does not see has a weight of zero, but zero times an infinity is NaN: in the stages with nodes V is looked through, and infinities and NaN, if any, are taken out of the
 // product.  Rows that see them, or whose result is not finite for another reason, are computed again, each by a wave, in fp32.
@@ -16,8 +17,8 @@
 // the workspace, and a second launch puts the parts together, in order: the result does not depend on which came first.
 //
 // What bounds it: up to 64 rows the cache's bytes (64 requests of 4096, 32 heads on 8: 4 nodes 176 us, 8 nodes 183, 16 nodes 209, 6.1 to 5.1 TB/s; 200 of 100 to 1500, 16 on 16 of 64, 123 us, 5.4 TB/s; 48 of
-// up to 4096 with 1 to 16 nodes 90, 4.5 TB/s and the second launch's 7); with 128 what is issued (2 documents of 80000 with trees of 64, 64 heads on 8: 0.336 TFLOP in 440 us, 0.76 PFLOP/s where a large matrix
-// product reaches 1.2; the matrix unit is busy a third of the time, the vector unit half: two exponentials, maxima and roundings per 512 flops); one short request is the chain of latencies (11.5 us).
+// up to 4096 with 1 to 16 nodes 90, 4.5 TB/s and the second launch's 7); with 128 what is issued (2 documents of 80000 with trees of 64, 64 heads on 8: 0.336 TFLOP in 545 us, 0.62 PFLOP/s where a large matrix
+// product reaches 1.2: an exponential, a maximum and two roundings per 512 flops, and a third of the matrix instructions for the second terms); one short request is the chain of latencies (11.5 us).
 #include "lanes.h"
 
 #include <type_traits>
@@ -67,6 +68,18 @@ __device__ __forceinline__ int ta_cut(int i, int stages, int n) { return (int)((
 __device__ __forceinline__ int ta_here(int v) {
     asm volatile("" : "+v"(v));
     return v;
+}
+
+// weights i and i + 1 as sums of two fp16 terms each
+__device__ __forceinline__ void ta_terms(const float (&p)[2], int i, half8_t &p8, half8_t &rest8) {
+    float one = 1.f;
+    half2_t h = {(half_t)p[0], (half_t)p[1]};
+    asm("" : "+v"(h), "+s"(one));                // (two are rounded by one instruction, and each one's rest is another)
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        p8[i + e] = h[e];
+        rest8[i + e] = (half_t)__builtin_fmaf(p[e], one, -(float)h[e]);
+    }
 }
 
 // the larger of v here and in the lane whose number differs by W (16 or 32), or (SUM) both together
@@ -504,7 +517,7 @@ __global__ __launch_bounds__(256, 2) void attention_tree_few_kernel(const ta_arg
                         for (int e = 0; e < 4; e++) s[t][i][e] = seen >> e & 1 ? s[t][i][e] : -INFINITY;
                     }
             }
-            half8_t p8[QT];
+            half8_t p8[QT], rest8[QT];
             float r[QT];
 #pragma unroll
             for (int t = 0; t < QT; t++) {
@@ -517,10 +530,14 @@ __global__ __launch_bounds__(256, 2) void attention_tree_few_kernel(const ta_arg
                 m[t] = mn;
                 float sum[2] = {0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i >> 2][i & 3], scale2, -from));
-                    sum[i & 1] += p;
-                    p8[t][i] = (half_t)p;
+                for (int i = 0; i < 8; i += 2) {
+                    float p[2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][(i + e) >> 2][(i + e) & 3], scale2, -from));
+                        sum[e] += p[e];
+                    }
+                    ta_terms(p, i, p8[t], rest8[t]);
                 }
                 l[t] = l[t] * r[t] + (sum[0] + sum[1]);
             }
@@ -558,6 +575,8 @@ __global__ __launch_bounds__(256, 2) void attention_tree_few_kernel(const ta_arg
                 const half8_t v = {v8[0][j], v8[1][j], v8[2][j], v8[3][j], v8[4][j], v8[5][j], v8[6][j], v8[7][j]};
 #pragma unroll
                 for (int t = 0; t < QT; t++) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p8[t], acc[t][j], 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < QT; t++) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, rest8[t], acc[t][j], 0, 0, 0);
             }
             if (next < st_end) fetch_v(next, rel);
             st = next;
@@ -807,7 +826,7 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
         // infinities and NaN in a stage's v become zeros, and their positions are noted
         auto clean = [&](half_t *sv, int st) {
 #pragma unroll 1
-            for (int i = tid; i < TA_P * D / 8; i += THREADS) {
+            for (int i = ta_here(tid); i < TA_P * D / 8; i += THREADS) {
                 half8_t v = *reinterpret_cast<const half8_t *>(sv + 8 * i);
                 bool odd = false;
 #pragma unroll
@@ -869,7 +888,7 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
             __builtin_amdgcn_sched_barrier(0);
         };
         float4_t sa[QT][2], sb[QT][2];
-        half8_t p8[QT];
+        half8_t p8[QT], rest8[QT];              // a weight is the sum of two
         half8_t vt[W];
         float r[QT];
         auto values = [&](const half_t *stage) __attribute__((always_inline)) {
@@ -895,15 +914,19 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
                 m[t] = mn;
                 float sum[2] = {0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i >> 2][i & 3], scale2, -from));
-                    sum[i & 1] += p;
-                    p8[t][i] = (half_t)p;
+                for (int i = 0; i < 8; i += 2) {
+                    float p[2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][(i + e) >> 2][(i + e) & 3], scale2, -from));
+                        sum[e] += p[e];
+                    }
+                    ta_terms(p, i, p8[t], rest8[t]);
                 }
                 l[t] = l[t] * r[t] + (sum[0] + sum[1]);
             }
 #pragma unroll
-            for (int t = 0; t < QT; t++) asm volatile("" : "+v"(p8[t]));   // (computed here, beside the products, and not behind the branch)
+            for (int t = 0; t < QT; t++) asm volatile("" : "+v"(p8[t]), "+v"(rest8[t]));   // (computed here, beside the products, and not behind the branch)
         };
         auto output = [&]() __attribute__((always_inline)) {
             if (__any(r[0] != 1.f || r[QT - 1] != 1.f)) {
@@ -916,6 +939,8 @@ __global__ __launch_bounds__(WR * 64, 2) void attention_tree_kernel(const ta_arg
             for (int j = 0; j < W; j++) {
 #pragma unroll
                 for (int t = 0; t < QT; t++) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[j], p8[t], acc[t][j], 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < QT; t++) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt[j], rest8[t], acc[t][j], 0, 0, 0);
             }
         };
         // a stage

@@ -559,7 +559,7 @@ int bs_tree_plan(const int32_t *parents, const int32_t *lengths, const int32_t *
  * that nothing is left for, are zeros.  Positions whose table entry is no page are left out.  What is masked or left out has no
  * influence, whatever stands there.  head_dim 64 or 128; B <= 65536, T * heads <= 2^22, B * heads <= 2^22 and B *
  * max_pages * page_size < 2^35.  out must not overlap q.
- * Scores, maximum and sums in fp32, the weights in fp16 for the product with v, the largest as 2^15.  A score of -inf weighs nothing, one of
+ * Scores, maximum and sums in fp32, the weights as two fp16 terms for the product with v (2^-22), the largest as 2^15.  A score of -inf weighs nothing, one of
  * +inf or NaN makes its row of its head NaN.  Deterministic.  Scratch: bs_attention_tree_workspace_bytes, 16-byte aligned (0: none; negative: an error status).
  */
 int64_t bs_attention_tree_workspace_bytes(int B, int T, int nodes, int heads, int kv_heads, int head_dim, int page_size, int max_pages);
