@@ -646,7 +646,7 @@ extern "C" int bs_logits_adjust_f16(const void *logits, int64_t ld, void *out, i
                                     const int32_t *drafted, int drafted_width, const int32_t *bias_tokens, const float *bias, int biases, const int32_t *allowed, int masks,
                                     const int32_t *allowed_rows, int R, int V, int B, void *stream) {
     if (sample_shape(R, V) != BS_OK || B < 0 || (R > 1 && (ld < V || ld_out < V)) || history_width < 0 || drafted_width < 0 || biases < 0 || masks < 0 ||
-        history_width > 1 << 30 || drafted_width > 1 << 30 || biases > 1 << 30 ||
+        history_width > 1 << 30 || drafted_width > 1 << 30 || (int64_t)history_width + drafted_width > INT32_MAX || biases > 1 << 30 ||   // (counts of 31 bits)
         ((history_lengths || prompt_lengths) && !history && history_width > 0) || (bias_tokens != nullptr) != (bias != nullptr) || (allowed_rows && !allowed && masks > 0) ||
         (allowed && !allowed_rows && masks < R) || (logits == out && ld != ld_out && R > 1) ||
         (!requests && B < R && (history || drafted || bias || repetition || frequency || presence)))

@@ -615,7 +615,7 @@ int bs_page_fork_f16(const int32_t *source, const int32_t *lengths, int32_t *blo
  *               allowed_rows[r] (NULL: mask r; a number that no mask has: none); -inf where the bit is 0
  * Any of them may be NULL, or have no width: history_lengths the whole width, prompt_lengths 0, repetition 1 (also where it is not above 0),
  * frequency and presence 0.  Tokens outside 0 .. V - 1 are none.  Finite logits stay finite up to here, at most 65504, unless a bias is infinite; settings other
- * than biases must be finite.  R <= 2^20, V <= 2^18, R * V <= 2^33, widths and biases <= 2^30.  No counterpart in the reference.
+ * than biases must be finite.  R <= 2^20, V <= 2^18, R * V <= 2^33, widths and biases <= 2^30, both widths together below 2^31.  No counterpart in the reference.
  */
 int bs_logits_adjust_f16(const void *logits, int64_t ld, void *out, int64_t ld_out, const int32_t *requests, const int32_t *history, int history_width,
                          const int32_t *history_lengths, const int32_t *prompt_lengths, const float *repetition, const float *frequency, const float *presence,
