@@ -7,14 +7,14 @@ namespace {
 
 constexpr int NODES = 64, THREADS = 256, WAVES = THREADS / 64;
 
-// request b's token rows start .. end - 1, the first `nodes` of them its tree: 0 without slots, or with more nodes than `most`
+// request b's token rows start .. end - 1, the first `nodes` of them its tree: 0 without slots, or with more nodes than `most` or (lengths not null) than its length
 struct tree_rows {
     int start, end, nodes;
-    __device__ __forceinline__ tree_rows(const int32_t *starts, const int32_t *granted, int b, int T, int most) {
+    __device__ __forceinline__ tree_rows(const int32_t *starts, const int32_t *granted, const int32_t *lengths, int b, int T, int most) {
         start = min(max(starts[b], 0), T);
         end = min(max(starts[b + 1], start), T);
         const int n = granted[b];
-        nodes = n > 0 && n <= most && n <= end - start ? n : 0;
+        nodes = n > 0 && n <= most && n <= end - start && (!lengths || n <= lengths[b]) ? n : 0;
     }
 };
 
@@ -37,7 +37,7 @@ __global__ __launch_bounds__(THREADS) void tree_plan_kernel(const int32_t *__res
     }
     const int b = blockIdx.x * WAVES + wave;
     if (b >= B) return;
-    const tree_rows r(starts, granted, b, T, NODES);
+    const tree_rows r(starts, granted, lengths, b, T, NODES);
     const int held = max(lengths[b] - granted[b], 0);
     int p = lane < r.nodes ? parents[r.start + lane] : -1;
     if (p >= lane) p = -1;
@@ -74,13 +74,13 @@ struct accept_args {
     int B, T, nodes, blocks, layers, kv_heads, pieces, shift, max_pages, pool;
 };
 
-// one request by one wave, a lane a node
+// One request by one wave, a lane a node.  `writes`: by the wave that writes what the caller gets, which looks at the length; the others, which move, cannot: that wave may have written on it.
 struct accept_path {
     tree_rows r;
     int parent;
     int64_t drafted, target, slot;
     int at, count, mine;                         // the last node of the path, nodes on it, lane i: node i of it
-    __device__ __forceinline__ accept_path(const accept_args &a, int b) : r(a.starts, a.granted, b, a.T, a.nodes) {
+    __device__ __forceinline__ accept_path(const accept_args &a, int b, bool writes) : r(a.starts, a.granted, writes ? a.lengths : nullptr, b, a.T, a.nodes) {
         const int lane = threadIdx.x & 63;
         const bool there = lane < r.nodes;
         parent = there ? a.parents[r.start + lane] : -1;
@@ -150,9 +150,10 @@ struct accept_path {
 // (10 MB to and fro).
 __global__ __launch_bounds__(THREADS) void tree_accept_kernel(const accept_args a) {
     const int b = blockIdx.x / a.blocks, block = blockIdx.x - b * a.blocks;
-    accept_path p(a, b);
+    const bool writes = block == 0 && threadIdx.x < 64;
+    accept_path p(a, b, writes);
     p.walk();
-    if (block == 0 && threadIdx.x < 64) {
+    if (writes) {
         const int2 back = p.write(a, b);
         if (threadIdx.x == 0) {
             a.back[2 * b] = back.x;
@@ -167,7 +168,7 @@ constexpr int FEW = 64, FEW_THREADS = 1024, FEW_WAVES = FEW_THREADS / 64;
 __global__ __launch_bounds__(FEW_THREADS) void tree_accept_few_kernel(const accept_args a, const int32_t *__restrict__ table, int32_t *ring, const int32_t *state, int32_t *state_out) {
     if (blockIdx.x > 0) {
         const int b = (blockIdx.x - 1) / a.blocks, block = (blockIdx.x - 1) - b * a.blocks;
-        accept_path p(a, b);
+        accept_path p(a, b, false);
         p.walk();
         return p.move(a, block * FEW_THREADS + threadIdx.x, a.blocks * FEW_THREADS);
     }
@@ -177,7 +178,7 @@ __global__ __launch_bounds__(FEW_THREADS) void tree_accept_few_kernel(const acce
     for (int b0 = 0; b0 < a.B; b0 += FEW_WAVES) {
         const int b = b0 + wave;
         if (b >= a.B) break;
-        accept_path p(a, b);
+        accept_path p(a, b, true);
         p.walk();
         const int2 back = p.write(a, b);
         if (lane == 0) {

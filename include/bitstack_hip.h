@@ -541,7 +541,7 @@ int bs_sample_f16(const void *logits, int64_t ld, const float *uniform, const fl
  * bs_page_plan has left for a step of that many tokens: request b held lengths[b] -
  * granted[b] positions and has granted[b] nodes (0: refused, or idle).  starts must not
  * decrease.  At most 64 nodes, and as many as `nodes` says where it is given; a request with
- * more, or with more than its token rows or its length, has none.  No counterpart in the reference.
+ * more, or with more than its token rows or its length, has none (what its slots hold may change then; no plan leaves more than the length).  No counterpart in the reference.
  *
  * bs_tree_plan, once per step: positions[T], the positions held plus the node's depth,
  * which its query and key are rotated by (bs_rope_store_paged_f16 with these and the plan's
@@ -555,8 +555,8 @@ int bs_tree_plan(const int32_t *parents, const int32_t *lengths, const int32_t *
  * Attention of the nodes, their keys and values being stored: out[T, heads * head_dim] =
  * softmax(q k^T / sqrt(head_dim)) v over the positions that the request held and those of
  * its nodes that masks[t] names (any mask, not only a tree's; bits of no node are ignored).  q [T, heads * head_dim] is
- * rotated (rows ldq halves apart).  Position p of request b, nodes behind the held ones, is at row p of its pages.  Rows that are no node, and rows
- * that nothing is left for, are zeros.  Positions whose table entry is no page are left out.  What is masked or left out has no
+ * rotated (rows ldq halves apart).  Position p of request b, nodes behind the held ones, is at row p of its pages.  Rows that are no node, rows
+ * that nothing is left for, and those of a length beyond the table's row, are zeros.  Positions whose table entry is no page are left out.  What is masked or left out has no
  * influence, whatever stands there.  head_dim 64 or 128; B <= 65536, T * heads <= 2^22, B * heads <= 2^22 and B *
  * max_pages * page_size < 2^35.  out must not overlap q.
  * Scores, maximum and sums in fp32, the weights as two fp16 terms for the product with v (2^-22), the largest as 2^15.  A score of -inf weighs nothing, one of
