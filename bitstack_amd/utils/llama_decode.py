@@ -662,7 +662,7 @@ class SyntheticLlamaDecoder:
             x = bitstack_forward_group_hip(grp["down"], act, EPI_RESIDUAL, residual=x)
         self.logits = self._head(rmsnorm_hip(x, self.final_norm, eps))
         if adjust:
-            logits_adjust_hip(self.logits, **adjust)
+            self.logits = logits_adjust_hip(self.logits, **adjust)         # (in place, or the caller's `out`)
         token = self._choose(uniform, **sampling)
         torch.where(plan.granted > 0, token, cache.token, out=cache.token)
         return plan
@@ -730,7 +730,7 @@ class SyntheticLlamaDecoder:
                 other = torch.arange(1, nodes, device=self.dev)
                 drafted = ids[(plan.starts[request].long()[:, None] + other).clamp(max=T - 1)]
                 adjust = {**adjust, "drafted": torch.where((tree.masks[:, None] >> other & 1) == 1, drafted, -1).int()}
-            logits_adjust_hip(self.logits, requests=request.int(), **adjust)
+            self.logits = logits_adjust_hip(self.logits, requests=request.int(), **adjust)
         targets = self._choose(uniform, **{name: None if t is None else t[request] for name, t in sampling.items()})
         done = tree_accept_hip(ids, parents, targets, plan.slots, cache.lengths, plan.granted, plan.starts, cache.block_table, cache.free_pages, cache.free_state, cache.kpages,
                                cache.vpages, nodes, inplace=True)
