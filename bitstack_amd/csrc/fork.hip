@@ -165,7 +165,9 @@ __device__ __forceinline__ void fork_few_tables(const fork_args &a) {
     }
 }
 
-// ... and as many as there are.
+// ... and as many as there are.  The choice goes by rows and the table's width, as lengths are known on the device alone.  us a call of a graph, 32 layers of 8 heads of 128: 4 rows of 300 positions 5.8 in tables of up to 64
+// pages (an entry to a lane), 7.0 in one of 256 (four), 7.5 in one of 512 and 7.9 in one of 1024 (here); 17 rows of 300 9.3 in one of 128 (four), 11.1 in one of 129 (here); 48 rows 15.9 in one of 64, 25 in one of 65 (here);
+// 4 rows of 8000, tables of 502 to 1024, 20 to 24.
 __device__ __forceinline__ void fork_tables(const fork_args &a) {
     __shared__ uint32_t waves[WAVES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

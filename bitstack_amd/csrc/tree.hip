@@ -146,8 +146,8 @@ struct accept_path {
     }
 };
 
-// Many requests: workgroups of one request each; the ring in a launch of its own.  What bounds both is the chain row -> parents, tokens, targets -> path -> slots -> moves: 48 requests of up to 32 nodes 8.3 us
-// (10 MB to and fro).
+// Many requests: workgroups of one request each; the ring in a launch of its own.  What bounds both is the chain row -> parents, tokens, targets -> path -> slots -> moves: 100 requests of up to 32 nodes, 32 layers
+// of 8 heads of 128, 11.9 us and 3.9 for the ring (21 MB to and fro).
 __global__ __launch_bounds__(THREADS) void tree_accept_kernel(const accept_args a) {
     const int b = blockIdx.x / a.blocks, block = blockIdx.x - b * a.blocks;
     const bool writes = block == 0 && threadIdx.x < 64;
@@ -163,7 +163,8 @@ __global__ __launch_bounds__(THREADS) void tree_accept_kernel(const accept_args 
     p.move(a, block * THREADS + threadIdx.x, a.blocks * THREADS);
 }
 
-// Up to 64: one workgroup writes what the caller gets, and the ring; beside it, the others move.  (one request of 8 nodes, 32 layers of 8 heads of 128: 7.2 us, with a second launch 10.3.)
+// Up to 64: one workgroup writes what the caller gets, and the ring; beside it, the others move.  (one request of 8 nodes, 32 layers of 8 heads of 128: 7.3 us a call, 4.8 on the device,
+// with a second launch 10.3; 48 requests of up to 32 nodes, 10 MB to and fro, 8.0.)
 constexpr int FEW = 64, FEW_THREADS = 1024, FEW_WAVES = FEW_THREADS / 64;
 __global__ __launch_bounds__(FEW_THREADS) void tree_accept_few_kernel(const accept_args a, const int32_t *__restrict__ table, int32_t *ring, const int32_t *state, int32_t *state_out) {
     if (blockIdx.x > 0) {

@@ -8,7 +8,8 @@
 // Up to 32 rows a wave takes every fourth stage with K and V in registers; beyond, every wave has 16 or 32 rows, and the stages come to LDS straight from the pages (no registers).
 // Maximum, sum and output are fp32, in base 2.  The weights enter the second product as two fp16 terms, p = hi + lo, the largest as 2^15: held to 2^-22 of themselves down to 2^-18 of the
 // largest, below that to 2^-40 of the largest.  (hi alone: an error against 64 bits of 2.2 to 2.7e-4 where the result's rounding is 2.1e-4, and where many weights are rounded up values of 65504
-// everywhere became infinities, as the sum below the line is that of the fp32 weights.  Up to 64 rows the second term's products cost nothing that shows, 128 rows 545 us instead of 441 for 2 documents of 80000.)
+// everywhere became infinities, as the sum below the line is that of the fp32 weights.  The second terms' products cost 0 to 2 % up to 32 rows
+// of a KV head, 0 to 5 with 64, a sixth to a quarter with 128: 64 requests of 4000, 32 heads on 8, 16 nodes 174 -> 183 us, 32 nodes 226 -> 266; 2 documents of 80000 with trees of 64 441 -> 545.)
 //
 // What a row does not see has a weight of zero, but zero times an infinity is NaN: in the stages with nodes V is looked through, and infinities and NaN, if any, are taken out of the
 // product.  Rows that see them, or whose result is not finite for another reason, are computed again, each by a wave, in fp32.
@@ -16,9 +17,9 @@
 // The split: as the lengths are known on the device alone, every workgroup works out from them what it is to do (ta_deal).  What is not a whole request's leaves (max, sum, weighted v) in
 // the workspace, and a second launch puts the parts together, in order: the result does not depend on which came first.
 //
-// What bounds it: up to 64 rows the cache's bytes (64 requests of 4096, 32 heads on 8: 4 nodes 176 us, 8 nodes 183, 16 nodes 209, 6.1 to 5.1 TB/s; 200 of 100 to 1500, 16 on 16 of 64, 123 us, 5.4 TB/s; 48 of
-// up to 4096 with 1 to 16 nodes 90, 4.5 TB/s and the second launch's 7); with 128 what is issued (2 documents of 80000 with trees of 64, 64 heads on 8: 0.336 TFLOP in 545 us, 0.62 PFLOP/s where a large matrix
-// product reaches 1.2: an exponential, a maximum and two roundings per 512 flops, and a third of the matrix instructions for the second terms); one short request is the chain of latencies (11.5 us).
+// What bounds it: up to 64 rows the cache's bytes (64 requests of 4000, 32 heads on 8: 4 nodes 169 us, 8 nodes 173, 16 nodes 183, 6.2 to 5.8 TB/s; 200 of 100 to 1500, 16 on 16 of 64, 123 us, 5.4 TB/s; 48 of
+// up to 4096 with 1 to 16 nodes 88, 4.6 TB/s and the second launch's 7); with 128 what is issued (2 documents of 80000 with trees of 64, 64 heads on 8: 0.336 TFLOP in 545 us, 0.62 PFLOP/s where a large matrix
+// product reaches 1.2: an exponential, a maximum and two roundings per 512 flops, and a third of the matrix instructions for the second terms); one short request is the chain of latencies (11.8 us).
 #include "lanes.h"
 
 #include <type_traits>
@@ -135,8 +136,8 @@ __device__ __forceinline__ ta_request ta_uniform(const ta_request &r, int lane) 
 // How the stages of all requests, `sum`, are dealt to a.shares workgroups of a unit.
 // Equal shares keep the workgroups busy to the end whatever the lengths are, but one may hold the end of a request and the beginning of another: each costs its chain of latencies (lengths, pages, K, what it
 // leaves), 4 us, and is a part.  Each request's own parts, one to a workgroup, have one chain, but may be unequal.  They are taken where they fit and none has `more` stages more than an equal share (16
-// up to 32 rows, whose stages take 0.3 us, else 32).  us, equal shares / own parts: 5 requests of up to 1000 with 8 nodes 19 / 14, 16 of up to 250 24 / 14, 64 of up to 1000 with 32 nodes 78 / 62, and
-// at a limit of 32 where 16 stands 32 requests of up to 4000 with 4 nodes 58 / 65.
+// up to 32 rows, whose stages take 0.3 us, else 32).  us, equal shares / own parts: 5 requests of up to 1000 with 8 nodes 22.5 / 14.0, 16 of up to 250 22.0 / 13.6, 64 of up to 1000 with 32 nodes 77 / 71, and without
+// the limit 32 requests of up to 4000 with 4 nodes 55 / 69.
 // A part has at least 4 stages; more where the longest request would be in many, which the second launch takes eight at a time (8 nodes, one request of 4000: 8 stages 16.6, 4 stages 20.1); and more
 // where all of them are many: what all units leave of one costs part_cost stages, so that parts of sqrt(part_cost sum) stages cost as much as they have (16 requests of 390: whole 15, in four 25).
 struct ta_deal {
@@ -1138,19 +1139,19 @@ struct ta_shape {
 ta_shape shape_of(int B, int nodes, int heads, int kv_heads, int64_t positions) {
     ta_shape p;
     const int64_t rows = (int64_t)(heads / kv_heads) * nodes;
-    // As many rows as there are, up to 128: K and V are read once for each tile of them.  (33 to 64 rows with K and V in registers, four tiles of columns to a wave: 118 us instead of 93 for 48 requests of up to
-    // 4096 with 16 nodes; 64 rows to a wave, 256 to a workgroup: 796 instead of 524 for 2 of 80000 with trees of 64, the sums no longer fit the registers.)
+    // As many rows as there are, up to 128: K and V are read once for each tile of them.  (33 to 64 rows with K and V in registers, four tiles of columns to a wave: a quarter slower for 48 requests of up to
+    // 4096 with 16 nodes; 64 rows to a wave, 256 to a workgroup: half slower for 2 of 80000 with trees of 64, the sums no longer fit the registers.)
     p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
     p.units = kv_heads * (int)bs_cdiv(rows, p.rows);
-    // Two workgroups to a CU (768 of them in all: 243 us, 1024 219, 512 201 for 64 requests of 4096).  Tables of up to 512 positions, 16 stages, are not cut: the second launch costs 2.5 us and parts their
-    // traffic (us, uncut / cut: one of 390 with 8 nodes 11.9 / 12.1, 16 of 390 12.4 / 16.8, 64 of 390 26 / 30; with 32 nodes 21 / 16, 22 / 28, 35 / 45).
+    // Two workgroups to a CU (768 of them in all: 233 us, 1024 208, 512 183 for 64 requests of 4000 with 16 nodes).  Tables of up to 512 positions, 16 stages, are not cut: the second launch costs 2.5 us and parts their
+    // traffic (us, uncut / cut: one of 390 with 8 nodes 11.8 / 11.9, 16 of 390 12.7 / 16.2, 64 of 390 23 / 27; with 32 nodes 24 / 16, 26 / 29, 40 / 48).
     p.shares = positions <= 512 ? 0 : 512 / p.units > 1 ? 512 / p.units : 1;
     return p;
 }
 int64_t before_bytes(int B) { return bs_cdiv(4ll * (B + 3), 16) * 16; }
 
-// A cache that the last-level cache cannot hold is read past it, where a workgroup of the unit has all of its rows (64 requests of 4096, 4 nodes 203 -> 188 us, 8 nodes 214 -> 205).  Where several read the
-// same positions the second one finds them there (32 nodes: 252, past it 323).
+// A cache that the last-level cache cannot hold is read past it, where a workgroup of the unit has all of its rows (64 requests of 4000, 4 nodes 186 -> 169 us, 8 nodes 189 -> 173, 16 nodes 199 -> 183).  Where several read the
+// same positions the second one finds them there (256 rows: a quarter slower past it).
 constexpr int64_t TA_STREAM = 256ll << 20;
 
 template <int D>

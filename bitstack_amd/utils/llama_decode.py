@@ -683,7 +683,8 @@ class SyntheticLlamaDecoder:
 
     @torch.no_grad()
     def step_tree(self, cache: PagedCache, tokens, parents, new_tokens, nodes=64, released=None, uniform=None, adjust=None, **sampling):
-        """Several drafted tokens per request in one step, of which as many are kept as the model would have given one by one.  Request b's new_tokens[b] (int32 [rows], up to
+        """Several drafted tokens per request in one step, of which those are kept that the model itself gives behind what is in front of them (as in steps of one token, up to the roundings of kernels for
+        other token counts; what is drawn depends on `uniform` [T], which is per node).  Request b's new_tokens[b] (int32 [rows], up to
         `nodes`; 0: idle) tokens are the next rows of tokens [T] (int64) and parents [T] (int32: a number among the request's own, smaller than the token's; -1 for the first): its first
         one is its cache.token, whatever `tokens` says, the others are drafts, each behind its parent (numbers outside the vocabulary, also in rows of no request, are none).  The model's token behind each is greedy, or drawn with uniform [T] and the
         requests' temperature, top_k, top_p, min_p [rows]; `adjust`: logits_adjust_hip's settings per request and allowed_rows per token (history with cache.token in it, the drafts are added).
