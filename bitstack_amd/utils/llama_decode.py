@@ -676,9 +676,9 @@ class SyntheticLlamaDecoder:
         """The token of every row of the logits, greedy or drawn."""
         if uniform is not None:
             return sample_hip(self.logits, uniform, **sampling)
-        if self.logits.shape[0] == 1 or self.logits.shape[1] % 8 == 0:
+        if (self.logits.shape[0] == 1 or self.logits.shape[1] % 8 == 0) and self.logits.is_contiguous() and self.logits.data_ptr() % 16 == 0:
             return argmax_hip(self.logits)
-        zeros = torch.zeros(self.logits.shape[0], device=self.dev)        # (rows that do not start on 16 bytes)
+        zeros = torch.zeros(self.logits.shape[0], device=self.dev)        # (rows that do not start on 16 bytes, or of a wider tensor)
         return sample_hip(self.logits, zeros, temperature=zeros)
 
     @torch.no_grad()

@@ -45,3 +45,17 @@ def test_a_step_with_drafts():
         assert done.accepted.tolist() == [3, 2] and cache.token.tolist() == [9, 8]
         results.append(dec.logits.clone())
     assert torch.equal(results[0], results[1])
+
+
+@pytest.mark.parametrize("wide,first", [(SHAPE.vocab + 24, 0), (SHAPE.vocab + 24, 8), (SHAPE.vocab, 1), (SHAPE.vocab + 3, 2)])
+def test_rows_of_a_wider_tensor(wide, first):
+    """Greedy tokens from an output whose rows are apart, or do not start on 16 bytes."""
+    results = []
+    for own in (False, True):
+        dec = decoder()
+        cache = cache_of(dec)
+        out = torch.zeros(2 * wide + first, dtype=torch.float16, device="cuda")[first:].view(2, wide)[:, :SHAPE.vocab]
+        bias = dict(bias_tokens=i32([[9], [8]]), bias=torch.full((2, 1), 2000.0, device="cuda"))
+        dec.step_paged(cache, adjust=dict(bias, **({"out": out} if own else {})))
+        results.append((dec.logits.clone(), cache.token.tolist()))
+    assert torch.equal(results[0][0], results[1][0]) and results[0][1] == results[1][1] == [9, 8]
